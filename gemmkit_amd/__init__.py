@@ -39,7 +39,10 @@ counterpart): f32 output for bf16 GEMMs (:func:`gemm_bf16_f32out`,
 :func:`gemm_batched_bf16_f32out`), per-column requant vectors
 (``RequantScale.PerCol``, ``Requantize(bias_axis="col")``), a ReLU after
 requantization (``Requantize(relu=True)``), and prepacked-B requantization
-(:func:`gemm_i8_packed_b_requant`).
+(:func:`gemm_i8_packed_b_requant`), products of ragged groups with their weight
+gradient (:func:`gemm_grouped`, :func:`gemm_grouped_wgrad`: the experts of a routed
+layer), and MXFP4 operands (:class:`MatMxfp4`, :func:`quantize_mxfp4`,
+:func:`dequantize_mxfp4`, :func:`gemm_mxfp4`, :func:`gemm_grouped_mxfp4`).
 
 All tensors must live on the HIP device; calls are synchronous by default and
 run on torch's current stream.  There is no CPU fallback: a missing library
@@ -54,7 +57,7 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _lib
-from ._lib import BiasC, MatMutC, MatRefC, RequantizeC
+from ._lib import BiasC, MatMutC, MatRefC, Mxfp4C, RequantizeC
 
 __all__ = [
     "GemmkitError", "MatRef", "MatMut", "Parallelism", "Workspace", "RequantScale",
@@ -66,7 +69,9 @@ __all__ = [
     "gemm_batched", "gemm_batched_unchecked", "gemm_batched_bf16_f32out", "prepack_rhs",
     "gemm_packed_b", "gemm_packed_b_unchecked", "Bias", "Activation", "gemm_fused",
     "gemm_fused_unchecked", "gemm_batched_fused", "gemm_batched_fused_unchecked",
-    "gemm_packed_b_fused", "gemm_packed_b_fused_unchecked", "set_synchronous",
+    "gemm_packed_b_fused", "gemm_packed_b_fused_unchecked", "gemm_grouped",
+    "gemm_grouped_wgrad", "MatMxfp4", "quantize_mxfp4", "dequantize_mxfp4", "gemm_mxfp4",
+    "gemm_grouped_mxfp4", "set_synchronous",
     "library_path", "version",
 ]
 
@@ -1007,3 +1012,165 @@ def gemm_packed_a_fused_unchecked(alpha, packed: PackedLhs, n, b, rsb, csb, beta
             _ws(ws), _bf16_bits(alpha), packed.handle, n, _ptr(b, b_off), rsb, csb,
             _bf16_bits(beta), _ptr(c, c_off), rsc, csc, bp, bd, hb, int(act), _bf16_bits(slope),
             _par(par)))
+
+
+# -------------------------------------------- ragged groups, MXFP4 operands
+
+def _here(*tensors: torch.Tensor) -> None:
+    """The tensors of a call lie on the current device, whose stream it goes to."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t.is_cuda and t.device.index != dev:
+            raise GemmkitError(-7, f"gemmkit_amd: a tensor lies on {t.device}, the current device "
+                                   f"is cuda:{dev}")
+
+
+def _offsets(offsets: torch.Tensor):
+    """(device pointer, number of groups) of a call's group offsets."""
+    d = _slice(offsets, "offsets")
+    if d.dtype != torch.int32 or d.dim() != 1 or d.numel() < 1:
+        raise TypeError("gemmkit_amd: offsets must be a 1-D int32 tensor of groups + 1 entries, got "
+                        f"{d.dtype} of shape {tuple(d.shape)}")
+    return d.data_ptr(), d.numel() - 1
+
+
+def _out_entry(c: MatMut, bf16_entry, f32_entry, what: str):
+    dt = c.data.dtype
+    if dt == torch.bfloat16:
+        return bf16_entry, dt
+    if dt == torch.float32:
+        return f32_entry, dt
+    raise TypeError(f"gemmkit_amd: {what} writes bfloat16 or float32, got {dt}")
+
+
+def gemm_grouped(alpha: float, a: MatRef, offsets: torch.Tensor, b: MatRef, b_group_stride: int,
+                 beta: float, c: MatMut, par: Optional[Parallelism] = None,
+                 ws: Optional[Workspace] = None) -> None:
+    """Extension: one product per group of rows, the experts of a routed layer.
+
+    ``C[rows of g] <- alpha * A[rows of g] @ B_g + beta * C[rows of g]``: A is rows x k and C
+    rows x n, B_g the k x n view ``b`` moved by ``g * b_group_stride`` elements; bfloat16
+    inputs, f32 sums, bfloat16 or float32 C.  ``offsets`` (int32, groups + 1 entries, on the
+    device, so that routing needs no copy to the host) bounds the groups: rows
+    ``offsets[g] .. offsets[g + 1]``, empty ones among them.  Offsets outside the rows or
+    not increasing are clamped (``s_i = min(rows, max(0, offsets[:i + 1]))``); rows of no
+    group are left as they are.
+
+    Weights stored output-major (n x k) are the view ``MatRef(w, k, n, 1, k)``.  The gradient
+    of A is the same call on the output's gradient with ``MatRef(w, n, k, k, 1)``."""
+    _bind_stream()
+    fn, dt = _out_entry(c, "gk_gemm_grouped_bf16", "gk_gemm_grouped_bf16_f32out", "gemm_grouped")
+    off, groups = _offsets(offsets)
+    _here(a.data, b.data, c.data, offsets)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c(torch.bfloat16, "A"), off, groups,
+                                   b._c(torch.bfloat16, "B"), b_group_stride, float(beta),
+                                   c._c(dt, "C"), _par(par)))
+
+
+def gemm_grouped_wgrad(alpha: float, a: MatRef, offsets: torch.Tensor, b: MatRef, beta: float,
+                       c: MatMut, c_group_stride: int, par: Optional[Parallelism] = None,
+                       ws: Optional[Workspace] = None) -> None:
+    """Extension: the gradient of :func:`gemm_grouped`'s weights.
+
+    ``C_g <- alpha * A[rows of g]^T @ B[rows of g] + beta * C_g``: A is rows x k (the product's
+    left operand), B rows x n (the gradient of its output), C_g the k x n view ``c`` moved by
+    ``g * c_group_stride`` elements; bfloat16 inputs, f32 sums, bfloat16 or float32 C.  An
+    empty group's C_g becomes ``beta * C_g``.  ``offsets`` as in :func:`gemm_grouped`."""
+    _bind_stream()
+    fn, dt = _out_entry(c, "gk_gemm_grouped_wgrad_bf16", "gk_gemm_grouped_wgrad_bf16_f32out",
+                        "gemm_grouped_wgrad")
+    off, groups = _offsets(offsets)
+    _here(a.data, b.data, c.data, offsets)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c(torch.bfloat16, "A"), off, groups,
+                                   b._c(torch.bfloat16, "B"), float(beta), c._c(dt, "C"),
+                                   c_group_stride, _par(par)))
+
+
+class MatMxfp4:
+    """Extension: a rows x cols matrix in MXFP4.  Row r's elements are e2m1 codes (0, 0.5, 1,
+    1.5, 2, 3, 4, 6 and their negatives), two a byte with the even element in the lower
+    nibble, 16 bytes per begun block of 32, at ``codes + r * ld``; each block has an e8m0
+    scale byte (2^(byte - 127), 255: NaN) at ``scales + r * lds``.  ``codes`` and ``scales`` are
+    contiguous uint8 device tensors, their row strides (bytes, multiples of 16) by default
+    those of whole rows: ``16 * ceil(cols / 32)`` and ``ceil(cols / 32)`` rounded up to 16."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int,
+                 ld: Optional[int] = None, lds: Optional[int] = None):
+        self.codes, self.scales = codes, scales
+        self.rows, self.cols = int(rows), int(cols)
+        blocks = -(-self.cols // 32)
+        self.ld = 16 * blocks if ld is None else int(ld)
+        self.lds = -(-blocks // 16) * 16 if lds is None else int(lds)
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device="cuda") -> "MatMxfp4":
+        """An uninitialised matrix to quantize into."""
+        blocks = -(-int(cols) // 32)
+        codes = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device)
+        scales = torch.empty((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device)
+        return cls(codes, scales, rows, cols)
+
+    def _c(self, what: str) -> Mxfp4C:
+        codes, scales = _slice(self.codes, what), _slice(self.scales, what)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"gemmkit_amd: {what} codes and scales must be uint8")
+        if min(self.rows, self.cols, self.ld, self.lds) < 0:
+            raise GemmkitError(-2, f"gemmkit_amd: {what} has a negative side or stride")
+        _here(codes, scales)
+        return Mxfp4C(codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
+                      self.rows, self.cols, self.ld, self.lds)
+
+
+def quantize_mxfp4(x: MatRef, q: Optional[MatMxfp4] = None) -> MatMxfp4:
+    """Extension: x (float32 or bfloat16, any strides) in MXFP4, into ``q`` if one is given.
+
+    A block of 32 columns with largest magnitude m gets the scale 2^e with
+    ``e = max(floor(log2 m) - 2, -127)`` and every element the nearest e2m1 value of
+    ``x / 2^e``, ties to the even code, magnitudes above 6 to 6; a block that holds a NaN or
+    an infinity becomes NaN."""
+    _bind_stream()
+    L = _lib.lib()
+    dt = x.data.dtype
+    if dt not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"gemmkit_amd: quantize_mxfp4 supports float32 and bfloat16, got {dt}")
+    view = x._c(dt, "X")
+    _here(x.data)
+    if q is None:
+        q = MatMxfp4.empty(x.rows, x.cols, x.data.device)
+    fn = L.gk_quantize_mxfp4_f32 if dt == torch.float32 else L.gk_quantize_mxfp4_bf16
+    _check(fn(view, q._c("MXFP4 output")))
+    return q
+
+
+def dequantize_mxfp4(q: MatMxfp4, c: MatMut) -> None:
+    """Extension: the values of q in c (float32 or bfloat16, any strides)."""
+    _bind_stream()
+    fn, dt = _out_entry(c, "gk_dequantize_mxfp4_bf16", "gk_dequantize_mxfp4_f32",
+                        "dequantize_mxfp4")
+    _here(c.data)
+    _check(getattr(_lib.lib(), fn)(q._c("MXFP4 input"), c._c(dt, "C")))
+
+
+def gemm_mxfp4(alpha: float, a: MatMxfp4, b: MatMxfp4, beta: float, c: MatMut,
+               par: Optional[Parallelism] = None, ws: Optional[Workspace] = None) -> None:
+    """Extension: ``C <- alpha * A @ B^T + beta * C`` on MXFP4 operands, A m x k and B n x k (a
+    linear layer's weight, output-major); f32 sums, bfloat16 or float32 C of any strides."""
+    _bind_stream()
+    fn, dt = _out_entry(c, "gk_gemm_mxfp4_bf16", "gk_gemm_mxfp4_f32", "gemm_mxfp4")
+    _here(c.data)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), b._c("B"), float(beta),
+                                   c._c(dt, "C"), _par(par)))
+
+
+def gemm_grouped_mxfp4(alpha: float, a: MatMxfp4, offsets: torch.Tensor, b: MatMxfp4,
+                       beta: float, c: MatMut, par: Optional[Parallelism] = None,
+                       ws: Optional[Workspace] = None) -> None:
+    """Extension: :func:`gemm_grouped` on MXFP4 operands.  ``b`` holds the groups' n x k
+    matrices one after the other (groups * n rows)."""
+    _bind_stream()
+    fn, dt = _out_entry(c, "gk_gemm_grouped_mxfp4_bf16", "gk_gemm_grouped_mxfp4_f32",
+                        "gemm_grouped_mxfp4")
+    off, groups = _offsets(offsets)
+    _here(c.data, offsets)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), off, groups, b._c("B"),
+                                   float(beta), c._c(dt, "C"), _par(par)))

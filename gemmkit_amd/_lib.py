@@ -72,10 +72,17 @@ class BatchProblemBf16C(C.Structure):
                 ("c", MatMutC)]
 
 
+class Mxfp4C(C.Structure):
+    """``gk_mxfp4``: rows of e2m1 codes and their e8m0 scales."""
+    _fields_ = [("codes", _vp), ("codes_len", _size), ("scales", _vp), ("scales_len", _size),
+                ("rows", _size), ("cols", _size), ("ld", _size), ("lds", _size)]
+
+
 _REF = C.POINTER(MatRefC)
 _MUT = C.POINTER(MatMutC)
 _REQ = C.POINTER(RequantizeC)
 _BIAS = C.POINTER(BiasC)
+_MX = C.POINTER(Mxfp4C)
 
 # name -> (restype, argtypes); one line per symbol of include/gemmkit_hip.h
 SIGNATURES: dict[str, tuple] = {
@@ -221,6 +228,22 @@ SIGNATURES: dict[str, tuple] = {
     "gk_gemm_packed_b_fused_bf16_unchecked": (C.c_int, [_vp, _u16, _size, _vp, _sdiff, _sdiff,
                                                         _vp, _u16, _vp, _sdiff, _sdiff, _vp,
                                                         _i32, _u8, _i32, _u16, _u32]),
+    "gk_gemm_grouped_bf16": (C.c_int, [_vp, _f32, _REF, _vp, _size, _REF, _sdiff, _f32, _MUT,
+                                       _u32]),
+    "gk_gemm_grouped_bf16_f32out": (C.c_int, [_vp, _f32, _REF, _vp, _size, _REF, _sdiff, _f32, _MUT,
+                                              _u32]),
+    "gk_gemm_grouped_wgrad_bf16": (C.c_int, [_vp, _f32, _REF, _vp, _size, _REF, _f32, _MUT,
+                                             _sdiff, _u32]),
+    "gk_gemm_grouped_wgrad_bf16_f32out": (C.c_int, [_vp, _f32, _REF, _vp, _size, _REF, _f32, _MUT,
+                                                    _sdiff, _u32]),
+    "gk_quantize_mxfp4_f32": (C.c_int, [_REF, _MX]),
+    "gk_dequantize_mxfp4_f32": (C.c_int, [_MX, _MUT]),
+    "gk_quantize_mxfp4_bf16": (C.c_int, [_REF, _MX]),
+    "gk_dequantize_mxfp4_bf16": (C.c_int, [_MX, _MUT]),
+    "gk_gemm_mxfp4_bf16": (C.c_int, [_vp, _f32, _MX, _MX, _f32, _MUT, _u32]),
+    "gk_gemm_grouped_mxfp4_bf16": (C.c_int, [_vp, _f32, _MX, _vp, _size, _MX, _f32, _MUT, _u32]),
+    "gk_gemm_mxfp4_f32": (C.c_int, [_vp, _f32, _MX, _MX, _f32, _MUT, _u32]),
+    "gk_gemm_grouped_mxfp4_f32": (C.c_int, [_vp, _f32, _MX, _vp, _size, _MX, _f32, _MUT, _u32]),
 }
 
 _LIB: C.CDLL | None = None

@@ -2137,6 +2137,372 @@ int packed_a_checked(gk_workspace *ws, InType in, EpiKind kind, size_t esz, floa
 // ---- pointer-array batched (src/api/batched.rs:711-799; run_ptr,
 // src/special/batched.rs:294-334: every problem as a standalone gemm)
 
+// ---- ragged groups and MXFP4 operands (no counterpart in the reference)
+
+// The longest row (bytes) of an operand of these products: with at most 256 rows a
+// tile's 32-bit offsets stay below kMaxRecords.
+constexpr int64_t kMaxRaggedRow = int64_t(4) << 20;
+
+int check_ragged_sizes(size_t rows, size_t k, size_t n, size_t groups) {
+    const size_t lim = (size_t)INT32_MAX - 1024;
+    if (rows > lim || k > lim || n > lim || groups > lim)
+        return fail(GK_ERR_OVERFLOW,
+                    "gemmkit: grouped product of %zu rows, k %zu, n %zu and %zu groups: each must "
+                    "be below 2^31 - 1024", rows, k, n, groups);
+    return GK_OK;
+}
+
+int check_offsets(const int32_t *offsets, size_t groups, const gk_mat_mut *c, size_t so) {
+    if (groups == 0) return GK_OK;
+    if (!offsets || (uintptr_t)offsets % alignof(int32_t))
+        return fail(GK_ERR_ARG, "gemmkit: group offsets are null or not 4-byte aligned");
+    if (overlaps_bytes(c->data, c->len, so, offsets, groups + 1, 4))
+        return fail(GK_ERR_ALIAS, "gemmkit: C aliases the group offsets");
+    return GK_OK;
+}
+
+int row_too_long(const char *name, int64_t bytes) {
+    return fail(GK_ERR_OVERFLOW, "gemmkit: %s rows of %lld bytes exceed the 4 MiB that a grouped "
+                                 "or MXFP4 product takes", name, (long long)bytes);
+}
+
+// A view's row and column strides as the kernels take them: the stride of a dimension
+// of one element is never used, so it may be anything.
+bool ragged_in_place(const Opnd &o, int64_t R, int64_t K, int64_t batch) {
+    return canonical(o, R, K, 2, batch) && (R <= 1 || o.rs * 2 <= kMaxRaggedRow) &&
+           (R <= 1 || o.rs >= K);
+}
+
+// Row stride in bytes of an operand read in place (one row: its own length).
+int64_t ragged_ld(const Opnd &o, int64_t R, int64_t K) {
+    return R <= 1 ? round_up64(K * 2, 16) : o.rs * 2;
+}
+
+int launch_failed(hipError_t e, const char *what) {
+    if (e == hipErrorInvalidValue)
+        return fail(GK_ERR_OVERFLOW, "gemmkit: %s: the product has more tiles than a launch takes",
+                    what);
+    return hip_fail(e, what);
+}
+
+// Packs the operands among jobs[0 .. n) that do not fit one launch's batch in pieces.
+int pack_groups(PackJob *jobs, int n) {
+    for (int i = 0; i < n; ++i)
+        if (jobs[i].batch > kMaxGridZ) {
+            for (int j = 0; j < n; ++j) {
+                const int64_t nb = jobs[j].batch;
+                for (int64_t z = 0; z < nb; z += kMaxGridZ) {
+                    PackJob p = jobs[j];
+                    p.src = (const uint8_t *)p.src + z * p.bs * 2;
+                    p.dst = (uint8_t *)p.dst + z * p.rows * p.ld * 2;
+                    p.batch = (int32_t)std::min<int64_t>(kMaxGridZ, nb - z);
+                    const hipError_t e = launch_pack(InType::BF16, &p, 1, tl_stream);
+                    if (e != hipSuccess) return hip_fail(e, "pack");
+                }
+            }
+            return GK_OK;
+        }
+    const hipError_t e = launch_pack(InType::BF16, jobs, n, tl_stream);
+    return e == hipSuccess ? GK_OK : hip_fail(e, "pack");
+}
+
+int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const gk_mat_ref *a,
+                    const int32_t *offsets, size_t groups, const gk_mat_ref *b, ptrdiff_t b_gs,
+                    float beta, const gk_mat_mut *c) {
+    int r;
+    if (!a || !b || !c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if (a->cols != b->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.cols (%zu) != B.rows (%zu)", a->cols, b->rows);
+    if (a->rows != c->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.rows (%zu) != C.rows (%zu)", a->rows, c->rows);
+    if (b->cols != c->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: B.cols (%zu) != C.cols (%zu)", b->cols, c->cols);
+    size_t eb = 0;
+    if ((r = check_view(a->len, a->rows, a->cols, a->rs, a->cs, "A"))) return r;
+    if (groups > 0 &&
+        (r = check_batched_view(b->len, b->rows, b->cols, b->rs, b->cs, groups, b_gs, "B", &eb)))
+        return r;
+    if ((r = check_view(c->len, c->rows, c->cols, c->rs, c->cs, "C"))) return r;
+    if (self_aliases(c->rows, c->cols, c->rs, c->cs))
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: C view aliases itself (strides %td,%td map distinct elements to the "
+                    "same memory); C must address each (i,j) uniquely",
+                    c->rs, c->cs);
+    if (overlaps_bytes(c->data, c->len, so, a->data, a->len, 2) ||
+        overlaps_bytes(c->data, c->len, so, b->data, b->len, 2))
+        return fail(GK_ERR_ALIAS, "gemmkit: C aliases A or B");
+    if ((r = check_offsets(offsets, groups, c, so))) return r;
+    if ((r = check_ragged_sizes(a->rows, a->cols, b->cols, groups))) return r;
+    const int64_t row_bytes = round_up64((int64_t)a->cols * 2, 16);
+    if (row_bytes > kMaxRaggedRow) return row_too_long("A", row_bytes);
+    if ((r = device_init())) return r;
+    const int64_t M = (int64_t)a->rows, N = (int64_t)b->cols, G = (int64_t)groups;
+    const int64_t K = alpha == 0.0f ? 0 : (int64_t)a->cols;  // (then nothing of A and B is read)
+    if (M == 0 || N == 0 || G == 0) return ok();
+
+    // B_g is read as N rows of K or as K rows of N.
+    Opnd A{a->data, a->rs, a->cs, 0};
+    Opnd Br{b->data, b->cs, b->rs, G > 1 ? b_gs : 0}, Bc{b->data, b->rs, b->cs, G > 1 ? b_gs : 0};
+    RaggedB bl = RaggedB::Rows;
+    int64_t lda = 0, ldb = 0, bs = 0;
+    if (K > 0) {
+        const bool a_ok = ragged_in_place(A, M, K, 1);
+        const bool rows_ok = ragged_in_place(Br, N, K, G);
+        const bool cols_ok = !rows_ok && ragged_in_place(Bc, K, N, G);
+        if (!a_ok || (!rows_ok && !cols_ok)) {
+            const bool b_pack = !rows_ok && !cols_ok;
+            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+            const size_t pb = b_pack ? pack_bytes(InType::BF16, N, K, G, Br) : 0;
+            void *buf = nullptr;
+            if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
+            PackJob jobs[2];
+            int nj = 0;
+            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
+            if (pb) jobs[nj++] = pack_job(InType::BF16, &Br, N, K, G, (uint8_t *)buf + pa);
+            if ((r = pack_groups(jobs, nj))) return r;
+        }
+        bl = cols_ok ? RaggedB::Cols : RaggedB::Rows;
+        lda = ragged_ld(A, M, K);
+        ldb = cols_ok ? ragged_ld(Bc, K, N) : ragged_ld(Br, N, K);
+        bs = (cols_ok ? Bc.bs : Br.bs) * 2;
+    }
+    EpiParams ep = epi_float(kind, alpha, beta);
+    ep.c = c->data;
+    ep.rsc = c->rs;
+    ep.csc = c->cs;
+    ep.vec4 = c->cs == 1;
+    RaggedArgs g{};
+    g.a = A.p;
+    g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.bsb = bs;
+    g.off = offsets;
+    g.G = (int32_t)G;
+    g.M = (int32_t)M;
+    g.N = (int32_t)N;
+    g.K = (int32_t)K;
+    const hipError_t e = launch_grouped_bf16(g, bl, ep, g_num_cus, tl_stream);
+    if (e != hipSuccess) return launch_failed(e, "grouped gemm");
+    return finish("grouped gemm");
+}
+
+int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const gk_mat_ref *a,
+                  const int32_t *offsets, size_t groups, const gk_mat_ref *b, float beta,
+                  const gk_mat_mut *c, ptrdiff_t c_gs) {
+    int r;
+    if (!a || !b || !c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if (a->rows != b->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.rows (%zu) != B.rows (%zu)", a->rows, b->rows);
+    if (a->cols != c->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.cols (%zu) != C.rows (%zu)", a->cols, c->rows);
+    if (b->cols != c->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: B.cols (%zu) != C.cols (%zu)", b->cols, c->cols);
+    size_t ec = 0;
+    if ((r = check_view(a->len, a->rows, a->cols, a->rs, a->cs, "A"))) return r;
+    if ((r = check_view(b->len, b->rows, b->cols, b->rs, b->cs, "B"))) return r;
+    if (groups > 0 &&
+        (r = check_batched_view(c->len, c->rows, c->cols, c->rs, c->cs, groups, c_gs, "C", &ec)))
+        return r;
+    if (self_aliases(c->rows, c->cols, c->rs, c->cs))
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: grouped C element aliases itself (strides %td,%td map distinct "
+                    "elements to the same memory); C must address each (i,j) uniquely",
+                    c->rs, c->cs);
+    if (groups > 1 && (size_t)c_gs < ec)
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: C group stride (%td) must be at least the element extent (%zu) so "
+                    "the groups' outputs stay disjoint", c_gs, ec);
+    if (overlaps_bytes(c->data, c->len, so, a->data, a->len, 2) ||
+        overlaps_bytes(c->data, c->len, so, b->data, b->len, 2))
+        return fail(GK_ERR_ALIAS, "gemmkit: C aliases A or B");
+    if ((r = check_offsets(offsets, groups, c, so))) return r;
+    if ((r = check_ragged_sizes(a->rows, a->cols, b->cols, groups))) return r;
+    const int64_t row_bytes = round_up64((int64_t)std::max(a->cols, b->cols) * 2, 16);
+    if (row_bytes > kMaxRaggedRow) return row_too_long("A or B", row_bytes);
+    if ((r = device_init())) return r;
+    if (groups == 0 || a->cols == 0 || b->cols == 0) return ok();
+    // C column-major-ish: C_g^T = B^T A, the same product with the roles swapped.
+    const bool swap = iabs64(c->cs) > iabs64(c->rs);
+    const gk_mat_ref *x = swap ? b : a, *y = swap ? a : b;
+    const int64_t M = alpha == 0.0f ? 0 : (int64_t)a->rows;
+    const int64_t K = (int64_t)x->cols, N = (int64_t)y->cols;
+    Opnd A{x->data, x->rs, x->cs, 0}, B{y->data, y->rs, y->cs, 0};
+    int64_t lda = 0, ldb = 0;
+    if (M > 0) {
+        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
+        if (!a_ok || !b_ok) {
+            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+            const size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
+            void *buf = nullptr;
+            if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
+            PackJob jobs[2];
+            int nj = 0;
+            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
+            if (pb) jobs[nj++] = pack_job(InType::BF16, &B, M, N, 1, (uint8_t *)buf + pa);
+            if ((r = pack_groups(jobs, nj))) return r;
+        }
+        lda = ragged_ld(A, M, K);
+        ldb = ragged_ld(B, M, N);
+    }
+    EpiParams ep = epi_float(kind, alpha, beta);
+    ep.c = c->data;
+    ep.rsc = swap ? c->cs : c->rs;
+    ep.csc = swap ? c->rs : c->cs;
+    ep.bsc = groups > 1 ? c_gs : 0;
+    ep.vec4 = ep.csc == 1;
+    RaggedArgs g{};
+    g.a = A.p;
+    g.b = B.p;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.off = offsets;
+    g.G = (int32_t)groups;
+    g.M = (int32_t)M;
+    g.N = (int32_t)N;
+    g.K = (int32_t)K;
+    const hipError_t e = launch_grouped_wgrad(g, ep, g_num_cus, tl_stream);
+    if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
+    return finish("grouped weight gradient");
+}
+
+int check_mxfp4(const gk_mxfp4 *q, const char *name) {
+    if (!q) return fail(GK_ERR_ARG, "gemmkit: null MXFP4 argument");
+    const size_t lim = (size_t)INT32_MAX - 1024;
+    if (q->rows > lim || q->cols > lim)
+        return fail(GK_ERR_OVERFLOW, "gemmkit: MXFP4 %s of %zux%zu: each side must be below "
+                                     "2^31 - 1024", name, q->rows, q->cols);
+    const size_t nb = (q->cols + kMxBlock - 1) / kMxBlock, sb = (nb + 15) / 16 * 16;
+    if (q->rows == 0 || nb == 0) return GK_OK;
+    if (q->ld < nb * 16 || q->ld % 16 || q->lds < sb || q->lds % 16 ||
+        (uintptr_t)q->codes % 16 || (uintptr_t)q->scales % 16)
+        return fail(GK_ERR_VIEW,
+                    "gemmkit: MXFP4 %s needs 16-byte aligned codes and scales and row strides that "
+                    "are multiples of 16, at least %zu and %zu bytes; got %zu and %zu",
+                    name, nb * 16, sb, q->ld, q->lds);
+    if ((int64_t)std::max(nb * 16, sb) > kMaxRaggedRow) return row_too_long(name, (int64_t)nb * 16);
+    const __int128 need_c = (__int128)(q->rows - 1) * q->ld + nb * 16;
+    const __int128 need_s = (__int128)(q->rows - 1) * q->lds + sb;
+    if (need_c > (__int128)q->codes_len || need_s > (__int128)q->scales_len)
+        return fail(GK_ERR_VIEW,
+                    "gemmkit: MXFP4 %s of %zux%zu (row strides %zu, %zu) needs more bytes of codes "
+                    "or scales than the %zu and %zu it has",
+                    name, q->rows, q->cols, q->ld, q->lds, q->codes_len, q->scales_len);
+    return GK_OK;
+}
+
+bool overlaps_mxfp4(const gk_mxfp4 *q, const void *p, size_t n, size_t s) {
+    return overlaps_bytes(q->codes, q->codes_len, 1, p, n, s) ||
+           overlaps_bytes(q->scales, q->scales_len, 1, p, n, s);
+}
+
+MxArgs mx_args(const gk_mxfp4 *q, void *x, ptrdiff_t rs, ptrdiff_t cs) {
+    return MxArgs{(uint8_t *)q->codes, (uint8_t *)q->scales, (int64_t)q->ld, (int64_t)q->lds, x,
+                  rs, cs, (int64_t)q->rows, (int64_t)q->cols};
+}
+
+int quantize_checked(InType in, const gk_mat_ref *x, const gk_mxfp4 *q) {
+    int r;
+    if (!x) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_mxfp4(q, "output"))) return r;
+    if (x->rows != q->rows || x->cols != q->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: MXFP4 output is %zux%zu, the matrix %zux%zu", q->rows,
+                    q->cols, x->rows, x->cols);
+    if ((r = check_view(x->len, x->rows, x->cols, x->rs, x->cs, "X"))) return r;
+    if (overlaps_mxfp4(q, x->data, x->len, in_size(in)) ||
+        overlaps_bytes(q->codes, q->codes_len, 1, q->scales, q->scales_len, 1))
+        return fail(GK_ERR_ALIAS, "gemmkit: MXFP4 codes, scales and the matrix overlap");
+    if ((r = device_init())) return r;
+    if (x->rows == 0 || x->cols == 0) return ok();
+    const hipError_t e = launch_mxfp4_quantize(
+        in, mx_args(q, const_cast<void *>(x->data), x->rs, x->cs), tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "mxfp4 quantize");
+    return finish("mxfp4 quantize");
+}
+
+int dequantize_checked(InType out, const gk_mxfp4 *q, const gk_mat_mut *c) {
+    int r;
+    if (!c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_mxfp4(q, "input"))) return r;
+    if (c->rows != q->rows || c->cols != q->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: MXFP4 input is %zux%zu, the matrix %zux%zu", q->rows,
+                    q->cols, c->rows, c->cols);
+    if ((r = check_view(c->len, c->rows, c->cols, c->rs, c->cs, "C"))) return r;
+    if (self_aliases(c->rows, c->cols, c->rs, c->cs))
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: C view aliases itself (strides %td,%td map distinct elements to the "
+                    "same memory); C must address each (i,j) uniquely",
+                    c->rs, c->cs);
+    if (overlaps_mxfp4(q, c->data, c->len, in_size(out)))
+        return fail(GK_ERR_ALIAS, "gemmkit: C aliases the MXFP4 codes or scales");
+    if ((r = device_init())) return r;
+    if (c->rows == 0 || c->cols == 0) return ok();
+    const hipError_t e =
+        launch_mxfp4_dequantize(out, mx_args(q, c->data, c->rs, c->cs), tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "mxfp4 dequantize");
+    return finish("mxfp4 dequantize");
+}
+
+// offsets == nullptr: the plain product.
+int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool grouped,
+                  const int32_t *offsets, size_t groups, const gk_mxfp4 *b, float beta,
+                  const gk_mat_mut *c) {
+    int r;
+    if (!c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_mxfp4(a, "A"))) return r;
+    if ((r = check_mxfp4(b, "B"))) return r;
+    if (a->cols != b->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.cols (%zu) != B.cols (%zu) (B holds the product's "
+                                  "columns as rows)", a->cols, b->cols);
+    if (a->rows != c->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.rows (%zu) != C.rows (%zu)", a->rows, c->rows);
+    if ((__int128)c->cols * groups != (__int128)b->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: B.rows (%zu) != C.cols (%zu) for each of %zu groups",
+                    b->rows, c->cols, groups);
+    if ((r = check_view(c->len, c->rows, c->cols, c->rs, c->cs, "C"))) return r;
+    if (self_aliases(c->rows, c->cols, c->rs, c->cs))
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: C view aliases itself (strides %td,%td map distinct elements to the "
+                    "same memory); C must address each (i,j) uniquely",
+                    c->rs, c->cs);
+    if (overlaps_mxfp4(a, c->data, c->len, so) || overlaps_mxfp4(b, c->data, c->len, so))
+        return fail(GK_ERR_ALIAS, "gemmkit: C aliases A or B");
+    if (grouped && (r = check_offsets(offsets, groups, c, so))) return r;
+    if ((r = check_ragged_sizes(a->rows, a->cols, c->cols, groups))) return r;
+    // (the kernels take a row's stride as a 32-bit offset)
+    if ((int64_t)std::max(std::max(a->ld, b->ld), std::max(a->lds, b->lds)) > kMaxRaggedRow)
+        return row_too_long("A or B", (int64_t)std::max(a->ld, b->ld));
+    if ((r = device_init())) return r;
+    if (c->rows == 0 || c->cols == 0 || groups == 0) return ok();
+    // C column-major-ish: C^T = B A^T.  (Groups are rows of C and stay where they are.)
+    const bool swap = !grouped && iabs64(c->cs) > iabs64(c->rs);
+    if (swap) std::swap(a, b);
+    EpiParams ep = epi_float(kind, alpha, beta);
+    ep.c = c->data;
+    ep.rsc = swap ? c->cs : c->rs;
+    ep.csc = swap ? c->rs : c->cs;
+    ep.vec4 = ep.csc == 1;
+    RaggedArgs g{};
+    g.a = a->codes;
+    g.b = b->codes;
+    g.sa = (const uint8_t *)a->scales;
+    g.sb = (const uint8_t *)b->scales;
+    g.lda = (int64_t)a->ld;
+    g.ldb = (int64_t)b->ld;
+    g.lsa = (int64_t)a->lds;
+    g.lsb = (int64_t)b->lds;
+    g.G = (int32_t)groups;
+    g.M = (int32_t)a->rows;
+    g.N = (int32_t)(b->rows / groups);
+    g.K = alpha == 0.0f ? 0 : (int32_t)a->cols;
+    g.bsb = (int64_t)g.N * g.ldb;
+    g.bssb = (int64_t)g.N * g.lsb;
+    g.off = grouped ? offsets : nullptr;
+    const hipError_t e = launch_mxfp4(g, ep, g_num_cus, tl_stream);
+    if (e != hipSuccess) return launch_failed(e, "mxfp4 gemm");
+    return finish("mxfp4 gemm");
+}
+
 // Element step of a run of problems: the pointer difference in elements, when
 // it is a whole number of elements.
 bool elem_step(const void *p0, const void *p1, size_t esz, ptrdiff_t *step) {
@@ -2871,6 +3237,71 @@ int gk_gemm_packed_b_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha, size_
     const FusedSpec fx{has_bias ? bias : nullptr, bias_dim, act, bf16_to_f32(slope)};
     return packed_b_unchecked(ws, InType::BF16, EpiKind::BF16, bf16_to_f32(alpha), m, a, rsa, csa,
                               packed, bf16_to_f32(beta), c, rsc, csc, &fx);
+}
+
+// ---- ragged groups and MXFP4 operands
+
+int gk_gemm_grouped_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                         const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                         ptrdiff_t b_gs, float beta, const gk_mat_mut *c, gk_par) {
+    return grouped_checked(ws, EpiKind::BF16, 2, alpha, a, offsets, groups, b, b_gs, beta, c);
+}
+
+int gk_gemm_grouped_bf16_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                                ptrdiff_t b_gs, float beta, const gk_mat_mut *c, gk_par) {
+    return grouped_checked(ws, EpiKind::F32, 4, alpha, a, offsets, groups, b, b_gs, beta, c);
+}
+
+int gk_gemm_grouped_wgrad_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                               const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                               float beta, const gk_mat_mut *c, ptrdiff_t c_gs, gk_par) {
+    return wgrad_checked(ws, EpiKind::BF16, 2, alpha, a, offsets, groups, b, beta, c, c_gs);
+}
+
+int gk_gemm_grouped_wgrad_bf16_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                      const int32_t *offsets, size_t groups,
+                                      const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                                      ptrdiff_t c_gs, gk_par) {
+    return wgrad_checked(ws, EpiKind::F32, 4, alpha, a, offsets, groups, b, beta, c, c_gs);
+}
+
+int gk_quantize_mxfp4_f32(const gk_mat_ref *x, const gk_mxfp4 *q) {
+    return quantize_checked(InType::F32, x, q);
+}
+
+int gk_quantize_mxfp4_bf16(const gk_mat_ref *x, const gk_mxfp4 *q) {
+    return quantize_checked(InType::BF16, x, q);
+}
+
+int gk_dequantize_mxfp4_f32(const gk_mxfp4 *q, const gk_mat_mut *c) {
+    return dequantize_checked(InType::F32, q, c);
+}
+
+int gk_dequantize_mxfp4_bf16(const gk_mxfp4 *q, const gk_mat_mut *c) {
+    return dequantize_checked(InType::BF16, q, c);
+}
+
+int gk_gemm_mxfp4_bf16(gk_workspace *, float alpha, const gk_mxfp4 *a, const gk_mxfp4 *b,
+                       float beta, const gk_mat_mut *c, gk_par) {
+    return mxfp4_checked(EpiKind::BF16, 2, alpha, a, false, nullptr, 1, b, beta, c);
+}
+
+int gk_gemm_mxfp4_f32(gk_workspace *, float alpha, const gk_mxfp4 *a, const gk_mxfp4 *b,
+                      float beta, const gk_mat_mut *c, gk_par) {
+    return mxfp4_checked(EpiKind::F32, 4, alpha, a, false, nullptr, 1, b, beta, c);
+}
+
+int gk_gemm_grouped_mxfp4_bf16(gk_workspace *, float alpha, const gk_mxfp4 *a,
+                               const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
+                               float beta, const gk_mat_mut *c, gk_par) {
+    return mxfp4_checked(EpiKind::BF16, 2, alpha, a, true, offsets, groups, b, beta, c);
+}
+
+int gk_gemm_grouped_mxfp4_f32(gk_workspace *, float alpha, const gk_mxfp4 *a,
+                              const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
+                              float beta, const gk_mat_mut *c, gk_par) {
+    return mxfp4_checked(EpiKind::F32, 4, alpha, a, true, offsets, groups, b, beta, c);
 }
 
 }  // extern "C"

@@ -237,4 +237,39 @@ hipError_t launch_split_reduce(InType in, const void *part, int splits, int64_t 
 hipError_t launch_fused_fill(const EpiParams &ep, int64_t m, int64_t n, int64_t batch,
                              hipStream_t stream);
 
+// Products of ragged groups (ragged.h, instantiated in grouped.hip and mxfp4.hip).
+// Group g of G has the rows [s_g, s_{g+1}) with s_i = min(M, max(0, off_0 .. off_i)), so
+// that any offsets, wrong ones too, give disjoint row ranges inside the matrix.
+//   forward: C[s_g + i, n] = epi(sum_k A[s_g + i, k] * B_g[n, k])
+//   wgrad:   C_g[m, n] = epi(sum_{i in group g} A[i, m] * B[i, n])
+// Without offsets (nullptr, G == 1) the one group has all M rows.
+struct RaggedArgs {
+    const void *a, *b;         // 16-byte aligned, as are the row strides (bytes)
+    int64_t lda, ldb, bsb;     // row strides of a and b, bytes from one B_g to the next
+    const uint8_t *sa, *sb;    // MXFP4 operands: their scale rows, likewise
+    int64_t lsa, lsb, bssb;
+    const int32_t *off;        // G + 1 offsets on the device, or nullptr
+    int32_t G, M, N, K;        // M: rows of A; wgrad: K is A's columns
+};
+// B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
+enum class RaggedB : int { Rows = 0, Cols = 1 };
+hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep, int cus,
+                               hipStream_t stream);
+hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, int cus,
+                                hipStream_t stream);
+
+// MXFP4 (mxfp4.hip): rows of e2m1 codes, two a byte, the lower nibble first, with one
+// e8m0 scale per 32 elements.
+constexpr int kMxBlock = 32;
+struct MxArgs {
+    uint8_t *codes, *scales;   // row r at codes + r*ld, scales + r*lds (bytes)
+    int64_t ld, lds;
+    void *x;                   // the values: element (r, k) at x + r*rs + k*cs
+    int64_t rs, cs, rows, K;
+};
+hipError_t launch_mxfp4_quantize(InType in, const MxArgs &g, hipStream_t stream);
+hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stream);
+// C = epi(A B^T) of MXFP4 operands per group: K in elements, lda/ldb bytes of code rows.
+hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, int cus, hipStream_t stream);
+
 }  // namespace gk

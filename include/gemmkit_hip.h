@@ -614,6 +614,96 @@ int gk_gemm_packed_a_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha,
                                           uint8_t has_bias, int32_t act, gk_bf16 slope,
                                           gk_par par);
 
+/* ----------------------------------------- ragged groups and MXFP4 operands */
+
+/* The entries below have no counterpart in the reference: the products of a
+ * routed layer, whose matrices each see a number of rows that only the device
+ * knows, and of 4-bit block-scaled operands.  alpha and beta are f32 whatever
+ * the output type; beta == 0 never reads C.  They run on the launch stream
+ * like every other entry, can be captured into a HIP graph (the workspace holds
+ * packed copies of operands that the kernels cannot read in place, and nothing
+ * else), and give the same bits on every run.
+ *
+ * Groups: `offsets` holds groups + 1 row offsets on the DEVICE.  Group g has
+ * the rows [s_g, s_{g+1}) with s_i = min(rows, max(0, offsets[0 .. i])): for
+ * increasing offsets within the rows simply offsets[g] .. offsets[g + 1], and
+ * any other contents give disjoint groups inside the matrix too.  Groups may be
+ * empty.  Rows before s_0 and from s_groups on belong to no group.
+ *
+ * Sizes: rows, groups, k and n below 2^31; a bf16 row of k (and, for wgrad, n)
+ * elements at most 4 MiB, a row of codes likewise.  GK_ERR_OVERFLOW beyond.
+ */
+
+/* C[rows of g] <- alpha * A[rows of g] * B_g + beta * C[rows of g], bf16 inputs, f32
+ * sums: A rows x k, C rows x n, B_g the k x n view b moved by g * b_gs
+ * elements (0: one matrix for all).  Rows of no group are left as they are.
+ * Read in place: rows of A of unit stride; B of unit k stride or unit n
+ * stride; 16-byte aligned.  Other layouts are packed first. */
+int gk_gemm_grouped_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                         const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                         ptrdiff_t b_gs, float beta, const gk_mat_mut *c, gk_par par);
+int gk_gemm_grouped_bf16_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                                ptrdiff_t b_gs, float beta, const gk_mat_mut *c, gk_par par);
+
+/* The gradient of B in the product above: C_g <- alpha * A[rows of g]^T * B[rows of g]
+ * + beta * C_g with A rows x k, B rows x n (the gradient of the product's
+ * output) and C_g the k x n view c moved by g * c_gs elements.  An empty
+ * group's C_g becomes beta * C_g.  (The gradient of A is the product itself, with
+ * the transposed view of B.) */
+int gk_gemm_grouped_wgrad_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                               const int32_t *offsets, size_t groups, const gk_mat_ref *b,
+                               float beta, const gk_mat_mut *c, ptrdiff_t c_gs, gk_par par);
+int gk_gemm_grouped_wgrad_bf16_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                      const int32_t *offsets, size_t groups,
+                                      const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                                      ptrdiff_t c_gs, gk_par par);
+
+/* A rows x cols matrix in MXFP4: row r's elements as e2m1 codes, two a byte
+ * with the even element in the lower nibble, at codes + r * ld; one e8m0 scale
+ * (2^(byte - 127), 255: NaN) per 32 consecutive elements at scales + r * lds.
+ * Strides are bytes, multiples of 16, and both arrays 16-byte aligned.  A row
+ * holds 16 bytes of codes per begun block (elements past cols: zero codes)
+ * and its scales padded to a multiple of 16 bytes (contents ignored).
+ * codes_len and scales_len are the arrays' sizes in bytes. */
+typedef struct gk_mxfp4 {
+    void *codes;
+    size_t codes_len;
+    void *scales;
+    size_t scales_len;
+    size_t rows;
+    size_t cols;
+    size_t ld;
+    size_t lds;
+} gk_mxfp4;
+
+/* Quantizes the matrix x into q (same rows and cols).  A block with largest
+ * magnitude m gets the scale 2^e, e = max(floor(log2 m) - 2, -127), and each
+ * element the nearest e2m1 value of x / 2^e (ties to the even code,
+ * magnitudes above 6 to 6); a block with a NaN or an infinity the scale byte
+ * 255 and zero codes. */
+int gk_quantize_mxfp4_f32(const gk_mat_ref *x, const gk_mxfp4 *q);
+int gk_quantize_mxfp4_bf16(const gk_mat_ref *x, const gk_mxfp4 *q);
+/* The values of q in c: exact in f32 and, but for magnitudes below bf16's
+ * smallest, in bf16. */
+int gk_dequantize_mxfp4_f32(const gk_mxfp4 *q, const gk_mat_mut *c);
+int gk_dequantize_mxfp4_bf16(const gk_mxfp4 *q, const gk_mat_mut *c);
+
+/* C <- alpha * A * B^T + beta * C, A m x k, B n x k (the columns of the product's right
+ * operand, as a linear layer holds its weight): exact products, f32 sums. */
+int gk_gemm_mxfp4_bf16(gk_workspace *ws, float alpha, const gk_mxfp4 *a, const gk_mxfp4 *b,
+                       float beta, const gk_mat_mut *c, gk_par par);
+int gk_gemm_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a, const gk_mxfp4 *b,
+                      float beta, const gk_mat_mut *c, gk_par par);
+/* The same per group: b holds the groups' n x k matrices one after the other
+ * (groups * n rows).  Rows of no group are left as they are. */
+int gk_gemm_grouped_mxfp4_bf16(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
+                               const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
+                               float beta, const gk_mat_mut *c, gk_par par);
+int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
+                              const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
+                              float beta, const gk_mat_mut *c, gk_par par);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
