@@ -2272,6 +2272,7 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     ep.csc = c->cs;
     ep.vec4 = c->cs == 1;
     RaggedArgs g{};
+    g.cus = g_num_cus;
     g.a = A.p;
     g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
     g.lda = lda;
@@ -2282,7 +2283,7 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
-    const hipError_t e = launch_grouped_bf16(g, bl, ep, g_num_cus, tl_stream);
+    const hipError_t e = launch_grouped_bf16(g, bl, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "grouped gemm");
     return finish("grouped gemm");
 }
@@ -2352,6 +2353,7 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     ep.bsc = groups > 1 ? c_gs : 0;
     ep.vec4 = ep.csc == 1;
     RaggedArgs g{};
+    g.cus = g_num_cus;
     g.a = A.p;
     g.b = B.p;
     g.lda = lda;
@@ -2361,7 +2363,7 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
-    const hipError_t e = launch_grouped_wgrad(g, ep, g_num_cus, tl_stream);
+    const hipError_t e = launch_grouped_wgrad(g, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
     return finish("grouped weight gradient");
 }
@@ -2483,6 +2485,7 @@ int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool 
     ep.csc = swap ? c->rs : c->cs;
     ep.vec4 = ep.csc == 1;
     RaggedArgs g{};
+    g.cus = g_num_cus;
     g.a = a->codes;
     g.b = b->codes;
     g.sa = (const uint8_t *)a->scales;
@@ -2498,7 +2501,7 @@ int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool 
     g.bsb = (int64_t)g.N * g.ldb;
     g.bssb = (int64_t)g.N * g.lsb;
     g.off = grouped ? offsets : nullptr;
-    const hipError_t e = launch_mxfp4(g, ep, g_num_cus, tl_stream);
+    const hipError_t e = launch_mxfp4(g, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "mxfp4 gemm");
     return finish("mxfp4 gemm");
 }

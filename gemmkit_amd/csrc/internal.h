@@ -250,13 +250,13 @@ struct RaggedArgs {
     int64_t lsa, lsb, bssb;
     const int32_t *off;        // G + 1 offsets on the device, or nullptr
     int32_t G, M, N, K;        // M: rows of A; wgrad: K is A's columns
+    int32_t cus;               // compute units of the device
 };
 // B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
 enum class RaggedB : int { Rows = 0, Cols = 1 };
-hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep, int cus,
+hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
                                hipStream_t stream);
-hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, int cus,
-                                hipStream_t stream);
+hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 
 // MXFP4 (mxfp4.hip): rows of e2m1 codes, two a byte, the lower nibble first, with one
 // e8m0 scale per 32 elements.
@@ -270,6 +270,6 @@ struct MxArgs {
 hipError_t launch_mxfp4_quantize(InType in, const MxArgs &g, hipStream_t stream);
 hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stream);
 // C = epi(A B^T) of MXFP4 operands per group: K in elements, lda/ldb bytes of code rows.
-hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, int cus, hipStream_t stream);
+hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 
 }  // namespace gk

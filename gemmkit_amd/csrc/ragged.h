@@ -35,22 +35,23 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------- groups
 
-// Inclusive scans over the wave.
-__device__ __forceinline__ int scan_max(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int t = __shfl_up(v, d);
-        if (lane >= d) v = v > t ? v : t;
-    }
+// Inclusive scans over the wave of non-negative values (0 is neutral for both), in
+// registers: shifts within rows of 16 lanes, then each row's last value to the rows after.
+template <typename F>
+__device__ __forceinline__ int scan(int v, F op) {
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true));   // row_shr:1
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));  // row_bcast:31
     return v;
 }
-__device__ __forceinline__ int scan_add(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int t = __shfl_up(v, d);
-        if (lane >= d) v += t;
-    }
-    return v;
+__device__ __forceinline__ int scan_max(int v) {
+    return scan(v, [](int a, int b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ int scan_add(int v) {
+    return scan(v, [](int a, int b) { return a + b; });
 }
 __device__ __forceinline__ int clamp_row(int v, int M) { return v < 0 ? 0 : (v > M ? M : v); }
 
@@ -60,12 +61,12 @@ __device__ __forceinline__ void group_rows(const int32_t *off, int G, int M, int
                                            int &top, int &s, int &e) {
     const int i = base + lane;
     int lo = i < G ? off[i] : 0, hi = i < G ? off[i + 1] : 0;
-    int m = scan_max(lo, lane);
+    int m = scan_max(lo > 0 ? lo : 0);
     m = m > top ? m : top;
     s = clamp_row(m, M);
     hi = hi > m ? hi : m;
     e = i < G ? clamp_row(hi, M) : s;
-    top = __shfl(hi, 63);
+    top = __builtin_amdgcn_readlane(hi, 63);
 }
 
 struct GroupTile {
@@ -74,34 +75,47 @@ struct GroupTile {
     int tn;           // tile column
 };
 
-// The tile of workgroup `bid`: the groups' tiles in order, a group's in tile_coords order.
-// Every workgroup adds up the groups' tile counts itself (G + 1 offsets, in L2 after the
-// first), so that nothing has to run before the product.  False: no tile left.
-template <int BM>
-__device__ __forceinline__ bool find_tile(const int32_t *off, int G, int M, int tiles_n,
+// The tile of workgroup `bid`: the groups' tiles in order, a group's in tile_coords order,
+// every XCD a contiguous range of them (xcd_logical).  Every workgroup adds up the groups'
+// tile counts itself (G + 1 offsets, in L2 after the first), so that nothing has to run
+// before the product.  False: no tile left.
+// HALVES: where the tiles of an XCD's last round would leave half of its CUs (cus / 8) or
+// more without one, each goes out as two tiles of half the rows.
+template <int BM, bool HALVES>
+__device__ __forceinline__ bool find_tile(const int32_t *off, int G, int M, int tiles_n, int cus,
                                           int64_t bid, int lane, GroupTile &t) {
-    int g = 0, s = 0, e = M, pid, tm_all;
+    int g = 0, s = 0, e = M, ls = 0, le = 0, incl = 0, total = 0;
     if (!off) {
-        tm_all = (M + BM - 1) / BM;
-        const int64_t all = (int64_t)tm_all * tiles_n;
-        if (bid >= all) return false;
-        pid = (int)xcd_logical(bid, all);
+        total = (M + BM - 1) / BM;
     } else {
-        int top = 0, ls = 0, le = 0, incl = 0, total = 0;
+        int top = 0;
         for (int base = 0; base < G; base += 64) {
             group_rows(off, G, M, base, lane, top, ls, le);
-            incl = total + scan_add((le - ls + BM - 1) / BM, lane);
-            total = __shfl(incl, 63);
+            incl = total + scan_add((le - ls + BM - 1) / BM);
+            total = __builtin_amdgcn_readlane(incl, 63);
         }
-        const int64_t all = (int64_t)total * tiles_n;
-        if (bid >= all) return false;
-        pid = (int)xcd_logical(bid, all);
+    }
+    const int all = total * tiles_n;  // (below 2^31: the host checks the upper bound)
+    const int xcd = (int)(bid % 8), per = all / 8, rem = all % 8;
+    const int mine = per + (xcd < rem ? 1 : 0);
+    int idx = (int)(bid / 8), half = -1;
+    if constexpr (HALVES) {
+        const int cx = cus / 8 > 0 ? cus / 8 : 1, whole = mine / cx * cx;
+        if (2 * (mine - whole) <= cx && idx >= whole) {
+            half = (idx - whole) & 1;
+            idx = whole + (idx - whole) / 2;
+        }
+    }
+    if (idx >= mine) return false;
+    int pid = xcd * per + (xcd < rem ? xcd : rem) + idx;
+    if (off) {
         if (G > 64) {
-            top = total = 0;
+            int top = 0;
+            total = 0;
             for (int base = 0;; base += 64) {
                 group_rows(off, G, M, base, lane, top, ls, le);
-                incl = total + scan_add((le - ls + BM - 1) / BM, lane);
-                total = __shfl(incl, 63);
+                incl = total + scan_add((le - ls + BM - 1) / BM);
+                total = __builtin_amdgcn_readlane(incl, 63);
                 g = base;
                 if (pid < total * tiles_n) break;
             }
@@ -111,14 +125,21 @@ __device__ __forceinline__ bool find_tile(const int32_t *off, int G, int M, int 
         g += l;
         s = __builtin_amdgcn_readlane(ls, l);
         e = __builtin_amdgcn_readlane(le, l);
-        tm_all = (e - s + BM - 1) / BM;
-        pid -= (__builtin_amdgcn_readlane(incl, l) - tm_all) * tiles_n;
+        total = (e - s + BM - 1) / BM;
+        pid -= (__builtin_amdgcn_readlane(incl, l) - total) * tiles_n;
     }
     int tm, tn;
-    tile_coords(pid, tm_all, tiles_n, tm, tn);
+    tile_coords(pid, total, tiles_n, tm, tn);
+    int row0 = s + tm * BM, rows = e - row0 < BM ? e - row0 : BM;
+    if (half >= 0) {
+        row0 += half * (BM / 2);
+        rows -= half * (BM / 2);
+        if (rows <= 0) return false;
+        rows = rows < BM / 2 ? rows : BM / 2;
+    }
     t.g = __builtin_amdgcn_readfirstlane(g);
-    t.row0 = __builtin_amdgcn_readfirstlane(s + tm * BM);
-    t.rows = __builtin_amdgcn_readfirstlane(e - (s + tm * BM) < BM ? e - (s + tm * BM) : BM);
+    t.row0 = __builtin_amdgcn_readfirstlane(row0);
+    t.rows = __builtin_amdgcn_readfirstlane(rows);
     t.tn = __builtin_amdgcn_readfirstlane(tn);
     return true;
 }
@@ -171,7 +192,12 @@ struct Panel {
     int ld;
     uint32_t num;         // k-contiguous: resource size from base
     int left;             // of the contraction from the next stage on: bytes, or rows (TR)
-    uint32_t vo[LP];      // this lane's offsets from the stage's base
+    // This lane's offsets from the stage's base: of loads 0 and 1; the layouts repeat
+    // after two loads, 2*RPI rows further on.
+    static constexpr int RPI = TR ? 1024 / (2 * W) : 8;  // rows one load fills
+    static constexpr bool PAIR = TR ? RPI == 2 && LP == 4 : LP % 2 == 0;
+    static constexpr int NVO = PAIR ? 2 : LP;
+    uint32_t vo[NVO];
     int wave, lane;
 
     // `cols`: bytes of the matrix's columns from the tile's first one (TR).
@@ -184,7 +210,7 @@ struct Panel {
         left = k;
         num = TR ? 0 : (uint32_t)((rows - 1) * ld + k);
 #pragma unroll
-        for (int i = 0; i < LP; ++i) {
+        for (int i = 0; i < NVO; ++i) {
             const int at = (wave * LP + i) * 64 + lane;  // 16-byte slot of the stage
             if constexpr (TR) {
                 const int row = at / (W / 8), slot = at % (W / 8);
@@ -201,11 +227,12 @@ struct Panel {
     // `spare`).
     __device__ __forceinline__ void load(uint8_t *dst, uint8_t *spare, int i) const {
         uint8_t *d = NI % NW == 0 || wave * LP + i < NI ? dst + (wave * LP + i) * 1024 : spare;
+        // (an out-of-range offset stays one with the rows added)
+        uint32_t v = PAIR ? vo[i % 2] + (uint32_t)(i / 2 * 2 * RPI * ld) : vo[i];
         if constexpr (TR) {
             // (rows at and past the end read zeros: their offsets reach left * ld)
-            dma16(base, size(), vo[i], d);
+            dma16(base, size(), v, d);
         } else {
-            uint32_t v = vo[i];
             if (left < 128) {  // the K tail's chunks read zeros
                 const int slot = (wave * LP + i) * 64 + lane;
                 if (((slot % 8) ^ swz_of<128>(slot / 8)) * 16 >= left) v = kOutOfRange;
@@ -296,8 +323,7 @@ __device__ __forceinline__ v4f bf_step(v4i b, v4i a, v4f c) {
 template <bool MX, int BM, int BN, int NS>
 struct RaggedLds {
     static constexpr int STAGE = (BM + BN) * 128;
-    static constexpr int SA_ROWS = (BM + 63) / 64 * 64, SB_ROWS = (BN + 63) / 64 * 64;
-    static constexpr int SSLOT = MX ? (SA_ROWS + SB_ROWS) * 16 : 0;
+    static constexpr int SSLOT = MX ? ((BM + 63) / 64 + (BN + 63) / 64) * 1024 : 0;
     static constexpr int NSS = NS / 2 + 1;
     static constexpr int SCALES = NS * STAGE;
     static constexpr int SPARE = SCALES + NSS * SSLOT;
@@ -310,6 +336,164 @@ constexpr int ragged_waves(int lds, int nw) {
     const int w = wgs * nw / 4;
     return w < 1 ? 1 : (w > 4 ? 4 : w);
 }
+
+// ---------------------------------------------------------------- tiles
+
+// What a workgroup computes.
+struct RaggedTile {
+    int row0, rows;   // rows of C (wgrad: of C_g) and how many of them
+    int n0, cols;     // columns
+    int g, z;         // group; batch element of C
+    int k;            // contraction: bytes of A (k-contiguous), rows (wgrad)
+    int KT;           // stages
+    const uint8_t *a, *b;
+};
+
+// wgrad: how many workgroups an XCD gets for each group's `per` tiles.
+__device__ __host__ __forceinline__ int wgrad_share(int per) { return (per + 7) / 8; }
+
+template <bool MX, bool AT, bool BT, int BM, int BN, bool HALVES>
+__device__ __forceinline__ bool ragged_tile(const RaggedArgs &g, int lane, RaggedTile &t) {
+    const int tiles_n = (g.N + BN - 1) / BN;
+    const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    t.a = (const uint8_t *)g.a;
+    t.b = (const uint8_t *)g.b;
+    t.z = 0;
+    int tn;
+    if constexpr (AT) {
+        // Every XCD takes an eighth of each group's tiles, a contiguous one: with whole
+        // groups per XCD the one with the longest group would work on alone.  (The
+        // eighths turn with the group, so that their roundings even out.)
+        const int tiles_m = (g.K + BM - 1) / BM, per = tiles_m * tiles_n, share = wgrad_share(per);
+        const int64_t idx = bid / 8;
+        t.g = (int)(idx / share);
+        if (t.g >= g.G) return false;
+        const int part = (int)((bid + t.g) % 8);
+        const int pid = (int)((int64_t)part * per / 8) + (int)(idx % share);
+        if (pid >= (int)((int64_t)(part + 1) * per / 8)) return false;
+        int tm, s, e;
+        tile_coords(pid, tiles_m, tiles_n, tm, tn);
+        one_group(g.off, g.G, g.M, t.g, lane, s, e);
+        t.row0 = tm * BM;
+        t.rows = g.K - t.row0 < BM ? g.K - t.row0 : BM;
+        t.k = e - s;
+        t.z = t.g;
+        t.KT = (t.k + 63) / 64;
+        t.a += s * g.lda + (int64_t)t.row0 * 2;
+        t.b += s * g.ldb;
+    } else {
+        GroupTile f;
+        if (!find_tile<BM, HALVES>(g.off, g.G, g.M, tiles_n, g.cus, bid, lane, f)) return false;
+        t.g = f.g;
+        t.row0 = f.row0;
+        t.rows = f.rows;
+        tn = f.tn;
+        t.k = MX ? (g.K + 31) / 32 * 16 : (g.K * 2 + 15) / 16 * 16;
+        t.KT = (t.k + 127) / 128;
+        t.a += t.row0 * g.lda;
+        t.b += t.g * g.bsb;
+    }
+    t.n0 = tn * BN;
+    t.cols = g.N - t.n0 < BN ? g.N - t.n0 : BN;
+    t.b += BT ? (int64_t)t.n0 * 2 : t.n0 * g.ldb;
+    return true;
+}
+
+// The scales of a MXFP4 tile: wave w loads rows 64*w .. +63 of the tile's A rows, then of
+// its B rows, 16 bytes each (two stages) at a time.
+template <int BM, int BN>
+struct ScalePanel {
+    static constexpr int A_ROWS = (BM + 63) / 64 * 64, B_ROWS = (BN + 63) / 64 * 64;
+    static constexpr int SLOT = (A_ROWS + B_ROWS) * 16;
+    const uint8_t *base;
+    int left;       // blocks of a row from the next two stages on
+    uint32_t vo;
+    uint8_t *dst;   // this wave's part of slot 0
+    bool mine;
+
+    __device__ __forceinline__ void init(const RaggedArgs &g, const RaggedTile &t, uint8_t *slots,
+                                         uint8_t *spare, int wave, int lane) {
+        constexpr int NA = A_ROWS / 64;
+        const bool is_a = wave < NA;
+        const int r0 = (is_a ? wave : wave - NA) * 64;
+        const int64_t lds = is_a ? g.lsa : g.lsb;
+        base = uniform(is_a ? g.sa + (t.row0 + r0) * lds
+                            : g.sb + t.g * g.bssb + (int64_t)(t.n0 + r0) * lds);
+        mine = wave < (A_ROWS + B_ROWS) / 64;
+        const int rows = mine ? (is_a ? t.rows : t.cols) - r0 : 0;
+        left = rows > 0 ? (g.K + 31) / 32 : 0;
+        vo = lane < rows ? (uint32_t)(lane * (int)lds) : kOutOfRange;
+        dst = mine ? slots + wave * 1024 : spare;
+    }
+    __device__ __forceinline__ void load(int slot) {
+        dma16(base, __builtin_amdgcn_readfirstlane(left > 0 ? kMaxRecords : 0), vo,
+              mine ? dst + slot * SLOT : dst);
+        base += 16;
+        left -= 16;
+    }
+};
+
+// The scales of N 64-row quads of a wave for one stage: rows from `row` of the slot at sc
+// (+ 8 in an odd stage); `nv` blocks of the row remain from this stage on.
+template <int N, int ROWS>
+__device__ __forceinline__ void read_scales(const uint8_t *sc, int row, int nv, int lane,
+                                            ScaleQuad (&x)[N]) {
+    // A row's bytes past its blocks hold anything: cleared, so that no NaN scale meets the
+    // zero codes there.
+    const uint32_t mx = nv >= 4 ? ~0u : (nv <= 0 ? 0u : (1u << (8 * nv)) - 1);
+    const uint32_t my = nv >= 8 ? ~0u : (nv <= 4 ? 0u : (1u << (8 * (nv - 4))) - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const v2u w = *(const v2u *)(sc + (row + 64 * i + (lane & (ROWS < 64 ? ROWS - 1 : 63))) * 16);
+        x[i].set(w[0] & mx, w[1] & my);
+    }
+}
+
+// acc[i][j] += the products of half SS of a stage.
+template <int SS>
+__device__ __forceinline__ v4f mx_half(v4i b, v4i a, v4f c, const ScaleQuad &y, const ScaleQuad &x,
+                                       int i, int j) {
+    // (the byte of a scale register is an immediate)
+    const int sx = x.q[i % 2], sy = y.q[j % 2];
+    const bool ia = (i / 2) % 2, jb = (j / 2) % 2;
+    return ia ? (jb ? mx_step<2 * SS + 1, 2 * SS + 1>(b, a, c, sy, sx)
+                    : mx_step<2 * SS + 1, 2 * SS>(b, a, c, sy, sx))
+              : (jb ? mx_step<2 * SS, 2 * SS + 1>(b, a, c, sy, sx)
+                    : mx_step<2 * SS, 2 * SS>(b, a, c, sy, sx));
+}
+
+// Epilogue: 16-row bands of a wave's TM x TN blocks staged through LDS and stored as rows.
+template <EpiKind E, int WTM, int WTN, int TM, int TN>
+__device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTile &t, int N,
+                                             const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                             int wm, int wn, int lane) {
+    constexpr int EPI_LD = WTN + 4;
+    float *const stg = (float *)smem + wave * 16 * EPI_LD;
+    constexpr int CPRE = WTN / 4;                          // 4-element chunks per row
+    constexpr int RPIT = 64 / CPRE < 16 ? 64 / CPRE : 16;  // rows per pass
+    const int l16 = lane & 15, lq = lane >> 4;
+    const int gcol0 = t.n0 + wn * WTN;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * EPI_LD + j * 16 + 4 * lq) = acc[i][j];
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int it = 0; it < 16 / RPIT; ++it) {
+            const int r = it * RPIT + lane / CPRE, c4 = (lane % CPRE) * 4;
+            const v4f v4 = *(const v4f *)(stg + r * EPI_LD + c4);
+            const float v[4] = {v4[0], v4[1], v4[2], v4[3]};
+            const int row = wm * WTM + i * 16 + r;
+            if (row < t.rows && gcol0 + c4 < N)
+                store4<E, float, StPol::Plain>(ep, t.z, t.row0 + row, gcol0 + c4, N, v);
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---------------------------------------------------------------- small tiles
 
 template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(WM * WN * 64)
@@ -324,80 +508,30 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
     using L = RaggedLds<MX, BM, BN, NS>;
     using PA = Panel<AT, BM, NW>;
     using PB = Panel<BT, BN, NW>;
+    using SP = ScalePanel<BM, BN>;
     constexpr int LPW = PA::LP + PB::LP;  // loads per wave and stage (without scales)
-    constexpr int EPI_LD = WTN + 4;
-    static_assert(L::BYTES <= 160 * 1024 && NW * 16 * EPI_LD * 4 <= L::BYTES, "LDS");
-    static_assert(!MX || (L::SA_ROWS + L::SB_ROWS) / 64 <= NW, "one scale load per wave");
+    static_assert(L::BYTES <= 160 * 1024 && NW * 16 * (WTN + 4) * 4 <= L::BYTES, "LDS");
+    static_assert(!MX || (SP::A_ROWS + SP::B_ROWS) / 64 <= NW, "one scale load per wave");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
 
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int tiles_n = (g.N + BN - 1) / BN;
-    const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-
-    GroupTile t;
-    int k, z = 0;   // contraction: bytes (k-contiguous A), rows (wgrad)
-    const uint8_t *pa = (const uint8_t *)g.a, *pb = (const uint8_t *)g.b;
-    if constexpr (AT) {
-        const int tiles_m = (g.K + BM - 1) / BM, per = tiles_m * tiles_n;
-        const int64_t all = (int64_t)per * g.G;
-        if (bid >= all) return;
-        const int64_t pid = xcd_logical(bid, all);
-        int tm, s, e;
-        t.g = (int)(pid / per);
-        tile_coords((int)(pid % per), tiles_m, tiles_n, tm, t.tn);
-        one_group(g.off, g.G, g.M, t.g, lane, s, e);
-        t.row0 = tm * BM;
-        t.rows = g.K - t.row0 < BM ? g.K - t.row0 : BM;
-        k = e - s;
-        z = t.g;
-        pa += s * g.lda + (int64_t)t.row0 * 2;
-        pb += s * g.ldb;
-    } else {
-        if (!find_tile<BM>(g.off, g.G, g.M, tiles_n, bid, lane, t)) return;
-        k = MX ? (g.K + 31) / 32 * 16 : (g.K * 2 + 15) / 16 * 16;
-        pa += t.row0 * g.lda;
-        pb += t.g * g.bsb;
-    }
-    const int n0 = t.tn * BN;
-    const int cols = g.N - n0 < BN ? g.N - n0 : BN;
-    pb += BT ? (int64_t)n0 * 2 : n0 * g.ldb;
-    const int KT = AT ? (k + 63) / 64 : (k + 127) / 128;
+    RaggedTile t;
+    if (!ragged_tile<MX, AT, BT, BM, BN, false>(g, lane, t)) return;
 
     PA A;
     PB B;
-    A.init(pa, g.lda, t.rows, k, t.rows * 2, wave, lane);
+    A.init(t.a, g.lda, t.rows, t.k, t.rows * 2, wave, lane);
     // (a transposed B against a k-contiguous A: g.K rows)
-    B.init(pb, g.ldb, cols, BT && !AT ? g.K : k, cols * 2, wave, lane);
+    B.init(t.b, g.ldb, t.cols, BT && !AT ? g.K : t.k, t.cols * 2, wave, lane);
     uint8_t *const spare = smem + L::SPARE;
-
-    // Scales: wave w loads rows 64*w .. +63 of the tile's A rows and B rows, 16 bytes each
-    // (two stages).
-    const uint8_t *s_base = nullptr;
-    int s_left = 0;  // blocks of a row from the next two stages on
-    uint32_t s_vo = 0;
+    SP S;
+    if constexpr (MX) S.init(g, t, smem + L::SCALES, spare, wave, lane);
     const int nb = (g.K + 31) / 32;  // blocks of a row
-    if constexpr (MX) {
-        constexpr int NA = L::SA_ROWS / 64;
-        const bool is_a = wave < NA;
-        const int r0 = (is_a ? wave : wave - NA) * 64;
-        const int64_t lds = is_a ? g.lsa : g.lsb;
-        s_base = uniform(is_a ? g.sa + (t.row0 + r0) * lds
-                              : g.sb + t.g * g.bssb + (int64_t)(n0 + r0) * lds);
-        const int rows = wave >= (L::SA_ROWS + L::SB_ROWS) / 64 ? 0 : (is_a ? t.rows : cols) - r0;
-        s_left = rows > 0 ? nb : 0;
-        s_vo = lane < rows ? (uint32_t)(lane * (int)lds) : kOutOfRange;
-    }
-    int s_slot = 0;
+    int s_slot = 0, r_slot = 0;      // scale slots: the next to fill, the one in use
     auto load_scales = [&]() {  // of the next two stages
-        uint8_t *d = wave < (L::SA_ROWS + L::SB_ROWS) / 64
-                         ? smem + L::SCALES + s_slot * L::SSLOT + wave * 1024
-                         : spare;
-        dma16(s_base, __builtin_amdgcn_readfirstlane(s_left > 0 ? kMaxRecords : 0), s_vo, d);
-        s_base += 16;
-        s_left -= 16;
+        S.load(s_slot);
         s_slot = s_slot == L::NSS - 1 ? 0 : s_slot + 1;
     };
     auto load_stage = [&](uint8_t *d) {
@@ -419,8 +553,9 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
 
-    int r_slot = 0;  // the scale slot in use
-    // Stage kt, in slot kt % NS; PAR: kt's parity.
+    // Stage kt; PAR: kt's parity.  wr: the slot to load into, sa: the stage's own.  The two
+    // differ, and `restrict` says so: else the compiler waits for every load in flight
+    // before the transposing reads.
     auto kstep = [&](int kt, auto par, uint8_t *__restrict__ wr, const uint8_t *__restrict__ sa) {
         constexpr int PAR = decltype(par)::value;
         // Loads in flight behind stage kt's: stages kt+1 .. kt+NS-2, the even ones with
@@ -433,23 +568,10 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
         const uint8_t *const sb = sa + PA::BYTES;
         ScaleQuad xa[QA], xb[QB];
         if constexpr (MX) {
-            const uint8_t *sc = smem + L::SCALES + r_slot * L::SSLOT + PAR * 8;
+            const uint8_t *sc = smem + L::SCALES + r_slot * SP::SLOT + PAR * 8;
             if (PAR) r_slot = r_slot == L::NSS - 1 ? 0 : r_slot + 1;
-            // A row's bytes past its blocks hold anything: cleared, so that no NaN
-            // scale meets the zero codes there.
-            const int nv = nb - kt * 8;
-            const uint32_t mx = nv >= 4 ? ~0u : (1u << (8 * nv)) - 1;
-            const uint32_t my = nv >= 8 ? ~0u : (nv <= 4 ? 0u : (1u << (8 * (nv - 4))) - 1);
-#pragma unroll
-            for (int i = 0; i < QA; ++i) {
-                const v2u w = *(const v2u *)(sc + (wm * WTM + 64 * i + (lane & (WTM - 1 < 63 ? WTM - 1 : 63))) * 16);
-                xa[i].set(w[0] & mx, w[1] & my);
-            }
-#pragma unroll
-            for (int i = 0; i < QB; ++i) {
-                const v2u w = *(const v2u *)(sc + (L::SA_ROWS + wn * WTN + 64 * i + (lane & (WTN - 1 < 63 ? WTN - 1 : 63))) * 16);
-                xb[i].set(w[0] & mx, w[1] & my);
-            }
+            read_scales<QA, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
+            read_scales<QB, WTN>(sc, SP::A_ROWS + wn * WTN, nb - kt * 8, lane, xb);
         }
         auto half = [&](auto hh) {
             constexpr int SS = decltype(hh)::value;
@@ -461,19 +583,9 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    if constexpr (MX) {
-                        // (the byte of a scale register is an immediate)
-                        const int x = xa[i / 4].q[i % 2], y = xb[j / 4].q[j % 2];
-                        const bool ia = (i / 2) % 2, jb = (j / 2) % 2;
-                        acc[i][j] = ia ? (jb ? mx_step<2 * SS + 1, 2 * SS + 1>(bf[j], af[i], acc[i][j], y, x)
-                                             : mx_step<2 * SS + 1, 2 * SS>(bf[j], af[i], acc[i][j], y, x))
-                                       : (jb ? mx_step<2 * SS, 2 * SS + 1>(bf[j], af[i], acc[i][j], y, x)
-                                             : mx_step<2 * SS, 2 * SS>(bf[j], af[i], acc[i][j], y, x));
-                    } else {
-                        acc[i][j] = bf_step(bf[j], af[i], acc[i][j]);
-                    }
-                }
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = MX ? mx_half<SS>(bf[j], af[i], acc[i][j], xb[j / 4], xa[i / 4], i, j)
+                                   : bf_step(bf[j], af[i], acc[i][j]);
         };
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
@@ -492,38 +604,208 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
         kstep(kt, par, smem + w * L::STAGE, smem + slot * L::STAGE);
         slot = slot == NS - 1 ? 0 : slot + 1;
     };
-    for (int kt = 0; kt < KT; kt += 2) {
+    for (int kt = 0; kt < t.KT; kt += 2) {
         step(kt, std::integral_constant<int, 0>{});
-        if (kt + 1 < KT) step(kt + 1, std::integral_constant<int, 1>{});
+        if (kt + 1 < t.KT) step(kt + 1, std::integral_constant<int, 1>{});
     }
 
-    // Epilogue: 16-row bands of the wave staged through LDS and stored as rows.  The loads
-    // past the end of K (zeros into ring slots) land first.
+    // (the loads past the end of K, zeros into ring slots, land first)
     wait_vmcnt<0>();
     __syncthreads();
-    float *const stg = (float *)smem + wave * 16 * EPI_LD;
-    constexpr int CPRE = WTN / 4;                       // 4-element chunks per row
-    constexpr int RPIT = 64 / CPRE < 16 ? 64 / CPRE : 16;  // rows per pass
-    const int l16 = lane & 15, lq = lane >> 4;
-    const int gcol0 = n0 + wn * WTN;
+    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+}
+
+// ---------------------------------------------------------------- 256 x 256 tile
+
+// Eight waves of 128 x 64, as mma16_kernel's: a stage is four phases of 16 matrix
+// instructions, fragments and loads of later stages spread among them.
+//   phase 0  half 0, block rows 0-3   reads half 1's A 0-3 and B;  (3 A slots) loads A of kt+2
+//   phase 1  half 0, block rows 4-7   reads half 1's A 4-7
+//   phase 2  half 1, block rows 0-3   then waits for stage kt+1, barrier
+//   phase 3  half 1, block rows 4-7   reads half 0 of stage kt+1; loads the rest of kt+2
+// bf16: three A slots and two B slots, all of the LDS; MXFP4: two of each and the scales.
+template <bool MX>
+struct RaggedBigLds {
+    static constexpr int NSA = MX ? 2 : 3, NSB = 2, OP = 256 * 128;
+    static constexpr int B = NSA * OP, SCALES = B + NSB * OP;
+    static constexpr int BYTES = SCALES + (MX ? 2 * ScalePanel<256, 256>::SLOT : 0);
+};
+
+template <bool MX, bool AT, bool BT, EpiKind E>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
+    constexpr int BM = 256, BN = 256, WN = 4, WTM = 128, WTN = 64, TM = 8, TN = 4;
+    using L = RaggedBigLds<MX>;
+    using PA = Panel<AT, BM, 8>;
+    using PB = Panel<BT, BN, 8>;
+    using SP = ScalePanel<BM, BN>;
+    constexpr int LPA = PA::LP, LPB = PB::LP;
+    constexpr bool A3 = L::NSA == 3;
+    static_assert(L::BYTES <= 160 * 1024 && LPA == 4 && LPB == 4, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    RaggedTile t;
+    if (!ragged_tile<MX, AT, BT, BM, BN, true>(g, lane, t)) return;
+
+    PA A;
+    PB B;
+    A.init(t.a, g.lda, t.rows, t.k, t.rows * 2, wave, lane);
+    B.init(t.b, g.ldb, t.cols, BT && !AT ? g.K : t.k, t.cols * 2, wave, lane);
+    SP S;
+    if constexpr (MX) S.init(g, t, smem + L::SCALES, nullptr, wave, lane);
+    const int nb = (g.K + 31) / 32;
+
+    Frag<AT, BM> fa;
+    Frag<BT, BN> fb;
+    fa.init(lane, wm * WTM);
+    fb.init(lane, wn * WTN);
+    v4f acc[TM][TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * EPI_LD + j * 16 + 4 * lq) = acc[i][j];
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int it = 0; it < 16 / RPIT; ++it) {
-            const int r = it * RPIT + lane / CPRE, c4 = (lane % CPRE) * 4;
-            const v4f v4 = *(const v4f *)(stg + r * EPI_LD + c4);
-            const float v[4] = {v4[0], v4[1], v4[2], v4[3]};
-            const int row = wm * WTM + i * 16 + r;
-            if (row < t.rows && gcol0 + c4 < g.N)
-                store4<E, float, StPol::Plain>(ep, z, t.row0 + row, gcol0 + c4, g.N, v);
+        for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
+    v4i af[2][TM], bf[2][TN];
+    ScaleQuad xa[2], xb[1];
+
+    auto mfma_rows = [&](auto hh, int r0) {
+        constexpr int SS = decltype(hh)::value;
+#pragma unroll
+        for (int i = r0; i < r0 + TM / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = MX ? mx_half<SS>(bf[SS][j], af[SS][i], acc[i][j], xb[0], xa[i / 4], i, j)
+                               : bf_step(bf[SS][j], af[SS][i], acc[i][j]);
+    };
+    // A fragments [alo, alo + na) and (wb) the B fragments of half ss, with nl loads spread
+    // among them.
+    auto ops = [&](const uint8_t *sa, const uint8_t *sb, auto ss, int alo, auto na, auto wb, auto nl,
+                   auto ld) {
+        constexpr int SS = decltype(ss)::value, NA = decltype(na)::value;
+        constexpr int NB = decltype(wb)::value ? TN : 0, NR = NA + NB, NL = decltype(nl)::value;
+        int l = 0;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            // A[alo], B, then A[alo+1 ..]: the next phase's first products pair A[alo]
+            // with every B fragment
+            const int ra = r == 0 ? 0 : (r <= NB ? -1 : r - NB);
+            if (ra >= 0) af[SS][alo + ra] = fa.read(sa, alo + ra, SS);
+            else bf[SS][r - 1] = fb.read(sb, r - 1, SS);
+            if ((r + 1) * NL / NR != r * NL / NR) ld(l++);
         }
-        __builtin_amdgcn_s_waitcnt(0xC07F);
-        __builtin_amdgcn_wave_barrier();
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using H = std::integral_constant<int, TM / 2>;
+    using FA = std::integral_constant<int, TM>;
+    constexpr int RA = AT ? 2 : 1, RB = BT ? 2 : 1;  // LDS reads per fragment
+    constexpr int NM = (TM / 2) * TN, SPAN = NM * 7 / 8;
+
+    auto a_slot = [&](int s) { return smem + s * L::OP; };
+    auto b_slot = [&](int s) { return smem + L::B + s * L::OP; };
+    auto scales = [&](int kt, int par) {  // of stage kt, which has landed
+        const uint8_t *sc = smem + L::SCALES + ((kt >> 1) & 1) * SP::SLOT + par * 8;
+        read_scales<2, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
+        read_scales<1, WTN>(sc, SP::A_ROWS + wn * WTN, nb - kt * 8, lane, xb);
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if constexpr (MX) {
+            if (s == 0) S.load(0);
+        }
+#pragma unroll
+        for (int i = 0; i < LPA; ++i) A.load(a_slot(s), nullptr, i);
+        A.next();
+#pragma unroll
+        for (int i = 0; i < LPB; ++i) B.load(b_slot(s), nullptr, i);
+        B.next();
     }
+    wait_vmcnt<LPA + LPB>();
+    stage_barrier();
+    ops(a_slot(0), b_slot(0), I0{}, 0, FA{}, std::true_type{}, I0{}, [](int) {});
+    if constexpr (MX) scales(0, 0);
+
+
+    // A stage in two parts, up to its barrier and behind it: within each, the slots that are
+    // loaded (wa, wb: stage kt+2's) and those that are read differ, and `restrict` says so
+    // (see ragged_kernel).  No branches: they would end the scheduled block.
+    constexpr int LA = A3 ? LPA : 0, LB = A3 ? LPB : LPA + LPB;
+    auto before = [&](uint8_t *__restrict__ wa, const uint8_t *__restrict__ sa,
+                      const uint8_t *__restrict__ sb) {
+        mfma_rows(I0{}, 0);
+        ops(sa, sb, I1{}, 0, H{}, std::true_type{}, std::integral_constant<int, LA>{},
+            [&](int i) { A.load(wa, nullptr, i); });
+        sched_ops<NM, TM / 2 * RA + TN * RB, LA, SPAN>();
+        if constexpr (A3) A.next();
+        mfma_rows(I0{}, TM / 2);
+        ops(sa, sb, I1{}, TM / 2, H{}, std::false_type{}, I0{}, [](int) {});
+        sched_ops<NM, TM / 2 * RA, 0, SPAN>();
+        mfma_rows(I1{}, 0);
+#pragma unroll
+        for (int m = 0; m < NM; ++m) __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        wait_vmcnt<LA>();
+        stage_barrier();
+    };
+    auto behind = [&](int kt, auto par, uint8_t *__restrict__ wa, uint8_t *__restrict__ wb,
+                      const uint8_t *__restrict__ na, const uint8_t *__restrict__ nbp) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(af[1][i]));
+#pragma unroll
+        for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(bf[1][j]));
+        mfma_rows(I1{}, TM / 2);
+        if constexpr (MX && decltype(par)::value == 0) S.load(((kt >> 1) + 1) & 1);
+        ops(na, nbp, I0{}, 0, FA{}, std::true_type{}, std::integral_constant<int, LB>{}, [&](int i) {
+            if constexpr (A3) B.load(wb, nullptr, i);
+            else if (i < LPA) A.load(wa, nullptr, i);
+            else B.load(wb, nullptr, i - LPA);
+        });
+        sched_ops<NM, TM * RA + TN * RB, LB, SPAN>();
+        if constexpr (!A3) A.next();
+        B.next();
+        if constexpr (MX) scales(kt + 1, 1 - decltype(par)::value);
+    };
+    int s = 0;
+    auto step = [&](int kt, auto par) {
+        const int s1 = s == L::NSA - 1 ? 0 : s + 1, s2 = A3 ? (s1 == L::NSA - 1 ? 0 : s1 + 1) : s;
+        constexpr int P = decltype(par)::value;
+        before(a_slot(s2), a_slot(s), b_slot(P));
+        behind(kt, par, a_slot(s2), b_slot(P), a_slot(s1), b_slot(1 - P));
+        s = s1;
+    };
+    if (wm == 0 || t.rows > WTM) {
+        for (int kt = 0; kt < t.KT; kt += 2) {
+            step(kt, I0{});
+            if (kt + 1 < t.KT) step(kt + 1, I1{});
+        }
+    } else {
+        // A tile of at most half the rows: the lower waves only load, and the upper ones,
+        // one on each SIMD, have the matrix cores to themselves.
+        for (int kt = 0; kt < t.KT; ++kt) {
+            if constexpr (A3) {
+#pragma unroll
+                for (int i = 0; i < LPA; ++i) A.load(a_slot((kt + 2) % 3), nullptr, i);
+                A.next();
+            }
+            wait_vmcnt<LA>();
+            stage_barrier();
+            if constexpr (MX) {
+                if (!(kt & 1)) S.load(((kt >> 1) + 1) & 1);
+            }
+            if constexpr (!A3) {
+#pragma unroll
+                for (int i = 0; i < LPA; ++i) A.load(a_slot(kt & 1), nullptr, i);
+                A.next();
+            }
+#pragma unroll
+            for (int i = 0; i < LPB; ++i) B.load(b_slot(kt & 1), nullptr, i);
+            B.next();
+        }
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
@@ -539,6 +821,8 @@ inline int64_t ragged_tiles(const RaggedArgs &g, int bm, int bn) {
     return tm * ((g.N + bn - 1) / bn);
 }
 
+// The tile shapes: BM x BN on WM x WN waves with NS stages in the ring, and the 256 x 256
+// kernel (NS == 0).
 template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS>
 static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     // 32-bit offsets inside a panel, with the loads of rows past its edge
@@ -547,11 +831,19 @@ static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
         (BT ? 64 * g.ldb + (int64_t)g.N * 2 : BN * g.ldb + kbytes) > (int64_t)kMaxRecords ||
         (MX && 64 * (g.lsa > g.lsb ? g.lsa : g.lsb) > (int64_t)kMaxRecords))
         return hipErrorInvalidValue;
-    const int64_t tiles = AT ? (int64_t)g.G * ((g.K + BM - 1) / BM) * ((g.N + BN - 1) / BN)
-                             : ragged_tiles(g, BM, BN);
+    const int64_t per = (int64_t)((g.K + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    if (AT && per > INT32_MAX - 8) return hipErrorInvalidValue;
+    const int64_t tiles = AT ? (int64_t)g.G * wgrad_share((int)per) * 8
+                             : ragged_tiles(g, BM, BN) + (NS == 0 ? g.cus : 8);
     if (tiles > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, WM, WN, NS>), ragged_grid(tiles),
-                       dim3(WM * WN * 64), 0, stream, g, ep);
+    const dim3 grid = ragged_grid(tiles), block(WM * WN * 64);
+    if constexpr (NS == 0) {
+        static_assert(BM == 256 && BN == 256 && WM == 2 && WN == 4, "the big tile");
+        hipLaunchKernelGGL((ragged_big_kernel<MX, AT, BT, E>), grid, block, 0, stream, g, ep);
+    } else {
+        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, WM, WN, NS>), grid, block, 0,
+                           stream, g, ep);
+    }
     return hipGetLastError();
 }
 
