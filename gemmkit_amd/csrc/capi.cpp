@@ -2273,6 +2273,7 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     ep.vec4 = c->cs == 1;
     RaggedArgs g{};
     g.cus = g_num_cus;
+    g.splits = 1;
     g.a = A.p;
     g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
     g.lda = lda;
@@ -2329,23 +2330,6 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     const int64_t M = alpha == 0.0f ? 0 : (int64_t)a->rows;
     const int64_t K = (int64_t)x->cols, N = (int64_t)y->cols;
     Opnd A{x->data, x->rs, x->cs, 0}, B{y->data, y->rs, y->cs, 0};
-    int64_t lda = 0, ldb = 0;
-    if (M > 0) {
-        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
-        if (!a_ok || !b_ok) {
-            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-            const size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
-            void *buf = nullptr;
-            if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
-            PackJob jobs[2];
-            int nj = 0;
-            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
-            if (pb) jobs[nj++] = pack_job(InType::BF16, &B, M, N, 1, (uint8_t *)buf + pa);
-            if ((r = pack_groups(jobs, nj))) return r;
-        }
-        lda = ragged_ld(A, M, K);
-        ldb = ragged_ld(B, M, N);
-    }
     EpiParams ep = epi_float(kind, alpha, beta);
     ep.c = c->data;
     ep.rsc = swap ? c->cs : c->rs;
@@ -2354,17 +2338,49 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     ep.vec4 = ep.csc == 1;
     RaggedArgs g{};
     g.cus = g_num_cus;
-    g.a = A.p;
-    g.b = B.p;
-    g.lda = lda;
-    g.ldb = ldb;
     g.off = offsets;
     g.G = (int32_t)groups;
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
-    const hipError_t e = launch_grouped_wgrad(g, ep, tl_stream);
+    g.splits = wgrad_splits(g);
+    uint8_t *part = nullptr;
+    if (M > 0) {
+        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
+        const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+        const size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
+        const size_t sums = g.splits > 1 ? (size_t)g.splits * groups * K * N * 4 : 0;
+        if (pa + pb + sums > 0) {
+            void *buf = nullptr;
+            if ((r = ws_reserve(resolve_ws(ws), pa + pb + sums, &buf))) return r;
+            part = (uint8_t *)buf + pa + pb;
+            PackJob jobs[2];
+            int nj = 0;
+            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
+            if (pb) jobs[nj++] = pack_job(InType::BF16, &B, M, N, 1, (uint8_t *)buf + pa);
+            if (nj && (r = pack_groups(jobs, nj))) return r;
+        }
+        g.lda = ragged_ld(A, M, K);
+        g.ldb = ragged_ld(B, M, N);
+    }
+    g.a = A.p;
+    g.b = B.p;
+    if (g.splits == 1) {
+        const hipError_t e = launch_grouped_wgrad(g, ep, tl_stream);
+        if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
+        return finish("grouped weight gradient");
+    }
+    // Partial sums of the row ranges, then their sum in range order with the epilogue.
+    EpiParams pe = epi_float(EpiKind::F32, 1.0f, 0.0f);
+    pe.c = part;
+    pe.rsc = N;
+    pe.csc = 1;
+    pe.bsc = K * N;
+    pe.vec4 = 1;
+    hipError_t e = launch_grouped_wgrad(g, pe, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
+    e = launch_split_reduce(InType::BF16, part, g.splits, K, N, (int64_t)groups, ep, tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "split reduce");
     return finish("grouped weight gradient");
 }
 
@@ -2486,6 +2502,7 @@ int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool 
     ep.vec4 = ep.csc == 1;
     RaggedArgs g{};
     g.cus = g_num_cus;
+    g.splits = 1;
     g.a = a->codes;
     g.b = b->codes;
     g.sa = (const uint8_t *)a->scales;

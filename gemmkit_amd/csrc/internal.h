@@ -251,11 +251,15 @@ struct RaggedArgs {
     const int32_t *off;        // G + 1 offsets on the device, or nullptr
     int32_t G, M, N, K;        // M: rows of A; wgrad: K is A's columns
     int32_t cus;               // compute units of the device
+    // wgrad: row ranges per group (1 = whole groups).  Range r of group g writes its sums
+    // to batch element g*splits + r of C, in whole stages of 64 rows.
+    int32_t splits;
 };
 // B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
 enum class RaggedB : int { Rows = 0, Cols = 1 };
 hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
                                hipStream_t stream);
+int wgrad_splits(const RaggedArgs &g);  // what a product should be given
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 
 // MXFP4 (mxfp4.hip): rows of e2m1 codes, two a byte, the lower nibble first, with one

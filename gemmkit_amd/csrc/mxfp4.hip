@@ -219,18 +219,9 @@ hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stre
                                : mx_walk<InType::F32>(g, false, stream);
 }
 
-template <EpiKind E>
-static hipError_t mxfp4_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-    const int64_t groups = g.G < g.M ? g.G : g.M;
-    const int64_t avg = (g.M + groups - 1) / groups;
-    if (avg <= 24) return ragged_go<true, false, false, E, 16, 64, 1, 4, 7>(g, ep, stream);
-    if (avg <= 96) return ragged_go<true, false, false, E, 64, 128, 2, 2, 3>(g, ep, stream);
-    return ragged_go<true, false, false, E, 256, 256, 2, 4, 0>(g, ep, stream);
-}
-
 hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-    if (ep.kind == EpiKind::BF16) return mxfp4_go<EpiKind::BF16>(g, ep, stream);
-    if (ep.kind == EpiKind::F32) return mxfp4_go<EpiKind::F32>(g, ep, stream);
+    if (ep.kind == EpiKind::BF16) return ragged_forward<true, false, EpiKind::BF16>(g, ep, stream);
+    if (ep.kind == EpiKind::F32) return ragged_forward<true, false, EpiKind::F32>(g, ep, stream);
     return hipErrorInvalidValue;
 }
 

@@ -246,16 +246,17 @@ struct Panel {
             TR ? (left >= 64 ? kMaxRecords : (left > 0 ? (uint32_t)(left * ld) : 0))
                : (left > 0 ? num : 0));
     }
-    __device__ __forceinline__ void next() {
+    __device__ __forceinline__ void skip(int stages) {
         if constexpr (TR) {
-            base += (int64_t)64 * ld;
-            left -= 64;
+            base += (int64_t)stages * 64 * ld;
+            left -= stages * 64;
         } else {
-            base += 128;
-            num -= 128;
-            left -= 128;
+            base += stages * 128;
+            num -= (uint32_t)stages * 128;
+            left -= stages * 128;
         }
     }
+    __device__ __forceinline__ void next() { skip(1); }
 };
 
 // Fragments of 16-row (16-column, TR) blocks from a stage.
@@ -364,7 +365,8 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &g, int lane, Ragge
         // Every XCD takes an eighth of each group's tiles, a contiguous one: with whole
         // groups per XCD the one with the longest group would work on alone.  (The
         // eighths turn with the group, so that their roundings even out.)
-        const int tiles_m = (g.K + BM - 1) / BM, per = tiles_m * tiles_n, share = wgrad_share(per);
+        const int tiles_m = (g.K + BM - 1) / BM, tiles = tiles_m * tiles_n;
+        const int per = tiles * g.splits, share = wgrad_share(per);
         const int64_t idx = bid / 8;
         t.g = (int)(idx / share);
         if (t.g >= g.G) return false;
@@ -372,12 +374,20 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &g, int lane, Ragge
         const int pid = (int)((int64_t)part * per / 8) + (int)(idx % share);
         if (pid >= (int)((int64_t)(part + 1) * per / 8)) return false;
         int tm, s, e;
-        tile_coords(pid, tiles_m, tiles_n, tm, tn);
+        tile_coords(pid % tiles, tiles_m, tiles_n, tm, tn);
         one_group(g.off, g.G, g.M, t.g, lane, s, e);
+        const int sp = pid / tiles;
+        if (g.splits > 1) {  // this part's stages of the group
+            const int stages = (e - s + 63) / 64;
+            const int lo = (int)((int64_t)stages * sp / g.splits);
+            const int hi = (int)((int64_t)stages * (sp + 1) / g.splits);
+            e = e < s + hi * 64 ? e : s + hi * 64;
+            s += lo * 64;
+        }
         t.row0 = tm * BM;
         t.rows = g.K - t.row0 < BM ? g.K - t.row0 : BM;
-        t.k = e - s;
-        t.z = t.g;
+        t.k = e > s ? e - s : 0;
+        t.z = t.g * g.splits + sp;
         t.KT = (t.k + 63) / 64;
         t.a += s * g.lda + (int64_t)t.row0 * 2;
         t.b += s * g.ldb;
@@ -462,31 +472,69 @@ __device__ __forceinline__ v4f mx_half(v4i b, v4i a, v4f c, const ScaleQuad &y, 
                     : mx_step<2 * SS, 2 * SS>(b, a, c, sy, sx));
 }
 
+// Elements a lane stores at once: 16 bytes.
+constexpr int chunk_of(EpiKind e) { return e == EpiKind::BF16 ? 8 : 4; }
+
+// A chunk of one row of C.  bf16 takes 16 bytes here instead of store4's 8: a weight
+// gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16 from 64 rows: 21.8 us
+// with 8 bytes a lane).
+template <EpiKind E>
+__device__ __forceinline__ void store_chunk(const EpiParams &ep, int64_t z, int row, int col, int N,
+                                            const v4f (&v)[chunk_of(E) / 4]) {
+    if constexpr (E == EpiKind::BF16) {
+        if (ep.vec4 && col + 8 <= N) {
+            typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+            typedef uint32_t v4u_any2 __attribute__((ext_vector_type(4), aligned(2)));
+            uint16_t *c = (uint16_t *)ep.c + z * ep.bsc + (int64_t)row * ep.rsc + col;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = ep.alpha_f * v[e / 4][e % 4];
+            if (ep.beta_f != 0.0f) {
+                const v4u old = *(const v4u_any2 *)c;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float w = bf16_widen((uint16_t)(old[e / 2] >> (16 * (e % 2))));
+                    f[e] = ep.beta_f == 1.0f ? w + f[e] : __builtin_fmaf(ep.beta_f, w, f[e]);
+                }
+            }
+            v4u o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
+            __builtin_nontemporal_store(o, (v4u_any2 *)c);
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < chunk_of(E) / 4; ++i) {
+        const float w[4] = {v[i][0], v[i][1], v[i][2], v[i][3]};
+        if (col + 4 * i < N) store4<E, float, StPol::Plain>(ep, z, row, col + 4 * i, N, w);
+    }
+}
+
 // Epilogue: 16-row bands of a wave's TM x TN blocks staged through LDS and stored as rows.
 template <EpiKind E, int WTM, int WTN, int TM, int TN>
 __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTile &t, int N,
                                              const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
                                              int wm, int wn, int lane) {
-    constexpr int EPI_LD = WTN + 4;
-    float *const stg = (float *)smem + wave * 16 * EPI_LD;
-    constexpr int CPRE = WTN / 4;                          // 4-element chunks per row
-    constexpr int RPIT = 64 / CPRE < 16 ? 64 / CPRE : 16;  // rows per pass
+    constexpr int LD = WTN + 4, CH = chunk_of(E);
+    constexpr int CPR = WTN / CH;                        // chunks per row
+    constexpr int RPP = 64 / CPR < 16 ? 64 / CPR : 16;   // rows per pass
+    float *const stg = (float *)smem + wave * 16 * LD;
     const int l16 = lane & 15, lq = lane >> 4;
-    const int gcol0 = t.n0 + wn * WTN;
+    const int r0 = lane / CPR, c = lane % CPR * CH, col = t.n0 + wn * WTN + c;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * EPI_LD + j * 16 + 4 * lq) = acc[i][j];
+        for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * LD + j * 16 + 4 * lq) = acc[i][j];
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-        for (int it = 0; it < 16 / RPIT; ++it) {
-            const int r = it * RPIT + lane / CPRE, c4 = (lane % CPRE) * 4;
-            const v4f v4 = *(const v4f *)(stg + r * EPI_LD + c4);
-            const float v[4] = {v4[0], v4[1], v4[2], v4[3]};
+        for (int r = r0; r < 16; r += RPP) {
+            v4f v[CH / 4];
+#pragma unroll
+            for (int e = 0; e < CH / 4; ++e) v[e] = *(const v4f *)(stg + r * LD + c + 4 * e);
             const int row = wm * WTM + i * 16 + r;
-            if (row < t.rows && gcol0 + c4 < N)
-                store4<E, float, StPol::Plain>(ep, t.z, t.row0 + row, gcol0 + c4, N, v);
+            if (row < t.rows && col < N) store_chunk<E>(ep, t.z, t.row0 + row, col, N, v);
         }
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_wave_barrier();
@@ -617,9 +665,9 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
 
 // ---------------------------------------------------------------- 256 x 256 tile
 
-// Eight waves of 128 x 64, as mma16_kernel's: a stage is four phases of 16 matrix
+// 256 x 256, eight waves of 128 x 64, as mma16_kernel's: a stage is four phases of 16 matrix
 // instructions, fragments and loads of later stages spread among them.
-//   phase 0  half 0, block rows 0-3   reads half 1's A 0-3 and B;  (3 A slots) loads A of kt+2
+//   phase 0  half 0, block rows 0-3   reads half 1's A 0-3 and B; (three A slots) loads A of kt+2
 //   phase 1  half 0, block rows 4-7   reads half 1's A 4-7
 //   phase 2  half 1, block rows 0-3   then waits for stage kt+1, barrier
 //   phase 3  half 1, block rows 4-7   reads half 0 of stage kt+1; loads the rest of kt+2
@@ -668,7 +716,7 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
     v4i af[2][TM], bf[2][TN];
-    ScaleQuad xa[2], xb[1];
+    ScaleQuad xa[TM / 4], xb[1];
 
     auto mfma_rows = [&](auto hh, int r0) {
         constexpr int SS = decltype(hh)::value;
@@ -707,7 +755,7 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
     auto b_slot = [&](int s) { return smem + L::B + s * L::OP; };
     auto scales = [&](int kt, int par) {  // of stage kt, which has landed
         const uint8_t *sc = smem + L::SCALES + ((kt >> 1) & 1) * SP::SLOT + par * 8;
-        read_scales<2, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
+        read_scales<TM / 4, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
         read_scales<1, WTN>(sc, SP::A_ROWS + wn * WTN, nb - kt * 8, lane, xb);
     };
 #pragma unroll
@@ -728,16 +776,22 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
     if constexpr (MX) scales(0, 0);
 
 
+    // Loads of stage kt+2 in phase 0 (L0, A's) and in phase 3 (L3, A's first).  The scales of
+    // stages kt+2 and kt+3 go out in phase 3 of even stages.
+    constexpr int L0 = A3 ? LPA : 0, L3 = LPA + LPB - L0;
+    auto load3 = [&](int i, uint8_t *wa, uint8_t *wb) {
+        if (!A3 && i < LPA) A.load(wa, nullptr, i);
+        else B.load(wb, nullptr, i - (A3 ? 0 : LPA));
+    };
     // A stage in two parts, up to its barrier and behind it: within each, the slots that are
     // loaded (wa, wb: stage kt+2's) and those that are read differ, and `restrict` says so
     // (see ragged_kernel).  No branches: they would end the scheduled block.
-    constexpr int LA = A3 ? LPA : 0, LB = A3 ? LPB : LPA + LPB;
     auto before = [&](uint8_t *__restrict__ wa, const uint8_t *__restrict__ sa,
                       const uint8_t *__restrict__ sb) {
         mfma_rows(I0{}, 0);
-        ops(sa, sb, I1{}, 0, H{}, std::true_type{}, std::integral_constant<int, LA>{},
+        ops(sa, sb, I1{}, 0, H{}, std::true_type{}, std::integral_constant<int, L0>{},
             [&](int i) { A.load(wa, nullptr, i); });
-        sched_ops<NM, TM / 2 * RA + TN * RB, LA, SPAN>();
+        sched_ops<NM, TM / 2 * RA + TN * RB, L0, SPAN>();
         if constexpr (A3) A.next();
         mfma_rows(I0{}, TM / 2);
         ops(sa, sb, I1{}, TM / 2, H{}, std::false_type{}, I0{}, [](int) {});
@@ -745,7 +799,7 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
         mfma_rows(I1{}, 0);
 #pragma unroll
         for (int m = 0; m < NM; ++m) __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-        wait_vmcnt<LA>();
+        wait_vmcnt<L0>();
         stage_barrier();
     };
     auto behind = [&](int kt, auto par, uint8_t *__restrict__ wa, uint8_t *__restrict__ wb,
@@ -756,56 +810,184 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
         for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(bf[1][j]));
         mfma_rows(I1{}, TM / 2);
         if constexpr (MX && decltype(par)::value == 0) S.load(((kt >> 1) + 1) & 1);
-        ops(na, nbp, I0{}, 0, FA{}, std::true_type{}, std::integral_constant<int, LB>{}, [&](int i) {
-            if constexpr (A3) B.load(wb, nullptr, i);
-            else if (i < LPA) A.load(wa, nullptr, i);
-            else B.load(wb, nullptr, i - LPA);
-        });
-        sched_ops<NM, TM * RA + TN * RB, LB, SPAN>();
+        ops(na, nbp, I0{}, 0, FA{}, std::true_type{}, std::integral_constant<int, L3>{},
+            [&](int i) { load3(i, wa, wb); });
+        sched_ops<NM, TM * RA + TN * RB, L3, SPAN>();
         if constexpr (!A3) A.next();
         B.next();
         if constexpr (MX) scales(kt + 1, 1 - decltype(par)::value);
     };
-    int s = 0;
+    int s = 0;  // A slot of stage kt
+    auto turn = [](int i) { return i == L::NSA - 1 ? 0 : i + 1; };
     auto step = [&](int kt, auto par) {
-        const int s1 = s == L::NSA - 1 ? 0 : s + 1, s2 = A3 ? (s1 == L::NSA - 1 ? 0 : s1 + 1) : s;
         constexpr int P = decltype(par)::value;
+        const int s1 = turn(s), s2 = turn(s1);  // of kt+1 and kt+2
         before(a_slot(s2), a_slot(s), b_slot(P));
         behind(kt, par, a_slot(s2), b_slot(P), a_slot(s1), b_slot(1 - P));
         s = s1;
     };
-    if (wm == 0 || t.rows > WTM) {
+    // A tile of at most half the rows: the lower waves only load, and the upper ones, one on
+    // each SIMD, have the matrix cores to themselves.
+    auto idle = [&](int kt, auto par) {
+        constexpr int P = decltype(par)::value;
+        const int s1 = turn(s);
+        uint8_t *const wa = a_slot(turn(s1));
+#pragma unroll
+        for (int i = 0; i < L0; ++i) A.load(wa, nullptr, i);
+        wait_vmcnt<L0>();
+        stage_barrier();
+        if constexpr (MX && P == 0) S.load(((kt >> 1) + 1) & 1);
+#pragma unroll
+        for (int i = 0; i < L3; ++i) load3(i, wa, b_slot(P));
+        A.next();
+        B.next();
+        s = s1;
+    };
+    auto stages = [&](auto one) {
         for (int kt = 0; kt < t.KT; kt += 2) {
-            step(kt, I0{});
-            if (kt + 1 < t.KT) step(kt + 1, I1{});
+            one(kt, I0{});
+            if (kt + 1 < t.KT) one(kt + 1, I1{});
         }
-    } else {
-        // A tile of at most half the rows: the lower waves only load, and the upper ones,
-        // one on each SIMD, have the matrix cores to themselves.
-        for (int kt = 0; kt < t.KT; ++kt) {
-            if constexpr (A3) {
-#pragma unroll
-                for (int i = 0; i < LPA; ++i) A.load(a_slot((kt + 2) % 3), nullptr, i);
-                A.next();
-            }
-            wait_vmcnt<LA>();
-            stage_barrier();
-            if constexpr (MX) {
-                if (!(kt & 1)) S.load(((kt >> 1) + 1) & 1);
-            }
-            if constexpr (!A3) {
-#pragma unroll
-                for (int i = 0; i < LPA; ++i) A.load(a_slot(kt & 1), nullptr, i);
-                A.next();
-            }
-#pragma unroll
-            for (int i = 0; i < LPB; ++i) B.load(b_slot(kt & 1), nullptr, i);
-            B.next();
-        }
-    }
+    };
+    if (wm == 0 || t.rows > WTM) stages(step);
+    else stages(idle);
     wait_vmcnt<0>();
     __syncthreads();
     ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+}
+
+// ---------------------------------------------------------------- few tiles
+
+// Products with too few tiles to keep the CUs busy by themselves: the KS waves of a
+// workgroup share one BM x BN tile and split K among them, stage kt to wave kt % KS.  Each
+// wave fills its own ring of NS stages and waits for nothing but its own loads (no
+// barriers); their sums are added in wave order through LDS at the end.
+template <bool MX, int BM, int BN, int KS, int NS>
+struct RaggedWaveLds {
+    static constexpr int STAGE = (BM + BN) * 128 + (MX ? 2048 : 0);  // operands, scales
+    static constexpr int RING = KS * NS * STAGE, SUMS = KS * BM * (BN + 4) * 4;
+    static constexpr int BYTES = RING > SUMS ? RING : SUMS;
+};
+
+template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int KS, int NS>
+__global__ __launch_bounds__(KS * 64)
+__attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS),
+                                   ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS))))
+void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
+    constexpr int TM = BM / 16, TN = BN / 16, QA = (TM + 3) / 4, QB = (TN + 3) / 4;
+    using L = RaggedWaveLds<MX, BM, BN, KS, NS>;
+    using PA = Panel<AT, BM, 1>;
+    using PB = Panel<BT, BN, 1>;
+    constexpr int LPW = PA::LP + PB::LP + (MX ? 2 : 0);
+    static_assert(L::BYTES <= 160 * 1024 && (!MX || (BM <= 64 && BN <= 64)),
+                  "LDS, one scale load per operand");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    RaggedTile t;
+    if (!ragged_tile<MX, AT, BT, BM, BN, false>(g, lane, t)) return;
+
+    PA A;
+    PB B;
+    A.init(t.a, g.lda, t.rows, t.k, t.rows * 2, 0, lane);
+    B.init(t.b, g.ldb, t.cols, BT && !AT ? g.K : t.k, t.cols * 2, 0, lane);
+    A.skip(wave);
+    B.skip(wave);
+    // Scales: 16 bytes of every row, of stage kt and its neighbour kt ^ 1.
+    const int nb = (g.K + 31) / 32;
+    const uint8_t *sa = nullptr, *sb = nullptr;
+    uint32_t va = 0, vb = 0;
+    if constexpr (MX) {
+        sa = uniform(g.sa + t.row0 * g.lsa);
+        sb = uniform(g.sb + t.g * g.bssb + (int64_t)t.n0 * g.lsb);
+        va = lane < t.rows ? (uint32_t)(lane * (int)g.lsa) : kOutOfRange;
+        vb = lane < t.cols ? (uint32_t)(lane * (int)g.lsb) : kOutOfRange;
+    }
+    uint8_t *const ring = smem + wave * (NS * L::STAGE);
+    auto load_stage = [&](int kt, uint8_t *d) {
+#pragma unroll
+        for (int i = 0; i < PA::LP; ++i) A.load(d, nullptr, i);
+#pragma unroll
+        for (int i = 0; i < PB::LP; ++i) B.load(d + PA::BYTES, nullptr, i);
+        if constexpr (MX) {
+            const uint32_t n = __builtin_amdgcn_readfirstlane(kt < t.KT ? kMaxRecords : 0);
+            dma16(sa + kt / 2 * 16, n, va, d + PA::BYTES + PB::BYTES);
+            dma16(sb + kt / 2 * 16, n, vb, d + PA::BYTES + PB::BYTES + 1024);
+        }
+        A.skip(KS);
+        B.skip(KS);
+    };
+
+    Frag<AT, BM> fa;
+    Frag<BT, BN> fb;
+    fa.init(lane, 0);
+    fb.init(lane, 0);
+    v4f acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
+
+    // (wr and sa differ: see ragged_kernel)
+    auto kstep = [&](int kt, uint8_t *__restrict__ wr, const uint8_t *__restrict__ s) {
+        wait_vmcnt<(NS - 2) * LPW>();
+        asm volatile("" ::: "memory");  // (no access moves over the wait)
+        load_stage(kt + (NS - 1) * KS, wr);
+        ScaleQuad xa[QA], xb[QB];
+        if constexpr (MX) {
+            const uint8_t *sc = s + PA::BYTES + PB::BYTES + (kt & 1) * 8;
+            read_scales<QA, BM>(sc, 0, nb - kt * 8, lane, xa);
+            read_scales<QB, BN>(sc + 1024, 0, nb - kt * 8, lane, xb);
+        }
+        auto half = [&](auto hh) {
+            constexpr int SS = decltype(hh)::value;
+            v4i af[TM], bf[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) bf[j] = fb.read(s + PA::BYTES, j, SS);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) af[i] = fa.read(s, i, SS);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = MX ? mx_half<SS>(bf[j], af[i], acc[i][j], xb[j / 4], xa[i / 4], i, j)
+                                   : bf_step(bf[j], af[i], acc[i][j]);
+        };
+        half(std::integral_constant<int, 0>{});
+        half(std::integral_constant<int, 1>{});
+    };
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load_stage(wave + i * KS, ring + i * L::STAGE);
+    int slot = 0;
+    for (int kt = wave; kt < t.KT; kt += KS) {
+        kstep(kt, ring + (slot == 0 ? NS - 1 : slot - 1) * L::STAGE, ring + slot * L::STAGE);
+        slot = slot == NS - 1 ? 0 : slot + 1;
+    }
+
+    wait_vmcnt<0>();
+    __syncthreads();
+    constexpr int LD = BN + 4, CH = chunk_of(E);
+    float *const sums = (float *)smem;
+    const int l16 = lane & 15, lq = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            *(v4f *)(sums + (wave * BM + i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i][j];
+    __syncthreads();
+#pragma unroll 1
+    for (int c = threadIdx.x; c < BM * BN / CH; c += KS * 64) {
+        const int row = c / (BN / CH), col = c % (BN / CH) * CH;
+        if (row >= t.rows || t.n0 + col >= g.N) continue;
+        v4f v[CH / 4] = {};
+#pragma unroll
+        for (int w = 0; w < KS; ++w)
+#pragma unroll
+            for (int i = 0; i < CH / 4; ++i)
+                v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
+        store_chunk<E>(ep, t.z, t.row0 + row, t.n0 + col, g.N, v);
+    }
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
@@ -821,30 +1003,99 @@ inline int64_t ragged_tiles(const RaggedArgs &g, int bm, int bn) {
     return tm * ((g.N + bn - 1) / bn);
 }
 
-// The tile shapes: BM x BN on WM x WN waves with NS stages in the ring, and the 256 x 256
-// kernel (NS == 0).
-template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS>
+// The kernels' tile shapes.
+// ring: BM x BN on WM x WN waves, NS stages; big: 256 x 256; wave: BM x BN, K split over KS
+// waves.
+template <int BM_, int BN_, int WM_, int WN_, int NS_>
+struct RingTile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, KIND = 0;
+};
+struct BigTile {
+    static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, NS = 0, KIND = 1;
+};
+template <int BM_, int BN_, int KS, int NS_>
+struct WaveTile {
+    static constexpr int BM = BM_, BN = BN_, WM = 1, WN = KS, NS = NS_, KIND = 2;
+};
+
+template <bool MX, bool AT, bool BT, EpiKind E, typename T>
 static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+    constexpr int BM = T::BM, BN = T::BN;
     // 32-bit offsets inside a panel, with the loads of rows past its edge
     const int64_t kbytes = MX ? (int64_t)(g.K + 31) / 32 * 16 : (int64_t)g.K * 2;
     if ((AT ? 64 : BM) * g.lda + kbytes > (int64_t)kMaxRecords ||
         (BT ? 64 * g.ldb + (int64_t)g.N * 2 : BN * g.ldb + kbytes) > (int64_t)kMaxRecords ||
         (MX && 64 * (g.lsa > g.lsb ? g.lsa : g.lsb) > (int64_t)kMaxRecords))
         return hipErrorInvalidValue;
-    const int64_t per = (int64_t)((g.K + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    const int64_t per =
+        (int64_t)((g.K + BM - 1) / BM) * ((g.N + BN - 1) / BN) * (AT ? g.splits : 1);
     if (AT && per > INT32_MAX - 8) return hipErrorInvalidValue;
     const int64_t tiles = AT ? (int64_t)g.G * wgrad_share((int)per) * 8
-                             : ragged_tiles(g, BM, BN) + (NS == 0 ? g.cus : 8);
+                             : ragged_tiles(g, BM, BN) + (T::KIND == 1 ? g.cus : 8);
     if (tiles > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid = ragged_grid(tiles), block(WM * WN * 64);
-    if constexpr (NS == 0) {
-        static_assert(BM == 256 && BN == 256 && WM == 2 && WN == 4, "the big tile");
+    const dim3 grid = ragged_grid(tiles), block(T::WM * T::WN * 64);
+    if constexpr (T::KIND == 1)
         hipLaunchKernelGGL((ragged_big_kernel<MX, AT, BT, E>), grid, block, 0, stream, g, ep);
-    } else {
-        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, WM, WN, NS>), grid, block, 0,
+    else if constexpr (T::KIND == 2)
+        hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, E, BM, BN, T::WN, T::NS>), grid, block, 0,
                            stream, g, ep);
-    }
+    else
+        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, T::WM, T::WN, T::NS>), grid, block,
+                           0, stream, g, ep);
     return hipGetLastError();
+}
+
+// Tiles of a forward product whose groups are alike.
+inline int64_t even_tiles(const RaggedArgs &g, int64_t avg, int bm, int bn) {
+    const int64_t groups = g.off ? (g.G < g.M ? g.G : g.M) : 1;
+    return groups * ((avg + bm - 1) / bm) * (((int64_t)g.N + bn - 1) / bn);
+}
+
+// The tile of a forward product, by the average rows of a group (the host does not know
+// more) and the tiles that makes.  Times in us, graph-timed with rotating weights, as
+// rows x groups x k x n with k-contiguous / n-contiguous bf16 / MXFP4 weights ("-": n/a).
+template <bool MX, bool BT, EpiKind E>
+static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+#define GK_GO(...) return ragged_go<MX, false, BT, E, __VA_ARGS__>(g, ep, stream)
+    const int64_t cus = g.cus;
+    const int64_t groups = g.off ? (g.G < g.M ? g.G : g.M) : 1;
+    const int64_t avg = (g.M + groups - 1) / groups;
+    const int64_t stages = ((MX ? (int64_t)g.K / 2 : (int64_t)g.K * 2) + 127) / 128;
+    if (avg <= 16) {
+        // One 16-row tile per group: the weights are read once, HBM-bound.  Where K is split
+        // over the waves nothing waits at barriers and a few tiles keep many loads in
+        // flight: 8x64x2048x1024 7.4 / 8.9 / 4.9 against 9.6 / 8.8 / 6.5 on the ring,
+        // 64x32x2048x4096 71 / 86 / 44 against 78 / 83 / 25.  It reads 64-byte pieces
+        // of n-contiguous rows (32 columns) and a scale load per stage, so those two
+        // layouts take it for few tiles only, and k of few stages never (128x100x512x600
+        // 15.4 / 17.1 / 16.9 against 11.1 / 12.5 / 7.0).
+        const int64_t few = even_tiles(g, avg, 16, 64);
+        if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16))
+            GK_GO(WaveTile<16, 32, 4, 3>);
+        // n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more: 64x32x2048x4096
+        // - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2 against
+        // - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few tiles)
+        if ((BT || (MX && avg > 4)) && even_tiles(g, avg, 64, 128) >= 2 * cus)
+            GK_GO(RingTile<64, 128, 2, 2, 3>);
+        GK_GO(RingTile<16, 64, 1, 4, 4>);
+    }
+    // Too few tiles for half of the CUs: K split over the waves.  500x2x8192x1024
+    // 34.7 / 33.7 / 12.5 against 35.4 / 36.0 / 16.8.
+    if (even_tiles(g, avg, 64, 64) <= cus / 2) GK_GO(WaveTile<64, 64, 4, 2>);
+    if (avg > 64) {
+        // 16384x8x4096x4096 487 / 475 / 182 against 531 / 522 / 206, one group of 4096x4096x4096
+        // 103 / 102 / 40 against 115 / 118 / 47; below two rounds of whole tiles the half
+        // tiles spread better: 8192x16x4096x2048 181 / 173 / 69 against 164 / 162 / 70.
+        const int64_t big = even_tiles(g, avg, 256, 256);
+        if (big >= 2 * cus || (groups == 1 && big <= cus && big * 4 >= cus * 3)) GK_GO(BigTile);
+        // 2048x16x4096x2048 73 / 68 / 26 against 89 / 86 / 34 with 64 x 128 tiles
+        if (even_tiles(g, avg, 128, 256) >= cus / 2) GK_GO(RingTile<128, 256, 2, 4, 3>);
+    }
+    // 4096x64x1024x1024 38 / 38 / 16 against 39 / 41 / 20 with 64 x 64 tiles;
+    // 1001x5x1504x776 (140 tiles) 12.7 / 12.8 / 8.3 against 10.2 / 10.7 / 7.3
+    if (even_tiles(g, avg, 64, 128) >= cus) GK_GO(RingTile<64, 128, 2, 2, 3>);
+    GK_GO(RingTile<64, 64, 2, 2, 4>);
+#undef GK_GO
 }
 
 }  // namespace gk

@@ -621,8 +621,9 @@ int gk_gemm_packed_a_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha,
  * knows, and of 4-bit block-scaled operands.  alpha and beta are f32 whatever
  * the output type; beta == 0 never reads C.  They run on the launch stream
  * like every other entry, can be captured into a HIP graph (the workspace holds
- * packed copies of operands that the kernels cannot read in place, and nothing
- * else), and give the same bits on every run.
+ * packed copies of operands that the kernels cannot read in place and, for a
+ * weight gradient of long groups over few tiles, partial sums), and give the
+ * same bits on every run.
  *
  * Groups: `offsets` holds groups + 1 row offsets on the DEVICE.  Group g has
  * the rows [s_g, s_{g+1}) with s_i = min(rows, max(0, offsets[0 .. i])): for

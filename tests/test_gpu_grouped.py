@@ -224,6 +224,31 @@ def test_wgrad(dev, sizes, k, n, out, c_lay, alpha, beta):
     run_wgrad(dev, offs(*sizes), sum(sizes) + 3, k, n, out, c_lay, alpha, beta)
 
 
+@pytest.mark.parametrize("sizes,k,n", [((9000,), 40, 72), ((0, 4500), 130, 264), ((70, 6100, 0), 24, 520),
+                                       ((4097, 4000), 264, 40)])
+@pytest.mark.parametrize("out,c_lay,alpha,beta", [(F32, "r", 1.0, 0.0), (BF16, "c+", -0.5, 1.0)])
+def test_wgrad_of_long_groups(dev, sizes, k, n, out, c_lay, alpha, beta):
+    """Row ranges per group, their partial sums added afterwards."""
+    run_wgrad(dev, offs(*sizes), sum(sizes) + 3, k, n, out, c_lay, alpha, beta)
+
+
+@pytest.mark.parametrize("layout", ["c", "r"])
+@pytest.mark.parametrize("k", [520, 1096, 4104])
+@pytest.mark.parametrize("sizes", [(1,), (3, 0, 1), (16, 5), (70, 30), (200,), (7, 0, 90, 64)])
+def test_long_k_on_few_tiles(dev, sizes, k, layout):
+    for n in (24, 200):
+        run_grouped(dev, offs(*sizes), sum(sizes) + 1, k, n, b_lay=layout, out=F32)
+
+
+@pytest.mark.parametrize("layout", ["c", "r"])
+@pytest.mark.parametrize("sizes,k,n", [((1400, 300, 800), 136, 2600), ((130,) * 40, 72, 1000),
+                                       ((40,) * 60, 200, 700), ((6,) * 100, 264, 1100),
+                                       ((2,) * 70, 1032, 1500), ((4096,), 72, 4096),
+                                       ((3000, 0, 2900, 100), 136, 4000)])
+def test_many_tiles(dev, sizes, k, n, layout):
+    run_grouped(dev, offs(*sizes), sum(sizes) + 1, k, n, b_lay=layout)
+
+
 @pytest.mark.parametrize("lays", ["r+ r", "r r+", "ro c", "m r", "c+ m"])
 def test_wgrad_operand_layouts(dev, lays):
     a_lay, b_lay = lays.split()

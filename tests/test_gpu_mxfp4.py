@@ -249,6 +249,20 @@ def test_grouped_product(dev, sizes, n, k, out, c_lay, alpha, beta):
     assert torch.equal(c.cpu()[mask], before.cpu()[mask])
 
 
+@pytest.mark.parametrize("sizes,n,k", [((1400, 300, 800), 2600, 160), ((130,) * 40, 1000, 288),
+                                       ((40,) * 60, 700, 400), ((6,) * 100, 1100, 520),
+                                       ((2,) * 70, 1500, 2080), ((3, 0, 1), 24, 8200),
+                                       ((200,), 136, 4100), ((3000, 0, 2900, 100), 4000, 288)])
+def test_grouped_tiles(dev, sizes, n, k):
+    test_grouped_product(dev, sizes, n, k, F32, "row", 1.0, 0.0)
+
+
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 288), (3000, 5000, 96), (300, 20000, 160),
+                                   (30, 9000, 1100), (8, 14336, 800)])
+def test_plain_tiles(dev, m, n, k):
+    test_product(dev, m, n, k, BF16, "row", 1.0, 0.0)
+
+
 def test_degenerate_products(dev):
     def product(m, n, k, alpha, beta):
         ca, cb = random_mx(max(m, 1), max(k, 1), 1), random_mx(max(n, 1), max(k, 1), 2)
