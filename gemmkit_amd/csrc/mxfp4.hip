@@ -9,8 +9,10 @@
 // which v_cvt_scalef32_pk_fp4_* computes from x and 2^e for two elements at a time.  A
 // block that holds a NaN or an infinity gets the scale byte 255, the format's NaN, and
 // zero codes.
-// Bound: HBM.  Four lanes hold a block, 16 bytes of bf16 (32 of f32) each, so a wave
-// reads 16 blocks of a row side by side and writes their 256 bytes of codes and 16 scales.
+// Bound: HBM.  Lanes hold 16 bytes of a row side by side, four (bf16) or eight (f32) of them
+// a block; their largest magnitude goes round by lane permutations.
+#include <algorithm>
+
 #include "ragged.h"
 
 namespace gk {
@@ -46,15 +48,44 @@ __device__ __forceinline__ int mx_byte(uint32_t top) {
     return e == 255 ? 255 : (e > 2 ? e - 2 : 0);
 }
 
+// Four (f32) or eight (bf16) consecutive values of a row from column k0 (zeros past its
+// end): 16 bytes.
+template <InType T, MxWalk W, int N>
+__device__ __forceinline__ void mx_read(const MxArgs &g, int64_t row, int64_t k0, float *v) {
+    if (W == MxWalk::Vec && k0 + N <= g.K) {
+        const v4i w = *(const v4i *)((const uint8_t *)g.x + (row * g.rs + k0) * (16 / N));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = __uint_as_float(N == 4 ? (uint32_t)w[i % 4]
+                                          : (uint32_t)w[i / 2 % 4] << (i % 2 ? 0 : 16) & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = k0 + i < g.K ? mx_load<T>(g.x, row * g.rs + (k0 + i) * g.cs) : 0.0f;
+    }
+}
+
+// A workgroup's four waves walk 2^wl segments of 16 blocks of each of its rows.
+struct MxGrid {
+    int64_t row, rows;  // this wave's first row, and how far to the next
+    int seg, lane;
+    __device__ __forceinline__ MxGrid(int wl) {
+        const int wave = threadIdx.x >> 6;
+        lane = threadIdx.x & 63;
+        row = ((int64_t)blockIdx.x << (2 - wl)) + (wave >> wl);
+        rows = (int64_t)gridDim.x << (2 - wl);
+        seg = ((int)blockIdx.y << wl) + (wave & ((1 << wl) - 1));
+    }
+};
+
 template <InType T, MxWalk W>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(const MxArgs g) {
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t waves = (int64_t)gridDim.x * 4;
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const MxArgs g, int wl) {
     const int64_t nb = (g.K + kMxBlock - 1) / kMxBlock;
     if constexpr (W == MxWalk::Rows) {
+        const int lane = threadIdx.x & 63;
         const int64_t bands = (g.rows + 63) / 64;
-        for (int64_t it = wave; it < bands * nb; it += waves) {
+        for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < bands * nb;
+             it += (int64_t)gridDim.x * 4) {
             const int64_t row = it % bands * 64 + lane, blk = it / bands;
             if (row >= g.rows) continue;
             float v[kMxBlock];
@@ -77,53 +108,57 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const MxArgs g) {
                 for (int64_t b = nb; b < (nb + 15) / 16 * 16; ++b) g.scales[row * g.lds + b] = 0;
         }
     } else {
-        const int64_t segs = (nb + 15) / 16;
-        for (int64_t it = wave; it < g.rows * segs; it += waves) {
-            const int64_t row = it / segs, blk = it % segs * 16 + (lane >> 2);
-            const int64_t k0 = blk * kMxBlock + (lane & 3) * 8;
-            float v[8];
-            if (W == MxWalk::Vec && k0 + 8 <= g.K) {
-                if constexpr (T == InType::BF16) {
-                    const v4i w = *(const v4i *)((const uint16_t *)g.x + row * g.rs + k0);
+        // A load of a wave is 1 KiB of the row: bf16 a segment's 16 blocks at four lanes each,
+        // f32 half of them at eight.
+        constexpr int N = T == InType::BF16 ? 8 : 4, LB = 32 / N, U = 8 / N;
+        const MxGrid w(wl);
+        if ((int64_t)w.seg * 16 >= nb) return;
+        for (int64_t row = w.row; row < g.rows; row += w.rows) {
+            float v[U][N];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = __uint_as_float((uint32_t)w[i / 2] << (i % 2 ? 0 : 16) & 0xFFFF0000u);
-                } else {
-                    const v4f *p = (const v4f *)((const float *)g.x + row * g.rs + k0);
-                    const v4f a = p[0], b = p[1];
+            for (int u = 0; u < U; ++u)
+                mx_read<T, W, N>(g, row, ((int64_t)w.seg * U + u) * 64 * N + w.lane * N, v[u]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = i < 4 ? a[i % 4] : b[i % 4];
+            for (int u = 0; u < U; ++u) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t m = __float_as_uint(v[u][i]) & 0x7FFFFFFFu;
+                    top = m > top ? m : top;
                 }
-            } else {
+                uint32_t o = __builtin_amdgcn_mov_dpp(top, 0xB1, 0xF, 0xF, true);  // lane ^ 1
+                top = o > top ? o : top;
+                o = __builtin_amdgcn_mov_dpp(top, 0x4E, 0xF, 0xF, true);           // lane ^ 2
+                top = o > top ? o : top;
+                if constexpr (LB == 8) {
+                    o = __builtin_amdgcn_mov_dpp(top, 0x141, 0xF, 0xF, true);      // 7 - lane % 8
+                    top = o > top ? o : top;
+                }
+                const int byte = mx_byte(top);
+                const float scale = mx_scale(byte);
+                const int64_t blk = ((int64_t)w.seg * U + u) * (64 / LB) + w.lane / LB;
+                uint32_t c = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = k0 + i < g.K ? mx_load<T>(g.x, row * g.rs + (k0 + i) * g.cs) : 0.0f;
+                for (int i = 0; i < N; i += 4) {
+                    uint32_t h = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v[u][i], v[u][i + 1], scale, 0);
+                    h = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(h, v[u][i + 2], v[u][i + 3], scale, 1);
+                    c |= h << (4 * i);
+                }
+                if (byte == 255) c = 0;
+                uint8_t *const at = g.codes + row * g.ld + blk * 16 + w.lane % LB * (N / 2);
+                if (blk < nb) {
+                    if constexpr (N == 8) *(uint32_t *)at = c;
+                    else *(uint16_t *)at = (uint16_t)c;
+                }
+                // (past the row's blocks: zeros, up to the row's 16 bytes)
+                if (w.lane % LB == 0) g.scales[row * g.lds + blk] = (uint8_t)byte;
             }
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t m = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-                top = m > top ? m : top;
-            }
-            uint32_t o = __builtin_amdgcn_mov_dpp(top, 0xB1, 0xF, 0xF, true);  // lane ^ 1
-            top = o > top ? o : top;
-            o = __builtin_amdgcn_mov_dpp(top, 0x4E, 0xF, 0xF, true);           // lane ^ 2
-            top = o > top ? o : top;
-            const int byte = mx_byte(top);
-            if (blk < nb)
-                *(uint32_t *)(g.codes + row * g.ld + blk * 16 + (lane & 3) * 4) =
-                    byte == 255 ? 0 : mx_codes8(v, mx_scale(byte));
-            // (past the row's blocks: zeros, up to the row's 16 bytes)
-            if ((lane & 3) == 0) g.scales[row * g.lds + blk] = (uint8_t)byte;
         }
     }
 }
 
 template <InType T, MxWalk W>
-__global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxArgs g) {
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t waves = (int64_t)gridDim.x * 4;
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxArgs g, int wl) {
     const int64_t nb = (g.K + kMxBlock - 1) / kMxBlock;
     auto decode = [](uint32_t w, int byte, float v[8]) {
         const float s = mx_scale(byte);
@@ -141,8 +176,10 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxArgs g) {
         else ((float *)g.x)[at] = v;
     };
     if constexpr (W == MxWalk::Rows) {
+        const int lane = threadIdx.x & 63;
         const int64_t bands = (g.rows + 63) / 64;
-        for (int64_t it = wave; it < bands * nb; it += waves) {
+        for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < bands * nb;
+             it += (int64_t)gridDim.x * 4) {
             const int64_t row = it % bands * 64 + lane, blk = it / bands;
             if (row >= g.rows) continue;
             const v4i w = *(const v4i *)(g.codes + row * g.ld + blk * 16);
@@ -159,11 +196,11 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxArgs g) {
             }
         }
     } else {
-        const int64_t segs = (nb + 15) / 16;
-        for (int64_t it = wave; it < g.rows * segs; it += waves) {
-            const int64_t row = it / segs, blk = it % segs * 16 + (lane >> 2);
-            const int64_t k0 = blk * kMxBlock + (lane & 3) * 8;
-            if (k0 >= g.K) continue;
+        const MxGrid at(wl);
+        const int lane = at.lane;
+        const int64_t blk = (int64_t)at.seg * 16 + (lane >> 2), k0 = blk * kMxBlock + (lane & 3) * 8;
+        if (k0 >= g.K) return;
+        for (int64_t row = at.row; row < g.rows; row += at.rows) {
             const uint32_t w = *(const uint32_t *)(g.codes + row * g.ld + blk * 16 + (lane & 3) * 4);
             float v[8];
             decode(w, g.scales[row * g.lds + blk], v);
@@ -188,14 +225,20 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxArgs g) {
 
 template <InType T, MxWalk W>
 static hipError_t mx_go(const MxArgs &g, bool quantize, hipStream_t stream) {
-    const int64_t nb = (g.K + kMxBlock - 1) / kMxBlock;
-    const int64_t items = W == MxWalk::Rows ? (g.rows + 63) / 64 * nb : g.rows * ((nb + 15) / 16);
-    const int64_t wgs = (items + 3) / 4;
-    const dim3 grid((uint32_t)(wgs < (1 << 20) ? wgs : (1 << 20)));
+    const int64_t nb = (g.K + kMxBlock - 1) / kMxBlock, segs = (nb + 15) / 16;
+    int wl = 0;
+    dim3 grid;
+    if (W == MxWalk::Rows) {
+        grid = dim3((uint32_t)std::min<int64_t>(((g.rows + 63) / 64 * nb + 3) / 4, 1 << 20));
+    } else {
+        wl = segs >= 4 ? 2 : segs >= 2 ? 1 : 0;
+        const int64_t wgs = (g.rows + (4 >> wl) - 1) >> (2 - wl);
+        grid = dim3((uint32_t)std::min<int64_t>(wgs, 1 << 20), (uint32_t)((segs + (1 << wl) - 1) >> wl));
+    }
     if (quantize)
-        hipLaunchKernelGGL((mx_quantize_kernel<T, W>), grid, dim3(256), 0, stream, g);
+        hipLaunchKernelGGL((mx_quantize_kernel<T, W>), grid, dim3(256), 0, stream, g, wl);
     else
-        hipLaunchKernelGGL((mx_dequantize_kernel<T, W>), grid, dim3(256), 0, stream, g);
+        hipLaunchKernelGGL((mx_dequantize_kernel<T, W>), grid, dim3(256), 0, stream, g, wl);
     return hipGetLastError();
 }
 
