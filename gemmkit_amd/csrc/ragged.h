@@ -181,9 +181,20 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
     return (const uint8_t *)((uint64_t)hi << 32 | lo);
 }
 
+// dma16 (mma_kernel.h); ONCE: nontemporally, the caches keep nothing of it.
+template <bool ONCE>
+__device__ __forceinline__ void load16(const uint8_t *base, uint32_t num, uint32_t voff,
+                                       uint8_t *lds) {
+    constexpr int kNt = 2;  // the instruction's nt bit
+    __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)num, kRsrcWord3);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16,
+                                             voff, 0, 0, ONCE ? kNt : 0);
+}
+
 // One operand of a tile: W rows (or columns, TR) of it, filled by NW waves.  Stages are
 // loaded in order; `base`, `num` and `left` move on with them.
-template <bool TR, int W, int NW>
+template <bool TR, int W, int NW, bool ONCE = false>
 struct Panel {
     static constexpr int BYTES = W * 128;             // of a stage, either layout
     static constexpr int NI = BYTES / 1024;           // load instructions per stage
@@ -231,13 +242,13 @@ struct Panel {
         uint32_t v = PAIR ? vo[i % 2] + (uint32_t)(i / 2 * 2 * RPI * ld) : vo[i];
         if constexpr (TR) {
             // (rows at and past the end read zeros: their offsets reach left * ld)
-            dma16(base, size(), v, d);
+            load16<ONCE>(base, size(), v, d);
         } else {
             if (left < 128) {  // the K tail's chunks read zeros
                 const int slot = (wave * LP + i) * 64 + lane;
                 if (((slot % 8) ^ swz_of<128>(slot / 8)) * 16 >= left) v = kOutOfRange;
             }
-            dma16(base, size(), v, d);
+            load16<ONCE>(base, size(), v, d);
         }
     }
     // The resource's size for the next stage.
@@ -475,7 +486,9 @@ __device__ __forceinline__ v4f mx_half(v4i b, v4i a, v4f c, const ScaleQuad &y, 
 // Elements a lane stores at once: 16 bytes.
 constexpr int chunk_of(EpiKind e) { return e == EpiKind::BF16 ? 8 : 4; }
 
-// A chunk of one row of C.  bf16 takes 16 bytes here instead of store4's 8: a weight
+// A chunk of one row of C, stored nontemporally: written through the L2 the output pushes the
+// operand panels out of it (weight gradient 16384x8x4096x4096 with f32 output 512 against 443
+// us).  bf16 takes 16 bytes here instead of store4's 8: a weight
 // gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16 from 64 rows: 21.8 us
 // with 8 bytes a lane).
 template <EpiKind E>
@@ -507,7 +520,7 @@ __device__ __forceinline__ void store_chunk(const EpiParams &ep, int64_t z, int 
 #pragma unroll
     for (int i = 0; i < chunk_of(E) / 4; ++i) {
         const float w[4] = {v[i][0], v[i][1], v[i][2], v[i][3]};
-        if (col + 4 * i < N) store4<E, float, StPol::Plain>(ep, z, row, col + 4 * i, N, w);
+        if (col + 4 * i < N) store4<E, float, StPol::NT>(ep, z, row, col + 4 * i, N, w);
     }
 }
 
@@ -543,7 +556,7 @@ __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTi
 
 // ---------------------------------------------------------------- small tiles
 
-template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS>
+template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS, bool ONCE>
 __global__ __launch_bounds__(WM * WN * 64)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedLds<MX, BM, BN, NS>::BYTES, WM * WN),
                                    ragged_waves(RaggedLds<MX, BM, BN, NS>::BYTES, WM * WN))))
@@ -555,7 +568,7 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
     constexpr int QA = (TM + 3) / 4, QB = (TN + 3) / 4;
     using L = RaggedLds<MX, BM, BN, NS>;
     using PA = Panel<AT, BM, NW>;
-    using PB = Panel<BT, BN, NW>;
+    using PB = Panel<BT, BN, NW, ONCE>;
     using SP = ScalePanel<BM, BN>;
     constexpr int LPW = PA::LP + PB::LP;  // loads per wave and stage (without scales)
     static_assert(L::BYTES <= 160 * 1024 && NW * 16 * (WTN + 4) * 4 <= L::BYTES, "LDS");
@@ -869,7 +882,7 @@ struct RaggedWaveLds {
     static constexpr int BYTES = RING > SUMS ? RING : SUMS;
 };
 
-template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int KS, int NS>
+template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int KS, int NS, bool ONCE>
 __global__ __launch_bounds__(KS * 64)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS),
                                    ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS))))
@@ -877,7 +890,7 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
     constexpr int TM = BM / 16, TN = BN / 16, QA = (TM + 3) / 4, QB = (TN + 3) / 4;
     using L = RaggedWaveLds<MX, BM, BN, KS, NS>;
     using PA = Panel<AT, BM, 1>;
-    using PB = Panel<BT, BN, 1>;
+    using PB = Panel<BT, BN, 1, ONCE>;
     constexpr int LPW = PA::LP + PB::LP + (MX ? 2 : 0);
     static_assert(L::BYTES <= 160 * 1024 && (!MX || (BM <= 64 && BN <= 64)),
                   "LDS, one scale load per operand");
@@ -1005,17 +1018,20 @@ inline int64_t ragged_tiles(const RaggedArgs &g, int bm, int bn) {
 
 // The kernels' tile shapes.
 // ring: BM x BN on WM x WN waves, NS stages; big: 256 x 256; wave: BM x BN, K split over KS
-// waves.
-template <int BM_, int BN_, int WM_, int WN_, int NS_>
+// waves.  ONCE: B nontemporally.
+template <int BM_, int BN_, int WM_, int WN_, int NS_, bool ONCE_ = false>
 struct RingTile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, KIND = 0;
+    static constexpr bool ONCE = ONCE_;
 };
 struct BigTile {
     static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, NS = 0, KIND = 1;
+    static constexpr bool ONCE = false;
 };
-template <int BM_, int BN_, int KS, int NS_>
+template <int BM_, int BN_, int KS, int NS_, bool ONCE_ = false>
 struct WaveTile {
     static constexpr int BM = BM_, BN = BN_, WM = 1, WN = KS, NS = NS_, KIND = 2;
+    static constexpr bool ONCE = ONCE_;
 };
 
 template <bool MX, bool AT, bool BT, EpiKind E, typename T>
@@ -1037,11 +1053,11 @@ static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
     if constexpr (T::KIND == 1)
         hipLaunchKernelGGL((ragged_big_kernel<MX, AT, BT, E>), grid, block, 0, stream, g, ep);
     else if constexpr (T::KIND == 2)
-        hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, E, BM, BN, T::WN, T::NS>), grid, block, 0,
+        hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, E, BM, BN, T::WN, T::NS, T::ONCE>), grid, block, 0,
                            stream, g, ep);
     else
-        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, T::WM, T::WN, T::NS>), grid, block,
-                           0, stream, g, ep);
+        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, T::WM, T::WN, T::NS, T::ONCE>), grid,
+                           block, 0, stream, g, ep);
     return hipGetLastError();
 }
 
@@ -1057,10 +1073,19 @@ inline int64_t even_tiles(const RaggedArgs &g, int64_t avg, int bm, int bn) {
 template <bool MX, bool BT, EpiKind E>
 static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
 #define GK_GO(...) return ragged_go<MX, false, BT, E, __VA_ARGS__>(g, ep, stream)
+#define GK_GO_ONCE(...) \
+    if (once) GK_GO(__VA_ARGS__, true>); \
+    GK_GO(__VA_ARGS__>)
     const int64_t cus = g.cus;
     const int64_t groups = g.off ? (g.G < g.M ? g.G : g.M) : 1;
     const int64_t avg = (g.M + groups - 1) / groups;
-    const int64_t stages = ((MX ? (int64_t)g.K / 2 : (int64_t)g.K * 2) + 127) / 128;
+    const int64_t kbytes = MX ? (int64_t)g.K / 2 : (int64_t)g.K * 2, stages = (kbytes + 127) / 128;
+    // Weights that tiles of 64 rows read once, and that would fill half of the 256 MB
+    // Infinity Cache, go past it: 64x32x2048x4096 72.7 / 73.3 / 24.6 against 65.6 / 66.0 / 22.6,
+    // 16x8x4096x11008 107 / 124 / 33.9 against 96 / 113 / 31.6.  Smaller ones stay there from
+    // one call to the next, and are read again by every further tile: 150x3x2048x2048
+    // 11.3 / 11.6 / 6.7 against 13.6 / 15.2 / 7.1 nontemporally.
+    const bool once = avg <= 64 && groups * g.N * kbytes >= (int64_t(128) << 20);
     if (avg <= 16) {
         // One 16-row tile per group: the weights are read once, HBM-bound.  Where K is split
         // over the waves nothing waits at barriers and a few tiles keep many loads in
@@ -1071,13 +1096,16 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         // 15.4 / 17.1 / 16.9 against 11.1 / 12.5 / 7.0).
         const int64_t few = even_tiles(g, avg, 16, 64);
         if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16))
-            GK_GO(WaveTile<16, 32, 4, 3>);
+            {
+            GK_GO_ONCE(WaveTile<16, 32, 4, 3);
+        }
         // n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more: 64x32x2048x4096
         // - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2 against
         // - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few tiles)
-        if ((BT || (MX && avg > 4)) && even_tiles(g, avg, 64, 128) >= 2 * cus)
-            GK_GO(RingTile<64, 128, 2, 2, 3>);
-        GK_GO(RingTile<16, 64, 1, 4, 4>);
+        if ((BT || (MX && avg > 4)) && even_tiles(g, avg, 64, 128) >= 2 * cus) {
+            GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
+        }
+        GK_GO_ONCE(RingTile<16, 64, 1, 4, 4);
     }
     // Too few tiles for half of the CUs: K split over the waves.  500x2x8192x1024
     // 34.7 / 33.7 / 12.5 against 35.4 / 36.0 / 16.8.
@@ -1093,8 +1121,11 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
     }
     // 4096x64x1024x1024 38 / 38 / 16 against 39 / 41 / 20 with 64 x 64 tiles;
     // 1001x5x1504x776 (140 tiles) 12.7 / 12.8 / 8.3 against 10.2 / 10.7 / 7.3
-    if (even_tiles(g, avg, 64, 128) >= cus) GK_GO(RingTile<64, 128, 2, 2, 3>);
-    GK_GO(RingTile<64, 64, 2, 2, 4>);
+    if (even_tiles(g, avg, 64, 128) >= cus) {
+        GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
+    }
+    GK_GO_ONCE(RingTile<64, 64, 2, 2, 4);
+#undef GK_GO_ONCE
 #undef GK_GO
 }
 
