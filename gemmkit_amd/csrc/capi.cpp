@@ -2173,6 +2173,12 @@ bool ragged_in_place(const Opnd &o, int64_t R, int64_t K, int64_t batch) {
            (R <= 1 || o.rs >= K);
 }
 
+// R rows of K with unit stride, 16 bytes or more each, at any alignment.
+bool ragged_unit_rows(const Opnd &o, int64_t R, int64_t K) {
+    return K >= 8 && o.ks == 1 && K * 2 + 16 <= kMaxRaggedRow &&
+           (R <= 1 || (o.rs >= K && o.rs * 2 <= kMaxRaggedRow));
+}
+
 // Row stride in bytes of an operand read in place (one row: its own length).
 int64_t ragged_ld(const Opnd &o, int64_t R, int64_t K) {
     return R <= 1 ? round_up64(K * 2, 16) : o.rs * 2;
@@ -2240,40 +2246,6 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     const int64_t K = alpha == 0.0f ? 0 : (int64_t)a->cols;  // (then nothing of A and B is read)
     if (M == 0 || N == 0 || G == 0) return ok();
 
-    // B_g is read as N rows of K or as K rows of N.
-    Opnd A{a->data, a->rs, a->cs, 0};
-    Opnd Br{b->data, b->cs, b->rs, G > 1 ? b_gs : 0}, Bc{b->data, b->rs, b->cs, G > 1 ? b_gs : 0};
-    RaggedB bl = RaggedB::Rows;
-    int64_t lda = 0, ldb = 0, bs = 0;
-    if (K > 0) {
-        const bool a_ok = ragged_in_place(A, M, K, 1);
-        const bool rows_ok = ragged_in_place(Br, N, K, G);
-        bool cols_ok = !rows_ok && ragged_in_place(Bc, K, N, G);
-        if (!a_ok || (!rows_ok && !cols_ok)) {
-            const bool b_pack = !rows_ok && !cols_ok;
-            // n-contiguous rows that only lack alignment are copied as they are, without
-            // a transposition (5 x 1501 x 777: 12.4 us transposed)
-            cols_ok = cols_ok || (b_pack && Bc.ks == 1 && N * 2 + 16 <= kMaxRaggedRow);
-            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-            const size_t pb = !b_pack ? 0
-                              : cols_ok ? pack_bytes(InType::BF16, K, N, G, Bc)
-                                        : pack_bytes(InType::BF16, N, K, G, Br);
-            void *buf = nullptr;
-            if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
-            uint8_t *const dst = (uint8_t *)buf + pa;
-            PackJob jobs[2];
-            int nj = 0;
-            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
-            if (pb)
-                jobs[nj++] = cols_ok ? pack_job(InType::BF16, &Bc, K, N, G, dst)
-                                     : pack_job(InType::BF16, &Br, N, K, G, dst);
-            if ((r = pack_groups(jobs, nj))) return r;
-        }
-        bl = cols_ok ? RaggedB::Cols : RaggedB::Rows;
-        lda = ragged_ld(A, M, K);
-        ldb = cols_ok ? ragged_ld(Bc, K, N) : ragged_ld(Br, N, K);
-        bs = (cols_ok ? Bc.bs : Br.bs) * 2;
-    }
     EpiParams ep = epi_float(kind, alpha, beta);
     ep.c = c->data;
     ep.rsc = c->rs;
@@ -2282,16 +2254,53 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     RaggedArgs g{};
     g.cus = g_num_cus;
     g.splits = 1;
-    g.a = A.p;
-    g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
-    g.lda = lda;
-    g.ldb = ldb;
-    g.bsb = bs;
     g.off = offsets;
     g.G = (int32_t)G;
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
+    // B_g is read as N rows of K or as K rows of N.
+    Opnd A{a->data, a->rs, a->cs, 0};
+    Opnd Br{b->data, b->cs, b->rs, G > 1 ? b_gs : 0}, Bc{b->data, b->rs, b->cs, G > 1 ? b_gs : 0};
+    RaggedB bl = RaggedB::Rows;
+    if (K > 0) {
+        const bool a_ok = ragged_in_place(A, M, K, 1);
+        const bool rows_ok = ragged_in_place(Br, N, K, G);
+        bool cols_ok = !rows_ok && ragged_in_place(Bc, K, N, G);
+        // Rows of unit stride that only lack alignment are read as they are by a kernel of
+        // their own, or copied row by row.
+        const bool rows_any = ragged_unit_rows(Br, N, K), cols_any = ragged_unit_rows(Bc, K, N);
+        if (!a_ok || (!rows_ok && !cols_ok)) {
+            g.any_align = ragged_unit_rows(A, M, K) && (rows_any || cols_any) &&
+                          grouped_takes_any_align(g, rows_any ? RaggedB::Rows : RaggedB::Cols);
+            if (g.any_align) {
+                cols_ok = !rows_any;
+            } else {
+                const bool b_pack = !rows_ok && !cols_ok;
+                cols_ok = cols_ok || (b_pack && cols_any);
+                const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+                const size_t pb = !b_pack ? 0
+                                  : cols_ok ? pack_bytes(InType::BF16, K, N, G, Bc)
+                                            : pack_bytes(InType::BF16, N, K, G, Br);
+                void *buf = nullptr;
+                if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
+                uint8_t *const dst = (uint8_t *)buf + pa;
+                PackJob jobs[2];
+                int nj = 0;
+                if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
+                if (pb)
+                    jobs[nj++] = cols_ok ? pack_job(InType::BF16, &Bc, K, N, G, dst)
+                                         : pack_job(InType::BF16, &Br, N, K, G, dst);
+                if ((r = pack_groups(jobs, nj))) return r;
+            }
+        }
+        bl = cols_ok ? RaggedB::Cols : RaggedB::Rows;
+        g.lda = ragged_ld(A, M, K);
+        g.ldb = cols_ok ? ragged_ld(Bc, K, N) : ragged_ld(Br, N, K);
+        g.bsb = (cols_ok ? Bc.bs : Br.bs) * 2;
+    }
+    g.a = A.p;
+    g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
     const hipError_t e = launch_grouped_bf16(g, bl, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "grouped gemm");
     return finish("grouped gemm");
@@ -2354,7 +2363,10 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     g.splits = wgrad_splits(g);
     uint8_t *part = nullptr;
     if (M > 0) {
-        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
+        bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
+        g.any_align = (!a_ok || !b_ok) && ragged_unit_rows(A, M, K) && ragged_unit_rows(B, M, N) &&
+                      wgrad_takes_any_align(g);
+        if (g.any_align) a_ok = b_ok = true;
         const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
         const size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
         const size_t sums = g.splits > 1 ? (size_t)g.splits * groups * K * N * 4 : 0;

@@ -254,9 +254,15 @@ struct RaggedArgs {
     // wgrad: row ranges per group (1 = whole groups).  Range r of group g writes its sums
     // to batch element g*splits + r of C, in whole stages of 64 rows.
     int32_t splits;
+    // bf16: the operands' rows are unit-stride, 16 bytes or more, at any alignment
+    int32_t any_align;
 };
 // B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
 enum class RaggedB : int { Rows = 0, Cols = 1 };
+// Whether a forward product whose operands lack the alignment should be given them as they
+// are (any_align) rather than aligned copies.
+bool grouped_takes_any_align(const RaggedArgs &g, RaggedB bl);
+bool wgrad_takes_any_align(const RaggedArgs &g);
 hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
                                hipStream_t stream);
 int wgrad_splits(const RaggedArgs &g);  // what a product should be given

@@ -875,6 +875,33 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
 // workgroup share one BM x BN tile and split K among them, stage kt to wave kt % KS.  Each
 // wave fills its own ring of NS stages and waits for nothing but its own loads (no
 // barriers); their sums are added in wave order through LDS at the end.
+template <EpiKind E, int BM, int BN, int KS, int TM, int TN>
+__device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile &t, int N,
+                                          const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                          int lane) {
+    constexpr int LD = BN + 4, CH = chunk_of(E);
+    float *const sums = (float *)smem;
+    const int l16 = lane & 15, lq = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            *(v4f *)(sums + (wave * BM + i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i][j];
+    __syncthreads();
+#pragma unroll 1
+    for (int c = threadIdx.x; c < BM * BN / CH; c += KS * 64) {
+        const int row = c / (BN / CH), col = c % (BN / CH) * CH;
+        if (row >= t.rows || t.n0 + col >= N) continue;
+        v4f v[CH / 4] = {};
+#pragma unroll
+        for (int w = 0; w < KS; ++w)
+#pragma unroll
+            for (int i = 0; i < CH / 4; ++i)
+                v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
+        store_chunk<E>(ep, t.z, t.row0 + row, t.n0 + col, N, v);
+    }
+}
+
 template <bool MX, int BM, int BN, int KS, int NS>
 struct RaggedWaveLds {
     static constexpr int STAGE = (BM + BN) * 128 + (MX ? 2048 : 0);  // operands, scales
@@ -980,27 +1007,225 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
 
     wait_vmcnt<0>();
     __syncthreads();
-    constexpr int LD = BN + 4, CH = chunk_of(E);
-    float *const sums = (float *)smem;
-    const int l16 = lane & 15, lq = lane >> 4;
+    wave_sums<E, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+}
+
+// ---------------------------------------------------------------- operands of any alignment
+
+// Rows that miss the 16-byte alignment of the direct-to-LDS loads (an odd k or n) go
+// through registers: 16-byte loads at any address, two stages ahead, written to the stage's
+// slots.  Several workgroups on a CU, whose small rings leave the LDS room for, keep the
+// loads in flight that a deep ring would.
+template <bool TR, int W, int NW>
+struct RegPanel {
+    static constexpr int BYTES = W * 128, NI = BYTES / 1024, LP = (NI + NW - 1) / NW;
+    const uint8_t *base;  // of the next stage
+    int ld, left;         // row stride in bytes; contraction left: bytes, or rows (TR)
+    int lim;              // rows of the tile; TR: bytes of its columns that are in the matrix
+    int wave, lane;
+
+    __device__ __forceinline__ void init(const uint8_t *b, int64_t ld_, int k, int lim_, int wave_,
+                                         int lane_) {
+        base = uniform(b);
+        ld = (int)ld_;
+        left = k;
+        lim = lim_;
+        wave = wave_;
+        lane = lane_;
+    }
+    __device__ __forceinline__ bool mine(int i) const { return NI % NW == 0 || wave * LP + i < NI; }
+    __device__ __forceinline__ void load(v4i (&r)[LP]) {
+        typedef int v4i_any2 __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const int at = (wave * LP + i) * 64 + lane;  // 16-byte slot of the stage
+            int row, ch, valid;                          // valid: bytes of the chunk that exist
+            if constexpr (TR) {
+                row = at / (W / 8);
+                const int slot = at % (W / 8);
+                ch = ((((slot >> 1) ^ tr_unit<W>(row)) << 1) | (slot & 1)) * 16;
+                valid = row < left ? lim - ch : 0;
+            } else {
+                row = at / 8;
+                ch = ((at % 8) ^ swz_of<128>(row)) * 16;
+                valid = row < lim ? left - ch : 0;
+            }
+            v4i v = {};
+            if (mine(i) && valid > 0) {
+                // A chunk across the row's end is read back from that end (rows have 16
+                // bytes or more) and shifted.
+                const int cut = valid < 16 ? 16 - valid : 0;
+                const int64_t off = (int64_t)row * ld + ch - cut;
+                v = *(const v4i_any2 *)(base + off);
+                if (cut) {
+                    typedef uint64_t v2l __attribute__((ext_vector_type(2)));
+                    v2l w = __builtin_bit_cast(v2l, v);
+                    const int s = cut * 8;  // 16 .. 112
+                    w[0] = s >= 64 ? w[1] >> (s - 64) : w[0] >> s | w[1] << (64 - s);
+                    w[1] = s >= 64 ? 0 : w[1] >> s;
+                    v = __builtin_bit_cast(v4i, w);
+                }
+            }
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void skip(int stages) {
+        base += TR ? (int64_t)stages * 64 * ld : stages * 128;
+        left -= stages * (TR ? 64 : 128);
+    }
+    __device__ __forceinline__ void store(const v4i (&r)[LP], uint8_t *dst) const {
+#pragma unroll
+        for (int i = 0; i < LP; ++i)
+            if (mine(i)) *(v4i *)(dst + (wave * LP + i) * 1024 + lane * 16) = r[i];
+    }
+};
+
+template <bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64)
+void ragged_reg_kernel(const RaggedArgs g, const EpiParams ep) {
+    constexpr int NW = WM * WN;
+    constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
+    using PA = RegPanel<AT, BM, NW>;
+    using PB = RegPanel<BT, BN, NW>;
+    constexpr int STAGE = PA::BYTES + PB::BYTES, SUMS = NW * 16 * (WTN + 4) * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE > SUMS ? 2 * STAGE : SUMS];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    RaggedTile t;
+    if (!ragged_tile<false, AT, BT, BM, BN, false>(g, lane, t)) return;
+    // (t.k is rounded up to 16 bytes, for rows that are padded)
+    const int kb = AT ? t.k : g.K * 2;
+    PA A;
+    PB B;
+    A.init(t.a, g.lda, kb, AT ? t.rows * 2 : t.rows, wave, lane);
+    B.init(t.b, g.ldb, BT && !AT ? g.K : kb, BT ? t.cols * 2 : t.cols, wave, lane);
+
+    Frag<AT, BM> fa;
+    Frag<BT, BN> fb;
+    fa.init(lane, wm * WTM);
+    fb.init(lane, wn * WTN);
+    v4f acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-            *(v4f *)(sums + (wave * BM + i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i][j];
-    __syncthreads();
-#pragma unroll 1
-    for (int c = threadIdx.x; c < BM * BN / CH; c += KS * 64) {
-        const int row = c / (BN / CH), col = c % (BN / CH) * CH;
-        if (row >= t.rows || t.n0 + col >= g.N) continue;
-        v4f v[CH / 4] = {};
+        for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
+
+    v4i ra[2][PA::LP], rb[2][PB::LP];
+    auto get = [&](int set) {
+        A.load(ra[set]);
+        B.load(rb[set]);
+        A.skip(1);
+        B.skip(1);
+    };
+    auto put = [&](int set, uint8_t *d) {
+        A.store(ra[set], d);
+        B.store(rb[set], d + PA::BYTES);
+        get(set);
+    };
+    // Stage kt from slot PAR; stage kt+1, in registers, goes to the other one, and the loads
+    // of stage kt+3 take its registers.
+    auto kstep = [&](auto par) {
+        constexpr int PAR = decltype(par)::value;
+        const uint8_t *const sa = smem + PAR * STAGE, *const sb = sa + PA::BYTES;
+        put(1 - PAR, smem + (1 - PAR) * STAGE);
 #pragma unroll
-        for (int w = 0; w < KS; ++w)
+        for (int ss = 0; ss < 2; ++ss) {
+            v4i af[TM], bf[TN];
 #pragma unroll
-            for (int i = 0; i < CH / 4; ++i)
-                v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
-        store_chunk<E>(ep, t.z, t.row0 + row, t.n0 + col, g.N, v);
+            for (int j = 0; j < TN; ++j) bf[j] = fb.read(sb, j, ss);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) af[i] = fa.read(sa, i, ss);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = bf_step(bf[j], af[i], acc[i][j]);
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's writes and reads
+        stage_barrier();
+    };
+    get(0);
+    get(1);
+    put(0, smem);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    stage_barrier();
+    for (int kt = 0; kt < t.KT; kt += 2) {
+        kstep(std::integral_constant<int, 0>{});
+        if (kt + 1 < t.KT) kstep(std::integral_constant<int, 1>{});
     }
+    __syncthreads();
+    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+}
+
+// The same with K split over the KS waves of a workgroup (see ragged_wave_kernel): a wave's
+// stages go through a slot of its own, so it waits for its own loads only.
+template <bool AT, bool BT, EpiKind E, int BM, int BN, int KS>
+__global__ __launch_bounds__(KS * 64)
+void ragged_reg_wave_kernel(const RaggedArgs g, const EpiParams ep) {
+    constexpr int TM = BM / 16, TN = BN / 16;
+    using PA = RegPanel<AT, BM, 1>;
+    using PB = RegPanel<BT, BN, 1>;
+    constexpr int STAGE = PA::BYTES + PB::BYTES, SUMS = KS * BM * (BN + 4) * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[KS * STAGE > SUMS ? KS * STAGE : SUMS];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    RaggedTile t;
+    if (!ragged_tile<false, AT, BT, BM, BN, false>(g, lane, t)) return;
+    const int kb = AT ? t.k : g.K * 2;
+    PA A;
+    PB B;
+    A.init(t.a, g.lda, kb, AT ? t.rows * 2 : t.rows, 0, lane);
+    B.init(t.b, g.ldb, BT && !AT ? g.K : kb, BT ? t.cols * 2 : t.cols, 0, lane);
+    A.skip(wave);
+    B.skip(wave);
+    uint8_t *const sa = smem + wave * STAGE, *const sb = sa + PA::BYTES;
+
+    Frag<AT, BM> fa;
+    Frag<BT, BN> fb;
+    fa.init(lane, 0);
+    fb.init(lane, 0);
+    v4f acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
+    v4i ra[2][PA::LP], rb[2][PB::LP];
+    auto get = [&](int set) {
+        A.load(ra[set]);
+        B.load(rb[set]);
+        A.skip(KS);
+        B.skip(KS);
+    };
+    auto kstep = [&](auto par) {
+        constexpr int PAR = decltype(par)::value;
+        A.store(ra[PAR], sa);
+        B.store(rb[PAR], sb);
+        get(PAR);
+        asm volatile("" ::: "memory");  // (a wave's LDS accesses take effect in order)
+#pragma unroll
+        for (int ss = 0; ss < 2; ++ss) {
+            v4i af[TM], bf[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) bf[j] = fb.read(sb, j, ss);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) af[i] = fa.read(sa, i, ss);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = bf_step(bf[j], af[i], acc[i][j]);
+        }
+        asm volatile("" ::: "memory");
+    };
+    get(0);
+    get(1);
+    for (int kt = wave; kt < t.KT; kt += 2 * KS) {
+        kstep(std::integral_constant<int, 0>{});
+        if (kt + KS < t.KT) kstep(std::integral_constant<int, 1>{});
+    }
+    __syncthreads();
+    wave_sums<E, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
@@ -1034,6 +1259,19 @@ struct WaveTile {
     static constexpr bool ONCE = ONCE_;
 };
 
+// reg: operands of any alignment.
+template <int BM_, int BN_, int WM_, int WN_>
+struct RegTile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = 0, KIND = 3;
+    static constexpr bool ONCE = false;
+};
+
+template <int BM_, int BN_, int KS>
+struct RegWaveTile {
+    static constexpr int BM = BM_, BN = BN_, WM = 1, WN = KS, NS = 0, KIND = 4;
+    static constexpr bool ONCE = false;
+};
+
 template <bool MX, bool AT, bool BT, EpiKind E, typename T>
 static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     constexpr int BM = T::BM, BN = T::BN;
@@ -1055,6 +1293,12 @@ static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
     else if constexpr (T::KIND == 2)
         hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, E, BM, BN, T::WN, T::NS, T::ONCE>), grid, block, 0,
                            stream, g, ep);
+    else if constexpr (T::KIND == 3)
+        hipLaunchKernelGGL((ragged_reg_kernel<AT, BT, E, BM, BN, T::WM, T::WN>), grid, block, 0,
+                           stream, g, ep);
+    else if constexpr (T::KIND == 4)
+        hipLaunchKernelGGL((ragged_reg_wave_kernel<AT, BT, E, BM, BN, T::WN>), grid, block, 0, stream,
+                           g, ep);
     else
         hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, T::WM, T::WN, T::NS, T::ONCE>), grid,
                            block, 0, stream, g, ep);

@@ -249,6 +249,22 @@ def test_many_tiles(dev, sizes, k, n, layout):
     run_grouped(dev, offs(*sizes), sum(sizes) + 1, k, n, b_lay=layout)
 
 
+@pytest.mark.parametrize("lays", ["ro co", "ro ro", "m rm", "r+ ro", "ro c+", "m c"])
+@pytest.mark.parametrize("sizes", [(1, 0, 3), (16, 40, 0, 64), (200, 90), (7,) * 60, (130,) * 40])
+@pytest.mark.parametrize("k,n", [(9, 15), (8, 8), (201, 137), (1031, 65), (66, 1101), (7, 40), (40, 7)])
+def test_rows_of_any_alignment(dev, lays, sizes, k, n):
+    a_lay, b_lay = lays.split()
+    run_grouped(dev, offs(*sizes), sum(sizes) + 2, k, n, a_lay=a_lay, b_lay=b_lay, out=F32)
+
+
+@pytest.mark.parametrize("lays", ["ro ro", "m r", "r ro"])
+@pytest.mark.parametrize("sizes", [(1, 0, 3), (64, 65, 0, 1), (300, 0, 128, 700)])
+@pytest.mark.parametrize("k,n", [(9, 15), (73, 137), (265, 301), (8, 9), (7, 9), (41, 521)])
+def test_wgrad_rows_of_any_alignment(dev, lays, sizes, k, n):
+    a_lay, b_lay = lays.split()
+    run_wgrad(dev, offs(*sizes), sum(sizes) + 3, k, n, BF16, "ro", 1.0, 0.0, a_lay, b_lay)
+
+
 @pytest.mark.parametrize("lays", ["r+ r", "r r+", "ro c", "m r", "c+ m"])
 def test_wgrad_operand_layouts(dev, lays):
     a_lay, b_lay = lays.split()
