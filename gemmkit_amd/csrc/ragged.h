@@ -23,6 +23,9 @@
 //
 // Accumulator block: register r of lane l holds C row l%16, column 4*(l/16) + r (B's
 // fragment is the first operand).
+#include <algorithm>
+#include <cmath>
+
 #include "mma_kernel.h"
 
 namespace gk {
@@ -1311,9 +1314,49 @@ inline int64_t even_tiles(const RaggedArgs &g, int64_t avg, int bm, int bn) {
     return groups * ((avg + bm - 1) / bm) * (((int64_t)g.N + bn - 1) / bn);
 }
 
+// Expected time in us of a forward product with more than 16 rows a group on a BM x BN tile:
+//   2 + sqrt(c^2 + m^2),  c = (a + b*stages) * (1 + h*(y' - 1)),  m = bytes / bw
+// with y tiles per CU (a group's last tile half full on average), y' = q*ceil(y) + (1-q)*y, at
+// least 1.  The constants are the least-squares fit of log times of 110 products x 3 operand
+// kinds (17..4096 rows a group, 1..128 groups, k and n 128..8192, graph-timed with rotating
+// weights); the tile they pick took 1.009 (bf16) and 1.004 (MXFP4) times the fastest of the seven
+// in the geometric mean, 1.29 at worst.  The seven are those of 13 shapes that leave the least
+// behind the fastest of all (1.02); a rule on rows and tile counts alone left 1.15.
+struct RaggedCost {
+    int bm, bn;
+    double a, b, h, bw, q;
+};
+constexpr RaggedCost kRaggedCost[2][7] = {
+    {{64, 64, 0.91, 0.287, 0.97, 4.29, 0.55},     // bf16
+     {64, 128, 1.26, 0.403, 0.99, 4.69, 0.67},
+     {128, 128, 1.84, 0.492, 1.31, 4.98, 0.96},
+     {128, 256, 2.72, 0.794, 1.29, 4.97, 0.79},
+     {256, 256, 4.25, 0.901, 1.17, 3.65, 1.00},
+     {32, 64, 1.52, 0.156, 1.28, 3.86, 0.96},
+     {16, 32, 1.04, 0.095, 0.86, 3.50, 0.87}},
+    {{64, 64, 1.64, 0.408, 0.74, 4.30, 0.58},     // MXFP4
+     {64, 128, 1.99, 0.549, 0.75, 4.53, 0.62},
+     {128, 128, 2.67, 0.713, 1.12, 4.55, 0.90},
+     {128, 256, 3.49, 1.051, 1.17, 4.72, 1.00},
+     {256, 256, 5.22, 1.164, 1.17, 3.24, 1.00},
+     {32, 64, 1.93, 0.162, 1.24, 3.26, 0.91},
+     {16, 32, 1.87, 0.086, 1.08, 3.10, 0.88}}};
+
+inline double ragged_cost(const RaggedCost &c, const RaggedArgs &g, int64_t groups, int64_t avg,
+                          int64_t kbytes) {
+    const double tm = groups == 1 ? (double)((avg + c.bm - 1) / c.bm)
+                                  : std::max(1.0, (double)avg / c.bm + 0.5);
+    const double y = groups * tm * (double)((g.N + c.bn - 1) / c.bn) / std::max(g.cus, 1);
+    const double rounds = std::max(1.0, c.q * std::ceil(y) + (1.0 - c.q) * y);
+    const double work = (c.a + c.b * (double)((kbytes + 127) / 128)) * (1.0 + c.h * (rounds - 1.0));
+    const double bytes = ((double)groups * g.N + g.M) * (double)kbytes + 2.0 * g.M * g.N;
+    const double mem = bytes / (c.bw * 1e6);
+    return 2.0 + std::sqrt(work * work + mem * mem);
+}
+
 // The tile of a forward product, by the average rows of a group (the host does not know
-// more) and the tiles that makes.  Times in us, graph-timed with rotating weights, as
-// rows x groups x k x n with k-contiguous / n-contiguous bf16 / MXFP4 weights ("-": n/a).
+// more).  Times in us, graph-timed with rotating weights, as rows x groups x k x n with
+// k-contiguous / n-contiguous bf16 / MXFP4 weights.
 template <bool MX, bool BT, EpiKind E>
 static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
 #define GK_GO(...) return ragged_go<MX, false, BT, E, __VA_ARGS__>(g, ep, stream)
@@ -1339,8 +1382,7 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         // layouts take it for few tiles only, and k of few stages never (128x100x512x600
         // 15.4 / 17.1 / 16.9 against 11.1 / 12.5 / 7.0).
         const int64_t few = even_tiles(g, avg, 16, 64);
-        if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16))
-            {
+        if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16)) {
             GK_GO_ONCE(WaveTile<16, 32, 4, 3);
         }
         // n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more: 64x32x2048x4096
@@ -1351,24 +1393,24 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         }
         GK_GO_ONCE(RingTile<16, 64, 1, 4, 4);
     }
-    // Too few tiles for half of the CUs: K split over the waves.  500x2x8192x1024
-    // 34.7 / 33.7 / 12.5 against 35.4 / 36.0 / 16.8.
-    if (even_tiles(g, avg, 64, 64) <= cus / 2) GK_GO(WaveTile<64, 64, 4, 2>);
-    if (avg > 64) {
-        // 16384x8x4096x4096 487 / 475 / 182 against 531 / 522 / 206, one group of 4096x4096x4096
-        // 103 / 102 / 40 against 115 / 118 / 47; below two rounds of whole tiles the half
-        // tiles spread better: 8192x16x4096x2048 181 / 173 / 69 against 164 / 162 / 70.
-        const int64_t big = even_tiles(g, avg, 256, 256);
-        if (big >= 2 * cus || (groups == 1 && big <= cus && big * 4 >= cus * 3)) GK_GO(BigTile);
-        // 2048x16x4096x2048 73 / 68 / 26 against 89 / 86 / 34 with 64 x 128 tiles
-        if (even_tiles(g, avg, 128, 256) >= cus / 2) GK_GO(RingTile<128, 256, 2, 4, 3>);
+    int best = 0;
+    double cost = 0;
+    for (int i = 0; i < 7; ++i) {
+        const double c = ragged_cost(kRaggedCost[MX ? 1 : 0][i], g, groups, avg, kbytes);
+        if (i == 0 || c < cost) {
+            best = i;
+            cost = c;
+        }
     }
-    // 4096x64x1024x1024 38 / 38 / 16 against 39 / 41 / 20 with 64 x 64 tiles;
-    // 1001x5x1504x776 (140 tiles) 12.7 / 12.8 / 8.3 against 10.2 / 10.7 / 7.3
-    if (even_tiles(g, avg, 64, 128) >= cus) {
-        GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
+    switch (best) {
+    case 1: GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
+    case 2: GK_GO_ONCE(RingTile<128, 128, 2, 4, 4);
+    case 3: GK_GO(RingTile<128, 256, 2, 4, 3>);
+    case 4: GK_GO(BigTile);
+    case 5: GK_GO(WaveTile<32, 64, 4, 2>);
+    case 6: GK_GO(WaveTile<16, 32, 4, 3>);
+    default: GK_GO_ONCE(RingTile<64, 64, 2, 2, 4);
     }
-    GK_GO_ONCE(RingTile<64, 64, 2, 2, 4);
 #undef GK_GO_ONCE
 #undef GK_GO
 }
