@@ -489,12 +489,20 @@ __device__ __forceinline__ v4f mx_half(v4i b, v4i a, v4f c, const ScaleQuad &y, 
 // Elements a lane stores at once: 16 bytes.
 constexpr int chunk_of(EpiKind e) { return e == EpiKind::BF16 ? 8 : 4; }
 
-// A chunk of one row of C, stored nontemporally: written through the L2 the output pushes the
-// operand panels out of it (weight gradient 16384x8x4096x4096 with f32 output 512 against 443
-// us).  bf16 takes 16 bytes here instead of store4's 8: a weight
+// Whether C's rows start at 128-byte lines.
+template <EpiKind E>
+__device__ __forceinline__ bool whole_lines(const EpiParams &ep) {
+    constexpr int ESZ = E == EpiKind::BF16 ? 2 : 4;
+    return (((uint64_t)ep.c | (uint64_t)(ep.rsc * ESZ) | (uint64_t)(ep.bsc * ESZ)) & 127) == 0;
+}
+
+// A chunk of one row of C; NT: stored nontemporally.  Written through the L2 the output
+// pushes the operand panels out of it (weight gradient 16384x8x4096x4096 with f32 output 512
+// against 443 us), but pieces of lines have to meet there (rows of 9632 bytes,
+// 39x56x512x2408: 97 us nontemporally, 60 without).  bf16 takes 16 bytes here instead of store4's 8: a weight
 // gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16 from 64 rows: 21.8 us
 // with 8 bytes a lane).
-template <EpiKind E>
+template <EpiKind E, bool NT>
 __device__ __forceinline__ void store_chunk(const EpiParams &ep, int64_t z, int row, int col, int N,
                                             const v4f (&v)[chunk_of(E) / 4]) {
     if constexpr (E == EpiKind::BF16) {
@@ -516,19 +524,21 @@ __device__ __forceinline__ void store_chunk(const EpiParams &ep, int64_t z, int 
             v4u o;
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
-            __builtin_nontemporal_store(o, (v4u_any2 *)c);
+            if constexpr (NT) __builtin_nontemporal_store(o, (v4u_any2 *)c);
+            else *(v4u_any2 *)c = o;
             return;
         }
     }
 #pragma unroll
     for (int i = 0; i < chunk_of(E) / 4; ++i) {
         const float w[4] = {v[i][0], v[i][1], v[i][2], v[i][3]};
-        if (col + 4 * i < N) store4<E, float, StPol::NT>(ep, z, row, col + 4 * i, N, w);
+        if (col + 4 * i < N)
+            store4<E, float, NT ? StPol::NT : StPol::Plain>(ep, z, row, col + 4 * i, N, w);
     }
 }
 
 // Epilogue: 16-row bands of a wave's TM x TN blocks staged through LDS and stored as rows.
-template <EpiKind E, int WTM, int WTN, int TM, int TN>
+template <EpiKind E, bool NT, int WTM, int WTN, int TM, int TN>
 __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTile &t, int N,
                                              const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
                                              int wm, int wn, int lane) {
@@ -550,7 +560,7 @@ __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTi
 #pragma unroll
             for (int e = 0; e < CH / 4; ++e) v[e] = *(const v4f *)(stg + r * LD + c + 4 * e);
             const int row = wm * WTM + i * 16 + r;
-            if (row < t.rows && col < N) store_chunk<E>(ep, t.z, t.row0 + row, col, N, v);
+            if (row < t.rows && col < N) store_chunk<E, NT>(ep, t.z, t.row0 + row, col, N, v);
         }
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_wave_barrier();
@@ -676,7 +686,8 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
     // (the loads past the end of K, zeros into ring slots, land first)
     wait_vmcnt<0>();
     __syncthreads();
-    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
 
 // ---------------------------------------------------------------- 256 x 256 tile
@@ -869,7 +880,8 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
     else stages(idle);
     wait_vmcnt<0>();
     __syncthreads();
-    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
 
 // ---------------------------------------------------------------- few tiles
@@ -878,7 +890,7 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
 // workgroup share one BM x BN tile and split K among them, stage kt to wave kt % KS.  Each
 // wave fills its own ring of NS stages and waits for nothing but its own loads (no
 // barriers); their sums are added in wave order through LDS at the end.
-template <EpiKind E, int BM, int BN, int KS, int TM, int TN>
+template <EpiKind E, bool NT, int BM, int BN, int KS, int TM, int TN>
 __device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile &t, int N,
                                           const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
                                           int lane) {
@@ -901,7 +913,7 @@ __device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile 
 #pragma unroll
             for (int i = 0; i < CH / 4; ++i)
                 v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
-        store_chunk<E>(ep, t.z, t.row0 + row, t.n0 + col, N, v);
+        store_chunk<E, NT>(ep, t.z, t.row0 + row, t.n0 + col, N, v);
     }
 }
 
@@ -1010,7 +1022,8 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
 
     wait_vmcnt<0>();
     __syncthreads();
-    wave_sums<E, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    else wave_sums<E, false, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // ---------------------------------------------------------------- operands of any alignment
@@ -1158,7 +1171,8 @@ void ragged_reg_kernel(const RaggedArgs g, const EpiParams ep) {
         if (kt + 1 < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    ragged_store<E, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
 
 // The same with K split over the KS waves of a workgroup (see ragged_wave_kernel): a wave's
@@ -1228,7 +1242,8 @@ void ragged_reg_wave_kernel(const RaggedArgs g, const EpiParams ep) {
         if (kt + KS < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    wave_sums<E, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    else wave_sums<E, false, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
