@@ -1334,9 +1334,9 @@ inline int64_t even_tiles(const RaggedArgs &g, int64_t avg, int bm, int bn) {
 // with y tiles per CU (a group's last tile half full on average), y' = q*ceil(y) + (1-q)*y, at
 // least 1.  The constants are the least-squares fit of log times of 110 products x 3 operand
 // kinds (17..4096 rows a group, 1..128 groups, k and n 128..8192, graph-timed with rotating
-// weights); the tile they pick took 1.009 (bf16) and 1.004 (MXFP4) times the fastest of the seven
-// in the geometric mean, 1.29 at worst.  The seven are those of 13 shapes that leave the least
-// behind the fastest of all (1.02); a rule on rows and tile counts alone left 1.15.
+// weights); the tile they pick took 1.009 (bf16) and 1.011 (MXFP4) times the fastest of the seven
+// in the geometric mean, 1.31 at worst.  The seven are those of 13 shapes that leave the least
+// behind the fastest of all (1.02).
 struct RaggedCost {
     int bm, bn;
     double a, b, h, bw, q;
@@ -1351,7 +1351,7 @@ constexpr RaggedCost kRaggedCost[2][7] = {
      {16, 32, 1.04, 0.095, 0.86, 3.50, 0.87}},
     {{64, 64, 1.64, 0.408, 0.74, 4.30, 0.58},     // MXFP4
      {64, 128, 1.99, 0.549, 0.75, 4.53, 0.62},
-     {128, 128, 2.67, 0.713, 1.12, 4.55, 0.90},
+     {128, 128, 2.22, 0.755, 0.83, 4.61, 0.50},
      {128, 256, 3.49, 1.051, 1.17, 4.72, 1.00},
      {256, 256, 5.22, 1.164, 1.17, 3.24, 1.00},
      {32, 64, 1.93, 0.162, 1.24, 3.26, 0.91},
@@ -1419,7 +1419,7 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
     }
     switch (best) {
     case 1: GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
-    case 2: GK_GO_ONCE(RingTile<128, 128, 2, 4, 4);
+    case 2: GK_GO_ONCE(RingTile<128, 128, 2, 4, MX ? 2 : 4);
     case 3: GK_GO(RingTile<128, 256, 2, 4, 3>);
     case 4: GK_GO(BigTile);
     case 5: GK_GO(WaveTile<32, 64, 4, 2>);
