@@ -276,6 +276,10 @@ struct gk_workspace {
     hipStream_t last_stream = nullptr;
     hipEvent_t done = nullptr;
     bool recorded = false;
+    // A captured call has put the arena's address into a graph, which may be replayed
+    // after the arena has grown: such arenas are kept until the workspace goes.
+    bool captured = false;
+    std::vector<void *> kept;
 };
 
 struct gk_packed_rhs {
@@ -309,6 +313,9 @@ void ws_release(gk_workspace *ws) {
     if (tl_ws_recorded == &ws->recorded) tl_ws_recorded = nullptr;
     ws_quiesce(ws);
     if (ws->ptr) (void)hipFree(ws->ptr);
+    for (void *p : ws->kept) (void)hipFree(p);
+    ws->kept.clear();
+    ws->captured = false;
     ws->ptr = nullptr;
     ws->bytes = 0;
     if (ws->done) (void)hipEventDestroy(ws->done);
@@ -364,7 +371,9 @@ int ws_reserve(gk_workspace *ws, size_t bytes, void **out) {
                 if (e != hipSuccess) return hip_fail(e, "workspace grow");
                 ws->recorded = false;
             }
-            (void)hipFree(ws->ptr);
+            if (ws->captured) ws->kept.push_back(ws->ptr);
+            else (void)hipFree(ws->ptr);
+            ws->captured = false;
             ws->ptr = nullptr;
             ws->bytes = 0;
         }
@@ -391,6 +400,8 @@ int ws_reserve(gk_workspace *ws, size_t bytes, void **out) {
         ws->last_stream = tl_stream;
         tl_ws_event = ws->done;
         tl_ws_recorded = &ws->recorded;
+    } else {
+        ws->captured = true;
     }
     *out = ws->ptr;
     return GK_OK;
