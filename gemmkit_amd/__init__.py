@@ -1101,7 +1101,6 @@ class MatMxfp4:
         blocks = -(-self.cols // 32)
         self.ld = 16 * blocks if ld is None else int(ld)
         self.lds = -(-blocks // 16) * 16 if lds is None else int(lds)
-        self._made = None  # the C structure and what it was made from
 
     @classmethod
     def empty(cls, rows: int, cols: int, device="cuda") -> "MatMxfp4":
@@ -1112,22 +1111,13 @@ class MatMxfp4:
         return cls(codes, scales, rows, cols)
 
     def _c(self, what: str) -> Mxfp4C:
-        # Made once for the arrays in hand (1.3 us, twice a product).
-        made = (self.codes, self.scales, self.codes.data_ptr(), self.scales.data_ptr(),
-                self.rows, self.cols, self.ld, self.lds)
-        last = self._made
-        if last is not None and last[1][0] is made[0] and last[1][1] is made[1] \
-                and last[1][2:] == made[2:]:
-            return last[0]
         codes, scales = _slice(self.codes, what), _slice(self.scales, what)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError(f"gemmkit_amd: {what} codes and scales must be uint8")
         if min(self.rows, self.cols, self.ld, self.lds) < 0:
             raise GemmkitError(-2, f"gemmkit_amd: {what} has a negative side or stride")
-        c = Mxfp4C(codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
-                   self.rows, self.cols, self.ld, self.lds)
-        self._made = (c, made)
-        return c
+        return Mxfp4C(codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
+                      self.rows, self.cols, self.ld, self.lds)
 
 
 def quantize_mxfp4(x: MatRef, q: Optional[MatMxfp4] = None) -> MatMxfp4:

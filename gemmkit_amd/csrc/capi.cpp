@@ -19,6 +19,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
@@ -371,8 +372,15 @@ int ws_reserve(gk_workspace *ws, size_t bytes, void **out) {
                 if (e != hipSuccess) return hip_fail(e, "workspace grow");
                 ws->recorded = false;
             }
-            if (ws->captured) ws->kept.push_back(ws->ptr);
-            else (void)hipFree(ws->ptr);
+            if (ws->captured) {
+                try {
+                    ws->kept.push_back(ws->ptr);
+                } catch (const std::bad_alloc &) {
+                    return fail(GK_ERR_NOMEM, "gemmkit: out of host memory for the workspace");
+                }
+            } else {
+                (void)hipFree(ws->ptr);
+            }
             ws->captured = false;
             ws->ptr = nullptr;
             ws->bytes = 0;
@@ -2145,9 +2153,6 @@ int packed_a_checked(gk_workspace *ws, InType in, EpiKind kind, size_t esz, floa
                               c->data, c->rs, c->cs, any ? &fx : nullptr);
 }
 
-// ---- pointer-array batched (src/api/batched.rs:711-799; run_ptr,
-// src/special/batched.rs:294-334: every problem as a standalone gemm)
-
 // ---- ragged groups and MXFP4 operands (no counterpart in the reference)
 
 // The longest row (bytes) of an operand of these products: with at most 256 rows a
@@ -2553,6 +2558,9 @@ int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool 
     if (e != hipSuccess) return launch_failed(e, "mxfp4 gemm");
     return finish("mxfp4 gemm");
 }
+
+// ---- pointer-array batched (src/api/batched.rs:711-799; run_ptr,
+// src/special/batched.rs:294-334: every problem as a standalone gemm)
 
 // Element step of a run of problems: the pointer difference in elements, when
 // it is a whole number of elements.

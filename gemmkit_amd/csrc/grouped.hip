@@ -6,13 +6,13 @@
 
 namespace gk {
 
-// Products of rows that lack the alignment, in us as rows x groups x k x n with
-// k-contiguous / n-contiguous weights, against aligned copies of every group's weights.
 static int64_t avg_rows(const RaggedArgs &g) {
     const int64_t groups = std::min(g.G, g.M);
     return (g.M + groups - 1) / groups;
 }
 
+// Products of rows that lack the alignment, in us as rows x groups x k x n with
+// k-contiguous / n-contiguous weights, against aligned copies of every group's weights.
 bool grouped_takes_any_align(const RaggedArgs &g, RaggedB bl) {
     const int64_t avg = avg_rows(g);
     const double flops = 2.0 * g.M * g.N * g.K;
@@ -77,6 +77,7 @@ int wgrad_splits(const RaggedArgs &g) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
 }
 
+// (the figures of both sides: wgrad_go; a longer product repays its copies)
 bool wgrad_takes_any_align(const RaggedArgs &g) {
     return g.splits == 1 && 2.0 * g.M * g.N * g.K < 2e10;
 }
@@ -86,9 +87,9 @@ template <EpiKind E>
 static hipError_t wgrad_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     const int64_t cus = g.cus, big = wgrad_tiles(g, 256), avg = g.M / g.G;
     // Rows that lack the alignment as they are, against aligned copies of both operands:
-    // 375x5x149x320 9.6 / 9.7 against 14.9 / 13.4, 39x56x513x2409 102 / 58 against 118 / 69 (125 / 82
-    // with 64 x 64 tiles: C's rows lack the alignment too, and long pieces cost less),
-    // 4000x8x513x1027 29 / 29 against 32 / 32.
+    // 375x5x149x320 9.6 / 9.7 against 14.9 / 13.4, 39x56x513x2409 102 / 58 against
+    // 118 / 69 (125 / 82 with 64 x 64 tiles: C's rows lack the alignment too, and long pieces
+    // cost less), 4000x8x513x1027 29 / 29 against 32 / 32.
     if (g.any_align) return ragged_go<false, true, true, E, RegTile<64, 128, 2, 2>>(g, ep, stream);
     // The 256 x 256 tile wherever half of the CUs get one: 16384x8x4096x4096 509 / 427 against
     // 675 / 551 with 128 x 128 tiles.  Short groups are bound by the stores, which two

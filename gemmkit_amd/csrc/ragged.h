@@ -499,9 +499,9 @@ __device__ __forceinline__ bool whole_lines(const EpiParams &ep) {
 // A chunk of one row of C; NT: stored nontemporally.  Written through the L2 the output
 // pushes the operand panels out of it (weight gradient 16384x8x4096x4096 with f32 output 512
 // against 443 us), but pieces of lines have to meet there (rows of 9632 bytes,
-// 39x56x512x2408: 97 us nontemporally, 60 without).  bf16 takes 16 bytes here instead of store4's 8: a weight
-// gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16 from 64 rows: 21.8 us
-// with 8 bytes a lane).
+// 39x56x512x2408: 97 us nontemporally, 60 without).  bf16 takes 16 bytes here instead of
+// store4's 8: a weight gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16
+// from 64 rows: 21.8 us with 8 bytes a lane).
 template <EpiKind E, bool NT>
 __device__ __forceinline__ void store_chunk(const EpiParams &ep, int64_t z, int row, int col, int N,
                                             const v4f (&v)[chunk_of(E) / 4]) {
@@ -801,7 +801,6 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
     stage_barrier();
     ops(a_slot(0), b_slot(0), I0{}, 0, FA{}, std::true_type{}, I0{}, [](int) {});
     if constexpr (MX) scales(0, 0);
-
 
     // Loads of stage kt+2 in phase 0 (L0, A's) and in phase 3 (L3, A's first).  The scales of
     // stages kt+2 and kt+3 go out in phase 3 of even stages.

@@ -92,7 +92,8 @@ int gk_set_synchronous(int on);
 
 /* Device scratch arena (src/workspace.rs:53): holds packed operands for
  * layouts the kernels cannot read in place and split-K partial sums.  Grows on
- * demand (synchronizing the device), never shrinks.  A call made while the
+ * demand (synchronizing the device), never shrinks; what a captured call was
+ * given stays until the workspace is freed.  A call made while the
  * launch stream is being captured into a HIP graph cannot grow it: such a call
  * fails with GK_ERR_NOMEM when it needs more than the arena holds, so size the
  * arena before capturing.  The NULL (per-thread) workspace is released when its
@@ -631,15 +632,18 @@ int gk_gemm_packed_a_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha,
  * any other contents give disjoint groups inside the matrix too.  Groups may be
  * empty.  Rows before s_0 and from s_groups on belong to no group.
  *
- * Sizes: rows, groups, k and n below 2^31; a bf16 row of k (and, for wgrad, n)
- * elements at most 4 MiB, a row of codes likewise.  GK_ERR_OVERFLOW beyond.
+ * Sizes: rows, groups, k and n below 2^31 - 1024; a bf16 row of k (and, for
+ * wgrad, n) elements at most 4 MiB, a row of codes likewise.  GK_ERR_OVERFLOW
+ * beyond.
  */
 
 /* C[rows of g] <- alpha * A[rows of g] * B_g + beta * C[rows of g], bf16 inputs, f32
  * sums: A rows x k, C rows x n, B_g the k x n view b moved by g * b_gs
  * elements (0: one matrix for all).  Rows of no group are left as they are.
- * Read in place: rows of A of unit stride; B of unit k stride or unit n
- * stride; 16-byte aligned.  Other layouts are packed first. */
+ * Read in place: A of unit k stride, B of unit k or unit n stride, with bases
+ * and strides that are multiples of 16 bytes, and products of moderate size
+ * without that alignment too.  Anything else is packed first: size a workspace
+ * for copies of A and of all of B before a capture. */
 int gk_gemm_grouped_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
                          const int32_t *offsets, size_t groups, const gk_mat_ref *b,
                          ptrdiff_t b_gs, float beta, const gk_mat_mut *c, gk_par par);

@@ -359,3 +359,74 @@ def test_mxfp4_offsets_past_32_bits(dev):
     want = torch.zeros(500, k, dtype=BF16, device=dev)
     gk.dequantize_mxfp4(tail, gk.MatMut.from_row_major(want, 500, k))
     assert torch.equal(back[-500:], want) and not back[:-500].any()
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+def test_many_groups(dev, aligned):
+    """More groups than a launch's z extent; without alignment the weights are copied in
+    pieces (k below the 16 bytes that reading them as they are takes)."""
+    groups, k, n = 70_000, 8 if aligned else 5, 8 if aligned else 6
+    g = torch.Generator(device="cuda").manual_seed(5)
+    sizes = torch.randint(0, 3, (groups,), generator=g, device=dev)
+    off = torch.cat([torch.zeros(1, dtype=torch.int64, device=dev), sizes.cumsum(0)]).int()
+    rows = int(off[-1])
+    x, w, dy = rand(1, rows, k), rand(2, groups, n, k), rand(3, rows, n)
+    y = forward(x, off, w, torch.zeros(rows, n, device=dev))
+    of = torch.repeat_interleave(torch.arange(groups, device=dev), sizes)
+    want = (w.double()[of] * x.double()[:, None, :]).sum(2)
+    tol = 8 * 2.0 ** -23 * (w.double()[of].abs() * x.double()[:, None, :].abs()).sum(2)
+    assert ((y.double() - want).abs() <= tol + 2.0 ** -24 * want.abs()).all()
+    dx, dw = torch.zeros(rows, k, device=dev), torch.full((groups, n, k), 7.0, device=dev)
+    backward(x, off, w, dy, dx, dw)
+    outer = dy.double()[:, :, None] * x.double()[:, None, :]
+    want = torch.zeros(groups, n, k, dtype=torch.float64, device=dev).index_add_(0, of, outer)
+    tol = torch.zeros_like(want).index_add_(0, of, outer.abs()) * 2.0 ** -22
+    assert ((dw.double() - want).abs() <= tol).all()
+
+
+def test_one_mxfp4_matrix_in_several_products(dev):
+    """A quantized matrix stays the caller's: its arrays may be replaced or grow, and both
+    operands may be the same one."""
+    x = rand(1, 96, 160)
+    q = gk.quantize_mxfp4(gk.MatRef.from_row_major(x, 96, 160))
+    xd = torch.zeros(96, 160, device=dev)
+    gk.dequantize_mxfp4(q, gk.MatMut.from_row_major(xd, 96, 160))
+    c = torch.zeros(96, 96, device=dev)
+    gk.gemm_mxfp4(1.0, q, q, 0.0, gk.MatMut.from_row_major(c, 96, 96))
+    want = xd.double() @ xd.double().t()
+    tol = 160 * 2.0 ** -23 * (xd.double().abs() @ xd.double().abs().t())
+    assert ((c.double() - want).abs() <= tol).all()
+    codes, scales = q.codes, q.scales
+    q.codes, q.scales = torch.zeros_like(codes), scales.clone()
+    gk.gemm_mxfp4(1.0, q, q, 0.0, gk.MatMut.from_row_major(c, 96, 96))
+    assert not c.any()
+    q.codes = codes[:95]
+    with pytest.raises(gk.GemmkitError):
+        gk.gemm_mxfp4(1.0, q, q, 0.0, gk.MatMut.from_row_major(c, 96, 96))
+
+
+def test_python_refusals(dev):
+    x = rand(1, 8, 8)
+    a, c = gk.MatRef.from_row_major(x, 8, 8), gk.MatMut.from_row_major(torch.zeros_like(x), 8, 8)
+    good = offsets_of([8])
+    for off, err in ((good.long(), TypeError), (good.view(1, 2), TypeError), (good[:0], TypeError),
+                     (good.cpu(), gk.GemmkitError), (offsets_of([4, 4])[::2], TypeError),
+                     ([0, 8], TypeError)):
+        with pytest.raises(err):
+            gk.gemm_grouped(1.0, a, off, a, 0, 0.0, c)
+        with pytest.raises(err):
+            gk.gemm_grouped_wgrad(1.0, a, off, a, 0.0, c, 64)
+    f32 = gk.MatRef.from_row_major(x.float(), 8, 8)
+    with pytest.raises(TypeError):
+        gk.gemm_grouped(1.0, f32, good, a, 0, 0.0, c)
+    half = gk.MatMut.from_row_major(x.half(), 8, 8)
+    for call in (lambda: gk.gemm_grouped(1.0, a, good, a, 0, 0.0, half),
+                 lambda: gk.gemm_grouped_wgrad(1.0, a, good, a, 0.0, half, 64),
+                 lambda: gk.quantize_mxfp4(gk.MatRef.from_row_major(x.half(), 8, 8)),
+                 lambda: gk.dequantize_mxfp4(gk.MatMxfp4.empty(8, 8), half)):
+        with pytest.raises(TypeError):
+            call()
+    bad = gk.MatMxfp4(torch.zeros(8, 16, dtype=torch.int8, device=dev),
+                      torch.zeros(8, 16, dtype=torch.uint8, device=dev), 8, 8)
+    with pytest.raises(TypeError):
+        gk.dequantize_mxfp4(bad, c)
