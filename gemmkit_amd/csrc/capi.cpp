@@ -2287,17 +2287,18 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
         // their own, or copied row by row.
         const bool rows_any = ragged_unit_rows(Br, N, K), cols_any = ragged_unit_rows(Bc, K, N);
         if (!a_ok || (!rows_ok && !cols_ok)) {
+            const bool b_pack = !rows_ok && !cols_ok, pack_cols = cols_ok || (b_pack && cols_any);
+            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+            const size_t pb = !b_pack     ? 0
+                              : pack_cols ? pack_bytes(InType::BF16, K, N, G, Bc)
+                                          : pack_bytes(InType::BF16, N, K, G, Br);
             g.any_align = ragged_unit_rows(A, M, K) && (rows_any || cols_any) &&
-                          grouped_takes_any_align(g, rows_any ? RaggedB::Rows : RaggedB::Cols);
+                          grouped_plan_any(g, rows_any ? RaggedB::Rows : RaggedB::Cols,
+                                           (int64_t)(pa + pb));
             if (g.any_align) {
                 cols_ok = !rows_any;
             } else {
-                const bool b_pack = !rows_ok && !cols_ok;
-                cols_ok = cols_ok || (b_pack && cols_any);
-                const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-                const size_t pb = !b_pack ? 0
-                                  : cols_ok ? pack_bytes(InType::BF16, K, N, G, Bc)
-                                            : pack_bytes(InType::BF16, N, K, G, Br);
+                cols_ok = pack_cols;
                 void *buf = nullptr;
                 if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
                 uint8_t *const dst = (uint8_t *)buf + pa;
@@ -2376,15 +2377,17 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
-    g.splits = wgrad_splits(g);
+    g.splits = 1;
     uint8_t *part = nullptr;
+    if (M == 0) wgrad_plan(g, kind, false, 0);
     if (M > 0) {
-        bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
-        g.any_align = (!a_ok || !b_ok) && ragged_unit_rows(A, M, K) && ragged_unit_rows(B, M, N) &&
-                      wgrad_takes_any_align(g);
-        if (g.any_align) a_ok = b_ok = true;
-        const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-        const size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
+        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
+        size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+        size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
+        wgrad_plan(g, kind,
+                   (!a_ok || !b_ok) && ragged_unit_rows(A, M, K) && ragged_unit_rows(B, M, N),
+                   (int64_t)(pa + pb));
+        if (g.any_align) pa = pb = 0;
         const size_t sums = g.splits > 1 ? (size_t)g.splits * groups * K * N * 4 : 0;
         if (pa + pb + sums > 0) {
             void *buf = nullptr;

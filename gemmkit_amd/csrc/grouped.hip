@@ -6,41 +6,56 @@
 
 namespace gk {
 
-static int64_t avg_rows(const RaggedArgs &g) {
-    const int64_t groups = std::min(g.G, g.M);
-    return (g.M + groups - 1) / groups;
-}
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Products of rows that lack the alignment, in us as rows x groups x k x n with
-// k-contiguous / n-contiguous weights, against aligned copies of every group's weights.
-bool grouped_takes_any_align(const RaggedArgs &g, RaggedB bl) {
-    const int64_t avg = avg_rows(g);
-    const double flops = 2.0 * g.M * g.N * g.K;
-    // The weights are read once or nearly, those of empty groups not at all: 7x40x2233x5347
-    // 24 / 30 against 392 / 481, 1936x56x1285x469 29 / 34 against 47 / 44.
-    if (avg <= 64) return true;
-    // 13236x82x217x2215 71 / 71 against 91 / 102, 4096x8x1025x1027 30 / 32 against 36 / 34;
-    // 16384x8x2049x2047 246 / 246 against 230 / 206
-    if (even_tiles(g, avg, 128, 128) >= g.cus) return flops < 6e10;
-    // 1001x5x1501x777 18 / 23 against 22 / 22, 5322x16x3633x153 34 / 49 against 57 / 52
-    return bl == RaggedB::Rows && flops < 1e10;
+// Forward products of rows that lack the alignment, k-contiguous and n-contiguous weights.
+// The constants are the least-squares fit of log times of 215 products (1..16384 rows, 1..128
+// groups, k and n 128..8192, odd ones among them); the tile they pick, or aligned copies where
+// those are expected to cost less, took 1.027 times the fastest of 15 tiles and the copies in
+// the geometric mean.
+constexpr TileTime kAnyTile[2][5] = {
+    {{128, 128, 2.36, 0.839, 2.81, 0.722, 5.90, 0.41},
+     {128, 64, 1.57, 0.610, 1.20, 0.463, 7.28, 0.38},
+     {32, 64, 1.53, 0.489, 0.28, 0.249, 5.62, 0.00},
+     {16, 32, 1.70, 0.169, 0.36, 0.107, 6.62, 0.02},
+     {16, 32, 2.15, 0.098, 1.79, 0.091, 6.37, 0.32}},
+    {{128, 128, 1.67, 1.247, 2.85, 0.634, 7.16, 0.07},
+     {128, 64, 1.18, 0.794, 1.64, 0.453, 7.28, 0.16},
+     {32, 64, 0.53, 0.850, 0.26, 0.231, 6.29, 0.00},
+     {16, 32, 1.32, 0.285, 0.25, 0.149, 5.52, 0.60},
+     {16, 32, 1.81, 0.168, 1.10, 0.155, 6.31, 0.58}}};
+
+bool grouped_plan_any(RaggedArgs &g, RaggedB bl, int64_t copies) {
+    const int64_t groups = std::min(g.G, g.M), avg = ceil_div(g.M, groups);
+    const int64_t kbytes = (int64_t)g.K * 2;
+    const double bytes = ((double)groups * g.N + g.M) * (double)kbytes + 2.0 * g.M * g.N;
+    double cost = 0;
+    for (int i = 0; i < 5; ++i) {
+        const TileTime &t = kAnyTile[bl == RaggedB::Cols ? 1 : 0][i];
+        const double tm = groups == 1 ? (double)ceil_div(avg, t.bm)
+                                      : std::max(1.0, (double)avg / t.bm + 0.5);
+        const double c = tile_time(t, groups * tm * (double)ceil_div(g.N, t.bn) / std::max(g.cus, 1),
+                                   (double)ceil_div(kbytes, 128), bytes);
+        if (i == 0 || c < cost) {
+            g.tile = i;
+            cost = c;
+        }
+    }
+    if (avg <= 16) return true;  // the weights are read once, those of empty groups not at all
+    double aligned = 0;
+    ragged_best<false>(g, groups, avg, ceil_div(kbytes, 16) * 16, &aligned);
+    return cost < 4.6 + (double)copies / 2.49e6 + aligned;
 }
 
 template <bool BT, EpiKind E>
 static hipError_t any_align_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-    const int64_t avg = avg_rows(g), stages = ((int64_t)g.K * 2 + 127) / 128;
-    const bool few = even_tiles(g, avg, 64, 64) <= g.cus / 2;
-    // 4x24x4647x2741 20 / 39 against 42 / 79 with 16 x 64 tiles, 17x55x193x6961 14 / 14
-    // against 12 / 12
-    if (avg <= 16 && stages < 8 && !few)
-        return ragged_go<false, false, BT, E, RegTile<16, 64, 1, 4>>(g, ep, stream);
-    if (avg <= 16 || (avg <= 64 && few))
-        return ragged_go<false, false, BT, E, RegWaveTile<16, 32, 4>>(g, ep, stream);
-    if (avg <= 64) return ragged_go<false, false, BT, E, RegTile<64, 64, 2, 2>>(g, ep, stream);
-    if (even_tiles(g, avg, 128, 128) >= g.cus)
-        return ragged_go<false, false, BT, E, RegTile<128, 128, 2, 4>>(g, ep, stream);
-    if constexpr (!BT) return ragged_go<false, false, BT, E, RegWaveTile<64, 32, 4>>(g, ep, stream);
-    return hipErrorInvalidValue;
+    switch (g.tile) {
+    case 0: return ragged_go<false, false, BT, E, RegTile<128, 128, 2, 4>>(g, ep, stream);
+    case 1: return ragged_go<false, false, BT, E, RegTile<128, 64, 4, 2>>(g, ep, stream);
+    case 2: return ragged_go<false, false, BT, E, RegTile<32, 64, 1, 4>>(g, ep, stream);
+    case 3: return ragged_go<false, false, BT, E, RegWaveTile<16, 32, 4>>(g, ep, stream);
+    default: return ragged_go<false, false, BT, E, RegWaveTile<16, 32, 8>>(g, ep, stream);
+    }
 }
 
 hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
@@ -64,43 +79,61 @@ hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams 
     return hipErrorInvalidValue;
 }
 
-static int64_t wgrad_tiles(const RaggedArgs &g, int side) {
-    return (int64_t)g.G * ((g.K + side - 1) / side) * ((g.N + side - 1) / side);
+// Weight gradients: aligned operands, and rows that lack the alignment.  Fitted as above to
+// 310 aligned products (among them 90 of 700 rows a group and more) and 250 others, f32 and
+// bf16 output, with groups whole and cut into 2..16 ranges; what they pick took 1.038 and
+// 1.028 times the fastest of all tiles, ranges and copies.
+constexpr TileTime kWgradTile[2][5] = {
+    {{256, 256, 8.01, 1.798, 6.14, 1.099, 5.61, 0.83},
+     {128, 128, 5.74, 0.899, 1.36, 0.426, 7.02, 0.00},
+     {64, 64, 5.22, 0.217, 0.72, 0.170, 7.28, 0.61},
+     {64, 128, 5.34, 0.678, 0.86, 0.238, 7.28, 0.00},
+     {32, 64, 5.37, 0.135, 2.37, 0.203, 3.58, 0.63}},
+    {{64, 64, 4.65, 1.358, 0.50, 0.330, 5.52, 0.00},
+     {128, 128, 5.18, 1.940, 1.40, 0.865, 5.72, 0.37}}};
+
+void wgrad_plan(RaggedArgs &g, EpiKind out, bool can_any, int64_t copies) {
+    const double elems = (double)g.G * g.K * g.N, read = 2.0 * g.M * ((double)g.K + g.N);
+    const int osz = out == EpiKind::F32 ? 4 : 2;
+    const int64_t avg = g.G > 0 ? g.M / g.G : 0;
+    double best = 0;
+    bool first = true;
+    for (int any = 0; any <= (can_any ? 1 : 0); ++any)
+        for (int i = 0; i < (any ? 2 : 5); ++i)
+            // A long contraction over few tiles is cut into ranges of 128 rows or more, up to
+            // four tiles per CU: partial sums in f32, then one launch that adds them.
+            for (int s = 1; s <= 16; s *= 2) {
+                const TileTime &t = kWgradTile[any][i];
+                const double tiles = (double)g.G * ceil_div(g.K, t.bm) * ceil_div(g.N, t.bn) * s;
+                if (s > 1 && (avg < s * 128 || tiles > 4.0 * g.cus)) break;
+                double c = tile_time(t, tiles / std::max(g.cus, 1),
+                                     (double)g.M / std::max(g.G, 1) / 64 / s + 0.5,
+                                     read + elems * s * (s > 1 ? 4 : osz));
+                if (s > 1) c += 4.0 + elems * (4 * s + osz) / 5e6;
+                if (!any && copies > 0) c += 6.0 + (double)copies / 1.89e6;
+                if (first || c < best) {
+                    first = false;
+                    best = c;
+                    g.tile = i;
+                    g.splits = s;
+                    g.any_align = any;
+                }
+            }
 }
 
-// Row ranges per group: a long contraction over few tiles is cut until about two 128 x 128
-// tiles per CU have work, each range of 512 rows or more on average.
-int wgrad_splits(const RaggedArgs &g) {
-    const int64_t avg = g.G > 0 ? g.M / g.G : 0, tiles = wgrad_tiles(g, 128);
-    if (avg < 2048 || tiles == 0) return 1;
-    const int64_t s = std::min<int64_t>(avg / 512, 2 * g.cus / tiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
-}
-
-// (the figures of both sides: wgrad_go; a longer product repays its copies)
-bool wgrad_takes_any_align(const RaggedArgs &g) {
-    return g.splits == 1 && 2.0 * g.M * g.N * g.K < 2e10;
-}
-
-// Times in us as rows x groups x k x n with f32 / bf16 output.
 template <EpiKind E>
 static hipError_t wgrad_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-    const int64_t cus = g.cus, big = wgrad_tiles(g, 256), avg = g.M / g.G;
-    // Rows that lack the alignment as they are, against aligned copies of both operands:
-    // 375x5x149x320 9.6 / 9.7 against 14.9 / 13.4, 39x56x513x2409 102 / 58 against
-    // 118 / 69 (125 / 82 with 64 x 64 tiles: C's rows lack the alignment too, and long pieces
-    // cost less), 4000x8x513x1027 29 / 29 against 32 / 32.
-    if (g.any_align) return ragged_go<false, true, true, E, RegTile<64, 128, 2, 2>>(g, ep, stream);
-    // The 256 x 256 tile wherever half of the CUs get one: 16384x8x4096x4096 509 / 427 against
-    // 675 / 551 with 128 x 128 tiles.  Short groups are bound by the stores, which two
-    // workgroups on a CU overlap better, up to four rounds: 1003x32x1024x704 25.4 / 18.8 against
-    // 21.7 / 15.5, but 1024x128x2048x512 109 / 66 against 117 / 72.
-    if (g.splits == 1 && (big >= 4 * cus || (big >= cus / 2 && avg > 48)))
-        return ragged_go<false, true, true, E, BigTile>(g, ep, stream);
-    if (g.splits > 1 || avg <= 48)
-        return ragged_go<false, true, true, E, RingTile<128, 128, 2, 4, 2>>(g, ep, stream);
-    // 4096x4x1024x1024 19.6 / 17.5 against 29.4 / 28.0 with 128 x 128 tiles
-    return ragged_go<false, true, true, E, RingTile<64, 64, 2, 2, 3>>(g, ep, stream);
+    if (g.any_align) {
+        if (g.tile == 0) return ragged_go<false, true, true, E, RegTile<64, 64, 2, 2>>(g, ep, stream);
+        return ragged_go<false, true, true, E, RegTile<128, 128, 2, 4>>(g, ep, stream);
+    }
+    switch (g.tile) {
+    case 0: return ragged_go<false, true, true, E, BigTile>(g, ep, stream);
+    case 1: return ragged_go<false, true, true, E, RingTile<128, 128, 2, 4, 2>>(g, ep, stream);
+    case 2: return ragged_go<false, true, true, E, RingTile<64, 64, 2, 2, 3>>(g, ep, stream);
+    case 3: return ragged_go<false, true, true, E, RingTile<64, 128, 2, 2, 2>>(g, ep, stream);
+    default: return ragged_go<false, true, true, E, WaveTile<32, 64, 4, 2>>(g, ep, stream);
+    }
 }
 
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {

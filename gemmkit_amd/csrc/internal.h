@@ -256,16 +256,18 @@ struct RaggedArgs {
     int32_t splits;
     // bf16: the operands' rows are unit-stride, 16 bytes or more, at any alignment
     int32_t any_align;
+    int32_t tile;              // what grouped_plan_any or wgrad_plan chose
 };
 // B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
 enum class RaggedB : int { Rows = 0, Cols = 1 };
-// Whether a forward product whose operands lack the alignment should be given them as they
-// are (any_align) rather than aligned copies.
-bool grouped_takes_any_align(const RaggedArgs &g, RaggedB bl);
-bool wgrad_takes_any_align(const RaggedArgs &g);
+// Chooses the tile (g.tile) of a forward product whose operands lack the alignment; whether it
+// should be given them as they are (g.any_align) rather than aligned copies of `copies` bytes.
+bool grouped_plan_any(RaggedArgs &g, RaggedB bl, int64_t copies);
 hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
                                hipStream_t stream);
-int wgrad_splits(const RaggedArgs &g);  // what a product should be given
+// Chooses g.tile, g.splits and (can_any: the operands allow it) g.any_align of a weight
+// gradient with `out` output, given the bytes that aligned copies of its operands take.
+void wgrad_plan(RaggedArgs &g, EpiKind out, bool can_any, int64_t copies);
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 
 // MXFP4 (mxfp4.hip): rows of e2m1 codes, two a byte, the lower nibble first, with one

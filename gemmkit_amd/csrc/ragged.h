@@ -1368,6 +1368,38 @@ inline double ragged_cost(const RaggedCost &c, const RaggedArgs &g, int64_t grou
     return 2.0 + std::sqrt(work * work + mem * mem);
 }
 
+// The cheapest of the seven for a product of more than 16 rows a group, and its time.
+template <bool MX>
+inline int ragged_best(const RaggedArgs &g, int64_t groups, int64_t avg, int64_t kbytes,
+                       double *cost) {
+    int best = 0;
+    for (int i = 0; i < 7; ++i) {
+        const double c = ragged_cost(kRaggedCost[MX ? 1 : 0][i], g, groups, avg, kbytes);
+        if (i == 0 || c < *cost) {
+            best = i;
+            *cost = c;
+        }
+    }
+    return best;
+}
+
+// Expected time in us of a weight gradient, or of a product of operands of any alignment, on
+// one tile shape: y tiles per CU, each of `stages` stages, over `bytes` of operands and output.
+//   2 + sqrt((a + b*stages + (c1 + c2*stages)*(y' - 1))^2 + (bytes / bw)^2)
+// with y' = q*ceil(y) + (1-q)*y, at least 1: the first tile of a CU takes its latency, and
+// several workgroups on a CU overlap those after it.
+struct TileTime {
+    int bm, bn;
+    double a, b, c1, c2, bw, q;
+};
+
+inline double tile_time(const TileTime &c, double y, double stages, double bytes) {
+    const double rounds = std::max(1.0, c.q * std::ceil(y - 1e-9) + (1.0 - c.q) * y);
+    const double work = c.a + c.b * stages + (c.c1 + c.c2 * stages) * (rounds - 1.0);
+    const double mem = bytes / (c.bw * 1e6);
+    return 2.0 + std::sqrt(work * work + mem * mem);
+}
+
 // The tile of a forward product, by the average rows of a group (the host does not know
 // more).  Times in us, graph-timed with rotating weights, as rows x groups x k x n with
 // k-contiguous / n-contiguous bf16 / MXFP4 weights.
@@ -1407,16 +1439,8 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         }
         GK_GO_ONCE(RingTile<16, 64, 1, 4, 4);
     }
-    int best = 0;
     double cost = 0;
-    for (int i = 0; i < 7; ++i) {
-        const double c = ragged_cost(kRaggedCost[MX ? 1 : 0][i], g, groups, avg, kbytes);
-        if (i == 0 || c < cost) {
-            best = i;
-            cost = c;
-        }
-    }
-    switch (best) {
+    switch (ragged_best<MX>(g, groups, avg, kbytes, &cost)) {
     case 1: GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
     case 2: GK_GO_ONCE(RingTile<128, 128, 2, 4, MX ? 2 : 4);
     case 3: GK_GO(RingTile<128, 256, 2, 4, 3>);

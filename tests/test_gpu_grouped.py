@@ -322,3 +322,37 @@ def run_wgrad(dev, offsets, rows, k, n, out, c_lay, alpha, beta, a_lay="r", b_la
             mags = abs(alpha) * (a[s:e].double().abs().t() @ b[s:e].double().abs())
         check(view, want + beta * base, mags, e - s, out, alpha, beta, base)
     assert same_bits(host[mask], cbuf[mask])
+
+
+def uneven(rows, groups):
+    """Group sizes that differ, an empty group among them where there are several."""
+    w = [0 if g == 1 else 1 + g * 7 % 5 for g in range(groups)]
+    sizes = [rows * v // sum(w) for v in w]
+    sizes[0] += rows - sum(sizes)
+    return sizes
+
+
+# products that reach each tile for rows of any alignment, and the copies
+@pytest.mark.parametrize("rows,groups,k,n,layout", [
+    (459, 8, 9, 3101, "co"), (6419, 5, 9, 65, "co"), (5722, 3, 9, 9, "co"), (459, 8, 333, 301, "co"),
+    (60, 8, 333, 301, "co"), (5, 3, 397, 9, "co"), (44, 7, 1397, 75, "co"), (404, 2, 11, 4345, "co"),
+    (2254, 8, 9, 985, "ro"), (8467, 51, 9, 89, "ro"), (867, 5, 209, 189, "ro"), (33, 3, 69, 9, "ro"),
+    (70, 3, 261, 77, "ro"), (23, 1, 3905, 9, "ro"), (4, 2, 517, 131, "ro"), (1500, 3, 129, 131, "ro"),
+])
+def test_tiles_for_any_alignment(dev, rows, groups, k, n, layout):
+    run_grouped(dev, offs(*uneven(rows, groups)), rows + 3, k, n, a_lay="ro", b_lay=layout, out=F32)
+
+
+# weight gradients that reach each tile, whole groups and ranges of them
+@pytest.mark.parametrize("rows,groups,k,n", [
+    (4, 35, 1288, 144), (6358, 1, 2088, 1688), (31, 32, 1032, 8), (7060, 1, 600, 1664), (9, 1, 8, 8),
+    (4637, 2, 320, 8), (35, 54, 264, 8), (8172, 1, 136, 5600), (86, 1, 8, 16), (2142, 1, 16, 16),
+    (9, 1, 9, 9), (635, 1, 9, 9), (9, 50, 69, 331), (8340, 4, 69, 327), (385, 2, 815, 2085),
+    (6358, 1, 2087, 481), (8, 40, 1731, 259), (7060, 1, 597, 1657), (2215, 5, 623, 139),
+    (8713, 1, 163, 211), (12, 44, 147, 631), (414, 1, 9, 9), (7833, 1, 9, 9), (3000, 2, 520, 1040),
+    (900, 3, 520, 1040), (1200, 3, 521, 1041),
+])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_wgrad_tiles(dev, rows, groups, k, n, out):
+    lay = "ro" if k % 8 else "r"
+    run_wgrad(dev, offs(*uneven(rows, groups)), rows + 3, k, n, out, "r", 1.0, 0.0, lay, lay)
