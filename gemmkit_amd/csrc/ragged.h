@@ -1440,6 +1440,18 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16)) {
             GK_GO_ONCE(WaveTile<16, 32, 4, 3);
         }
+        // Up to a tile per CU: MXFP4 in 64-row pieces of the weights, split alike: 8x1x4096x14336
+        // 8.4 against 10.0, 64x16x4096x896 8.1 / 9.8 (16 x 32: 10.0); n-contiguous weights do
+        // not gain (8x2x4096x8192 29.1 / 27.7).  Up to two: one of 128 columns instead, which a
+        // CU reads in longer pieces: - / 16.0 / 6.6 against - / 21.0 / 7.4 (12x12x1536x2560),
+        // - / 38.0 / 14.8 against - / 48.3 / 14.5 (8x4x4096x5120); k-contiguous ones do not
+        // (8x4x4096x5120 39.5 / 33.3).
+        if (MX && stages >= 8 && few <= cus) {
+            GK_GO_ONCE(WaveTile<16, 64, 4, 2);
+        }
+        if ((MX || BT) && few > cus && few <= 2 * cus) {
+            GK_GO_ONCE(RingTile<16, 128, 1, 4, 4);
+        }
         // n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more: 64x32x2048x4096
         // - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2 against
         // - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few tiles)

@@ -356,3 +356,11 @@ def test_tiles_for_any_alignment(dev, rows, groups, k, n, layout):
 def test_wgrad_tiles(dev, rows, groups, k, n, out):
     lay = "ro" if k % 8 else "r"
     run_wgrad(dev, offs(*uneven(rows, groups)), rows + 3, k, n, out, "r", 1.0, 0.0, lay, lay)
+
+
+@pytest.mark.parametrize("layout", ["c", "r"])
+@pytest.mark.parametrize("sizes,k,n", [((2, 0, 5, 1), 520, 5000), ((1, 2, 3), 72, 9000),
+                                       ((4,) * 12, 264, 2560), ((16,), 1032, 20000),
+                                       ((1,) * 9, 8, 3336)])
+def test_short_groups_of_many_columns(dev, sizes, k, n, layout):
+    run_grouped(dev, offs(*sizes), sum(sizes) + 2, k, n, b_lay=layout)

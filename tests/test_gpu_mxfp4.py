@@ -278,3 +278,16 @@ def test_degenerate_products(dev):
     assert (product(4, 6, 64, 0.0, 2.0) == 6.0).all()
     assert (product(0, 6, 64, 1.0, 0.0) == 3.0).all()
     assert (product(4, 0, 64, 1.0, 0.0) == 3.0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 9000, 2080), (16, 12288, 2300), (1, 14336, 2048), (5, 25000, 520),
+                                   (16, 32768, 96), (9, 20000, 31)])
+def test_short_products_of_many_columns(dev, m, n, k):
+    """Up to 16 rows on one or two 64-column tiles per compute unit."""
+    test_product(dev, m, n, k, F32, "row", 1.0, 0.0)
+
+
+@pytest.mark.parametrize("sizes,n,k", [((2, 0, 5, 1), 3000, 2080), ((1, 2, 3), 6000, 2100),
+                                       ((4,) * 12, 2560, 160), ((1,) * 9, 3333, 31)])
+def test_short_groups_of_many_columns(dev, sizes, n, k):
+    test_grouped_product(dev, sizes, n, k, BF16, "row", 1.0, 0.0)
