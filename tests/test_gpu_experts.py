@@ -430,3 +430,76 @@ def test_python_refusals(dev):
                       torch.zeros(8, 16, dtype=torch.uint8, device=dev), 8, 8)
     with pytest.raises(TypeError):
         gk.dequantize_mxfp4(bad, c)
+
+
+def test_two_graphs_share_a_workspace(dev):
+    """Replayed in turn, with eager work on the same workspace between them."""
+    ws = gk.Workspace.with_capacity(64 << 20)
+    steps = [build_step(dev, ws, False), build_step(dev, ws, True)]
+    gk.set_synchronous(False)
+    try:
+        for _, call, _ in steps:
+            call()
+        torch.cuda.synchronize()
+        want = [[o.clone() for o in outs] for outs, _, _ in steps]
+        graphs = [capture(call, torch.cuda.Stream()) for _, call, _ in steps]
+        for i in (0, 1, 1, 0, 1, 0):
+            for o in steps[i][0]:
+                o.fill_(7.0)
+            steps[1 - i][1]()
+            graphs[i].replay()
+            steps[1 - i][1]()
+            torch.cuda.synchronize()
+            for o, v in zip(steps[i][0], want[i]):
+                assert torch.equal(o, v)
+    finally:
+        gk.set_synchronous(True)
+
+
+def test_a_capture_cannot_grow_its_workspace(dev):
+    """Operands that have to be copied need a workspace of the size before the capture."""
+    rows, k, n = 64, 40, 48
+    a, w = rand(1, k, rows), rand(2, n, k)  # A column-major
+    c, off = torch.zeros(rows, n, dtype=BF16, device=dev), offsets_of([30, 34])
+    ws = gk.Workspace()
+
+    def call():
+        gk.gemm_grouped(1.0, gk.MatRef(a, rows, k, 1, rows), off, gk.MatRef(w, k, n, 1, k), 0, 0.0,
+                        gk.MatMut.from_row_major(c, rows, n), ws=ws)
+
+    gk.set_synchronous(False)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            with torch.cuda.graph(graph):
+                with pytest.raises(gk.GemmkitError, match="captur"):
+                    call()
+                c.fill_(3.0)
+        call()
+        torch.cuda.synchronize()
+        want = c.clone()
+        graph = capture(call, torch.cuda.Stream())
+        for _ in range(3):
+            c.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(c, want)
+    finally:
+        gk.set_synchronous(True)
+    at = torch.cat([a.t()[:30].double() @ w.double().t(), a.t()[30:].double() @ w.double().t()])
+    assert ((want.double() - at).abs() <= 2.0 ** -8 * at.abs() * 1.001 + 1e-4).all()
+
+
+def test_tensors_of_another_device_are_refused(dev, monkeypatch):
+    x = rand(1, 8, 32)
+    a, c = gk.MatRef.from_row_major(x, 8, 32), gk.MatMut.from_row_major(torch.zeros(8, 8, device=dev), 8, 8)
+    q, off = gk.quantize_mxfp4(a), offsets_of([8])
+    w = gk.MatRef(rand(2, 8, 32), 32, 8, 1, 32)
+    monkeypatch.setattr(gk, "_raw_stream", lambda device: 0)  # (there is no second device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: gk.gemm_grouped(1.0, a, off, w, 0, 0.0, c),
+                 lambda: gk.gemm_grouped_wgrad(1.0, a, off, a, 0.0, c, 0),
+                 lambda: gk.quantize_mxfp4(a, q), lambda: gk.gemm_mxfp4(1.0, q, q, 0.0, c),
+                 lambda: gk.gemm_grouped_mxfp4(1.0, q, off, q, 0.0, c)):
+        with pytest.raises(gk.GemmkitError, match="current device"):
+            call()
