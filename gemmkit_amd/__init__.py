@@ -1016,13 +1016,17 @@ def gemm_packed_a_fused_unchecked(alpha, packed: PackedLhs, n, b, rsb, csb, beta
 
 # -------------------------------------------- ragged groups, MXFP4 operands
 
-def _here(*tensors: torch.Tensor) -> None:
-    """The tensors of a call lie on the current device, whose stream it goes to."""
+def _bind_here(*tensors: torch.Tensor) -> None:
+    """_bind_stream for a call whose tensors must lie on the current device, whose stream it
+    goes to."""
+    if _raw_stream is None:
+        _init_streams()
     dev = torch.cuda.current_device()
     for t in tensors:
         if t.get_device() != dev and t.is_cuda:
             raise GemmkitError(-7, f"gemmkit_amd: a tensor lies on {t.device}, the current device "
                                    f"is cuda:{dev}")
+    _lib.lib().gk_set_stream(_raw_stream(dev))
 
 
 def _offsets(offsets: torch.Tensor):
@@ -1058,10 +1062,9 @@ def gemm_grouped(alpha: float, a: MatRef, offsets: torch.Tensor, b: MatRef, b_gr
 
     Weights stored output-major (n x k) are the view ``MatRef(w, k, n, 1, k)``.  The gradient
     of A is the same call on the output's gradient with ``MatRef(w, n, k, k, 1)``."""
-    _bind_stream()
     fn, dt = _out_entry(c, "gk_gemm_grouped_bf16", "gk_gemm_grouped_bf16_f32out", "gemm_grouped")
     off, groups = _offsets(offsets)
-    _here(a.data, b.data, c.data, offsets)
+    _bind_here(a.data, b.data, c.data, offsets)
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c(torch.bfloat16, "A"), off, groups,
                                    b._c(torch.bfloat16, "B"), b_group_stride, float(beta),
                                    c._c(dt, "C"), _par(par)))
@@ -1076,11 +1079,10 @@ def gemm_grouped_wgrad(alpha: float, a: MatRef, offsets: torch.Tensor, b: MatRef
     left operand), B rows x n (the gradient of its output), C_g the k x n view ``c`` moved by
     ``g * c_group_stride`` elements; bfloat16 inputs, f32 sums, bfloat16 or float32 C.  An
     empty group's C_g becomes ``beta * C_g``.  ``offsets`` as in :func:`gemm_grouped`."""
-    _bind_stream()
     fn, dt = _out_entry(c, "gk_gemm_grouped_wgrad_bf16", "gk_gemm_grouped_wgrad_bf16_f32out",
                         "gemm_grouped_wgrad")
     off, groups = _offsets(offsets)
-    _here(a.data, b.data, c.data, offsets)
+    _bind_here(a.data, b.data, c.data, offsets)
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c(torch.bfloat16, "A"), off, groups,
                                    b._c(torch.bfloat16, "B"), float(beta), c._c(dt, "C"),
                                    c_group_stride, _par(par)))
@@ -1112,9 +1114,9 @@ class MatMxfp4:
 
     def _c(self, what: str) -> Mxfp4C:
         codes, scales = _slice(self.codes, what), _slice(self.scales, what)
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
             raise TypeError(f"gemmkit_amd: {what} codes and scales must be uint8")
-        if min(self.rows, self.cols, self.ld, self.lds) < 0:
+        if self.rows < 0 or self.cols < 0 or self.ld < 0 or self.lds < 0:
             raise GemmkitError(-2, f"gemmkit_amd: {what} has a negative side or stride")
         return Mxfp4C(codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
                       self.rows, self.cols, self.ld, self.lds)
@@ -1127,7 +1129,6 @@ def quantize_mxfp4(x: MatRef, q: Optional[MatMxfp4] = None) -> MatMxfp4:
     ``e = max(floor(log2 m) - 2, -127)`` and every element the nearest e2m1 value of
     ``x / 2^e``, ties to the even code, magnitudes above 6 to 6; a block that holds a NaN or
     an infinity becomes NaN."""
-    _bind_stream()
     L = _lib.lib()
     dt = x.data.dtype
     if dt not in (torch.float32, torch.bfloat16):
@@ -1135,7 +1136,7 @@ def quantize_mxfp4(x: MatRef, q: Optional[MatMxfp4] = None) -> MatMxfp4:
     view = x._c(dt, "X")
     if q is None:
         q = MatMxfp4.empty(x.rows, x.cols, x.data.device)
-    _here(x.data, q.codes, q.scales)
+    _bind_here(x.data, q.codes, q.scales)
     fn = L.gk_quantize_mxfp4_f32 if dt == torch.float32 else L.gk_quantize_mxfp4_bf16
     _check(fn(view, q._c("MXFP4 output")))
     return q
@@ -1143,10 +1144,9 @@ def quantize_mxfp4(x: MatRef, q: Optional[MatMxfp4] = None) -> MatMxfp4:
 
 def dequantize_mxfp4(q: MatMxfp4, c: MatMut) -> None:
     """Extension: the values of q in c (float32 or bfloat16, any strides)."""
-    _bind_stream()
     fn, dt = _out_entry(c, "gk_dequantize_mxfp4_bf16", "gk_dequantize_mxfp4_f32",
                         "dequantize_mxfp4")
-    _here(c.data, q.codes, q.scales)
+    _bind_here(c.data, q.codes, q.scales)
     _check(getattr(_lib.lib(), fn)(q._c("MXFP4 input"), c._c(dt, "C")))
 
 
@@ -1154,9 +1154,8 @@ def gemm_mxfp4(alpha: float, a: MatMxfp4, b: MatMxfp4, beta: float, c: MatMut,
                par: Optional[Parallelism] = None, ws: Optional[Workspace] = None) -> None:
     """Extension: ``C <- alpha * A @ B^T + beta * C`` on MXFP4 operands, A m x k and B n x k (a
     linear layer's weight, output-major); f32 sums, bfloat16 or float32 C of any strides."""
-    _bind_stream()
     fn, dt = _out_entry(c, "gk_gemm_mxfp4_bf16", "gk_gemm_mxfp4_f32", "gemm_mxfp4")
-    _here(c.data, a.codes, a.scales, b.codes, b.scales)
+    _bind_here(c.data, a.codes, a.scales, b.codes, b.scales)
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), b._c("B"), float(beta),
                                    c._c(dt, "C"), _par(par)))
 
@@ -1166,10 +1165,9 @@ def gemm_grouped_mxfp4(alpha: float, a: MatMxfp4, offsets: torch.Tensor, b: MatM
                        ws: Optional[Workspace] = None) -> None:
     """Extension: :func:`gemm_grouped` on MXFP4 operands.  ``b`` holds the groups' n x k
     matrices one after the other (groups * n rows)."""
-    _bind_stream()
     fn, dt = _out_entry(c, "gk_gemm_grouped_mxfp4_bf16", "gk_gemm_grouped_mxfp4_f32",
                         "gemm_grouped_mxfp4")
     off, groups = _offsets(offsets)
-    _here(c.data, offsets, a.codes, a.scales, b.codes, b.scales)
+    _bind_here(c.data, offsets, a.codes, a.scales, b.codes, b.scales)
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), off, groups, b._c("B"),
                                    float(beta), c._c(dt, "C"), _par(par)))
