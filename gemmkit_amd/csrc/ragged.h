@@ -1043,52 +1043,64 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
 template <bool TR, int W, int NW>
 struct RegPanel {
     static constexpr int BYTES = W * 128, NI = BYTES / 1024, LP = (NI + NW - 1) / NW;
-    const uint8_t *base;  // of the next stage
-    int ld, left;         // row stride in bytes; contraction left: bytes, or rows (TR)
-    int lim;              // rows of the tile; TR: bytes of its columns that are in the matrix
+    static constexpr int kNone = INT32_MAX;
+    // 16 bytes before the next stage (a chunk across the end of a row is read back from that
+    // end, which may lie before the stage's first byte).
+    const uint8_t *base;
+    int ld, left;      // row stride in bytes; contraction left: bytes, or rows (TR)
+    uint32_t vo[LP];   // this lane's offsets from `base`
+    int pos[LP];       // where they lie in the contraction, kNone: outside the tile
+    int cut[TR ? LP : 1];  // TR: bytes of the chunk past the matrix's columns
     int wave, lane;
 
-    __device__ __forceinline__ void init(const uint8_t *b, int64_t ld_, int k, int lim_, int wave_,
+    // lim: rows of the tile; TR: bytes of its columns that are in the matrix
+    __device__ __forceinline__ void init(const uint8_t *b, int64_t ld_, int k, int lim, int wave_,
                                          int lane_) {
-        base = uniform(b);
+        base = uniform(b) - 16;
         ld = (int)ld_;
         left = k;
-        lim = lim_;
         wave = wave_;
         lane = lane_;
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const int at = (wave * LP + i) * 64 + lane;  // 16-byte slot of the stage
+            if constexpr (TR) {
+                const int row = at / (W / 8), slot = at % (W / 8);
+                const int ch = ((((slot >> 1) ^ tr_unit<W>(row)) << 1) | (slot & 1)) * 16;
+                cut[i] = lim - ch < 16 ? 16 - (lim - ch) : 0;
+                vo[i] = (uint32_t)(16 + row * ld + ch - cut[i]);
+                pos[i] = mine(i) && ch < lim ? row : kNone;
+            } else {
+                const int row = at / 8, ch = ((at % 8) ^ swz_of<128>(row)) * 16;
+                vo[i] = (uint32_t)(16 + row * ld + ch);
+                pos[i] = mine(i) && row < lim ? ch : kNone;
+            }
+        }
     }
     __device__ __forceinline__ bool mine(int i) const { return NI % NW == 0 || wave * LP + i < NI; }
+    // A chunk's last 16 - c bytes, moved to its beginning (c: 2 .. 14).
+    __device__ __forceinline__ static v4i shifted(v4i v, int c) {
+        typedef uint64_t v2l __attribute__((ext_vector_type(2)));
+        v2l w = __builtin_bit_cast(v2l, v);
+        const int s = c * 8;
+        w[0] = s >= 64 ? w[1] >> (s - 64) : w[0] >> s | w[1] << (64 - s);
+        w[1] = s >= 64 ? 0 : w[1] >> s;
+        return __builtin_bit_cast(v4i, w);
+    }
     __device__ __forceinline__ void load(v4i (&r)[LP]) {
         typedef int v4i_any2 __attribute__((ext_vector_type(4), aligned(2)));
 #pragma unroll
         for (int i = 0; i < LP; ++i) {
-            const int at = (wave * LP + i) * 64 + lane;  // 16-byte slot of the stage
-            int row, ch, valid;                          // valid: bytes of the chunk that exist
-            if constexpr (TR) {
-                row = at / (W / 8);
-                const int slot = at % (W / 8);
-                ch = ((((slot >> 1) ^ tr_unit<W>(row)) << 1) | (slot & 1)) * 16;
-                valid = row < left ? lim - ch : 0;
-            } else {
-                row = at / 8;
-                ch = ((at % 8) ^ swz_of<128>(row)) * 16;
-                valid = row < lim ? left - ch : 0;
-            }
             v4i v = {};
-            if (mine(i) && valid > 0) {
-                // A chunk across the row's end is read back from that end (rows have 16
-                // bytes or more) and shifted.
-                const int cut = valid < 16 ? 16 - valid : 0;
-                const int64_t off = (int64_t)row * ld + ch - cut;
-                v = *(const v4i_any2 *)(base + off);
-                if (cut) {
-                    typedef uint64_t v2l __attribute__((ext_vector_type(2)));
-                    v2l w = __builtin_bit_cast(v2l, v);
-                    const int s = cut * 8;  // 16 .. 112
-                    w[0] = s >= 64 ? w[1] >> (s - 64) : w[0] >> s | w[1] << (64 - s);
-                    w[1] = s >= 64 ? 0 : w[1] >> s;
-                    v = __builtin_bit_cast(v4i, w);
+            if constexpr (TR) {
+                if (pos[i] < left) {
+                    v = *(const v4i_any2 *)(base + vo[i]);
+                    if (cut[i]) v = shifted(v, cut[i]);
                 }
+            } else if (pos[i] < left) {
+                const int c = left - pos[i] < 16 ? 16 - (left - pos[i]) : 0;
+                v = *(const v4i_any2 *)(base + (vo[i] - (uint32_t)c));
+                if (c) v = shifted(v, c);
             }
             r[i] = v;
         }
@@ -1416,8 +1428,10 @@ template <bool MX, bool BT, EpiKind E>
 static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
 #define GK_GO(...) return ragged_go<MX, false, BT, E, __VA_ARGS__>(g, ep, stream)
 #define GK_GO_ONCE(...) \
-    if (once) GK_GO(__VA_ARGS__, true>); \
-    GK_GO(__VA_ARGS__>)
+    do { \
+        if (once) GK_GO(__VA_ARGS__, true>); \
+        GK_GO(__VA_ARGS__>); \
+    } while (0)
     const int64_t cus = g.cus;
     const int64_t groups = g.off ? (g.G < g.M ? g.G : g.M) : 1;
     const int64_t avg = (g.M + groups - 1) / groups;
@@ -1442,21 +1456,23 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
         }
         // Up to a tile per CU: MXFP4 in 64-row pieces of the weights, split alike: 8x1x4096x14336
         // 8.4 against 10.0, 64x16x4096x896 8.1 / 9.8 (16 x 32: 10.0); n-contiguous weights do
-        // not gain (8x2x4096x8192 29.1 / 27.7).  Up to two: one of 128 columns instead, which a
-        // CU reads in longer pieces: - / 16.0 / 6.6 against - / 21.0 / 7.4 (12x12x1536x2560),
-        // - / 38.0 / 14.8 against - / 48.3 / 14.5 (8x4x4096x5120); k-contiguous ones do not
-        // (8x4x4096x5120 39.5 / 33.3).
-        if (MX && stages >= 8 && few <= cus) {
-            GK_GO_ONCE(WaveTile<16, 64, 4, 2);
+        // not gain (8x2x4096x8192 29.1 / 27.7).
+        if constexpr (MX) {
+            if (stages >= 8 && few <= cus) GK_GO_ONCE(WaveTile<16, 64, 4, 2);
         }
-        if ((MX || BT) && few > cus && few <= 2 * cus) {
-            GK_GO_ONCE(RingTile<16, 128, 1, 4, 4);
-        }
-        // n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more: 64x32x2048x4096
-        // - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2 against
-        // - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few tiles)
-        if ((BT || (MX && avg > 4)) && even_tiles(g, avg, 64, 128) >= 2 * cus) {
-            GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
+        // Up to two: 128 columns instead, which a CU reads in longer pieces and in one tile:
+        // - / 16.0 / 6.6 against - / 21.0 / 7.4 (12x12x1536x2560), - / 38.0 / 14.8 against
+        // - / 48.3 / 14.5 (8x4x4096x5120); k-contiguous ones do not gain (39.5 / 33.3).  Where
+        // uneven groups of more rows need second tiles beyond those, 64 rows hold them:
+        // 64x8x4096x4096 - / 48 / 17.4 against - / 70 / 23.9.
+        // Many tiles: n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more:
+        // 64x32x2048x4096 - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2
+        // against - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few)
+        if constexpr (MX || BT) {
+            const bool two = few > cus && few <= 2 * cus;
+            if (two && (avg <= 4 || 2 * few <= 3 * cus)) GK_GO_ONCE(RingTile<16, 128, 1, 4, 4);
+            if (two || ((BT || avg > 4) && even_tiles(g, avg, 64, 128) >= 2 * cus))
+                GK_GO_ONCE(RingTile<64, 128, 2, 2, 3);
         }
         GK_GO_ONCE(RingTile<16, 64, 1, 4, 4);
     }

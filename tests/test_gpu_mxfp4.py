@@ -291,3 +291,7 @@ def test_short_products_of_many_columns(dev, m, n, k):
                                        ((4,) * 12, 2560, 160), ((1,) * 9, 3333, 31)])
 def test_short_groups_of_many_columns(dev, sizes, n, k):
     test_grouped_product(dev, sizes, n, k, BF16, "row", 1.0, 0.0)
+
+
+def test_groups_of_several_rows_over_many_columns(dev):
+    test_grouped_product(dev, (0, 20, 5, 11, 3, 9, 7, 9), 3900, 160, F32, "row", 1.0, 0.0)
