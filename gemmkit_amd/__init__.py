@@ -1092,7 +1092,9 @@ class MatMxfp4:
     """Extension: a rows x cols matrix in MXFP4.  Row r's elements are e2m1 codes (0, 0.5, 1,
     1.5, 2, 3, 4, 6 and their negatives), two a byte with the even element in the lower
     nibble, 16 bytes per begun block of 32, at ``codes + r * ld``; each block has an e8m0
-    scale byte (2^(byte - 127), 255: NaN) at ``scales + r * lds``.  ``codes`` and ``scales`` are
+    scale byte (2^(byte - 127), 255: NaN) at ``scales + r * lds``.  Codes past ``cols`` and
+    scales past the last block do not count, so the first columns of a matrix are a
+    ``MatMxfp4`` on the same arrays and strides.  ``codes`` and ``scales`` are
     contiguous uint8 device tensors, their row strides (bytes, multiples of 16) by default
     those of whole rows: ``16 * ceil(cols / 32)`` and ``ceil(cols / 32)`` rounded up to 16."""
 

@@ -473,6 +473,23 @@ __device__ __forceinline__ void read_scales(const uint8_t *sc, int row, int nv, 
     }
 }
 
+// A row's last block may hold codes past its k columns, which do not count: cleared in the W
+// rows of one operand of that stage, in LDS (a code of zero makes the other operand's
+// products there zero whatever they are).  Thread r does row r.  The kernels run that stage
+// behind their loops: a test in every stage costs up to 5% (and the 256 x 256 tile spills).
+template <int W>
+__device__ __forceinline__ void mx_cut(uint8_t *stage, int r, int k) {
+    if (r >= W) return;
+    v4i *const p = (v4i *)(stage + r * 128 + (((k >> 5 & 7) ^ swz_of<128>(r)) << 4));
+    v4i v = *p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = (k & 31) - 8 * i;  // codes of this word that count
+        v[i] = n >= 8 ? v[i] : (n <= 0 ? 0 : v[i] & ((1 << (4 * n)) - 1));
+    }
+    *p = v;
+}
+
 // acc[i][j] += the products of half SS of a stage.
 template <int SS>
 __device__ __forceinline__ v4f mx_half(v4i b, v4i a, v4f c, const ScaleQuad &y, const ScaleQuad &x,
@@ -631,6 +648,28 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
 
+    ScaleQuad xa[QA], xb[QB];
+    auto scales = [&](int kt, int par) {  // of stage kt, which has landed
+        const uint8_t *sc = smem + L::SCALES + r_slot * SP::SLOT + par * 8;
+        read_scales<QA, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
+        read_scales<QB, WTN>(sc, SP::A_ROWS + wn * WTN, nb - kt * 8, lane, xb);
+    };
+    auto half = [&](const uint8_t *sa, const uint8_t *sb, auto hh) {
+        constexpr int SS = decltype(hh)::value;
+        v4i af[TM], bf[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) bf[j] = fb.read(sb, j, SS);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) af[i] = fa.read(sa, i, SS);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = MX ? mx_half<SS>(bf[j], af[i], acc[i][j], xb[j / 4], xa[i / 4], i, j)
+                               : bf_step(bf[j], af[i], acc[i][j]);
+    };
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
     // Stage kt; PAR: kt's parity.  wr: the slot to load into, sa: the stage's own.  The two
     // differ, and `restrict` says so: else the compiler waits for every load in flight
     // before the transposing reads.
@@ -643,30 +682,12 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
         stage_barrier();
         if constexpr (MX && (PAR + NS - 1) % 2 == 0) load_scales();
         load_stage(wr);
-        const uint8_t *const sb = sa + PA::BYTES;
-        ScaleQuad xa[QA], xb[QB];
         if constexpr (MX) {
-            const uint8_t *sc = smem + L::SCALES + r_slot * SP::SLOT + PAR * 8;
+            scales(kt, PAR);
             if (PAR) r_slot = r_slot == L::NSS - 1 ? 0 : r_slot + 1;
-            read_scales<QA, WTM>(sc, wm * WTM, nb - kt * 8, lane, xa);
-            read_scales<QB, WTN>(sc, SP::A_ROWS + wn * WTN, nb - kt * 8, lane, xb);
         }
-        auto half = [&](auto hh) {
-            constexpr int SS = decltype(hh)::value;
-            v4i af[TM], bf[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) bf[j] = fb.read(sb, j, SS);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) af[i] = fa.read(sa, i, SS);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    acc[i][j] = MX ? mx_half<SS>(bf[j], af[i], acc[i][j], xb[j / 4], xa[i / 4], i, j)
-                                   : bf_step(bf[j], af[i], acc[i][j]);
-        };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
+        half(sa, sa + PA::BYTES, H0{});
+        half(sa, sa + PA::BYTES, H1{});
     };
 
 #pragma unroll
@@ -682,14 +703,24 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
         kstep(kt, par, smem + w * L::STAGE, smem + slot * L::STAGE);
         slot = slot == NS - 1 ? 0 : slot + 1;
     };
-    for (int kt = 0; kt < t.KT; kt += 2) {
-        step(kt, std::integral_constant<int, 0>{});
-        if (kt + 1 < t.KT) step(kt + 1, std::integral_constant<int, 1>{});
+    const int whole = MX && g.K % 32 ? t.KT - 1 : t.KT;  // stages without a cut block
+    for (int kt = 0; kt < whole; kt += 2) {
+        step(kt, H0{});
+        if (kt + 1 < whole) step(kt + 1, H1{});
     }
 
     // (the loads past the end of K, zeros into ring slots, land first)
     wait_vmcnt<0>();
     __syncthreads();
+    if (MX && whole < t.KT) {
+        uint8_t *const sa = smem + slot * L::STAGE;
+        mx_cut<BM>(sa, threadIdx.x, g.K);
+        __syncthreads();
+        scales(whole, whole & 1);
+        half(sa, sa + PA::BYTES, H0{});
+        half(sa, sa + PA::BYTES, H1{});
+        __syncthreads();
+    }
     if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
     else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
@@ -876,16 +907,32 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
         B.next();
         s = s1;
     };
+    const int whole = MX && g.K % 32 ? t.KT - 1 : t.KT;  // stages without a cut block
     auto stages = [&](auto one) {
-        for (int kt = 0; kt < t.KT; kt += 2) {
+        for (int kt = 0; kt < whole; kt += 2) {
             one(kt, I0{});
-            if (kt + 1 < t.KT) one(kt + 1, I1{});
+            if (kt + 1 < whole) one(kt + 1, I1{});
         }
     };
-    if (wm == 0 || t.rows > WTM) stages(step);
+    const bool idles = wm != 0 && t.rows <= WTM;
+    if (!idles) stages(step);
     else stages(idle);
     wait_vmcnt<0>();
     __syncthreads();
+    if (MX && whole < t.KT) {  // (its scales are in the registers, and half 0 uncut)
+        mx_cut<BM>(a_slot(s), threadIdx.x, g.K);
+        __syncthreads();
+        if (!idles) {
+            auto half = [&](auto hh) {
+                ops(a_slot(s), b_slot(whole & 1), hh, 0, FA{}, std::true_type{}, I0{}, [](int) {});
+                mfma_rows(hh, 0);
+                mfma_rows(hh, TM / 2);
+            };
+            half(I0{});
+            half(I1{});
+        }
+        __syncthreads();
+    }
     if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
     else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
 }
@@ -991,11 +1038,7 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
 
-    // (wr and sa differ: see ragged_kernel)
-    auto kstep = [&](int kt, uint8_t *__restrict__ wr, const uint8_t *__restrict__ s) {
-        wait_vmcnt<(NS - 2) * LPW>();
-        asm volatile("" ::: "memory");  // (no access moves over the wait)
-        load_stage(kt + (NS - 1) * KS, wr);
+    auto products = [&](int kt, const uint8_t *s) {  // of stage kt, which has landed
         ScaleQuad xa[QA], xb[QB];
         if constexpr (MX) {
             const uint8_t *sc = s + PA::BYTES + PB::BYTES + (kt & 1) * 8;
@@ -1019,15 +1062,29 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
     };
+    // (wr and sa differ: see ragged_kernel)
+    auto kstep = [&](int kt, uint8_t *__restrict__ wr, const uint8_t *__restrict__ s) {
+        wait_vmcnt<(NS - 2) * LPW>();
+        asm volatile("" ::: "memory");  // (no access moves over the wait)
+        load_stage(kt + (NS - 1) * KS, wr);
+        products(kt, s);
+    };
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) load_stage(wave + i * KS, ring + i * L::STAGE);
-    int slot = 0;
-    for (int kt = wave; kt < t.KT; kt += KS) {
+    int slot = 0, kt = wave;
+    const int whole = MX && g.K % 32 ? t.KT - 1 : t.KT;  // stages without a cut block
+    for (; kt < whole; kt += KS) {
         kstep(kt, ring + (slot == 0 ? NS - 1 : slot - 1) * L::STAGE, ring + slot * L::STAGE);
         slot = slot == NS - 1 ? 0 : slot + 1;
     }
 
     wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    if (MX && kt < t.KT) {  // this wave's: its LDS accesses take effect in order
+        mx_cut<BM>(ring + slot * L::STAGE, lane, g.K);
+        asm volatile("" ::: "memory");
+        products(kt, ring + slot * L::STAGE);
+    }
     __syncthreads();
     if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
     else wave_sums<E, false, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);

@@ -668,8 +668,9 @@ int gk_gemm_grouped_wgrad_bf16_f32out(gk_workspace *ws, float alpha, const gk_ma
  * with the even element in the lower nibble, at codes + r * ld; one e8m0 scale
  * (2^(byte - 127), 255: NaN) per 32 consecutive elements at scales + r * lds.
  * Strides are bytes, multiples of 16, and both arrays 16-byte aligned.  A row
- * holds 16 bytes of codes per begun block (elements past cols: zero codes)
- * and its scales padded to a multiple of 16 bytes (contents ignored).
+ * holds 16 bytes of codes per begun block and its scales padded to a multiple
+ * of 16 bytes; codes past cols and scales past the last block do not count
+ * (quantization writes zeros there).
  * codes_len and scales_len are the arrays' sizes in bytes. */
 typedef struct gk_mxfp4 {
     void *codes;
