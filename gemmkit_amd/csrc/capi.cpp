@@ -2200,6 +2200,13 @@ int64_t ragged_ld(const Opnd &o, int64_t R, int64_t K) {
     return R <= 1 ? round_up64(K * 2, 16) : o.rs * 2;
 }
 
+// The same of an operand whose rows run along a tile's columns: of a single row a tile reads
+// its own columns only (512 bytes at most), and any stride past those keeps the rows that
+// are not there out of range, however long the row is.
+int64_t ragged_ld_cols(const Opnd &o, int64_t R, int64_t K) {
+    return std::min(ragged_ld(o, R, K), R <= 1 ? int64_t(4096) : INT64_MAX);
+}
+
 int launch_failed(hipError_t e, const char *what) {
     if (e == hipErrorInvalidValue)
         return fail(GK_ERR_OVERFLOW, "gemmkit: %s: the product has more tiles than a launch takes",
@@ -2313,7 +2320,7 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
         }
         bl = cols_ok ? RaggedB::Cols : RaggedB::Rows;
         g.lda = ragged_ld(A, M, K);
-        g.ldb = cols_ok ? ragged_ld(Bc, K, N) : ragged_ld(Br, N, K);
+        g.ldb = cols_ok ? ragged_ld_cols(Bc, K, N) : ragged_ld(Br, N, K);
         g.bsb = (cols_ok ? Bc.bs : Br.bs) * 2;
     }
     g.a = A.p;

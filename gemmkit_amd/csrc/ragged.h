@@ -1373,7 +1373,7 @@ static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
     // 32-bit offsets inside a panel, with the loads of rows past its edge
     const int64_t kbytes = MX ? (int64_t)(g.K + 31) / 32 * 16 : (int64_t)g.K * 2;
     if ((AT ? 64 : BM) * g.lda + kbytes > (int64_t)kMaxRecords ||
-        (BT ? 64 * g.ldb + (int64_t)g.N * 2 : BN * g.ldb + kbytes) > (int64_t)kMaxRecords ||
+        (BT ? 64 * g.ldb + BN * 2 : BN * g.ldb + kbytes) > (int64_t)kMaxRecords ||
         (MX && 64 * (g.lsa > g.lsb ? g.lsa : g.lsb) > (int64_t)kMaxRecords))
         return hipErrorInvalidValue;
     const int64_t per =

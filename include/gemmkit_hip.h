@@ -632,8 +632,9 @@ int gk_gemm_packed_a_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha,
  * any other contents give disjoint groups inside the matrix too.  Groups may be
  * empty.  Rows before s_0 and from s_groups on belong to no group.
  *
- * Sizes: rows, groups, k and n below 2^31 - 1024; a bf16 row of k (and, for
- * wgrad, n) elements at most 4 MiB, a row of codes likewise.  GK_ERR_OVERFLOW
+ * Sizes: rows, groups, k and n at most 2^31 - 1025; a bf16 row of k (and, for
+ * wgrad, n) elements at most 4 MiB, a row of codes likewise; fewer than 2^31
+ * tiles in all (a weight gradient: fewer than 2^28 groups).  GK_ERR_OVERFLOW
  * beyond.
  */
 

@@ -1,0 +1,93 @@
+"""Grouped products at the edges of what their documentation allows: rows of one element
+with very many columns, group strides of any alignment, values below the normal range.
+Tolerances as in test_gpu_grouped.py."""
+import pytest
+import torch
+
+import gemmkit_amd as gk
+from test_gpu_grouped import bounds_of, check, offs, rand
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def offsets(sizes, dev):
+    return torch.tensor(offs(*sizes), dtype=torch.int32, device=dev)
+
+
+@pytest.mark.parametrize("k,n", [(1, 3_000_000), (1, 16_600_008), (1, 20_000_000), (1, 17_000_001),
+                                 (2, 17_000_000), (3, 17_000_001)])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_few_k_and_very_many_columns(dev, k, n, groups):
+    """Sums of up to three exact products: two roundings at most in f32."""
+    sizes = (2,) if groups == 1 else (2, 0, 1)
+    rows = sum(sizes)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a = torch.randn(rows, k, generator=g, device=dev).to(BF16)
+    b = torch.randn(groups, k, n, generator=g, device=dev).to(BF16)
+    c = torch.full((rows, n), float("nan"), device=dev)
+    gk.gemm_grouped(1.0, gk.MatRef.from_row_major(a, rows, k), offsets(sizes, dev),
+                    gk.MatRef.from_row_major(b, k, n), k * n, 0.0,
+                    gk.MatMut.from_row_major(c, rows, n))
+    for z, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
+        for r in range(s, e):
+            terms = a[r].double()[:, None] * b[z].double()
+            err = (c[r].double() - terms.sum(0)).abs()
+            assert (err <= (k - 1) * 2.0 ** -23 * terms.abs().sum(0)).all(), r
+
+
+def test_most_columns(dev):
+    """One row, one k, the most columns that the entry takes in whole 16 bytes."""
+    n = 2 ** 31 - 1024 - 8
+    g = torch.Generator(device="cuda").manual_seed(2)
+    a = torch.full((1, 1), -1.5, dtype=BF16, device=dev)
+    b = torch.empty(n, dtype=BF16, device=dev).random_(-64, 64, generator=g)
+    c = torch.full((n,), float("nan"), dtype=BF16, device=dev)
+    gk.gemm_grouped(1.0, gk.MatRef.from_row_major(a, 1, 1), offsets((1,), dev),
+                    gk.MatRef.from_row_major(b, 1, n), 0, 0.0, gk.MatMut.from_row_major(c, 1, n))
+    for at in range(0, n, 1 << 28):
+        assert torch.equal(c[at:at + (1 << 28)], b[at:at + (1 << 28)] * -1.5)
+
+
+@pytest.mark.parametrize("layout", ["c", "r"])
+@pytest.mark.parametrize("sizes,k,n", [((3, 0, 2), 64, 72), ((20, 33, 9), 200, 136), ((300, 0, 257), 520, 264),
+                                       ((1, 2, 1), 1032, 4000)])
+@pytest.mark.parametrize("more", [1, 4, 1000])
+def test_group_strides_of_any_alignment(dev, sizes, k, n, layout, more):
+    groups, rows = len(sizes), sum(sizes)
+    a, b = rand(1, rows, k), rand(2, groups, k, n)
+    step = k * n + more
+    buf = torch.full((groups * step,), float("nan"), dtype=BF16)
+    for g in range(groups):
+        flat = b[g] if layout == "r" else b[g].t().contiguous()
+        buf[g * step:g * step + k * n] = flat.flatten()
+    c = torch.full((rows, n), float("nan"), device=dev)
+    rs, cs = (n, 1) if layout == "r" else (1, k)
+    gk.gemm_grouped(1.0, gk.MatRef.from_row_major(a.to(dev), rows, k), offsets(sizes, dev),
+                    gk.MatRef(buf.to(dev), k, n, rs, cs), step, 0.0,
+                    gk.MatMut.from_row_major(c, rows, n))
+    for g, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
+        if e > s:
+            x, w = a[s:e].double(), b[g].double()
+            check(c[s:e].cpu(), x @ w, x.abs() @ w.abs(), k, F32, 1.0, 0.0, torch.zeros(e - s, n).double())
+
+
+@pytest.mark.parametrize("sizes", [(2, 1), (40, 30), (300, 200)])
+def test_values_below_the_normal_range(dev, sizes):
+    """Subnormal inputs count as what they are, and subnormal sums are kept."""
+    k, n, rows, groups = 64, 72, sum(sizes), len(sizes)
+    g = torch.Generator().manual_seed(3)
+
+    def ints(*shape):
+        return torch.randint(-3, 4, shape, generator=g).double()
+
+    for ea, eb in ((-133, 20), (-133, 0), (-70, -70), (20, -133)):
+        a, b = (ints(rows, k) * 2.0 ** ea).to(BF16), (ints(groups, k, n) * 2.0 ** eb).to(BF16)
+        c = torch.full((rows, n), float("nan"), device=dev)
+        gk.gemm_grouped(1.0, gk.MatRef.from_row_major(a.to(dev), rows, k), offsets(sizes, dev),
+                        gk.MatRef.from_row_major(b.to(dev), k, n), k * n, 0.0,
+                        gk.MatMut.from_row_major(c, rows, n))
+        for z, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
+            # whole numbers below 2^10 times a power of two of at least 2^-149: exact
+            assert torch.equal(c[s:e].cpu().double(), a[s:e].double() @ b[z].double()), (ea, eb)
