@@ -691,8 +691,8 @@ typedef struct gk_mxfp4 {
  * 255 and zero codes. */
 int gk_quantize_mxfp4_f32(const gk_mat_ref *x, const gk_mxfp4 *q);
 int gk_quantize_mxfp4_bf16(const gk_mat_ref *x, const gk_mxfp4 *q);
-/* The values of q in c: exact in f32 and, but for magnitudes below bf16's
- * smallest, in bf16. */
+/* The values of q in c, exact in f32 and in bf16; those of 2^128 and more (scale
+ * bytes 253 and 254, which quantization never writes) are infinite. */
 int gk_dequantize_mxfp4_f32(const gk_mxfp4 *q, const gk_mat_mut *c);
 int gk_dequantize_mxfp4_bf16(const gk_mxfp4 *q, const gk_mat_mut *c);
 

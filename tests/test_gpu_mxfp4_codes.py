@@ -17,9 +17,9 @@ NO_C = torch.zeros(())
 
 
 def spoiled(rows, k, seed, more=0):
-    """(codes, scales) of `more` blocks beyond k's own, no code past k zero but by chance."""
+    """(codes, scales) of `more` blocks beyond k's own, no code past k zero."""
     code, byte = random_mx(rows, (-(-k // 32) + more) * 32, seed)
-    code[:, k:] |= 1  # (an odd code is no zero)
+    code[:, k:] |= 1
     return code, byte
 
 
