@@ -121,6 +121,9 @@ __device__ __forceinline__ bool find_tile(const int32_t *off, int G, int M, int 
                 total = __builtin_amdgcn_readlane(incl, 63);
                 g = base;
                 if (pid < total * tiles_n) break;
+                // (Something wrote the offsets while the product runs, and this second
+                // reading has fewer tiles than the first.)
+                if (G - base <= 64) return false;
             }
         }
         // the first lane whose tiles reach past pid (one does: pid is below the total)
