@@ -123,6 +123,28 @@ def debug_plan(in_type: str, kind: str, m: int, n: int, kbytes: int, batch: int 
     return _PLAN_NAMES[t.value], na.value, _PLAN_NAMES[tb.value]
 
 
+_RAGGED_KERNELS = ("ring", "big", "wave", "reg", "regwave")
+_RAGGED_OPS = {"grouped_c": 0, "grouped_r": 1, "wgrad": 2, "mxfp4": 3}
+
+
+def debug_plan_grouped(op: str, rows: int, groups: int, k: int, n: int, out: str = "bf16",
+                       aligned: bool = True) -> str:
+    """Extension (no reference counterpart): what a product of ragged groups runs, as
+    "kernel ROWSxCOLS[xWAVES][ once][ /ranges][ any]".  op: "grouped_c" (k-contiguous weights),
+    "grouped_r" (n-contiguous), "wgrad", "mxfp4" (plain: one group); ``aligned``: operands of
+    16-byte alignment, else rows without any.  Kernels: "ring" of LDS stages, "big" (the
+    scheduled 256x256 tile), "wave" (K split over the waves of a workgroup), "reg" and
+    "regwave" (the first and the last for rows of any alignment, then with "any"); "once":
+    weights read nontemporally; "/ranges": row ranges per group of a weight gradient.
+    Host-only."""
+    p = (C.c_int32 * 7)()
+    _check(_lib.lib().gk_debug_plan_grouped(_RAGGED_OPS[op], rows, groups, k, n, out == "f32",
+                                            aligned, p))
+    return (f"{_RAGGED_KERNELS[p[0]]} {p[1]}x{p[2]}" + (f"x{p[3]}" if p[3] > 1 else "")
+            + (" once" if p[4] else "") + (f" /{p[5]}" if p[5] > 1 else "")
+            + (" any" if p[6] else ""))
+
+
 def set_synchronous(on: bool) -> None:
     """True (default): every call waits for its kernels, like the reference."""
     _lib.lib().gk_set_synchronous(1 if on else 0)

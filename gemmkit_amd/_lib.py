@@ -92,6 +92,8 @@ SIGNATURES: dict[str, tuple] = {
                                 C.c_int64, C.POINTER(C.c_int32), C.POINTER(C.c_int64),
                                 C.POINTER(C.c_int32), C.POINTER(C.c_int32),
                                 C.POINTER(C.c_int32)]),
+    "gk_debug_plan_grouped": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                                        C.c_int32, C.c_int32, C.POINTER(C.c_int32)]),
     "gk_init": (C.c_int, []),
     "gk_set_stream": (C.c_int, [_vp]),
     "gk_get_stream": (_vp, []),

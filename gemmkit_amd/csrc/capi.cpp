@@ -2698,6 +2698,55 @@ int gk_debug_plan(int32_t in, int32_t kind, int64_t m, int64_t n, int64_t batch,
     return ok();
 }
 
+int gk_debug_plan_grouped(int32_t op, int64_t rows, int64_t groups, int64_t k, int64_t n,
+                          int32_t f32_out, int32_t aligned, int32_t *plan) {
+    const int64_t lim = INT32_MAX - 1024;
+    if (op < 0 || op > 3 || rows <= 0 || groups <= 0 || k <= 0 || n <= 0 || rows > lim ||
+        groups > lim || k > lim || n > lim || !plan)
+        return fail(GK_ERR_ARG, "gemmkit: gk_debug_plan_grouped: bad argument");
+    static const int32_t some_offsets = 0;
+    RaggedArgs g{};
+    g.cus = g_num_cus;
+    g.splits = 1;
+    g.off = &some_offsets;  // (only whether there are any counts)
+    g.G = (int32_t)groups;
+    g.M = (int32_t)rows;
+    g.K = (int32_t)k;
+    g.N = (int32_t)n;
+    RaggedPlan p;
+    if (op == 3) {
+        p = mxfp4_plan(g);
+    } else if (op == 2) {
+        const bool in_place = aligned && k % 8 == 0 && n % 8 == 0;
+        const Opnd none{};
+        const size_t copies = in_place ? 0
+                                       : pack_bytes(InType::BF16, rows, k, 1, none) +
+                                             pack_bytes(InType::BF16, rows, n, 1, none);
+        wgrad_plan(g, f32_out ? EpiKind::F32 : EpiKind::BF16, !in_place && k >= 8 && n >= 8,
+                   (int64_t)copies);
+        p = grouped_wgrad_plan(g);
+    } else {
+        const bool cols = op == 1;
+        const bool in_place = aligned && k % 8 == 0 && (!cols || n % 8 == 0);
+        RaggedB bl = cols ? RaggedB::Cols : RaggedB::Rows;
+        if (!in_place) {
+            const bool unit = k >= 8 && (!cols || n >= 8);  // (rows of 16 bytes and more)
+            if (cols && n < 8) bl = RaggedB::Rows;
+            Opnd b{};
+            b.bs = 1;
+            const size_t copies = pack_bytes(InType::BF16, rows, k, 1, b) +
+                                  (bl == RaggedB::Cols
+                                       ? pack_bytes(InType::BF16, k, n, groups, b)
+                                       : pack_bytes(InType::BF16, n, k, groups, b));
+            g.any_align = unit && grouped_plan_any(g, bl, (int64_t)copies);
+        }
+        p = grouped_plan(g, bl);
+    }
+    const int32_t out[7] = {p.kind, p.bm, p.bn, p.ks, p.once, g.splits, g.any_align};
+    std::copy(out, out + 7, plan);
+    return ok();
+}
+
 int gk_init(void) {
     int r = device_init();
     return r ? r : ok();

@@ -47,15 +47,28 @@ bool grouped_plan_any(RaggedArgs &g, RaggedB bl, int64_t copies) {
     return cost < 4.6 + (double)copies / 2.49e6 + aligned;
 }
 
+template <typename F>
+static auto any_align_tile(const RaggedArgs &g, F f) {
+    switch (g.tile) {
+    case 0: return f(RegTile<128, 128, 2, 4>{});
+    case 1: return f(RegTile<128, 64, 4, 2>{});
+    case 2: return f(RegTile<32, 64, 1, 4>{});
+    case 3: return f(RegWaveTile<16, 32, 4>{});
+    default: return f(RegWaveTile<16, 32, 8>{});
+    }
+}
+
 template <bool BT, EpiKind E>
 static hipError_t any_align_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-    switch (g.tile) {
-    case 0: return ragged_go<false, false, BT, E, RegTile<128, 128, 2, 4>>(g, ep, stream);
-    case 1: return ragged_go<false, false, BT, E, RegTile<128, 64, 4, 2>>(g, ep, stream);
-    case 2: return ragged_go<false, false, BT, E, RegTile<32, 64, 1, 4>>(g, ep, stream);
-    case 3: return ragged_go<false, false, BT, E, RegWaveTile<16, 32, 4>>(g, ep, stream);
-    default: return ragged_go<false, false, BT, E, RegWaveTile<16, 32, 8>>(g, ep, stream);
-    }
+    return any_align_tile(
+        g, [&](auto t) { return ragged_go<false, false, BT, E, decltype(t)>(g, ep, stream); });
+}
+
+RaggedPlan grouped_plan(const RaggedArgs &g, RaggedB bl) {
+    const auto plan = [](auto t) { return plan_of(t); };
+    if (g.any_align) return any_align_tile(g, plan);
+    return bl == RaggedB::Cols ? forward_tile<false, true>(g, plan)
+                               : forward_tile<false, false>(g, plan);
 }
 
 hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams &ep,
@@ -122,19 +135,29 @@ void wgrad_plan(RaggedArgs &g, EpiKind out, bool can_any, int64_t copies) {
             }
 }
 
-template <EpiKind E>
-static hipError_t wgrad_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+template <typename F>
+static auto wgrad_tile(const RaggedArgs &g, F f) {
     if (g.any_align) {
-        if (g.tile == 0) return ragged_go<false, true, true, E, RegTile<64, 64, 2, 2>>(g, ep, stream);
-        return ragged_go<false, true, true, E, RegTile<128, 128, 2, 4>>(g, ep, stream);
+        if (g.tile == 0) return f(RegTile<64, 64, 2, 2>{});
+        return f(RegTile<128, 128, 2, 4>{});
     }
     switch (g.tile) {
-    case 0: return ragged_go<false, true, true, E, BigTile>(g, ep, stream);
-    case 1: return ragged_go<false, true, true, E, RingTile<128, 128, 2, 4, 2>>(g, ep, stream);
-    case 2: return ragged_go<false, true, true, E, RingTile<64, 64, 2, 2, 3>>(g, ep, stream);
-    case 3: return ragged_go<false, true, true, E, RingTile<64, 128, 2, 2, 2>>(g, ep, stream);
-    default: return ragged_go<false, true, true, E, WaveTile<32, 64, 4, 2>>(g, ep, stream);
+    case 0: return f(BigTile{});
+    case 1: return f(RingTile<128, 128, 2, 4, 2>{});
+    case 2: return f(RingTile<64, 64, 2, 2, 3>{});
+    case 3: return f(RingTile<64, 128, 2, 2, 2>{});
+    default: return f(WaveTile<32, 64, 4, 2>{});
     }
+}
+
+template <EpiKind E>
+static hipError_t wgrad_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+    return wgrad_tile(
+        g, [&](auto t) { return ragged_go<false, true, true, E, decltype(t)>(g, ep, stream); });
+}
+
+RaggedPlan grouped_wgrad_plan(const RaggedArgs &g) {
+    return wgrad_tile(g, [](auto t) { return plan_of(t); });
 }
 
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {

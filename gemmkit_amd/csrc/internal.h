@@ -269,6 +269,13 @@ hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams 
 // gradient with `out` output, given the bytes that aligned copies of its operands take.
 void wgrad_plan(RaggedArgs &g, EpiKind out, bool can_any, int64_t copies);
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
+// What such a launch runs: the kernel (ragged.h: 0 ring, 1 256 x 256, 2 K split over the waves,
+// 3 and 4 the same for rows of any alignment), its tile, how many waves K is split over, whether B is read nontemporally.
+struct RaggedPlan {
+    int kind, bm, bn, ks, once;
+};
+RaggedPlan grouped_plan(const RaggedArgs &g, RaggedB bl);  // (with g.any_align its g.tile)
+RaggedPlan grouped_wgrad_plan(const RaggedArgs &g);        // (as wgrad_plan left it)
 
 // MXFP4 (mxfp4.hip): rows of e2m1 codes, two a byte, the lower nibble first, with one
 // e8m0 scale per 32 elements.
@@ -283,5 +290,6 @@ hipError_t launch_mxfp4_quantize(InType in, const MxArgs &g, hipStream_t stream)
 hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stream);
 // C = epi(A B^T) of MXFP4 operands per group: K in elements, lda/ldb bytes of code rows.
 hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
+RaggedPlan mxfp4_plan(const RaggedArgs &g);
 
 }  // namespace gk

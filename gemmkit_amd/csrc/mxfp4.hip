@@ -263,6 +263,10 @@ hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stre
                                : mx_walk<InType::F32>(g, false, stream);
 }
 
+RaggedPlan mxfp4_plan(const RaggedArgs &g) {
+    return forward_tile<true, false>(g, [](auto t) { return plan_of(t); });
+}
+
 hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     if (ep.kind == EpiKind::BF16) return ragged_forward<true, false, EpiKind::BF16>(g, ep, stream);
     if (ep.kind == EpiKind::F32) return ragged_forward<true, false, EpiKind::F32>(g, ep, stream);

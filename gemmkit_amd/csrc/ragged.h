@@ -1481,12 +1481,12 @@ inline double tile_time(const TileTime &c, double y, double stages, double bytes
     return 2.0 + std::sqrt(work * work + mem * mem);
 }
 
-// The tile of a forward product, by the average rows of a group (the host does not know
+// f(the tile of a forward product), by the average rows of a group (the host does not know
 // more).  Times in us, graph-timed with rotating weights, as rows x groups x k x n with
 // k-contiguous / n-contiguous bf16 / MXFP4 weights.
-template <bool MX, bool BT, EpiKind E>
-static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
-#define GK_GO(...) return ragged_go<MX, false, BT, E, __VA_ARGS__>(g, ep, stream)
+template <bool MX, bool BT, typename F>
+static auto forward_tile(const RaggedArgs &g, F f) {
+#define GK_GO(...) return f(__VA_ARGS__{})
 #define GK_GO_ONCE(...) \
     do { \
         if (once) GK_GO(__VA_ARGS__, true>); \
@@ -1548,6 +1548,17 @@ static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipSt
     }
 #undef GK_GO_ONCE
 #undef GK_GO
+}
+
+template <bool MX, bool BT, EpiKind E>
+static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+    return forward_tile<MX, BT>(
+        g, [&](auto t) { return ragged_go<MX, false, BT, E, decltype(t)>(g, ep, stream); });
+}
+
+template <typename T>
+RaggedPlan plan_of(T) {
+    return RaggedPlan{T::KIND, T::BM, T::BN, T::KIND == 2 || T::KIND == 4 ? T::WN : 1, T::ONCE};
 }
 
 }  // namespace gk

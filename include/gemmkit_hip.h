@@ -66,6 +66,17 @@ int gk_debug_plan(int32_t in, int32_t kind, int64_t m, int64_t n, int64_t batch,
                   int64_t ld_b, int32_t *tile, int64_t *na, int32_t *tile_b, int32_t *pn_a,
                   int32_t *pn_b);
 
+/* The same of the products of ragged groups and of MXFP4 operands: `op` 0 a grouped product of
+ * k-contiguous weights, 1 of n-contiguous ones, 2 a weight gradient, 3 MXFP4 (plain:
+ * one group), with f32 or bf16 output, of operands that are 16-byte aligned or of rows without
+ * alignment.  plan[7]: kernel (0 ring of stages, 1 the scheduled 256 x 256 tile, 2 K split
+ * over the waves of a workgroup, 3 and 4 like 0 and 2 for rows of any alignment), tile rows,
+ * tile columns, waves that K is split over, whether the weights are read nontemporally, row
+ * ranges per group (weight gradient), whether operands without alignment are read as they
+ * are instead of copied.  Host-only, no device needed. */
+int gk_debug_plan_grouped(int32_t op, int64_t rows, int64_t groups, int64_t k, int64_t n,
+                          int32_t f32_out, int32_t aligned, int32_t *plan);
+
 /* ---------------------------------------------------------------- runtime */
 
 /* Parallelism request (src/parallel.rs:25): 1 = Serial, 0 = Rayon(0) "all",
