@@ -73,6 +73,58 @@ def test_group_strides_of_any_alignment(dev, sizes, k, n, layout, more):
             check(c[s:e].cpu(), x @ w, x.abs() @ w.abs(), k, F32, 1.0, 0.0, torch.zeros(e - s, n).double())
 
 
+def near(c, a, b, k):
+    """f32 rows of an MXFP4 product of the values a and b against 64 bits."""
+    a, b = a.double(), b.double()
+    want = a @ b.t()
+    tol = k * 2.0 ** -23 * (a.abs() @ b.abs().t()) + 2.0 ** -24 * want.abs()
+    assert ((c.double() - want).abs() <= tol).all()
+
+
+def mx_values(codes, scales, k):
+    rows = codes.shape[0]
+    v = torch.zeros(rows, k, device=codes.device)
+    gk.dequantize_mxfp4(gk.MatMxfp4(codes, scales, rows, k), gk.MatMut.from_row_major(v, rows, k))
+    return v
+
+
+def test_mxfp4_rows_past_32_bits(dev):
+    """Activations of more than 2^32 bytes: the last rows."""
+    rows, k, n, last = 2_200_000, 4096, 72, 300
+    g = torch.Generator(device="cuda").manual_seed(4)
+    codes = torch.zeros(rows, k // 2, dtype=torch.uint8, device=dev)
+    scales = torch.full((rows, k // 32), 120, dtype=torch.uint8, device=dev)
+    codes[-last:] = torch.randint(0, 256, (last, k // 2), generator=g, device=dev, dtype=torch.uint8)
+    wc = torch.randint(0, 256, (2 * n, k // 2), generator=g, device=dev, dtype=torch.uint8)
+    ws = torch.randint(115, 130, (2 * n, k // 32), generator=g, device=dev, dtype=torch.uint8)
+    c = torch.full((rows, n), float("nan"), device=dev)
+    gk.gemm_grouped_mxfp4(1.0, gk.MatMxfp4(codes, scales, rows, k), offsets((rows - 100, 100), dev),
+                          gk.MatMxfp4(wc, ws, 2 * n, k), 0.0, gk.MatMut.from_row_major(c, rows, n))
+    av, wv = mx_values(codes[-last:], scales[-last:], k), mx_values(wc, ws, k)
+    near(c[-last:-100], av[:-100], wv[:n], k)
+    near(c[-100:], av[-100:], wv[n:], k)
+    assert not c[:-last].any()
+
+
+def test_mxfp4_weights_past_32_bits(dev):
+    """Weights of more than 2^32 bytes: the last group's."""
+    groups, k, n = 300, 4096, 8192
+    g = torch.Generator(device="cuda").manual_seed(5)
+    wc = torch.zeros(groups * n, k // 2, dtype=torch.uint8, device=dev)
+    ws = torch.full((groups * n, k // 32), 120, dtype=torch.uint8, device=dev)
+    wc[-n:] = torch.randint(0, 256, (n, k // 2), generator=g, device=dev, dtype=torch.uint8)
+    for rows in (20, 700):  # all but one of the last group
+        ac = torch.randint(0, 256, (rows, k // 2), generator=g, device=dev, dtype=torch.uint8)
+        asc = torch.randint(115, 130, (rows, k // 32), generator=g, device=dev, dtype=torch.uint8)
+        c = torch.full((rows, n), float("nan"), device=dev)
+        gk.gemm_grouped_mxfp4(1.0, gk.MatMxfp4(ac, asc, rows, k),
+                              offsets((1,) + (0,) * (groups - 2) + (rows - 1,), dev),
+                              gk.MatMxfp4(wc, ws, groups * n, k), 0.0,
+                              gk.MatMut.from_row_major(c, rows, n))
+        near(c[1:], mx_values(ac, asc, k)[1:], mx_values(wc[-n:], ws[-n:], k), k)
+        assert not c[:1].any()
+
+
 @pytest.mark.parametrize("sizes", [(2, 1), (40, 30), (300, 200)])
 def test_values_below_the_normal_range(dev, sizes):
     """Subnormal inputs count as what they are, and subnormal sums are kept."""
