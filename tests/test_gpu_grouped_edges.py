@@ -143,3 +143,75 @@ def test_values_below_the_normal_range(dev, sizes):
         for z, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
             # whole numbers below 2^10 times a power of two of at least 2^-149: exact
             assert torch.equal(c[s:e].cpu().double(), a[s:e].double() @ b[z].double()), (ea, eb)
+
+
+@pytest.mark.parametrize("sizes,k,n", [((3, 0, 2), 64, 72), ((40, 33, 9), 200, 136), ((300, 0, 257), 96, 264)])
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("beta", [0.0, -0.5])
+def test_output_of_any_strides(dev, sizes, k, n, out, beta):
+    """C with neither stride 1: elements between stay as they are, for all three products."""
+    rows, groups = sum(sizes), len(sizes)
+    bounds = bounds_of(offs(*sizes), rows)
+    a, b = rand(1, rows, k), rand(2, groups, k, n)
+    for rs, cs in ((2 * n + 1, 2), (3, 3 * rows + 1)):
+        buf0 = torch.randn((rows - 1) * rs + (n - 1) * cs + 1, generator=torch.Generator().manual_seed(3)).to(out)
+        buf = buf0.to(dev)
+        gk.gemm_grouped(1.0, gk.MatRef.from_row_major(a.to(dev), rows, k), offsets(sizes, dev),
+                        gk.MatRef.from_row_major(b.to(dev), k, n), k * n, beta,
+                        gk.MatMut(buf, rows, n, rs, cs))
+        got, old = buf.cpu(), torch.as_strided(buf0, (rows, n), (rs, cs)).double()
+        view = torch.as_strided(got, (rows, n), (rs, cs))
+        for g, (s, e) in enumerate(bounds):
+            if e > s:
+                x, w = a[s:e].double(), b[g].double()
+                check(view[s:e], x @ w + beta * old[s:e], x.abs() @ w.abs(), k, out, 1.0, beta, old[s:e])
+        mask = torch.ones(buf0.numel(), dtype=torch.bool)
+        torch.as_strided(mask, (rows, n), (rs, cs)).fill_(False)
+        assert torch.equal(got[mask], buf0[mask])
+    d = rand(4, rows, n)
+    for rs, cs in ((2 * n + 1, 2), (3, 3 * k + 1)):
+        step = (k - 1) * rs + (n - 1) * cs + 4
+        buf0 = torch.randn(groups * step, generator=torch.Generator().manual_seed(5)).to(out)
+        buf = buf0.to(dev)
+        gk.gemm_grouped_wgrad(1.0, gk.MatRef.from_row_major(a.to(dev), rows, k), offsets(sizes, dev),
+                              gk.MatRef.from_row_major(d.to(dev), rows, n), beta,
+                              gk.MatMut(buf, k, n, rs, cs), step)
+        got, mask = buf.cpu(), torch.ones(buf0.numel(), dtype=torch.bool)
+        for g, (s, e) in enumerate(bounds):
+            old = torch.as_strided(buf0, (k, n), (rs, cs), g * step).double()
+            x, w = a[s:e].double().t(), d[s:e].double()
+            check(torch.as_strided(got, (k, n), (rs, cs), g * step), x @ w + beta * old,
+                  x.abs() @ w.abs(), e - s, out, 1.0, beta, old)
+            torch.as_strided(mask, (k, n), (rs, cs), g * step).fill_(False)
+        assert torch.equal(got[mask], buf0[mask])
+
+
+@pytest.mark.parametrize("sizes", [(3, 0, 2), (40, 30), (300, 100)])
+def test_operands_that_overlap_themselves(dev, sizes):
+    """Broadcast and sliding rows, columns and group matrices."""
+    rows, k, n, groups = sum(sizes), 72, 88, len(sizes)
+    flat, w = rand(1, rows + k + 8), rand(2, groups, k + n + 8)
+    for a_rs, a_cs in ((0, 1), (1, 1), (1, 0), (0, 0), (1, 2)):
+        for b_rs, b_cs, b_gs in ((0, 1, 168), (1, 0, 168), (1, 1, 168), (1, 1, 3), (0, 0, 1)):
+            if a_rs * (rows - 1) + a_cs * (k - 1) >= flat.numel():
+                continue
+            c = torch.full((rows, n), float("nan"), device=dev)
+            gk.gemm_grouped(1.0, gk.MatRef(flat.to(dev), rows, k, a_rs, a_cs), offsets(sizes, dev),
+                            gk.MatRef(w.to(dev), k, n, b_rs, b_cs), b_gs, 0.0,
+                            gk.MatMut.from_row_major(c, rows, n))
+            a = torch.as_strided(flat, (rows, k), (a_rs, a_cs)).double()
+            for g, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
+                if e > s:
+                    b = torch.as_strided(w, (k, n), (b_rs, b_cs), g * b_gs).double()
+                    check(c[s:e].cpu(), a[s:e] @ b, a[s:e].abs() @ b.abs(), k, F32, 1.0, 0.0,
+                          torch.zeros(e - s, n).double())
+        d = rand(3, rows + n + 8)
+        c = torch.full((groups, k, n), float("nan"), device=dev)
+        if a_rs * (rows - 1) + a_cs * (k - 1) < flat.numel():
+            gk.gemm_grouped_wgrad(1.0, gk.MatRef(flat.to(dev), rows, k, a_rs, a_cs), offsets(sizes, dev),
+                                  gk.MatRef(d.to(dev), rows, n, 1, 1), 0.0,
+                                  gk.MatMut.from_row_major(c, k, n), k * n)
+            dv = torch.as_strided(d, (rows, n), (1, 1)).double()
+            for g, (s, e) in enumerate(bounds_of(offs(*sizes), rows)):
+                x, y = a[s:e].t(), dv[s:e]
+                check(c[g].cpu(), x @ y, x.abs() @ y.abs(), e - s, F32, 1.0, 0.0, torch.zeros(k, n).double())

@@ -1,10 +1,10 @@
 """MXFP4 over the whole range of its scales: every scale byte with every code, blocks below the
-normal range, products whose scales meet at either end."""
+normal range, products whose scales meet at either end; and matrices whose rows lie apart."""
 import pytest
 import torch
 
 import gemmkit_amd as gk
-from test_gpu_mxfp4 import mx, quantize_ref, random_mx, unpack, values_of
+from test_gpu_mxfp4 import mx, quantize_ref, random_mx, sample, unpack, values_of
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,35 @@ def test_products_over_the_range_of_scales(dev, m):
     assert torch.equal(got[normal], want[normal])
     low = scale - 2 < -126
     assert ((got - want)[low].abs() <= 64 * 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("rows,k", [(1, 33), (7, 1000), (70, 520), (300, 96), (5, 4100)])
+@pytest.mark.parametrize("how", ["row", "col", "odd", "one"])
+def test_rows_of_codes_that_lie_apart(dev, dt, rows, k, how):
+    """Quantization writes a row's blocks and its padded scales, nothing between the rows;
+    "one": every row is the same memory."""
+    nb = -(-k // 32)
+    ld, lds = nb * 16 + 48, -(-nb // 16) * 16 + 32
+    x = sample(rows, k, dt, 7)
+    if how == "one":
+        x = x[:1].expand(rows, k)
+        t, rs, cs = x[0].contiguous().to(dev), 0, 1
+    elif how == "col":
+        t, rs, cs = x.t().contiguous().flatten().to(dev), 1, rows
+    else:
+        rs, cs = k + (how == "odd"), 1
+        t = torch.zeros(rows, rs, dtype=dt)
+        t[:, :k] = x
+        t = t.flatten().to(dev)
+    codes = torch.full((rows, ld), 0x5A, dtype=torch.uint8, device=dev)
+    scales = torch.full((rows, lds), 0x5A, dtype=torch.uint8, device=dev)
+    q = gk.MatMxfp4(codes, scales, rows, k, ld, lds)
+    gk.quantize_mxfp4(gk.MatRef(t, rows, k, rs, cs), q)
+    code, byte = unpack(q)
+    want_code, want_byte = quantize_ref(x)
+    assert torch.equal(code, want_code) and torch.equal(byte, want_byte)
+    assert (codes[:, nb * 16:] == 0x5A).all() and (scales[:, -(-nb // 16) * 16:] == 0x5A).all()
+    back = torch.zeros(rows, k, device=dev)
+    gk.dequantize_mxfp4(q, gk.MatMut.from_row_major(back, rows, k))
+    assert torch.equal(back.cpu().double(), values_of(want_code, want_byte)[:, :k])
