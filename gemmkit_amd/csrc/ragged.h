@@ -517,9 +517,10 @@ __device__ __forceinline__ bool whole_lines(const EpiParams &ep) {
 }
 
 // A chunk of one row of C; NT: stored nontemporally.  Written through the L2 the output
-// pushes the operand panels out of it (weight gradient 16384x8x4096x4096 with f32 output 512
-// against 443 us), but pieces of lines have to meet there (rows of 9632 bytes,
-// 39x56x512x2408: 97 us nontemporally, 60 without).  bf16 takes 16 bytes here instead of
+// pushes the operand panels out of it (weight gradients in turn on one card: 16384x8x4096x4096
+// with f32 output 519 against 459 us, 1003x32x1024x704 with bf16 output 18.8 against 16.0), but
+// pieces of lines have to meet there (rows of 9632 bytes, 39x56x512x2408: 97 us
+// nontemporally, 60 without).  bf16 takes 16 bytes here instead of
 // store4's 8: a weight gradient of short groups is bound by its stores (32 x 1024 x 1024 bf16
 // from 64 rows: 21.8 us with 8 bytes a lane).
 template <EpiKind E, bool NT>
@@ -590,9 +591,10 @@ __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTi
 // ---------------------------------------------------------------- small tiles
 
 // BM x BN tiles on a ring of NS stages: stage kt + NS - 1 is loaded while kt is multiplied, one
-// barrier a stage.  Bound by loads in flight where groups are short: 16 x 64 reads 64x32x2048x4096's
-// 4-bit weights at 4.7 TB/s (23.9 us); small outputs leave the CUs' matrix cores waiting for
-// their first stages (1003x32x1024x704's weight gradient 16.5 us, 2.8 TB/s of stores).
+// barrier a stage.  Bound by loads in flight where groups are short: 16 x 64, nontemporal, reads
+// 64x32x2048x4096's 4-bit weights (107 MB of the 24 groups that have rows) in 21.9 us, 4.9 TB/s;
+// small outputs leave the CUs' matrix cores waiting for their first stages (1003x32x1024x704's
+// weight gradient 16.0 us, 2.9 TB/s of stores).
 template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS, bool ONCE>
 __global__ __launch_bounds__(WM * WN * 64)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedLds<MX, BM, BN, NS>::BYTES, WM * WN),
@@ -737,9 +739,12 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
 //   phase 2  half 1, block rows 0-3   then waits for stage kt+1, barrier
 //   phase 3  half 1, block rows 4-7   reads half 0 of stage kt+1; loads the rest of kt+2
 // bf16: three A slots and two B slots, all of the LDS; MXFP4: two of each and the scales.
-// Bound by the matrix cores at the clock that the power limit leaves: a full round's stage takes
-// 1.39 us (bf16) or 1.76 us (MXFP4, four times the k), 8192 x 4096 x 8192 367 and 130 us (1.50 and
-// 4.2 PFLOP/s); prologue, epilogue and launch take 7 to 9 us.
+// A full round's stage, 2048 cycles of matrix instructions on each SIMD, takes 1.39 us (bf16) or
+// 1.76 us (MXFP4, four times the k): 8192 x 4096 x 8192 367 and 130 us (1.50 and 4.2 PFLOP/s);
+// prologue, epilogue and launch take 7 to 9 us.  bf16 is bound by the matrix cores, 0.8 of them
+// at the 1.8 GHz that the power limit leaves.  MXFP4 is not: at 2.08 GHz a stage is 3660 cycles,
+// of which the scales' LDS reads, waits and lane swaps at its end, and eight loads and twelve
+// fragment reads in one phase, take their part.
 template <bool MX>
 struct RaggedBigLds {
     static constexpr int NSA = MX ? 2 : 3, NSB = 2, OP = 256 * 128;
@@ -946,7 +951,8 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
 // workgroup share one BM x BN tile and split K among them, stage kt to wave kt % KS.  Each
 // wave fills its own ring of NS stages and waits for nothing but its own loads (no
 // barriers); their sums are added in wave order through LDS at the end.  Bound by latency:
-// 8x64x2048x1024 5.1 us, 6.6 TB/s of the eight matrices that are used.
+// 8x64x2048x1024 7.6 us (3.9 TB/s of the seven matrices that are used), 5.2 where the caches
+// hold them from the call before.
 template <EpiKind E, bool NT, int BM, int BN, int KS, int TM, int TN>
 __device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile &t, int N,
                                           const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
@@ -1482,8 +1488,12 @@ inline double tile_time(const TileTime &c, double y, double stages, double bytes
 }
 
 // f(the tile of a forward product), by the average rows of a group (the host does not know
-// more).  Times in us, graph-timed with rotating weights, as rows x groups x k x n with
-// k-contiguous / n-contiguous bf16 / MXFP4 weights.
+// more).  Times in us, graph-timed with rotating weights on one card, as rows x groups x k x n
+// with k-contiguous / n-contiguous bf16 / MXFP4 weights.  For up to 16 rows a group the
+// rules below took 1.08 / 1.12 / 1.05 times the fastest of 9 to 13 tiles in the geometric mean
+// (103 products, 1..128 groups, k and n 128..8192; 1.45 at worst), and 1.12 / 1.13 / 1.08 where
+// one group has eight ninths of the rows (47 products; 1.71 at worst: tiles follow the average
+// group, and that one reads its weights again every 16 rows).
 template <bool MX, bool BT, typename F>
 static auto forward_tile(const RaggedArgs &g, F f) {
 #define GK_GO(...) return f(__VA_ARGS__{})
@@ -1497,37 +1507,38 @@ static auto forward_tile(const RaggedArgs &g, F f) {
     const int64_t avg = (g.M + groups - 1) / groups;
     const int64_t kbytes = MX ? (int64_t)g.K / 2 : (int64_t)g.K * 2, stages = (kbytes + 127) / 128;
     // Weights that tiles of 64 rows read once, and that would fill half of the 256 MB
-    // Infinity Cache, go past it: 64x32x2048x4096 72.7 / 73.3 / 24.6 against 65.6 / 66.0 / 22.6,
-    // 16x8x4096x11008 107 / 124 / 33.9 against 96 / 113 / 31.6.  Smaller ones stay there from
-    // one call to the next, and are read again by every further tile: 150x3x2048x2048
-    // 11.3 / 11.6 / 6.7 against 13.6 / 15.2 / 7.1 nontemporally.
+    // Infinity Cache, go past it: on the tiles picked 64x32x2048x4096 takes 72.4 / 70.9 / 23.8
+    // through it and 64.4 / 63.8 / 21.9 past it, 16x8x4096x11008 111 / 120 / 32.7 and
+    // 97 / 110 / 30.6.  Smaller ones stay there from one call to the next, and are read again
+    // by every further tile: 150x3x2048x2048 on 64 x 128 13.7 / 14.4 / 8.0 through it, 17.8 /
+    // 18.3 / 8.2 past it.
     const bool once = avg <= 64 && groups * g.N * kbytes >= (int64_t(128) << 20);
     if (avg <= 16) {
         // One 16-row tile per group: the weights are read once, HBM-bound.  Where K is split
         // over the waves nothing waits at barriers and a few tiles keep many loads in
-        // flight: 8x64x2048x1024 7.4 / 8.9 / 4.9 against 9.6 / 8.8 / 6.5 on the ring,
-        // 64x32x2048x4096 71 / 86 / 44 against 78 / 83 / 25.  It reads 64-byte pieces
+        // flight: 8x64x2048x1024 7.6 / 9.0 / 5.1 against 9.5 / 8.8 / 6.4 on the ring,
+        // 64x32x2048x4096 64 / 94 / 44 against 66 / 70 / 22.  It reads 64-byte pieces
         // of n-contiguous rows (32 columns) and a scale load per stage, so those two
         // layouts take it for few tiles only, and k of few stages never (128x100x512x600
-        // 15.4 / 17.1 / 16.9 against 11.1 / 12.5 / 7.0).
+        // 15.1 / 15.3 / 17.2 against 10.5 / 11.0 / 6.8).
         const int64_t few = even_tiles(g, avg, 16, 64);
         if (stages >= 8 && (MX ? few <= cus / 2 : BT ? few <= cus / 4 : stages >= 16)) {
             GK_GO_ONCE(WaveTile<16, 32, 4, 3);
         }
         // Up to a tile per CU: MXFP4 in 64-row pieces of the weights, split alike: 8x1x4096x14336
-        // 8.4 against 10.0, 64x16x4096x896 8.1 / 9.8 (16 x 32: 10.0); n-contiguous weights do
-        // not gain (8x2x4096x8192 29.1 / 27.7).
+        // 8.3 against 9.5 on the ring, 64x16x4096x896 8.0 / 9.4 (16 x 32: 10.0); n-contiguous
+        // weights do not gain (8x2x4096x8192 29.1 / 27.7).
         if constexpr (MX) {
             if (stages >= 8 && few <= cus) GK_GO_ONCE(WaveTile<16, 64, 4, 2);
         }
         // Up to two: 128 columns instead, which a CU reads in longer pieces and in one tile:
-        // - / 16.0 / 6.6 against - / 21.0 / 7.4 (12x12x1536x2560), - / 38.0 / 14.8 against
-        // - / 48.3 / 14.5 (8x4x4096x5120); k-contiguous ones do not gain (39.5 / 33.3).  Where
+        // - / 15.7 / 6.6 against - / 21.5 / 7.3 (12x12x1536x2560), - / 34.4 / 11.2 against
+        // - / 42.8 / 12.4 (8x4x4096x5120); k-contiguous ones do not gain (39.5 / 33.3).  Where
         // uneven groups of more rows need second tiles beyond those, 64 rows hold them:
-        // 64x8x4096x4096 - / 48 / 17.4 against - / 70 / 23.9.
+        // 64x8x4096x4096 - / 42 / 16.4 against - / 62 / 23.8.
         // Many tiles: n-contiguous rows in 256-byte pieces, MXFP4 tiles of 8 rows and more:
-        // 64x32x2048x4096 - / 74 / 24.5 against - / 83 / 24.9, 256x32x2048x2048 - / 51 / 18.2
-        // against - / 54 / 19.1; 8x1x4096x14336 - / 37 / 12.7 against - / 25 / 9.9 (too few)
+        // 64x32x2048x4096 - / 64 against - / 70, 256x32x2048x2048 - / 44 / 17.1 against
+        // - / 48 / 18.7; 8x1x4096x14336 - / 35 / 12.0 against - / 26 / 9.5 (too few)
         if constexpr (MX || BT) {
             const bool two = few > cus && few <= 2 * cus;
             if (two && (avg <= 4 || 2 * few <= 3 * cus)) GK_GO_ONCE(RingTile<16, 128, 1, 4, 4);
