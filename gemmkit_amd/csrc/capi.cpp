@@ -2717,27 +2717,25 @@ int gk_debug_plan_grouped(int32_t op, int64_t rows, int64_t groups, int64_t k, i
     if (op == 3) {
         p = mxfp4_plan(g);
     } else if (op == 2) {
-        const bool in_place = aligned && k % 8 == 0 && n % 8 == 0;
-        const Opnd none{};
-        const size_t copies = in_place ? 0
-                                       : pack_bytes(InType::BF16, rows, k, 1, none) +
-                                             pack_bytes(InType::BF16, rows, n, 1, none);
-        wgrad_plan(g, f32_out ? EpiKind::F32 : EpiKind::BF16, !in_place && k >= 8 && n >= 8,
-                   (int64_t)copies);
+        const bool a_ok = aligned && k % 8 == 0, b_ok = aligned && n % 8 == 0;
+        const Opnd o{};
+        const size_t copies = (a_ok ? 0 : pack_bytes(InType::BF16, rows, k, 1, o)) +
+                              (b_ok ? 0 : pack_bytes(InType::BF16, rows, n, 1, o));
+        wgrad_plan(g, f32_out ? EpiKind::F32 : EpiKind::BF16,
+                   (!a_ok || !b_ok) && k >= 8 && n >= 8, (int64_t)copies);
         p = grouped_wgrad_plan(g);
     } else {
         const bool cols = op == 1;
-        const bool in_place = aligned && k % 8 == 0 && (!cols || n % 8 == 0);
+        const bool a_ok = aligned && k % 8 == 0, b_ok = aligned && (cols ? n : k) % 8 == 0;
         RaggedB bl = cols ? RaggedB::Cols : RaggedB::Rows;
-        if (!in_place) {
+        if (!a_ok || !b_ok) {
             const bool unit = k >= 8 && (!cols || n >= 8);  // (rows of 16 bytes and more)
             if (cols && n < 8) bl = RaggedB::Rows;
-            Opnd b{};
-            b.bs = 1;
-            const size_t copies = pack_bytes(InType::BF16, rows, k, 1, b) +
-                                  (bl == RaggedB::Cols
-                                       ? pack_bytes(InType::BF16, k, n, groups, b)
-                                       : pack_bytes(InType::BF16, n, k, groups, b));
+            Opnd o{};
+            o.bs = 1;
+            const size_t pb = bl == RaggedB::Cols ? pack_bytes(InType::BF16, k, n, groups, o)
+                                                  : pack_bytes(InType::BF16, n, k, groups, o);
+            const size_t copies = (a_ok ? 0 : pack_bytes(InType::BF16, rows, k, 1, o)) + (b_ok ? 0 : pb);
             g.any_align = unit && grouped_plan_any(g, bl, (int64_t)copies);
         }
         p = grouped_plan(g, bl);

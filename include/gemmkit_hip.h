@@ -641,7 +641,9 @@ int gk_gemm_packed_a_fused_bf16_unchecked(gk_workspace *ws, gk_bf16 alpha,
  * the rows [s_g, s_{g+1}) with s_i = min(rows, max(0, offsets[0 .. i])): for
  * increasing offsets within the rows simply offsets[g] .. offsets[g + 1], and
  * any other contents give disjoint groups inside the matrix too.  Groups may be
- * empty.  Rows before s_0 and from s_groups on belong to no group.
+ * empty.  Rows before s_0 and from s_groups on belong to no group.  Every
+ * workgroup reads all offsets (64 at a time), which costs little for hundreds
+ * of groups and is most of the time for thousands.
  *
  * Sizes: rows, groups, k and n at most 2^31 - 1025; a bf16 row of k (and, for
  * wgrad, n) elements at most 4 MiB, a row of codes likewise; fewer than 2^31
