@@ -2702,7 +2702,8 @@ int gk_debug_plan_grouped(int32_t op, int64_t rows, int64_t groups, int64_t k, i
                           int32_t f32_out, int32_t aligned, int32_t *plan) {
     const int64_t lim = INT32_MAX - 1024;
     if (op < 0 || op > 3 || rows <= 0 || groups <= 0 || k <= 0 || n <= 0 || rows > lim ||
-        groups > lim || k > lim || n > lim || !plan)
+        groups > lim || k > lim || n > lim || !plan ||
+        (__int128)(rows + n + 8) * groups * (k + 8) > INT64_MAX / 4)
         return fail(GK_ERR_ARG, "gemmkit: gk_debug_plan_grouped: bad argument");
     static const int32_t some_offsets = 0;
     RaggedArgs g{};

@@ -121,7 +121,8 @@ def test_every_plan_is_listed():
 
 
 def test_plan_refusals():
-    for rows, groups, k, n in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0), (2 ** 31, 1, 1, 1)):
+    for rows, groups, k, n in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0), (2 ** 31, 1, 1, 1),
+                             (1, 2 ** 30, 2 ** 30, 2 ** 30)):
         with pytest.raises(gk.GemmkitError):
             gk.debug_plan_grouped("mxfp4", rows, groups, k, n)
 
