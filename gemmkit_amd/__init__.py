@@ -41,8 +41,12 @@ counterpart): f32 output for bf16 GEMMs (:func:`gemm_bf16_f32out`,
 requantization (``Requantize(relu=True)``), and prepacked-B requantization
 (:func:`gemm_i8_packed_b_requant`), products of ragged groups with their weight
 gradient (:func:`gemm_grouped`, :func:`gemm_grouped_wgrad`: the experts of a routed
-layer), and MXFP4 operands (:class:`MatMxfp4`, :func:`quantize_mxfp4`,
-:func:`dequantize_mxfp4`, :func:`gemm_mxfp4`, :func:`gemm_grouped_mxfp4`).
+layer), MXFP4 operands (:class:`MatMxfp4`, :func:`quantize_mxfp4`,
+:func:`dequantize_mxfp4`, :func:`gemm_mxfp4`, :func:`gemm_grouped_mxfp4`), and linear layers in
+training: products with bias, activation and residual and their gradients
+(:func:`gemm_linear`, :func:`gemm_linear_dgrad`, :func:`activation_grad`), and 8-bit checkpoints
+of activations (:class:`MatMxint8`, :func:`quantize_mxint8`, :func:`dequantize_mxint8`,
+:func:`gemm_wgrad_mxint8`).
 
 All tensors must live on the HIP device; calls are synchronous by default and
 run on torch's current stream.  There is no CPU fallback: a missing library
@@ -57,7 +61,7 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _lib
-from ._lib import BiasC, MatMutC, MatRefC, Mxfp4C, RequantizeC
+from ._lib import BiasC, MatMutC, MatRefC, Mxfp4C, Mxint8C, RequantizeC
 
 __all__ = [
     "GemmkitError", "MatRef", "MatMut", "Parallelism", "Workspace", "RequantScale",
@@ -71,7 +75,8 @@ __all__ = [
     "gemm_fused_unchecked", "gemm_batched_fused", "gemm_batched_fused_unchecked",
     "gemm_packed_b_fused", "gemm_packed_b_fused_unchecked", "gemm_grouped",
     "gemm_grouped_wgrad", "MatMxfp4", "quantize_mxfp4", "dequantize_mxfp4", "gemm_mxfp4",
-    "gemm_grouped_mxfp4", "set_synchronous",
+    "gemm_grouped_mxfp4", "gemm_linear", "gemm_linear_dgrad", "activation_grad", "MatMxint8",
+    "quantize_mxint8", "dequantize_mxint8", "gemm_wgrad_mxint8", "set_synchronous",
     "library_path", "version",
 ]
 
@@ -763,7 +768,9 @@ class Bias:
 
 
 class Activation:
-    """Activation (src/api/fused.rs:25-31): ``Relu`` or ``LeakyRelu(slope)``."""
+    """Activation (src/api/fused.rs:25-31): ``Relu`` or ``LeakyRelu(slope)``; the linear-layer
+    and MXINT8 functions also take ``Gelu`` (z * normal distribution), ``GeluTanh`` (its
+    approximation by tanh) and ``Silu`` (z * sigmoid)."""
 
     def __init__(self, kind: int, slope: float = 0.0):
         self.kind, self.slope = kind, float(slope)
@@ -774,6 +781,9 @@ class Activation:
 
 
 Activation.Relu = Activation(1)  # type: ignore[attr-defined]
+Activation.Gelu = Activation(3)  # type: ignore[attr-defined]
+Activation.GeluTanh = Activation(4)  # type: ignore[attr-defined]
+Activation.Silu = Activation(5)  # type: ignore[attr-defined]
 
 
 def _fused_args(dt: torch.dtype, bias: Optional[Bias], act: Optional[Activation]):
@@ -1195,3 +1205,180 @@ def gemm_grouped_mxfp4(alpha: float, a: MatMxfp4, offsets: torch.Tensor, b: MatM
     _bind_here(c.data, offsets, a.codes, a.scales, b.codes, b.scales)
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), off, groups, b._c("B"),
                                    float(beta), c._c(dt, "C"), _par(par)))
+
+
+# ------------------------------------- linear layers, 8-bit activation checkpoints
+
+class MatMxint8:
+    """Extension: a rows x cols matrix in MXINT8, the checkpoint of a layer's activations.  Row r's
+    elements are int8 codes at ``codes + r * ld``, in whole blocks of 32; each block has an e8m0
+    scale byte at ``scales + r * lds``, and a code stands for ``code * 2^(byte - 133)`` (255: NaN).
+    Codes past ``cols`` and scales past the last block do not count.  ``codes`` (int8) and
+    ``scales`` (uint8) are contiguous device tensors, their row strides (bytes, multiples of 16) by
+    default those of whole rows: ``32 * ceil(cols / 32)`` and ``ceil(cols / 32)`` rounded up to
+    16."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int,
+                 ld: Optional[int] = None, lds: Optional[int] = None):
+        self.codes, self.scales = codes, scales
+        self.rows, self.cols = int(rows), int(cols)
+        blocks = -(-self.cols // 32)
+        self.ld = 32 * blocks if ld is None else int(ld)
+        self.lds = -(-blocks // 16) * 16 if lds is None else int(lds)
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device="cuda") -> "MatMxint8":
+        """An uninitialised matrix to quantize into."""
+        blocks = -(-int(cols) // 32)
+        codes = torch.empty((rows, 32 * blocks), dtype=torch.int8, device=device)
+        scales = torch.empty((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device)
+        return cls(codes, scales, rows, cols)
+
+    def _c(self, what: str) -> Mxint8C:
+        codes, scales = _slice(self.codes, what), _slice(self.scales, what)
+        if codes.dtype is not torch.int8 or scales.dtype is not torch.uint8:
+            raise TypeError(f"gemmkit_amd: {what} codes must be int8 and scales uint8")
+        if self.rows < 0 or self.cols < 0 or self.ld < 0 or self.lds < 0:
+            raise GemmkitError(-2, f"gemmkit_amd: {what} has a negative side or stride")
+        return Mxint8C(codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
+                       self.rows, self.cols, self.ld, self.lds)
+
+
+def _act_args(act: Optional[Activation]):
+    return (0, 0.0) if act is None else (act.kind, act.slope)
+
+
+def quantize_mxint8(x: MatRef, q: Optional[MatMxint8] = None) -> MatMxint8:
+    """Extension: x (float32 or bfloat16, any strides) in MXINT8, into ``q`` if one is given.
+
+    A block of 32 columns with largest magnitude m has ``e = max(floor(log2 m), -120)``, the scale
+    byte ``e + 127``, and as codes the whole numbers nearest ``x / 2^(e - 6)``, ties to even, at
+    most 127 either way; a block that holds a NaN or an infinity becomes NaN."""
+    L = _lib.lib()
+    dt = x.data.dtype
+    if dt not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"gemmkit_amd: quantize_mxint8 supports float32 and bfloat16, got {dt}")
+    view = MatRef._c(x, dt, "X")
+    if q is None:
+        q = MatMxint8.empty(x.rows, x.cols, x.data.device)
+    _bind_here(x.data, q.codes, q.scales)
+    fn = L.gk_quantize_mxint8_f32 if dt == torch.float32 else L.gk_quantize_mxint8_bf16
+    _check(fn(view, q._c("MXINT8 output")))
+    return q
+
+
+def dequantize_mxint8(q: MatMxint8, c: MatMut, act: Optional[Activation] = None) -> None:
+    """Extension: act(values of q) in c (float32 or bfloat16, any strides)."""
+    fn, dt = _out_entry(c, "gk_dequantize_mxint8_bf16", "gk_dequantize_mxint8_f32",
+                        "dequantize_mxint8")
+    _bind_here(c.data, q.codes, q.scales)
+    _check(getattr(_lib.lib(), fn)(q._c("MXINT8 input"), *_act_args(act), c._c(dt, "C")))
+
+
+def gemm_wgrad_mxint8(alpha: float, a: MatMxint8, b: MatRef, beta: float, c: MatMut,
+                      act: Optional[Activation] = None, par: Optional[Parallelism] = None,
+                      ws: Optional[Workspace] = None) -> None:
+    """Extension: a linear layer's weight gradient from the checkpoint of its input.
+
+    ``C <- alpha * H^T @ B + beta * C`` with ``H = act(values of a)``, rounded to bfloat16 (without
+    ``act`` exact): a is rows x k, B (bfloat16) rows x n, C k x n, bfloat16 or float32.  ``act`` is
+    the activation of the layer before, where a holds that layer's pre-activations."""
+    fn, dt = _out_entry(c, "gk_gemm_wgrad_mxint8_bf16", "gk_gemm_wgrad_mxint8_f32",
+                        "gemm_wgrad_mxint8")
+    _bind_here(a.codes, a.scales, b.data, c.data)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), a._c("A"), *_act_args(act),
+                                   MatRef._c(b, torch.bfloat16, "B"), float(beta), c._c(dt, "C"),
+                                   _par(par)))
+
+
+def _kept(z, *tensors):
+    """(bfloat16 view or None, MXINT8 matrix or None) of pre-activations that are read; binds the
+    stream for them and the call's other tensors."""
+    if z is None:
+        _bind_here(*tensors)
+        return None, None
+    if isinstance(z, MatMxint8):
+        _bind_here(z.codes, z.scales, *tensors)
+        return None, z._c("Z")
+    _bind_here(z.data, *tensors)
+    return MatRef._c(z, torch.bfloat16, "Z"), None
+
+
+def _dbias(dbias: Optional[torch.Tensor]):
+    if dbias is None:
+        return None, 0
+    d = _slice(dbias, "dbias")
+    if d.dtype != torch.float32:
+        raise TypeError(f"gemmkit_amd: dbias must be float32, got {d.dtype}")
+    return d.data_ptr(), d.numel()
+
+
+def gemm_linear(alpha: float, a: MatRef, b: MatRef, c: MatMut, bias: Optional[Bias] = None,
+                act: Optional[Activation] = None, residual: Optional[MatRef] = None,
+                z: Union[MatMut, MatMxint8, None] = None, par: Optional[Parallelism] = None,
+                ws: Optional[Workspace] = None) -> None:
+    """Extension: a linear layer, ``C <- act(Z) + residual`` with ``Z = alpha * A @ B + bias``.
+
+    A and B are bfloat16, sums f32, C bfloat16 or float32.  ``bias`` is ``Bias.PerCol`` (bfloat16
+    or float32); ``residual`` has C's type and may be C itself.  ``z`` keeps Z for the backward
+    pass, a bfloat16 matrix or an 8-bit checkpoint; the activation takes it before it is rounded.
+    Weights stored output-major (n x k) are the view ``MatRef(w, k, n, 1, k)``."""
+    fn, dt = _out_entry(c, "gk_gemm_linear_bf16", "gk_gemm_linear_f32out", "gemm_linear")
+    bc, wide = None, 0
+    tensors = [a.data, b.data, c.data]
+    if bias is not None:
+        wide = 1 if bias.data.dtype == torch.float32 else 0
+        bc = bias._c(torch.float32 if wide else torch.bfloat16)
+        tensors.append(bias.data)
+    rc = zc = zq = None
+    if residual is not None:
+        rc = MatRef._c(residual, dt, "residual")
+        tensors.append(residual.data)
+    if isinstance(z, MatMxint8):
+        zq = z._c("Z")
+        tensors += [z.codes, z.scales]
+    elif z is not None:
+        if not isinstance(z, MatMut):
+            raise TypeError("gemmkit_amd: gemm_linear keeps Z in a MatMut or a MatMxint8")
+        zc = z._c(torch.bfloat16, "Z")
+        tensors.append(z.data)
+    _bind_here(*tensors)
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), MatRef._c(a, torch.bfloat16, "A"),
+                                   MatRef._c(b, torch.bfloat16, "B"), bc, wide, *_act_args(act),
+                                   rc, zc, zq, c._c(dt, "C"), _par(par)))
+
+
+def gemm_linear_dgrad(alpha: float, a: MatRef, b: MatRef, d: MatMut,
+                      act: Optional[Activation] = None, z: Union[MatRef, MatMxint8, None] = None,
+                      dbias: Optional[torch.Tensor] = None, par: Optional[Parallelism] = None,
+                      ws: Optional[Workspace] = None) -> None:
+    """Extension: the gradient at the pre-activations of the layer before a linear layer.
+
+    ``D <- (alpha * A @ B) * act'(Z)``: A (m x k) is the gradient of the linear layer's output, B
+    its transposed weights (k x n; stored output-major they are ``MatRef(w, k, n, n, 1)``), ``z`` the
+    m x n pre-activations as :func:`gemm_linear` kept them (none without ``act``).  A and B are
+    bfloat16, D bfloat16 or float32.  ``dbias`` (float32, n) becomes the column sums of D before it
+    is rounded, the gradient of that layer's bias."""
+    fn, dt = _out_entry(d, "gk_gemm_linear_dgrad_bf16", "gk_gemm_linear_dgrad_f32out",
+                        "gemm_linear_dgrad")
+    sums = _dbias(dbias)
+    zc, zq = _kept(z, a.data, b.data, d.data, *(() if dbias is None else (dbias,)))
+    _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), MatRef._c(a, torch.bfloat16, "A"),
+                                   MatRef._c(b, torch.bfloat16, "B"), *_act_args(act), zc, zq,
+                                   *sums, d._c(dt, "D"), _par(par)))
+
+
+def activation_grad(g: MatRef, d: MatMut, act: Optional[Activation] = None,
+                    z: Union[MatRef, MatMxint8, None] = None,
+                    dbias: Optional[torch.Tensor] = None, ws: Optional[Workspace] = None) -> None:
+    """Extension: ``D <- G * act'(Z)`` for a gradient G that is there already (bfloat16, which may
+    be D itself, or float32); D is bfloat16.  ``z`` and ``dbias`` as in :func:`gemm_linear_dgrad`;
+    without ``act`` D is G, and dbias its column sums."""
+    dt = g.data.dtype
+    if dt not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"gemmkit_amd: activation_grad supports float32 and bfloat16, got {dt}")
+    fn = "gk_activation_grad_f32" if dt == torch.float32 else "gk_activation_grad_bf16"
+    sums = _dbias(dbias)
+    zc, zq = _kept(z, g.data, d.data, *(() if dbias is None else (dbias,)))
+    _check(getattr(_lib.lib(), fn)(_ws(ws), MatRef._c(g, dt, "G"), *_act_args(act), zc, zq, *sums,
+                                   d._c(torch.bfloat16, "D")))

@@ -78,11 +78,17 @@ class Mxfp4C(C.Structure):
                 ("rows", _size), ("cols", _size), ("ld", _size), ("lds", _size)]
 
 
+class Mxint8C(C.Structure):
+    """``gk_mxint8``: rows of int8 codes and their e8m0 scales."""
+    _fields_ = Mxfp4C._fields_
+
+
 _REF = C.POINTER(MatRefC)
 _MUT = C.POINTER(MatMutC)
 _REQ = C.POINTER(RequantizeC)
 _BIAS = C.POINTER(BiasC)
 _MX = C.POINTER(Mxfp4C)
+_Q8 = C.POINTER(Mxint8C)
 
 # name -> (restype, argtypes); one line per symbol of include/gemmkit_hip.h
 SIGNATURES: dict[str, tuple] = {
@@ -246,6 +252,22 @@ SIGNATURES: dict[str, tuple] = {
     "gk_gemm_grouped_mxfp4_bf16": (C.c_int, [_vp, _f32, _MX, _vp, _size, _MX, _f32, _MUT, _u32]),
     "gk_gemm_mxfp4_f32": (C.c_int, [_vp, _f32, _MX, _MX, _f32, _MUT, _u32]),
     "gk_gemm_grouped_mxfp4_f32": (C.c_int, [_vp, _f32, _MX, _vp, _size, _MX, _f32, _MUT, _u32]),
+    "gk_quantize_mxint8_f32": (C.c_int, [_REF, _Q8]),
+    "gk_quantize_mxint8_bf16": (C.c_int, [_REF, _Q8]),
+    "gk_dequantize_mxint8_f32": (C.c_int, [_Q8, _i32, _f32, _MUT]),
+    "gk_dequantize_mxint8_bf16": (C.c_int, [_Q8, _i32, _f32, _MUT]),
+    "gk_gemm_wgrad_mxint8_bf16": (C.c_int, [_vp, _f32, _Q8, _i32, _f32, _REF, _f32, _MUT, _u32]),
+    "gk_gemm_wgrad_mxint8_f32": (C.c_int, [_vp, _f32, _Q8, _i32, _f32, _REF, _f32, _MUT, _u32]),
+    "gk_gemm_linear_bf16": (C.c_int, [_vp, _f32, _REF, _REF, _BIAS, _i32, _i32, _f32, _REF, _MUT,
+                                      _Q8, _MUT, _u32]),
+    "gk_gemm_linear_f32out": (C.c_int, [_vp, _f32, _REF, _REF, _BIAS, _i32, _i32, _f32, _REF,
+                                        _MUT, _Q8, _MUT, _u32]),
+    "gk_gemm_linear_dgrad_bf16": (C.c_int, [_vp, _f32, _REF, _REF, _i32, _f32, _REF, _Q8, _vp,
+                                            _size, _MUT, _u32]),
+    "gk_gemm_linear_dgrad_f32out": (C.c_int, [_vp, _f32, _REF, _REF, _i32, _f32, _REF, _Q8, _vp,
+                                              _size, _MUT, _u32]),
+    "gk_activation_grad_bf16": (C.c_int, [_vp, _REF, _i32, _f32, _REF, _Q8, _vp, _size, _MUT]),
+    "gk_activation_grad_f32": (C.c_int, [_vp, _REF, _i32, _f32, _REF, _Q8, _vp, _size, _MUT]),
 }
 
 _LIB: C.CDLL | None = None

@@ -2235,6 +2235,61 @@ int pack_groups(PackJob *jobs, int n) {
     return e == hipSuccess ? GK_OK : hip_fail(e, "pack");
 }
 
+// How a forward product reads its operands: in place, or from copies in the workspace.  The
+// constructor decides (with g's sizes), pack() makes the copies and place() sets g's
+// pointers and strides.  B_g is read as N rows of K or as K rows of N.
+struct ForwardOperands {
+    RaggedArgs &g;
+    Opnd A, Br, Bc;
+    bool cols = false;  // B as K rows of N
+    size_t pa = 0, pb = 0;
+
+    ForwardOperands(RaggedArgs &g_, const Opnd &a, const void *b, ptrdiff_t rsb, ptrdiff_t csb,
+                    ptrdiff_t b_gs)
+        : g(g_), A(a), Br{b, csb, rsb, b_gs}, Bc{b, rsb, csb, b_gs} {
+        const int64_t M = g.M, N = g.N, K = g.K, G = g.G;
+        if (K == 0) return;
+        const bool a_ok = ragged_in_place(A, M, K, 1);
+        const bool rows_ok = ragged_in_place(Br, N, K, G);
+        cols = !rows_ok && ragged_in_place(Bc, K, N, G);
+        if (a_ok && (rows_ok || cols)) return;
+        // Rows of unit stride that only lack alignment are read as they are by a kernel of
+        // their own, or copied row by row.
+        const bool rows_any = ragged_unit_rows(Br, N, K), cols_any = ragged_unit_rows(Bc, K, N);
+        const bool b_pack = !rows_ok && !cols, pack_cols = cols || (b_pack && cols_any);
+        pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+        pb = !b_pack     ? 0
+             : pack_cols ? pack_bytes(InType::BF16, K, N, G, Bc)
+                         : pack_bytes(InType::BF16, N, K, G, Br);
+        g.any_align = ragged_unit_rows(A, M, K) && (rows_any || cols_any) &&
+                      grouped_plan_any(g, rows_any ? RaggedB::Rows : RaggedB::Cols,
+                                       (int64_t)(pa + pb));
+        cols = g.any_align ? !rows_any : pack_cols;
+        if (g.any_align) pa = pb = 0;
+    }
+    size_t packed() const { return pa + pb; }
+    RaggedB layout() const { return cols ? RaggedB::Cols : RaggedB::Rows; }
+    int pack(uint8_t *buf) {
+        PackJob jobs[2];
+        int nj = 0;
+        if (pa) jobs[nj++] = pack_job(InType::BF16, &A, g.M, g.K, 1, buf);
+        if (pb)
+            jobs[nj++] = cols ? pack_job(InType::BF16, &Bc, g.K, g.N, g.G, buf + pa)
+                              : pack_job(InType::BF16, &Br, g.N, g.K, g.G, buf + pa);
+        return pack_groups(jobs, nj);
+    }
+    RaggedB place() {
+        if (g.K > 0) {
+            g.lda = ragged_ld(A, g.M, g.K);
+            g.ldb = cols ? ragged_ld_cols(Bc, g.K, g.N) : ragged_ld(Br, g.N, g.K);
+            g.bsb = (cols ? Bc.bs : Br.bs) * 2;
+        }
+        g.a = A.p;
+        g.b = cols ? Bc.p : Br.p;
+        return layout();
+    }
+};
+
 int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const gk_mat_ref *a,
                     const int32_t *offsets, size_t groups, const gk_mat_ref *b, ptrdiff_t b_gs,
                     float beta, const gk_mat_mut *c) {
@@ -2282,52 +2337,108 @@ int grouped_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, cons
     g.M = (int32_t)M;
     g.N = (int32_t)N;
     g.K = (int32_t)K;
-    // B_g is read as N rows of K or as K rows of N.
-    Opnd A{a->data, a->rs, a->cs, 0};
-    Opnd Br{b->data, b->cs, b->rs, G > 1 ? b_gs : 0}, Bc{b->data, b->rs, b->cs, G > 1 ? b_gs : 0};
-    RaggedB bl = RaggedB::Rows;
-    if (K > 0) {
-        const bool a_ok = ragged_in_place(A, M, K, 1);
-        const bool rows_ok = ragged_in_place(Br, N, K, G);
-        bool cols_ok = !rows_ok && ragged_in_place(Bc, K, N, G);
-        // Rows of unit stride that only lack alignment are read as they are by a kernel of
-        // their own, or copied row by row.
-        const bool rows_any = ragged_unit_rows(Br, N, K), cols_any = ragged_unit_rows(Bc, K, N);
-        if (!a_ok || (!rows_ok && !cols_ok)) {
-            const bool b_pack = !rows_ok && !cols_ok, pack_cols = cols_ok || (b_pack && cols_any);
-            const size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-            const size_t pb = !b_pack     ? 0
-                              : pack_cols ? pack_bytes(InType::BF16, K, N, G, Bc)
-                                          : pack_bytes(InType::BF16, N, K, G, Br);
-            g.any_align = ragged_unit_rows(A, M, K) && (rows_any || cols_any) &&
-                          grouped_plan_any(g, rows_any ? RaggedB::Rows : RaggedB::Cols,
-                                           (int64_t)(pa + pb));
-            if (g.any_align) {
-                cols_ok = !rows_any;
-            } else {
-                cols_ok = pack_cols;
-                void *buf = nullptr;
-                if ((r = ws_reserve(resolve_ws(ws), pa + pb, &buf))) return r;
-                uint8_t *const dst = (uint8_t *)buf + pa;
-                PackJob jobs[2];
-                int nj = 0;
-                if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
-                if (pb)
-                    jobs[nj++] = cols_ok ? pack_job(InType::BF16, &Bc, K, N, G, dst)
-                                         : pack_job(InType::BF16, &Br, N, K, G, dst);
-                if ((r = pack_groups(jobs, nj))) return r;
-            }
-        }
-        bl = cols_ok ? RaggedB::Cols : RaggedB::Rows;
-        g.lda = ragged_ld(A, M, K);
-        g.ldb = cols_ok ? ragged_ld_cols(Bc, K, N) : ragged_ld(Br, N, K);
-        g.bsb = (cols_ok ? Bc.bs : Br.bs) * 2;
+    ForwardOperands f(g, Opnd{a->data, a->rs, a->cs, 0}, b->data, b->rs, b->cs, G > 1 ? b_gs : 0);
+    if (f.packed() > 0) {
+        void *buf = nullptr;
+        if ((r = ws_reserve(resolve_ws(ws), f.packed(), &buf)) || (r = f.pack((uint8_t *)buf))) return r;
     }
-    g.a = A.p;
-    g.b = bl == RaggedB::Cols ? Bc.p : Br.p;
+    const RaggedB bl = f.place();
     const hipError_t e = launch_grouped_bf16(g, bl, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "grouped gemm");
     return finish("grouped gemm");
+}
+
+// A left operand that is an 8-bit checkpoint: its rows and the activation they go through.
+struct Checkpoint {
+    const MxArgs *args;
+    int32_t act;
+    float slope;
+};
+
+// C_g <- alpha * A[rows of g]^T B[rows of g] + beta * C_g, A rows x na (or the checkpoint q), B
+// rows x nb; offsets == nullptr: one group of all rows.
+int wgrad_run(gk_workspace *ws, EpiKind kind, float alpha, Opnd a, int64_t na, Opnd b, int64_t nb,
+              int64_t rows, const int32_t *offsets, size_t groups, float beta, const gk_mat_mut *c,
+              ptrdiff_t c_gs, const Checkpoint *q) {
+    int r;
+    // C column-major-ish: C_g^T = B^T A, the same product with the roles swapped.
+    const bool swap = iabs64(c->cs) > iabs64(c->rs);
+    const int64_t M = alpha == 0.0f ? 0 : rows;  // (then nothing of A and B is read)
+    const int64_t K = swap ? nb : na, N = swap ? na : nb;
+    // The decoded values of a checkpoint lie in the workspace, in aligned rows.
+    const int64_t qld = round_up64(na, 8);
+    const size_t pq = q && M > 0 ? (size_t)M * qld * 2 : 0;
+    if (q) a = Opnd{nullptr, qld, 1, 0};
+    Opnd A = swap ? b : a, B = swap ? a : b;
+    EpiParams ep = epi_float(kind, alpha, beta);
+    ep.c = c->data;
+    ep.rsc = swap ? c->cs : c->rs;
+    ep.csc = swap ? c->rs : c->cs;
+    ep.bsc = groups > 1 ? c_gs : 0;
+    ep.vec4 = ep.csc == 1;
+    RaggedArgs g{};
+    g.cus = g_num_cus;
+    g.off = offsets;
+    g.G = (int32_t)groups;
+    g.M = (int32_t)M;
+    g.N = (int32_t)N;
+    g.K = (int32_t)K;
+    g.splits = 1;
+    uint8_t *part = nullptr;
+    if (M == 0) wgrad_plan(g, kind, false, 0);
+    if (M > 0) {
+        const bool a_ok = (q && !swap) || ragged_in_place(A, M, K, 1);
+        const bool b_ok = (q && swap) || ragged_in_place(B, M, N, 1);
+        size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
+        size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
+        wgrad_plan(g, kind,
+                   (!a_ok || !b_ok) && ragged_unit_rows(A, M, K) && ragged_unit_rows(B, M, N),
+                   (int64_t)(pa + pb));
+        if (g.any_align) pa = pb = 0;
+        const size_t sums = g.splits > 1 ? (size_t)g.splits * groups * K * N * 4 : 0;
+        if (pq + pa + pb + sums > 0) {
+            void *buf = nullptr;
+            if ((r = ws_reserve(resolve_ws(ws), pq + pa + pb + sums, &buf))) return r;
+            uint8_t *const packs = (uint8_t *)buf + pq;
+            part = packs + pa + pb;
+            if (q) {
+                (swap ? B : A).p = buf;
+                MxArgs m = *q->args;
+                m.x = buf;
+                m.rs = qld;
+                m.cs = 1;
+                const hipError_t e = launch_mxint8_dequantize(InType::BF16, m, q->act, q->slope,
+                                                              tl_stream);
+                if (e != hipSuccess) return hip_fail(e, "mxint8 dequantize");
+            }
+            PackJob jobs[2];
+            int nj = 0;
+            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, packs);
+            if (pb) jobs[nj++] = pack_job(InType::BF16, &B, M, N, 1, packs + pa);
+            if (nj && (r = pack_groups(jobs, nj))) return r;
+        }
+        g.lda = ragged_ld(A, M, K);
+        g.ldb = ragged_ld(B, M, N);
+    }
+    g.a = A.p;
+    g.b = B.p;
+    if (g.splits == 1) {
+        const hipError_t e = launch_grouped_wgrad(g, ep, tl_stream);
+        if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
+        return finish("grouped weight gradient");
+    }
+    // Partial sums of the row ranges, then their sum in range order with the epilogue.
+    EpiParams pe = epi_float(EpiKind::F32, 1.0f, 0.0f);
+    pe.c = part;
+    pe.rsc = N;
+    pe.csc = 1;
+    pe.bsc = K * N;
+    pe.vec4 = 1;
+    hipError_t e = launch_grouped_wgrad(g, pe, tl_stream);
+    if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
+    e = launch_split_reduce(InType::BF16, part, g.splits, K, N, (int64_t)groups, ep, tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "split reduce");
+    return finish("grouped weight gradient");
 }
 
 int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const gk_mat_ref *a,
@@ -2365,69 +2476,9 @@ int wgrad_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const 
     if (row_bytes > kMaxRaggedRow) return row_too_long("A or B", row_bytes);
     if ((r = device_init())) return r;
     if (groups == 0 || a->cols == 0 || b->cols == 0) return ok();
-    // C column-major-ish: C_g^T = B^T A, the same product with the roles swapped.
-    const bool swap = iabs64(c->cs) > iabs64(c->rs);
-    const gk_mat_ref *x = swap ? b : a, *y = swap ? a : b;
-    const int64_t M = alpha == 0.0f ? 0 : (int64_t)a->rows;
-    const int64_t K = (int64_t)x->cols, N = (int64_t)y->cols;
-    Opnd A{x->data, x->rs, x->cs, 0}, B{y->data, y->rs, y->cs, 0};
-    EpiParams ep = epi_float(kind, alpha, beta);
-    ep.c = c->data;
-    ep.rsc = swap ? c->cs : c->rs;
-    ep.csc = swap ? c->rs : c->cs;
-    ep.bsc = groups > 1 ? c_gs : 0;
-    ep.vec4 = ep.csc == 1;
-    RaggedArgs g{};
-    g.cus = g_num_cus;
-    g.off = offsets;
-    g.G = (int32_t)groups;
-    g.M = (int32_t)M;
-    g.N = (int32_t)N;
-    g.K = (int32_t)K;
-    g.splits = 1;
-    uint8_t *part = nullptr;
-    if (M == 0) wgrad_plan(g, kind, false, 0);
-    if (M > 0) {
-        const bool a_ok = ragged_in_place(A, M, K, 1), b_ok = ragged_in_place(B, M, N, 1);
-        size_t pa = a_ok ? 0 : pack_bytes(InType::BF16, M, K, 1, A);
-        size_t pb = b_ok ? 0 : pack_bytes(InType::BF16, M, N, 1, B);
-        wgrad_plan(g, kind,
-                   (!a_ok || !b_ok) && ragged_unit_rows(A, M, K) && ragged_unit_rows(B, M, N),
-                   (int64_t)(pa + pb));
-        if (g.any_align) pa = pb = 0;
-        const size_t sums = g.splits > 1 ? (size_t)g.splits * groups * K * N * 4 : 0;
-        if (pa + pb + sums > 0) {
-            void *buf = nullptr;
-            if ((r = ws_reserve(resolve_ws(ws), pa + pb + sums, &buf))) return r;
-            part = (uint8_t *)buf + pa + pb;
-            PackJob jobs[2];
-            int nj = 0;
-            if (pa) jobs[nj++] = pack_job(InType::BF16, &A, M, K, 1, (uint8_t *)buf);
-            if (pb) jobs[nj++] = pack_job(InType::BF16, &B, M, N, 1, (uint8_t *)buf + pa);
-            if (nj && (r = pack_groups(jobs, nj))) return r;
-        }
-        g.lda = ragged_ld(A, M, K);
-        g.ldb = ragged_ld(B, M, N);
-    }
-    g.a = A.p;
-    g.b = B.p;
-    if (g.splits == 1) {
-        const hipError_t e = launch_grouped_wgrad(g, ep, tl_stream);
-        if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
-        return finish("grouped weight gradient");
-    }
-    // Partial sums of the row ranges, then their sum in range order with the epilogue.
-    EpiParams pe = epi_float(EpiKind::F32, 1.0f, 0.0f);
-    pe.c = part;
-    pe.rsc = N;
-    pe.csc = 1;
-    pe.bsc = K * N;
-    pe.vec4 = 1;
-    hipError_t e = launch_grouped_wgrad(g, pe, tl_stream);
-    if (e != hipSuccess) return launch_failed(e, "grouped weight gradient");
-    e = launch_split_reduce(InType::BF16, part, g.splits, K, N, (int64_t)groups, ep, tl_stream);
-    if (e != hipSuccess) return hip_fail(e, "split reduce");
-    return finish("grouped weight gradient");
+    return wgrad_run(ws, kind, alpha, Opnd{a->data, a->rs, a->cs, 0}, (int64_t)a->cols,
+                     Opnd{b->data, b->rs, b->cs, 0}, (int64_t)b->cols, (int64_t)a->rows, offsets,
+                     groups, beta, c, c_gs, nullptr);
 }
 
 int check_mxfp4(const gk_mxfp4 *q, const char *name) {
@@ -2567,6 +2618,401 @@ int mxfp4_checked(EpiKind kind, size_t so, float alpha, const gk_mxfp4 *a, bool 
     const hipError_t e = launch_mxfp4(g, ep, tl_stream);
     if (e != hipSuccess) return launch_failed(e, "mxfp4 gemm");
     return finish("mxfp4 gemm");
+}
+
+// ---- MXINT8 checkpoints and linear layers
+
+int check_mxint8(const gk_mxint8 *q, const char *name) {
+    const size_t lim = (size_t)INT32_MAX - 1024;
+    if (q->rows > lim || q->cols > lim)
+        return fail(GK_ERR_OVERFLOW, "gemmkit: MXINT8 %s of %zux%zu: each side must be below "
+                                     "2^31 - 1024", name, q->rows, q->cols);
+    const size_t nb = (q->cols + kMxBlock - 1) / kMxBlock, sb = (nb + 15) / 16 * 16;
+    if (q->rows == 0 || nb == 0) return GK_OK;
+    if (q->ld < nb * 32 || q->ld % 16 || q->lds < sb || q->lds % 16 ||
+        (uintptr_t)q->codes % 16 || (uintptr_t)q->scales % 16 || !q->codes || !q->scales)
+        return fail(GK_ERR_VIEW,
+                    "gemmkit: MXINT8 %s needs 16-byte aligned codes and scales and row strides that "
+                    "are multiples of 16, at least %zu and %zu bytes; got %zu and %zu",
+                    name, nb * 32, sb, q->ld, q->lds);
+    if (q->ld > (size_t)PTRDIFF_MAX / lim || q->lds > (size_t)PTRDIFF_MAX / lim)
+        return fail(GK_ERR_OVERFLOW, "gemmkit: MXINT8 %s row strides of %zu and %zu are too large",
+                    name, q->ld, q->lds);
+    const __int128 need_c = (__int128)(q->rows - 1) * q->ld + nb * 32;
+    const __int128 need_s = (__int128)(q->rows - 1) * q->lds + sb;
+    if (need_c > (__int128)q->codes_len || need_s > (__int128)q->scales_len)
+        return fail(GK_ERR_VIEW,
+                    "gemmkit: MXINT8 %s of %zux%zu (row strides %zu, %zu) needs more bytes of codes "
+                    "or scales than the %zu and %zu it has",
+                    name, q->rows, q->cols, q->ld, q->lds, q->codes_len, q->scales_len);
+    return GK_OK;
+}
+
+// Memory that a call reads or writes, for the checks that its outputs overlap nothing.
+struct Span {
+    const void *p;
+    size_t n, s;
+    const char *name;
+};
+bool overlaps(const Span &a, const Span &b) { return overlaps_bytes(a.p, a.n, a.s, b.p, b.n, b.s); }
+
+// Every output against every other span.
+int check_disjoint(const Span *outs, int no, const Span *ins, int ni) {
+    for (int i = 0; i < no; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (overlaps(outs[i], outs[j]))
+                return fail(GK_ERR_ALIAS, "gemmkit: %s aliases %s", outs[i].name, outs[j].name);
+        for (int j = 0; j < ni; ++j)
+            if (overlaps(outs[i], ins[j]))
+                return fail(GK_ERR_ALIAS, "gemmkit: %s aliases %s", outs[i].name, ins[j].name);
+    }
+    return GK_OK;
+}
+
+MxArgs mx_args(const gk_mxint8 *q, void *x, ptrdiff_t rs, ptrdiff_t cs) {
+    return MxArgs{(uint8_t *)q->codes, (uint8_t *)q->scales, (int64_t)q->ld, (int64_t)q->lds, x,
+                  rs, cs, (int64_t)q->rows, (int64_t)q->cols};
+}
+
+int check_linear_act(int32_t act, float slope) {
+    if (act < GK_ACT_NONE || act > GK_ACT_SILU)
+        return fail(GK_ERR_ARG, "gemmkit: activation (%d) must be 0 (none), 1 (Relu), 2 (LeakyRelu), "
+                                "3 (Gelu), 4 (GeluTanh) or 5 (Silu)", act);
+    if (act == GK_ACT_LEAKY_RELU && !std::isfinite(slope))
+        return fail(GK_ERR_ARG, "gemmkit: LeakyRelu slope must be finite");
+    return GK_OK;
+}
+
+int check_output(const gk_mat_mut *c, const char *name) {
+    int r;
+    if ((r = check_view(c->len, c->rows, c->cols, c->rs, c->cs, name))) return r;
+    if (self_aliases(c->rows, c->cols, c->rs, c->cs))
+        return fail(GK_ERR_ALIAS,
+                    "gemmkit: %s view aliases itself (strides %td,%td map distinct elements to the "
+                    "same memory); %s must address each (i,j) uniquely",
+                    name, c->rs, c->cs, name);
+    return GK_OK;
+}
+
+int check_sides(const char *name, size_t rows, size_t cols, size_t m, size_t n) {
+    if (rows != m || cols != n)
+        return fail(GK_ERR_SHAPE, "gemmkit: %s is %zux%zu, the output %zux%zu", name, rows, cols, m, n);
+    return GK_OK;
+}
+
+// Whether two views address the same element at every (i, j).
+template <typename X, typename Y>
+bool same_view(const X &a, const Y &b) {
+    return a.data == b.data && a.rows == b.rows && a.cols == b.cols &&
+           (a.rows <= 1 || a.rs == b.rs) && (a.cols <= 1 || a.cs == b.cs);
+}
+
+int quantize8_checked(InType in, const gk_mat_ref *x, const gk_mxint8 *q) {
+    int r;
+    if (!x || !q) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_mxint8(q, "output"))) return r;
+    if (x->rows != q->rows || x->cols != q->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: MXINT8 output is %zux%zu, the matrix %zux%zu", q->rows,
+                    q->cols, x->rows, x->cols);
+    if ((r = check_view(x->len, x->rows, x->cols, x->rs, x->cs, "X"))) return r;
+    const Span outs[2] = {{q->codes, q->codes_len, 1, "codes"}, {q->scales, q->scales_len, 1, "scales"}};
+    const Span ins[1] = {{x->data, x->len, in_size(in), "X"}};
+    if ((r = check_disjoint(outs, 2, ins, 1))) return r;
+    if ((r = device_init())) return r;
+    if (x->rows == 0 || x->cols == 0) return ok();
+    const hipError_t e = launch_mxint8_quantize(
+        in, mx_args(q, const_cast<void *>(x->data), x->rs, x->cs), tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "mxint8 quantize");
+    return finish("mxint8 quantize");
+}
+
+int dequantize8_checked(InType out, const gk_mxint8 *q, int32_t act, float slope,
+                        const gk_mat_mut *c) {
+    int r;
+    if (!c || !q) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_linear_act(act, slope))) return r;
+    if ((r = check_mxint8(q, "input"))) return r;
+    if (c->rows != q->rows || c->cols != q->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: MXINT8 input is %zux%zu, the matrix %zux%zu", q->rows,
+                    q->cols, c->rows, c->cols);
+    if ((r = check_output(c, "C"))) return r;
+    const Span outs[1] = {{c->data, c->len, in_size(out), "C"}};
+    const Span ins[2] = {{q->codes, q->codes_len, 1, "codes"}, {q->scales, q->scales_len, 1, "scales"}};
+    if ((r = check_disjoint(outs, 1, ins, 2))) return r;
+    if ((r = device_init())) return r;
+    if (c->rows == 0 || c->cols == 0) return ok();
+    const hipError_t e = launch_mxint8_dequantize(out, mx_args(q, c->data, c->rs, c->cs), act, slope,
+                                                  tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "mxint8 dequantize");
+    return finish("mxint8 dequantize");
+}
+
+int wgrad8_checked(gk_workspace *ws, EpiKind kind, size_t so, float alpha, const gk_mxint8 *a,
+                   int32_t act, float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c) {
+    int r;
+    if (!a || !b || !c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_linear_act(act, slope))) return r;
+    if ((r = check_mxint8(a, "A"))) return r;
+    if (a->rows != b->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.rows (%zu) != B.rows (%zu)", a->rows, b->rows);
+    if (a->cols != c->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.cols (%zu) != C.rows (%zu)", a->cols, c->rows);
+    if (b->cols != c->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: B.cols (%zu) != C.cols (%zu)", b->cols, c->cols);
+    if ((r = check_view(b->len, b->rows, b->cols, b->rs, b->cs, "B"))) return r;
+    if ((r = check_output(c, "C"))) return r;
+    const Span outs[1] = {{c->data, c->len, so, "C"}};
+    const Span ins[3] = {{a->codes, a->codes_len, 1, "A"}, {a->scales, a->scales_len, 1, "A"},
+                         {b->data, b->len, 2, "B"}};
+    if ((r = check_disjoint(outs, 1, ins, 3))) return r;
+    if ((r = check_ragged_sizes(a->rows, a->cols, b->cols, 1))) return r;
+    const int64_t row_bytes = round_up64((int64_t)std::max(a->cols, b->cols) * 2, 16);
+    if (row_bytes > kMaxRaggedRow) return row_too_long("A or B", row_bytes);
+    if ((r = device_init())) return r;
+    if (a->cols == 0 || b->cols == 0) return ok();
+    const MxArgs args = mx_args(a, nullptr, 0, 0);
+    const Checkpoint q{&args, act, slope};
+    return wgrad_run(ws, kind, alpha, Opnd{}, (int64_t)a->cols, Opnd{b->data, b->rs, b->cs, 0},
+                     (int64_t)b->cols, (int64_t)a->rows, nullptr, 1, beta, c, 0, &q);
+}
+
+// What a linear layer's call says beside its product.
+struct LinearSpec {
+    const gk_bias *bias = nullptr;
+    int32_t bias_f32 = 0;
+    int32_t act = 0;
+    float slope = 0;
+    const gk_mat_ref *res = nullptr;  // the residual; activation_grad: the gradient
+    size_t res_size = 0;
+    const gk_mat_ref *z = nullptr;    // the pre-activations, read or (z_out) written
+    const gk_mxint8 *zq = nullptr;
+    bool z_out = false;
+    float *dbias = nullptr;
+    size_t dbias_len = 0;
+};
+
+// Checks everything but the product's own operands (`ins`, ni of them, up to 2).
+int check_linear(const LinearSpec &s, const gk_mat_mut *c, size_t so, const char *cname,
+                 const char *rname, Span *ins, int ni) {
+    int r;
+    const size_t m = c->rows, n = c->cols;
+    if ((r = check_linear_act(s.act, s.slope))) return r;
+    if (s.z && s.zq) return fail(GK_ERR_ARG, "gemmkit: pre-activations given twice");
+    if (!s.z_out && (s.z || s.zq) != (s.act != GK_ACT_NONE))
+        return fail(GK_ERR_ARG, s.act != GK_ACT_NONE
+                                    ? "gemmkit: an activation's gradient needs its pre-activations"
+                                    : "gemmkit: pre-activations without an activation");
+    if ((r = check_output(c, cname))) return r;
+    Span outs[4] = {{c->data, c->len, so, cname}};
+    Span more[6];
+    int no = 1, nm = 0;
+    for (int i = 0; i < ni; ++i) more[nm++] = ins[i];
+    if (s.bias) {
+        if (s.bias->dim != GK_BIAS_PER_COL)
+            return fail(GK_ERR_ARG, "gemmkit: bias dim (%d) must be 1 (PerCol)", s.bias->dim);
+        if (s.bias->len != n)
+            return fail(GK_ERR_SHAPE, "gemmkit: PerCol bias length (%zu) != B.cols (%zu)",
+                        s.bias->len, n);
+        if (n > 0 && (!s.bias->data || (uintptr_t)s.bias->data % (s.bias_f32 ? 4 : 2)))
+            return fail(GK_ERR_ARG, "gemmkit: bias is null or not aligned to its type");
+        more[nm++] = {s.bias->data, s.bias->len, s.bias_f32 ? size_t(4) : size_t(2), "bias"};
+    }
+    if (s.res) {
+        if ((r = check_sides(rname, s.res->rows, s.res->cols, m, n))) return r;
+        if ((r = check_view(s.res->len, m, n, s.res->rs, s.res->cs, rname))) return r;
+        // (in place: every element is read where it is written)
+        if (s.res_size != so || !same_view(*s.res, *c))
+            more[nm++] = {s.res->data, s.res->len, s.res_size, rname};
+        else if (s.z_out && s.z && overlaps_bytes(s.z->data, s.z->len, 2, s.res->data, s.res->len, so))
+            return fail(GK_ERR_ALIAS, "gemmkit: Z aliases %s", rname);
+    }
+    if (s.z) {
+        if ((r = check_sides("Z", s.z->rows, s.z->cols, m, n))) return r;
+        const gk_mat_mut zm{const_cast<void *>(s.z->data), s.z->len, m, n, s.z->rs, s.z->cs};
+        if ((r = s.z_out ? check_output(&zm, "Z") : check_view(zm.len, m, n, zm.rs, zm.cs, "Z")))
+            return r;
+        const Span sp{s.z->data, s.z->len, 2, "Z"};
+        if (s.z_out) outs[no++] = sp;
+        else more[nm++] = sp;
+    }
+    if (s.zq) {
+        if ((r = check_mxint8(s.zq, "Z"))) return r;
+        if ((r = check_sides("Z", s.zq->rows, s.zq->cols, m, n))) return r;
+        const Span codes{s.zq->codes, s.zq->codes_len, 1, "Z's codes"};
+        const Span scales{s.zq->scales, s.zq->scales_len, 1, "Z's scales"};
+        if (s.z_out) {
+            outs[no++] = codes;
+            outs[no++] = scales;
+        } else {
+            more[nm++] = codes;
+            more[nm++] = scales;
+        }
+    }
+    if (s.dbias) {
+        if (s.dbias_len != n)
+            return fail(GK_ERR_SHAPE, "gemmkit: dbias length (%zu) != the output's columns (%zu)",
+                        s.dbias_len, n);
+        if ((uintptr_t)s.dbias % 4) return fail(GK_ERR_ARG, "gemmkit: dbias is not aligned to its type");
+        outs[no++] = {s.dbias, n, 4, "dbias"};
+    }
+    return check_disjoint(outs, no, more, nm);
+}
+
+LinearParams linear_params(const LinearSpec &s, float alpha, const gk_mat_mut *c) {
+    LinearParams p{};
+    p.c = c->data;
+    p.rsc = c->rs;
+    p.csc = c->cs;
+    p.alpha = alpha;
+    p.act = s.act;
+    p.slope = s.slope;
+    if (s.bias) {
+        p.bias = s.bias->data;
+        p.bias_f32 = s.bias_f32;
+    }
+    if (s.res) {
+        p.res = s.res->data;
+        p.rsr = s.res->rs;
+        p.csr = s.res->cs;
+    }
+    if (s.z) {
+        p.z = (uint16_t *)const_cast<void *>(s.z->data);
+        p.rsz = s.z->rs;
+        p.csz = s.z->cs;
+    }
+    if (s.zq) {
+        p.codes = (uint8_t *)s.zq->codes;
+        p.scales = (uint8_t *)s.zq->scales;
+        p.ld = (int64_t)s.zq->ld;
+        p.lds = (int64_t)s.zq->lds;
+    }
+    return p;
+}
+
+// dbias <- the sum of `rows` rows of partial column sums.
+int add_col_sums(const float *part, int64_t rows, const LinearSpec &s) {
+    const hipError_t e = launch_col_sums(part, rows, (int64_t)s.dbias_len, s.dbias, tl_stream);
+    return e == hipSuccess ? GK_OK : hip_fail(e, "column sums");
+}
+
+// Z = alpha*A*B + bias, C = act(Z) + residual; or (grad) C = (alpha*A*B) * act'(Z).
+int linear_checked(gk_workspace *ws, EpiKind kind, bool grad, float alpha, const gk_mat_ref *a,
+                   const gk_mat_ref *b, const LinearSpec &s, const gk_mat_mut *c) {
+    int r;
+    const char *const cname = grad ? "D" : "C";
+    if (!a || !b || !c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if (a->cols != b->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.cols (%zu) != B.rows (%zu)", a->cols, b->rows);
+    if (a->rows != c->rows)
+        return fail(GK_ERR_SHAPE, "gemmkit: A.rows (%zu) != %s.rows (%zu)", a->rows, cname, c->rows);
+    if (b->cols != c->cols)
+        return fail(GK_ERR_SHAPE, "gemmkit: B.cols (%zu) != %s.cols (%zu)", b->cols, cname, c->cols);
+    if ((r = check_view(a->len, a->rows, a->cols, a->rs, a->cs, "A"))) return r;
+    if ((r = check_view(b->len, b->rows, b->cols, b->rs, b->cs, "B"))) return r;
+    Span ins[2] = {{a->data, a->len, 2, "A"}, {b->data, b->len, 2, "B"}};
+    if ((r = check_linear(s, c, kind == EpiKind::F32 ? 4 : 2, cname, "the residual", ins, 2))) return r;
+    if ((r = check_ragged_sizes(a->rows, a->cols, b->cols, 1))) return r;
+    const int64_t row_bytes = round_up64((int64_t)a->cols * 2, 16);
+    if (row_bytes > kMaxRaggedRow) return row_too_long("A", row_bytes);
+    if ((r = device_init())) return r;
+    const int64_t M = (int64_t)a->rows, N = (int64_t)b->cols;
+    if (N == 0) return ok();
+    if (M == 0) {
+        if (!s.dbias) return ok();
+        return (r = add_col_sums(nullptr, 0, s)) ? r : finish("linear gradient");
+    }
+    RaggedArgs g{};
+    g.cus = g_num_cus;
+    g.splits = 1;
+    g.G = 1;
+    g.M = (int32_t)M;
+    g.N = (int32_t)N;
+    g.K = alpha == 0.0f ? 0 : (int32_t)a->cols;  // (then nothing of A and B is read)
+    ForwardOperands f(g, Opnd{a->data, a->rs, a->cs, 0}, b->data, b->rs, b->cs, 0);
+    LinearParams p = linear_params(s, alpha, c);
+    const int64_t unit = linear_unit(g, f.layout()), parts = s.dbias ? (M + unit - 1) / unit : 0;
+    const size_t sums = parts > 1 ? (size_t)parts * N * 4 : 0;
+    void *buf = nullptr;
+    if (f.packed() + sums > 0) {
+        if ((r = ws_reserve(resolve_ws(ws), f.packed() + sums, &buf))) return r;
+        if (f.packed() > 0 && (r = f.pack((uint8_t *)buf))) return r;
+    }
+    float *const part = sums ? (float *)((uint8_t *)buf + f.packed()) : nullptr;
+    p.sums = sums ? part : s.dbias;
+    const RaggedB bl = f.place();
+    const hipError_t e = grad ? launch_linear_grad(g, bl, kind, p, tl_stream)
+                              : launch_linear(g, bl, kind, p, tl_stream);
+    if (e != hipSuccess) return launch_failed(e, grad ? "linear gradient" : "linear layer");
+    if (sums && (r = add_col_sums(part, parts, s))) return r;
+    return finish(grad ? "linear gradient" : "linear layer");
+}
+
+int act_grad_checked(gk_workspace *ws, InType in, const LinearSpec &s, const gk_mat_mut *c) {
+    int r;
+    if (!s.res || !c) return fail(GK_ERR_ARG, "gemmkit: null view argument");
+    if ((r = check_linear(s, c, 2, "D", "G", nullptr, 0))) return r;
+    if ((r = check_ragged_sizes(c->rows, 0, c->cols, 1))) return r;
+    if ((r = device_init())) return r;
+    const int64_t M = (int64_t)c->rows, N = (int64_t)c->cols;
+    if (N == 0) return ok();
+    if (M == 0) {
+        if (!s.dbias) return ok();
+        return (r = add_col_sums(nullptr, 0, s)) ? r : finish("activation gradient");
+    }
+    LinearParams p = linear_params(s, 1.0f, c);
+    const int64_t unit = act_grad_unit(M, N, g_num_cus), parts = s.dbias ? (M + unit - 1) / unit : 0;
+    void *part = nullptr;
+    if (parts > 1 && (r = ws_reserve(resolve_ws(ws), (size_t)parts * N * 4, &part))) return r;
+    p.sums = parts > 1 ? (float *)part : s.dbias;
+    const hipError_t e = launch_act_grad(in, M, N, g_num_cus, p, tl_stream);
+    if (e != hipSuccess) return hip_fail(e, "activation gradient");
+    if (parts > 1 && (r = add_col_sums((const float *)part, parts, s))) return r;
+    return finish("activation gradient");
+}
+
+LinearSpec linear_spec(const gk_bias *bias, int32_t bias_f32, int32_t act, float slope,
+                       const gk_mat_ref *residual, size_t so, const gk_mat_ref *z,
+                       const gk_mxint8 *zq) {
+    LinearSpec s;
+    s.bias = bias;
+    s.bias_f32 = bias_f32;
+    s.act = act;
+    s.slope = slope;
+    s.res = residual;
+    s.res_size = so;
+    s.z = z;
+    s.zq = zq;
+    return s;
+}
+
+int linear_entry(gk_workspace *ws, EpiKind kind, float alpha, const gk_mat_ref *a,
+                 const gk_mat_ref *b, const gk_bias *bias, int32_t bias_f32, int32_t act,
+                 float slope, const gk_mat_ref *residual, const gk_mat_mut *z, const gk_mxint8 *zq,
+                 const gk_mat_mut *c) {
+    gk_mat_ref zr{};
+    if (z) zr = gk_mat_ref{z->data, z->len, z->rows, z->cols, z->rs, z->cs};
+    LinearSpec s = linear_spec(bias, bias_f32, act, slope, residual, kind == EpiKind::F32 ? 4 : 2,
+                               z ? &zr : nullptr, zq);
+    s.z_out = true;
+    return linear_checked(ws, kind, false, alpha, a, b, s, c);
+}
+
+int dgrad_entry(gk_workspace *ws, EpiKind kind, float alpha, const gk_mat_ref *a,
+                const gk_mat_ref *b, int32_t act, float slope, const gk_mat_ref *z,
+                const gk_mxint8 *zq, float *dbias, size_t dbias_len, const gk_mat_mut *d) {
+    LinearSpec s = linear_spec(nullptr, 0, act, slope, nullptr, 0, z, zq);
+    s.dbias = dbias;
+    s.dbias_len = dbias_len;
+    return linear_checked(ws, kind, true, alpha, a, b, s, d);
+}
+
+int act_grad_entry(gk_workspace *ws, InType in, const gk_mat_ref *gr, int32_t act, float slope,
+                   const gk_mat_ref *z, const gk_mxint8 *zq, float *dbias, size_t dbias_len,
+                   const gk_mat_mut *d) {
+    LinearSpec s = linear_spec(nullptr, 0, act, slope, gr, in_size(in), z, zq);
+    s.dbias = dbias;
+    s.dbias_len = dbias_len;
+    return act_grad_checked(ws, in, s, d);
 }
 
 // ---- pointer-array batched (src/api/batched.rs:711-799; run_ptr,
@@ -3419,6 +3865,74 @@ int gk_gemm_grouped_mxfp4_f32(gk_workspace *, float alpha, const gk_mxfp4 *a,
                               const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
                               float beta, const gk_mat_mut *c, gk_par) {
     return mxfp4_checked(EpiKind::F32, 4, alpha, a, true, offsets, groups, b, beta, c);
+}
+
+int gk_quantize_mxint8_f32(const gk_mat_ref *x, const gk_mxint8 *q) {
+    return quantize8_checked(InType::F32, x, q);
+}
+
+int gk_quantize_mxint8_bf16(const gk_mat_ref *x, const gk_mxint8 *q) {
+    return quantize8_checked(InType::BF16, x, q);
+}
+
+int gk_dequantize_mxint8_f32(const gk_mxint8 *q, int32_t act, float slope, const gk_mat_mut *c) {
+    return dequantize8_checked(InType::F32, q, act, slope, c);
+}
+
+int gk_dequantize_mxint8_bf16(const gk_mxint8 *q, int32_t act, float slope, const gk_mat_mut *c) {
+    return dequantize8_checked(InType::BF16, q, act, slope, c);
+}
+
+int gk_gemm_wgrad_mxint8_bf16(gk_workspace *ws, float alpha, const gk_mxint8 *a, int32_t act,
+                              float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                              gk_par) {
+    return wgrad8_checked(ws, EpiKind::BF16, 2, alpha, a, act, slope, b, beta, c);
+}
+
+int gk_gemm_wgrad_mxint8_f32(gk_workspace *ws, float alpha, const gk_mxint8 *a, int32_t act,
+                             float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                             gk_par) {
+    return wgrad8_checked(ws, EpiKind::F32, 4, alpha, a, act, slope, b, beta, c);
+}
+
+int gk_gemm_linear_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a, const gk_mat_ref *b,
+                        const gk_bias *bias, int32_t bias_f32, int32_t act, float slope,
+                        const gk_mat_ref *residual, const gk_mat_mut *z, const gk_mxint8 *zq,
+                        const gk_mat_mut *c, gk_par) {
+    return linear_entry(ws, EpiKind::BF16, alpha, a, b, bias, bias_f32, act, slope, residual, z, zq, c);
+}
+
+int gk_gemm_linear_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a, const gk_mat_ref *b,
+                          const gk_bias *bias, int32_t bias_f32, int32_t act, float slope,
+                          const gk_mat_ref *residual, const gk_mat_mut *z, const gk_mxint8 *zq,
+                          const gk_mat_mut *c, gk_par) {
+    return linear_entry(ws, EpiKind::F32, alpha, a, b, bias, bias_f32, act, slope, residual, z, zq, c);
+}
+
+int gk_gemm_linear_dgrad_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                              const gk_mat_ref *b, int32_t act, float slope, const gk_mat_ref *z,
+                              const gk_mxint8 *zq, float *dbias, size_t dbias_len,
+                              const gk_mat_mut *d, gk_par) {
+    return dgrad_entry(ws, EpiKind::BF16, alpha, a, b, act, slope, z, zq, dbias, dbias_len, d);
+}
+
+int gk_gemm_linear_dgrad_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                const gk_mat_ref *b, int32_t act, float slope, const gk_mat_ref *z,
+                                const gk_mxint8 *zq, float *dbias, size_t dbias_len,
+                                const gk_mat_mut *d, gk_par) {
+    return dgrad_entry(ws, EpiKind::F32, alpha, a, b, act, slope, z, zq, dbias, dbias_len, d);
+}
+
+int gk_activation_grad_bf16(gk_workspace *ws, const gk_mat_ref *g, int32_t act, float slope,
+                            const gk_mat_ref *z, const gk_mxint8 *zq, float *dbias,
+                            size_t dbias_len, const gk_mat_mut *d) {
+    return act_grad_entry(ws, InType::BF16, g, act, slope, z, zq, dbias, dbias_len, d);
+}
+
+int gk_activation_grad_f32(gk_workspace *ws, const gk_mat_ref *g, int32_t act, float slope,
+                           const gk_mat_ref *z, const gk_mxint8 *zq, float *dbias,
+                           size_t dbias_len, const gk_mat_mut *d) {
+    return act_grad_entry(ws, InType::F32, g, act, slope, z, zq, dbias, dbias_len, d);
 }
 
 }  // extern "C"

@@ -47,21 +47,10 @@ bool grouped_plan_any(RaggedArgs &g, RaggedB bl, int64_t copies) {
     return cost < 4.6 + (double)copies / 2.49e6 + aligned;
 }
 
-template <typename F>
-static auto any_align_tile(const RaggedArgs &g, F f) {
-    switch (g.tile) {
-    case 0: return f(RegTile<128, 128, 2, 4>{});
-    case 1: return f(RegTile<128, 64, 4, 2>{});
-    case 2: return f(RegTile<32, 64, 1, 4>{});
-    case 3: return f(RegWaveTile<16, 32, 4>{});
-    default: return f(RegWaveTile<16, 32, 8>{});
-    }
-}
-
 template <bool BT, EpiKind E>
 static hipError_t any_align_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     return any_align_tile(
-        g, [&](auto t) { return ragged_go<false, false, BT, E, decltype(t)>(g, ep, stream); });
+        g, [&](auto t) { return ragged_go<false, false, BT, PlainOut<E>, decltype(t)>(g, ep, stream); });
 }
 
 RaggedPlan grouped_plan(const RaggedArgs &g, RaggedB bl) {
@@ -153,7 +142,7 @@ static auto wgrad_tile(const RaggedArgs &g, F f) {
 template <EpiKind E>
 static hipError_t wgrad_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     return wgrad_tile(
-        g, [&](auto t) { return ragged_go<false, true, true, E, decltype(t)>(g, ep, stream); });
+        g, [&](auto t) { return ragged_go<false, true, true, PlainOut<E>, decltype(t)>(g, ep, stream); });
 }
 
 RaggedPlan grouped_wgrad_plan(const RaggedArgs &g) {

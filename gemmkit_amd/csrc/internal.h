@@ -48,7 +48,8 @@ struct EpiParams {
     const void *fbias;     // bias vector or nullptr
 };
 
-enum FusedAct : int32_t { kActNone = 0, kActRelu = 1, kActLeakyRelu = 2 };
+enum FusedAct : int32_t { kActNone = 0, kActRelu = 1, kActLeakyRelu = 2,
+                          kActGelu = 3, kActGeluTanh = 4, kActSilu = 5 };  // (3..5: LinearParams)
 
 // Largest operand row stride and row length (bytes) the matrix-core kernels
 // address: 256 row strides plus a row stay below 2^31 bytes of 32-bit buffer
@@ -291,5 +292,49 @@ hipError_t launch_mxfp4_dequantize(InType out, const MxArgs &g, hipStream_t stre
 // C = epi(A B^T) of MXFP4 operands per group: K in elements, lda/ldb bytes of code rows.
 hipError_t launch_mxfp4(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 RaggedPlan mxfp4_plan(const RaggedArgs &g);
+
+
+// MXINT8 (mxint8.hip): rows of int8 codes with one e8m0 scale per 32 elements; the value of
+// a code is code * 2^(byte - 133).  The scale of a block whose largest magnitude has the f32
+// exponent field E is max(E, kMxint8Min): steps are normal numbers.
+constexpr int kMxint8Min = 7;
+hipError_t launch_mxint8_quantize(InType in, const MxArgs &g, hipStream_t stream);
+// x = act(values), rounded to x's type.
+hipError_t launch_mxint8_dequantize(InType out, const MxArgs &g, int32_t act, float slope,
+                                    hipStream_t stream);
+
+// Linear layers (linear.h).  Forward: Z = alpha*A*B + bias, C = act(Z) + res, Z kept in z
+// (bf16) or in codes and scales (MXINT8).  Backward (the gradient at the layer before's
+// pre-activations, kept the same ways): C = (alpha*A*B) * act'(Z) and sums, C's column sums
+// before rounding.  Pointers that are not there are null.
+struct LinearParams {
+    void *c;                   // bf16 or f32: element (i, j) at c + i*rsc + j*csc
+    int64_t rsc, csc;
+    float alpha;
+    int32_t act;               // FusedAct
+    float slope;
+    const void *bias;          // per column
+    int32_t bias_f32;          // f32 (1) or bf16 (0)
+    const void *res;           // of C's type; may be C itself
+    int64_t rsr, csr;
+    uint16_t *z;
+    int64_t rsz, csz;
+    uint8_t *codes, *scales;   // row i at codes + i*ld, scales + i*lds
+    int64_t ld, lds;
+    float *sums;               // row of N column sums for each linear_unit() rows of the product
+};
+// A product without offsets (one group).  kind: C's type.
+hipError_t launch_linear(const RaggedArgs &g, RaggedB bl, EpiKind kind, const LinearParams &p,
+                         hipStream_t stream);
+hipError_t launch_linear_grad(const RaggedArgs &g, RaggedB bl, EpiKind kind, const LinearParams &p,
+                              hipStream_t stream);
+int linear_unit(const RaggedArgs &g, RaggedB bl);
+// C = A * act'(Z), elementwise over M x N (A of either type at p.res, C bf16), with column
+// sums per act_grad_unit() rows.
+int act_grad_unit(int64_t m, int64_t n, int cus);
+hipError_t launch_act_grad(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,
+                           hipStream_t stream);
+// out[j] = the sum over i < rows of part[i*n + j], in a fixed order.
+hipError_t launch_col_sums(const float *part, int64_t rows, int64_t n, float *out, hipStream_t stream);
 
 }  // namespace gk

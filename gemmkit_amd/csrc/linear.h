@@ -1,0 +1,523 @@
+#pragma once
+// linear.h -- what a linear layer's products do on their way out of the accumulators:
+// bias, activation, residual and the pre-activation kept for the backward pass; or, in the
+// backward pass, the activation's derivative and the bias gradient.
+//
+// Activations and derivatives, with P(z) the normal distribution and p(z) its density:
+//   gelu       z P(z)                 P + z p
+//   gelu_tanh  z s, s = sigmoid(2u)   s + z s (1 - s) 2u',  u = c (z + 0.044715 z^3), c^2 = 2/pi
+//   silu       z s, s = sigmoid(z)    s + z s (1 - s)
+// P(-|z|) = q e / 2 with e = exp(-z^2/2) and q a polynomial of degree 5 in
+// 1 / (1 + 0.3275911 |z| / sqrt 2): Hastings' approximation (Abramowitz and Stegun 7.1.26,
+// off by at most 1.5e-7 of erf), whose exponential is the density's too.
+#include "ragged.h"
+
+namespace gk {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGeluC2 = 1.5957691216057308f;  // 2 sqrt(2/pi)
+constexpr float kGeluCubic = 0.044715f;
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+struct Normal {  // the distribution and exp(-z^2/2)
+    float p, e;
+    __device__ __forceinline__ explicit Normal(float z) {
+        const float t = fast_rcp(__builtin_fmaf(__builtin_fabsf(z), 0.3275911f * 0.70710678f, 1.0f));
+        e = fast_exp2(z * z * (-0.5f * kLog2e));
+        float q = 1.061405429f;
+        q = __builtin_fmaf(q, t, -1.453152027f);
+        q = __builtin_fmaf(q, t, 1.421413741f);
+        q = __builtin_fmaf(q, t, -0.284496736f);
+        q = __builtin_fmaf(q, t, 0.254829592f);
+        q = q * t * (0.5f * e);
+        p = z > 0.0f ? 1.0f - q : q;
+    }
+};
+
+__device__ __forceinline__ float sigmoid(float z) {
+    return fast_rcp(1.0f + fast_exp2(-kLog2e * z));
+}
+__device__ __forceinline__ float gelu_inner(float z) {
+    return z * __builtin_fmaf(kGeluC2 * kGeluCubic, z * z, kGeluC2);
+}
+
+// f = act(f).  (ReLU and LeakyReLU as fused_apply's: NaN and -0 give 0.)
+template <int N>
+__device__ __forceinline__ void act_apply(float (&f)[N], int act, float slope) {
+    if (act == kActGelu) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= Normal(f[e]).p;
+    } else if (act == kActGeluTanh) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= sigmoid(gelu_inner(f[e]));
+    } else if (act == kActSilu) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= sigmoid(f[e]);
+    } else if (act != kActNone) {
+        const float s = act == kActRelu ? 0.0f : slope;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float hi = f[e] > 0.0f ? f[e] : 0.0f, lo = f[e] < 0.0f ? f[e] : 0.0f;
+            f[e] = act == kActRelu ? hi : __builtin_fmaf(s, lo, hi);
+        }
+    }
+}
+
+// f *= act'(z); at 0 ReLU's derivative is 0 and LeakyReLU's the slope.
+template <int N>
+__device__ __forceinline__ void act_scale(float (&f)[N], const float (&z)[N], int act, float slope) {
+    if (act == kActGelu) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const Normal d(z[e]);
+            f[e] *= __builtin_fmaf(z[e] * 0.3989422804f, d.e, d.p);
+        }
+    } else if (act == kActGeluTanh) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            // (s (1 - s) from exp(-|2u|): as 1 - s it would lose what z and u' multiply)
+            const float u = gelu_inner(z[e]), t = fast_exp2(-kLog2e * __builtin_fabsf(u));
+            const float r = fast_rcp(1.0f + t), q = t * r;
+            // (beyond 16 q is 0, and the square would overflow far out)
+            const float b = __builtin_amdgcn_fmed3f(z[e], -16.0f, 16.0f);
+            const float du = __builtin_fmaf(3.0f * kGeluC2 * kGeluCubic, b * b, kGeluC2);
+            f[e] *= __builtin_fmaf(q * r, b * du, u > 0.0f ? r : q);
+        }
+    } else if (act == kActSilu) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float s = sigmoid(z[e]);
+            f[e] *= s * __builtin_fmaf(z[e], 1.0f - s, 1.0f);
+        }
+    } else if (act != kActNone) {
+        const float s = act == kActRelu ? 0.0f : slope;
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= z[e] > 0.0f ? 1.0f : s;
+    }
+}
+
+// ---------------------------------------------------------------- MXINT8
+
+// The scale byte of a block whose largest magnitude has the bits `top`.
+__device__ __forceinline__ int mxint8_byte(uint32_t top) {
+    const int e = (int)(top >> 23);
+    return e > kMxint8Min ? e : kMxint8Min;
+}
+// Four values as codes: nearest whole multiple of the step, ties to even, at most 127.  A
+// value times 1/step is below 2^7 (1.5 * 2^23 added to it leaves the whole number, rounded,
+// in the low bits).
+__device__ __forceinline__ uint32_t mxint8_codes4(const float *v, int byte) {
+    if (byte == 255) return 0;
+    const float inv = __uint_as_float((uint32_t)(260 - byte) << 23);
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(v[i] * inv, -127.0f, 127.0f) + 12582912.0f);
+    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400);
+    const uint32_t hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000C0C);
+    return lo | hi;
+}
+__device__ __forceinline__ float mxint8_step(int byte) {
+    return byte == 255 ? __builtin_nanf("") : __builtin_ldexpf(1.0f, byte - 133);
+}
+__device__ __forceinline__ void mxint8_values4(uint32_t w, float step, float *v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)((int32_t)(w << (24 - 8 * i)) >> 24) * step;
+}
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// The largest of `top` over the LB lanes (4 or 8) of a block.
+template <int LB>
+__device__ __forceinline__ uint32_t block_max(uint32_t top) {
+    top = max_bits(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, true));  // lane ^ 1
+    top = max_bits(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+    if constexpr (LB == 8)
+        top = max_bits(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x141, 0xF, 0xF, true));  // 7 - lane % 8
+    return top;
+}
+
+// ---------------------------------------------------------------- output
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+// CH consecutive bf16 or f32 values of a row at p (element stride cs; cols of them exist), as
+// they lie in memory.
+template <bool F32, int CH>
+__device__ __forceinline__ v4u read_raw(const void *p, int64_t at, int64_t cs, int cols) {
+    v4u w = {};
+    if constexpr (F32) {
+        static_assert(CH == 4, "16 bytes");
+        typedef v4u v4u_any4 __attribute__((aligned(4)));
+        const uint32_t *q = (const uint32_t *)p + at;
+        if (cs == 1 && cols >= CH) return *(const v4u_any4 *)q;
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (e < cols) w[e] = q[e * cs];
+    } else {
+        const uint16_t *q = (const uint16_t *)p + at;
+        if (cs == 1 && cols >= CH) {
+            if constexpr (CH == 8) {
+                typedef v4u v4u_any2 __attribute__((aligned(2)));
+                return *(const v4u_any2 *)q;
+            } else {
+                const v2u_any2 h = *(const v2u_any2 *)q;
+                w[0] = h[0];
+                w[1] = h[1];
+                return w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (e < cols) w[e / 2] |= (uint32_t)q[e * cs] << (16 * (e % 2));
+    }
+    return w;
+}
+
+template <bool F32, int CH>
+__device__ __forceinline__ void widen(const v4u &w, float (&f)[CH]) {
+#pragma unroll
+    for (int e = 0; e < CH; ++e)
+        f[e] = __uint_as_float(F32 ? w[e % 4] : e % 2 ? w[e / 2 % 4] & 0xFFFF0000u : w[e / 2 % 4] << 16);
+}
+
+// CH values of a row, rounded once; NT: whole lines, stored nontemporally.
+template <bool F32, int CH>
+__device__ __forceinline__ void write_row(void *p, int64_t at, int64_t cs, int cols, bool nt,
+                                          const float (&f)[CH]) {
+    v4u w = {};
+    if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) w[e] = __float_as_uint(f[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < CH / 2; ++e) w[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
+    }
+    if (cs == 1 && cols >= CH) {
+        typedef v4u v4u_any2 __attribute__((aligned(2)));
+        if constexpr (CH * (F32 ? 4 : 2) == 16) {
+            v4u_any2 *q = (v4u_any2 *)((uint8_t *)p + at * (F32 ? 4 : 2));
+            if (nt) __builtin_nontemporal_store(w, q);
+            else *q = w;
+        } else {
+            *(v2u_any2 *)((uint16_t *)p + at) = v2u_any2{w[0], w[1]};
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < CH; ++e)
+        if (e < cols) {
+            if constexpr (F32) ((uint32_t *)p)[at + e * cs] = w[e];
+            else ((uint16_t *)p)[at + e * cs] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+        }
+}
+
+__device__ __forceinline__ bool row_lines(const void *p, int64_t row_bytes) {
+    return (((uint64_t)p | (uint64_t)row_bytes) & 127) == 0;
+}
+
+// Rows of a product for which sums holds one row: a tile's, or (256 x 256) half a tile's,
+// since the last round's tiles may go out as halves.
+constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }
+
+template <EpiKind E, bool GRAD>
+struct LinearOut {
+    using Params = LinearParams;
+    static constexpr bool F32 = E == EpiKind::F32;
+    static constexpr int CH = chunk_of(E);
+    static constexpr int LB = 32 / CH;  // lanes of a checkpoint's block
+
+    // What a chunk reads: the residual, or the pre-activations (v) with their scale.
+    struct In {
+        v4u v;
+        int byte;
+    };
+    __device__ __forceinline__ static In load(const Params &p, int row, int col, int N, bool live) {
+        In in = {};
+        if (!live || col >= N) return in;
+        if constexpr (!GRAD) {
+            if (p.res)
+                in.v = read_raw<F32, CH>(p.res, row * p.rsr + col * p.csr, p.csr, N - col);
+        } else if (p.codes) {
+            // (a begun block's codes are all there)
+            const uint8_t *q = p.codes + row * p.ld + col;
+            if constexpr (CH == 8) {
+                const v2u w = *(const v2u *)q;
+                in.v[0] = w[0];
+                in.v[1] = w[1];
+            } else {
+                in.v[0] = *(const uint32_t *)q;
+            }
+            in.byte = p.scales[row * p.lds + (col >> 5)];
+        } else if (p.z) {
+            in.v = read_raw<false, CH>(p.z, row * p.rsz + col * p.csz, p.csz, N - col);
+        }
+        return in;
+    }
+    struct Flags {
+        bool nt_c, nt_z;
+        __device__ __forceinline__ explicit Flags(const Params &p) {
+            nt_c = row_lines(p.c, p.rsc * (F32 ? 4 : 2));
+            nt_z = row_lines(p.z, p.rsz * 2);
+        }
+    };
+    __device__ __forceinline__ static void bias_of(const Params &p, int col, int N, float (&b)[CH]) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) b[e] = 0.0f;
+        if (GRAD || !p.bias) return;
+#pragma unroll
+        for (int e = 0; e < CH; ++e)
+            if (col + e < N)
+                b[e] = p.bias_f32 ? ((const float *)p.bias)[col + e]
+                                  : bf16_widen(((const uint16_t *)p.bias)[col + e]);
+    }
+    // f: sums of products in, the output before rounding out.  Every lane of a row's block
+    // comes along.
+    __device__ __forceinline__ static void store(const Params &p, const Flags &fl, int row, int col,
+                                                 int N, const float (&bias)[CH], const In &in,
+                                                 float (&f)[CH]) {
+        const int cols = N - col;  // (0 or less: outside the matrix)
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) f[e] *= p.alpha;
+            if (p.act != kActNone) {
+                float z[CH];
+                if (p.codes) {
+                    const float step = mxint8_step(in.byte);
+#pragma unroll
+                    for (int e = 0; e < CH; e += 4) mxint8_values4(in.v[e / 4], step, z + e);
+                } else {
+                    widen<false, CH>(in.v, z);
+                }
+                act_scale(f, z, p.act, p.slope);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) f[e] = __builtin_fmaf(p.alpha, f[e], bias[e]);
+            if (p.codes) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < CH; ++e) {
+                    if (e >= cols) f[e] = 0.0f;
+                    top = max_bits(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+                }
+                const int byte = mxint8_byte(block_max<LB>(top));
+                if ((col >> 5) < (N + 31) >> 5) {
+                    uint8_t *q = p.codes + row * p.ld + col;
+                    if constexpr (CH == 8)
+                        *(v2u *)q = v2u{mxint8_codes4(f, byte), mxint8_codes4(f + 4, byte)};
+                    else
+                        *(uint32_t *)q = mxint8_codes4(f, byte);
+                    if ((col & 31) == 0) p.scales[row * p.lds + (col >> 5)] = (uint8_t)byte;
+                }
+            } else if (p.z && cols > 0) {
+                write_row<false, CH>(p.z, row * p.rsz + col * p.csz, p.csz, cols, fl.nt_z, f);
+            }
+            act_apply(f, p.act, p.slope);
+            if (p.res) {
+                float r[CH];
+                widen<F32, CH>(in.v, r);
+#pragma unroll
+                for (int e = 0; e < CH; ++e) f[e] += r[e];
+            }
+        }
+        if (cols > 0) write_row<F32, CH>(p.c, row * p.rsc + col * p.csc, p.csc, cols, fl.nt_c, f);
+    }
+
+    // Column sums of a tile from the first row of its unit on.
+    template <int BM>
+    __device__ __forceinline__ static void put_sum(const Params &p, const RaggedTile &t, int N,
+                                                   int c, float s) {
+        constexpr int UNIT = sum_unit(BM);
+        if (t.n0 + c >= N) return;
+        float *q = p.sums + (int64_t)(t.row0 / UNIT) * N + t.n0 + c;
+        q[0] = s;
+        if (UNIT < BM && t.rows > UNIT) q[N] = 0.0f;
+    }
+
+    // Tiles that lie in LDS whole, SLABS partial sums of each element one after the other, of
+    // which every thread takes chunks.
+    template <int BM, int BN, int THREADS, int SLABS>
+    __device__ __forceinline__ static void slabs(const Params &p, const RaggedTile &t, int N,
+                                                 float *sums) {
+        constexpr int LD = BN + 4, CPR = BN / CH, CHUNKS = BM * CPR;
+        constexpr int U = (CHUNKS + THREADS - 1) / THREADS;
+        static_assert(CHUNKS % 64 == 0 && BN % 32 == 0, "whole waves, whole blocks");
+        const Flags fl(p);
+        In in[U];
+        float bias[U][CH];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {  // (on their way while the sums meet)
+            const int c = threadIdx.x + u * THREADS, row = c / CPR, col = t.n0 + c % CPR * CH;
+            const bool live = c < CHUNKS && row < t.rows;
+            in[u] = load(p, t.row0 + row, col, N, live);
+            bias_of(p, live ? col : N, N, bias[u]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = threadIdx.x + u * THREADS, row = c / CPR, at = c % CPR * CH;
+            if (c >= CHUNKS || row >= t.rows) continue;
+            float f[CH];
+#pragma unroll
+            for (int i = 0; i < CH; i += 4) {
+                v4f v = {};
+#pragma unroll
+                for (int w = 0; w < SLABS; ++w) v += *(const v4f *)(sums + (w * BM + row) * LD + at + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[i + e] = v[e];
+            }
+            store(p, fl, t.row0 + row, t.n0 + at, N, bias[u], in[u], f);
+            if (GRAD && p.sums) {
+#pragma unroll
+                for (int i = 0; i < CH; i += 4)
+                    *(v4f *)(sums + row * LD + at + i) = v4f{f[i], f[i + 1], f[i + 2], f[i + 3]};
+            }
+        }
+        if (GRAD && p.sums) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < BN; c += THREADS) {
+                float s = 0.0f;
+                for (int r = 0; r < t.rows; ++r) s += sums[r * LD + c];
+                put_sum<BM>(p, t, N, c, s);
+            }
+        }
+    }
+
+    template <int BM, int BN, int KS, int SMEM, int TM, int TN>
+    __device__ __forceinline__ static void waves(const Params &p, const RaggedTile &t, int N,
+                                                 const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                                 int lane) {
+        constexpr int LD = BN + 4;
+        static_assert(KS * BM * LD * 4 <= SMEM, "LDS");
+        float *const sums = (float *)smem;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                *(v4f *)(sums + (wave * BM + i * 16 + (lane & 15)) * LD + j * 16 + 4 * (lane >> 4)) =
+                    acc[i][j];
+        slabs<BM, BN, KS * 64, KS>(p, t, N, sums);
+    }
+
+    template <int BM, int BN, int WM, int WN, int SMEM, int TM, int TN>
+    __device__ __forceinline__ static void tile(const Params &p, const RaggedTile &t, int N,
+                                                const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                                int lane) {
+        constexpr int WTM = BM / WM, WTN = BN / WN;
+        const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, lq = lane >> 4;
+        if constexpr (WTN < 32) {
+            // A wave's columns are no whole block of a checkpoint: the tile goes through LDS
+            // whole.
+            constexpr int LD = BN + 4;
+            static_assert(BM * LD * 4 <= SMEM, "LDS");
+            float *const sums = (float *)smem;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    *(v4f *)(sums + (wm * WTM + i * 16 + l16) * LD + wn * WTN + j * 16 + 4 * lq) =
+                        acc[i][j];
+            slabs<BM, BN, WM * WN * 64, 1>(p, t, N, sums);
+        } else {
+            // Bands of 16 rows staged per wave, GB of them at a time, and read back as rows.
+            // (The row loop stays rolled: its code, five activations long, would not fit the
+            // instruction cache.)
+            constexpr int LD = WTN + 4, NW = WM * WN;
+            constexpr int GB = TM % 4 == 0 && NW * 64 * LD * 4 <= SMEM ? 4
+                               : TM % 2 == 0 && NW * 32 * LD * 4 <= SMEM ? 2 : 1;
+            static_assert(NW * GB * 16 * LD * 4 <= SMEM && WM * BN * 4 <= SMEM, "LDS");
+            constexpr int CPR = WTN / CH, RPP = 64 / CPR;  // chunks per row, rows per pass
+            constexpr int PASSES = GB * 16 / RPP;          // ... and group of bands
+            static_assert(RPP <= 16, "a pass lies in one band group");
+            float *const stg = (float *)smem + wave * GB * 16 * LD;
+            const int r0 = lane / CPR, c = lane % CPR * CH, col = t.n0 + wn * WTN + c;
+            const Flags fl(p);
+            float bias[CH], sum[CH] = {};
+            bias_of(p, col, N, bias);
+            const int last = t.rows < (wm + 1) * WTM ? t.rows : (wm + 1) * WTM;
+            int row = wm * WTM + r0;  // of the tile, this lane's in the next pass
+            In next = load(p, t.row0 + row, col, N, row < last);
+#pragma unroll
+            for (int h = 0; h < TM / GB; ++h) {
+#pragma unroll
+                for (int i = 0; i < GB; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        *(v4f *)(stg + (i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[h * GB + i][j];
+                __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+                for (int s = 0; s < PASSES; ++s) {
+                    const In in = next;
+                    const int at = row;
+                    row += RPP;
+                    next = load(p, t.row0 + row, col, N, row < last);
+                    float f[CH];
+#pragma unroll
+                    for (int i = 0; i < CH; i += 4) {
+                        const v4f v = *(const v4f *)(stg + (s * RPP + r0) * LD + c + i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[i + e] = v[e];
+                    }
+                    if (at < last) {
+                        store(p, fl, t.row0 + at, col, N, bias, in, f);
+                        if constexpr (GRAD) {
+#pragma unroll
+                            for (int e = 0; e < CH; ++e) sum[e] += f[e];
+                        }
+                    }
+                }
+                __builtin_amdgcn_s_waitcnt(0xC07F);
+                __builtin_amdgcn_wave_barrier();
+            }
+            if (GRAD && p.sums) {
+                // Lanes of the same columns, then the waves above each other, in order.
+#pragma unroll
+                for (int d = CPR; d < 64; d <<= 1)
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) sum[e] += __shfl_xor(sum[e], d);
+                __syncthreads();
+                float *const red = (float *)smem;
+                if (lane < CPR) {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) red[wm * BN + wn * WTN + c + e] = sum[e];
+                }
+                __syncthreads();
+                for (int j = threadIdx.x; j < BN; j += NW * 64) {
+                    float s = red[j];
+#pragma unroll
+                    for (int w = 1; w < WM; ++w) s += red[w * BN + j];
+                    put_sum<BM>(p, t, N, j, s);
+                }
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------- launch
+
+// The tiles of grouped.hip's rule.
+template <bool BT, EpiKind E, bool GRAD>
+static hipError_t linear_go(const RaggedArgs &g, const LinearParams &p, hipStream_t stream) {
+    const auto go = [&](auto t) {
+        return ragged_go<false, false, BT, LinearOut<E, GRAD>, decltype(t)>(g, p, stream);
+    };
+    if (g.any_align) return any_align_tile(g, go);
+    return forward_tile<false, BT>(g, go);
+}
+
+template <bool GRAD>
+static hipError_t linear_launch(const RaggedArgs &g, RaggedB bl, EpiKind kind,
+                                const LinearParams &p, hipStream_t stream) {
+    const bool cols = bl == RaggedB::Cols;
+    if (kind == EpiKind::BF16)
+        return cols ? linear_go<true, EpiKind::BF16, GRAD>(g, p, stream)
+                    : linear_go<false, EpiKind::BF16, GRAD>(g, p, stream);
+    if (kind == EpiKind::F32)
+        return cols ? linear_go<true, EpiKind::F32, GRAD>(g, p, stream)
+                    : linear_go<false, EpiKind::F32, GRAD>(g, p, stream);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace gk

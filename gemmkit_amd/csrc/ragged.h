@@ -392,7 +392,9 @@ __device__ __forceinline__ bool ragged_tile(const RaggedArgs &g, int lane, Ragge
         if (pid >= (int)((int64_t)(part + 1) * per / 8)) return false;
         int tm, s, e;
         tile_coords(pid % tiles, tiles_m, tiles_n, tm, tn);
-        one_group(g.off, g.G, g.M, t.g, lane, s, e);
+        s = 0;
+        e = g.M;
+        if (g.off) one_group(g.off, g.G, g.M, t.g, lane, s, e);
         const int sp = pid / tiles;
         if (g.splits > 1) {  // this part's stages of the group
             const int stages = (e - s + 63) / 64;
@@ -588,6 +590,58 @@ __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTi
     }
 }
 
+// The sums of the KS waves that share a BM x BN tile, added in wave order and stored.
+template <EpiKind E, bool NT, int BM, int BN, int KS, int TM, int TN>
+__device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile &t, int N,
+                                          const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                          int lane) {
+    constexpr int LD = BN + 4, CH = chunk_of(E);
+    float *const sums = (float *)smem;
+    const int l16 = lane & 15, lq = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            *(v4f *)(sums + (wave * BM + i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i][j];
+    __syncthreads();
+#pragma unroll 1
+    for (int c = threadIdx.x; c < BM * BN / CH; c += KS * 64) {
+        const int row = c / (BN / CH), col = c % (BN / CH) * CH;
+        if (row >= t.rows || t.n0 + col >= N) continue;
+        v4f v[CH / 4] = {};
+#pragma unroll
+        for (int w = 0; w < KS; ++w)
+#pragma unroll
+            for (int i = 0; i < CH / 4; ++i)
+                v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
+        store_chunk<E, NT>(ep, t.z, t.row0 + row, t.n0 + col, N, v);
+    }
+}
+
+// How a tile leaves the kernels: tile() of waves that each hold WTM x WTN of it, waves() of
+// waves that each hold sums of all of it, with SMEM bytes of LDS that nothing else uses any
+// more.  PlainOut: EpiParams' map.
+template <EpiKind E>
+struct PlainOut {
+    using Params = EpiParams;
+    template <int BM, int BN, int WM, int WN, int SMEM, int TM, int TN>
+    __device__ __forceinline__ static void tile(const Params &ep, const RaggedTile &t, int N,
+                                                const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                                int lane) {
+        constexpr int WTM = BM / WM, WTN = BN / WN;
+        const int wm = wave / WN, wn = wave % WN;
+        if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, N, acc, smem, wave, wm, wn, lane);
+        else ragged_store<E, false, WTM, WTN>(ep, t, N, acc, smem, wave, wm, wn, lane);
+    }
+    template <int BM, int BN, int KS, int SMEM, int TM, int TN>
+    __device__ __forceinline__ static void waves(const Params &ep, const RaggedTile &t, int N,
+                                                 const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                                 int lane) {
+        if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, N, acc, smem, wave, lane);
+        else wave_sums<E, false, BM, BN, KS>(ep, t, N, acc, smem, wave, lane);
+    }
+};
+
 // ---------------------------------------------------------------- small tiles
 
 // BM x BN tiles on a ring of NS stages: stage kt + NS - 1 is loaded while kt is multiplied, one
@@ -595,11 +649,11 @@ __device__ __forceinline__ void ragged_store(const EpiParams &ep, const RaggedTi
 // 64x32x2048x4096's 4-bit weights (107 MB of the 24 groups that have rows) in 21.9 us, 4.9 TB/s;
 // small outputs leave the CUs' matrix cores waiting for their first stages (1003x32x1024x704's
 // weight gradient 16.0 us, 2.9 TB/s of stores).
-template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN, int NS, bool ONCE>
+template <bool MX, bool AT, bool BT, typename O, int BM, int BN, int WM, int WN, int NS, bool ONCE>
 __global__ __launch_bounds__(WM * WN * 64)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedLds<MX, BM, BN, NS>::BYTES, WM * WN),
                                    ragged_waves(RaggedLds<MX, BM, BN, NS>::BYTES, WM * WN))))
-void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
+void ragged_kernel(const RaggedArgs g, const typename O::Params ep) {
     static_assert(!MX || (!AT && !BT), "MXFP4 operands are k-contiguous");
     static_assert(!AT || BT, "A transposed: the weights' gradient");
     constexpr int NW = WM * WN;
@@ -726,8 +780,7 @@ void ragged_kernel(const RaggedArgs g, const EpiParams ep) {
         half(sa, sa + PA::BYTES, H1{});
         __syncthreads();
     }
-    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
-    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // ---------------------------------------------------------------- 256 x 256 tile
@@ -752,10 +805,10 @@ struct RaggedBigLds {
     static constexpr int BYTES = SCALES + (MX ? 2 * ScalePanel<256, 256>::SLOT : 0);
 };
 
-template <bool MX, bool AT, bool BT, EpiKind E>
+template <bool MX, bool AT, bool BT, typename O>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
-    constexpr int BM = 256, BN = 256, WN = 4, WTM = 128, WTN = 64, TM = 8, TN = 4;
+void ragged_big_kernel(const RaggedArgs g, const typename O::Params ep) {
+    constexpr int BM = 256, BN = 256, WM = 2, WN = 4, WTM = 128, WTN = 64, TM = 8, TN = 4;
     using L = RaggedBigLds<MX>;
     using PA = Panel<AT, BM, 8>;
     using PB = Panel<BT, BN, 8>;
@@ -941,8 +994,7 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
         }
         __syncthreads();
     }
-    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
-    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // ---------------------------------------------------------------- few tiles
@@ -953,33 +1005,6 @@ void ragged_big_kernel(const RaggedArgs g, const EpiParams ep) {
 // barriers); their sums are added in wave order through LDS at the end.  Bound by latency:
 // 8x64x2048x1024 7.6 us (3.9 TB/s of the seven matrices that are used), 5.2 where the caches
 // hold them from the call before.
-template <EpiKind E, bool NT, int BM, int BN, int KS, int TM, int TN>
-__device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile &t, int N,
-                                          const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
-                                          int lane) {
-    constexpr int LD = BN + 4, CH = chunk_of(E);
-    float *const sums = (float *)smem;
-    const int l16 = lane & 15, lq = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-            *(v4f *)(sums + (wave * BM + i * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i][j];
-    __syncthreads();
-#pragma unroll 1
-    for (int c = threadIdx.x; c < BM * BN / CH; c += KS * 64) {
-        const int row = c / (BN / CH), col = c % (BN / CH) * CH;
-        if (row >= t.rows || t.n0 + col >= N) continue;
-        v4f v[CH / 4] = {};
-#pragma unroll
-        for (int w = 0; w < KS; ++w)
-#pragma unroll
-            for (int i = 0; i < CH / 4; ++i)
-                v[i] += *(const v4f *)(sums + (w * BM + row) * LD + col + 4 * i);
-        store_chunk<E, NT>(ep, t.z, t.row0 + row, t.n0 + col, N, v);
-    }
-}
-
 template <bool MX, int BM, int BN, int KS, int NS>
 struct RaggedWaveLds {
     static constexpr int STAGE = (BM + BN) * 128 + (MX ? 2048 : 0);  // operands, scales
@@ -987,11 +1012,11 @@ struct RaggedWaveLds {
     static constexpr int BYTES = RING > SUMS ? RING : SUMS;
 };
 
-template <bool MX, bool AT, bool BT, EpiKind E, int BM, int BN, int KS, int NS, bool ONCE>
+template <bool MX, bool AT, bool BT, typename O, int BM, int BN, int KS, int NS, bool ONCE>
 __global__ __launch_bounds__(KS * 64)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS),
                                    ragged_waves(RaggedWaveLds<MX, BM, BN, KS, NS>::BYTES, KS))))
-void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
+void ragged_wave_kernel(const RaggedArgs g, const typename O::Params ep) {
     constexpr int TM = BM / 16, TN = BN / 16, QA = (TM + 3) / 4, QB = (TN + 3) / 4;
     using L = RaggedWaveLds<MX, BM, BN, KS, NS>;
     using PA = Panel<AT, BM, 1>;
@@ -1095,8 +1120,7 @@ void ragged_wave_kernel(const RaggedArgs g, const EpiParams ep) {
         products(kt, ring + slot * L::STAGE);
     }
     __syncthreads();
-    if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
-    else wave_sums<E, false, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // ---------------------------------------------------------------- operands of any alignment
@@ -1182,9 +1206,9 @@ struct RegPanel {
     }
 };
 
-template <bool AT, bool BT, EpiKind E, int BM, int BN, int WM, int WN>
+template <bool AT, bool BT, typename O, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64)
-void ragged_reg_kernel(const RaggedArgs g, const EpiParams ep) {
+void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
     constexpr int NW = WM * WN;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     using PA = RegPanel<AT, BM, NW>;
@@ -1257,15 +1281,14 @@ void ragged_reg_kernel(const RaggedArgs g, const EpiParams ep) {
         if (kt + 1 < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
-    else ragged_store<E, false, WTM, WTN>(ep, t, g.N, acc, smem, wave, wm, wn, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // The same with K split over the KS waves of a workgroup (see ragged_wave_kernel): a wave's
 // stages go through a slot of its own, so it waits for its own loads only.
-template <bool AT, bool BT, EpiKind E, int BM, int BN, int KS>
+template <bool AT, bool BT, typename O, int BM, int BN, int KS>
 __global__ __launch_bounds__(KS * 64)
-void ragged_reg_wave_kernel(const RaggedArgs g, const EpiParams ep) {
+void ragged_reg_wave_kernel(const RaggedArgs g, const typename O::Params ep) {
     constexpr int TM = BM / 16, TN = BN / 16;
     using PA = RegPanel<AT, BM, 1>;
     using PB = RegPanel<BT, BN, 1>;
@@ -1328,8 +1351,7 @@ void ragged_reg_wave_kernel(const RaggedArgs g, const EpiParams ep) {
         if (kt + KS < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
-    else wave_sums<E, false, BM, BN, KS>(ep, t, g.N, acc, smem, wave, lane);
+    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
@@ -1376,8 +1398,8 @@ struct RegWaveTile {
     static constexpr bool ONCE = false;
 };
 
-template <bool MX, bool AT, bool BT, EpiKind E, typename T>
-static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+template <bool MX, bool AT, bool BT, typename O, typename T>
+static hipError_t ragged_go(const RaggedArgs &g, const typename O::Params &ep, hipStream_t stream) {
     constexpr int BM = T::BM, BN = T::BN;
     // 32-bit offsets inside a panel, with the loads of rows past its edge
     const int64_t kbytes = MX ? (int64_t)(g.K + 31) / 32 * 16 : (int64_t)g.K * 2;
@@ -1393,18 +1415,18 @@ static hipError_t ragged_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
     if (tiles > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid = ragged_grid(tiles), block(T::WM * T::WN * 64);
     if constexpr (T::KIND == 1)
-        hipLaunchKernelGGL((ragged_big_kernel<MX, AT, BT, E>), grid, block, 0, stream, g, ep);
+        hipLaunchKernelGGL((ragged_big_kernel<MX, AT, BT, O>), grid, block, 0, stream, g, ep);
     else if constexpr (T::KIND == 2)
-        hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, E, BM, BN, T::WN, T::NS, T::ONCE>), grid, block, 0,
+        hipLaunchKernelGGL((ragged_wave_kernel<MX, AT, BT, O, BM, BN, T::WN, T::NS, T::ONCE>), grid, block, 0,
                            stream, g, ep);
     else if constexpr (T::KIND == 3)
-        hipLaunchKernelGGL((ragged_reg_kernel<AT, BT, E, BM, BN, T::WM, T::WN>), grid, block, 0,
+        hipLaunchKernelGGL((ragged_reg_kernel<AT, BT, O, BM, BN, T::WM, T::WN>), grid, block, 0,
                            stream, g, ep);
     else if constexpr (T::KIND == 4)
-        hipLaunchKernelGGL((ragged_reg_wave_kernel<AT, BT, E, BM, BN, T::WN>), grid, block, 0, stream,
+        hipLaunchKernelGGL((ragged_reg_wave_kernel<AT, BT, O, BM, BN, T::WN>), grid, block, 0, stream,
                            g, ep);
     else
-        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, E, BM, BN, T::WM, T::WN, T::NS, T::ONCE>), grid,
+        hipLaunchKernelGGL((ragged_kernel<MX, AT, BT, O, BM, BN, T::WM, T::WN, T::NS, T::ONCE>), grid,
                            block, 0, stream, g, ep);
     return hipGetLastError();
 }
@@ -1561,10 +1583,22 @@ static auto forward_tile(const RaggedArgs &g, F f) {
 #undef GK_GO
 }
 
+// f(the tile of a forward product of operands of any alignment) that grouped_plan_any chose.
+template <typename F>
+static auto any_align_tile(const RaggedArgs &g, F f) {
+    switch (g.tile) {
+    case 0: return f(RegTile<128, 128, 2, 4>{});
+    case 1: return f(RegTile<128, 64, 4, 2>{});
+    case 2: return f(RegTile<32, 64, 1, 4>{});
+    case 3: return f(RegWaveTile<16, 32, 4>{});
+    default: return f(RegWaveTile<16, 32, 8>{});
+    }
+}
+
 template <bool MX, bool BT, EpiKind E>
 static hipError_t ragged_forward(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
     return forward_tile<MX, BT>(
-        g, [&](auto t) { return ragged_go<MX, false, BT, E, decltype(t)>(g, ep, stream); });
+        g, [&](auto t) { return ragged_go<MX, false, BT, PlainOut<E>, decltype(t)>(g, ep, stream); });
 }
 
 template <typename T>

@@ -220,6 +220,10 @@ int gk_gemm_i8_unchecked_noalloc(size_t m, size_t k, size_t n, int32_t alpha,
 #define GK_ACT_RELU 1
 /* Fused-epilogue entries only (Activation::LeakyRelu, src/api/fused.rs:26-31). */
 #define GK_ACT_LEAKY_RELU 2
+/* Linear-layer and MXINT8 entries only. */
+#define GK_ACT_GELU 3
+#define GK_ACT_GELU_TANH 4
+#define GK_ACT_SILU 5
 
 /* Requantize (src/api/int8.rs:185-209) plus the two extension fields.
  * scales == NULL selects RequantScale::PerTensor(scale); otherwise `scales`
@@ -723,6 +727,111 @@ int gk_gemm_grouped_mxfp4_bf16(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
 int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
                               const int32_t *offsets, size_t groups, const gk_mxfp4 *b,
                               float beta, const gk_mat_mut *c, gk_par par);
+
+/* ------------------------- linear layers and 8-bit activation checkpoints */
+
+/* The entries below have no counterpart in the reference either: the products of a
+ * linear layer in training and serving, with what surrounds them in their
+ * epilogues, and the 8-bit matrices that keep a layer's activations for its
+ * backward pass.  For a layer H = act(X W + b), Y = H V + c + X:
+ *   forward   gk_gemm_linear_bf16(X, W, b, act) -> H, Z as MXINT8;
+ *             gk_gemm_linear_bf16(H, V, c, residual X) -> Y;
+ *             gk_quantize_mxint8_bf16(X).  H and Z itself need not be kept.
+ *   backward  gk_gemm_wgrad_mxint8(Z, act, dY) -> dV = act(Z)^T dY;
+ *             gk_activation_grad(dY, dbias) -> dc;
+ *             gk_gemm_linear_dgrad(dY, V^T, act, Z, dbias) -> dZ and db;
+ *             gk_gemm_wgrad_mxint8(X, dZ) -> dW;
+ *             gk_gemm_linear(dZ, W^T, residual dY) -> dX.
+ *
+ * Products take bf16 operands and f32 sums, alpha is f32, and alpha == 0 reads
+ * neither operand.  Views may have any non-negative strides; operands are read in place
+ * as in gk_gemm_grouped_bf16, outputs, residuals and pre-activations fastest with unit
+ * column stride.  Outputs may overlap nothing else that a call reads or writes, but for the
+ * two cases named below.  All can be captured into a HIP graph (the workspace
+ * holds packed copies, decoded checkpoints and partial sums) and give the same bits
+ * on every run.  Sizes as for the grouped products.
+ *
+ * Activations (act, slope) and their derivatives, in f32:
+ *   GK_ACT_NONE        z                              1
+ *   GK_ACT_RELU        z > 0 ? z : 0                  z > 0 ? 1 : 0
+ *   GK_ACT_LEAKY_RELU  max(z,0) + slope*min(z,0)      z > 0 ? 1 : slope
+ *   GK_ACT_GELU        z*P(z)                         P(z) + z*p(z)
+ *   GK_ACT_GELU_TANH   z*s, s = sigmoid(2u)           s + z*s*(1-s)*2u',
+ *                      u = sqrt(2/pi)*(z + 0.044715*z^3)
+ *   GK_ACT_SILU        z*s, s = sigmoid(z)            s + z*s*(1-s)
+ * with the normal distribution P and its density p.  The last three are off by at most
+ * 2^-20 * max(|z|, 1) (derivatives: 2^-20 * max(|z|, 1) too), and NaN at -infinity.
+ */
+
+/* A rows x cols matrix in MXINT8: row r's elements as int8 codes at codes + r * ld,
+ * whole blocks of 32; one e8m0 scale per block at scales + r * lds.  A code stands for
+ * code * 2^(byte - 133), 255 for NaN.  Strides are bytes, multiples of 16, and both
+ * arrays 16-byte aligned; a row's scales are padded to a multiple of 16 bytes.  Codes
+ * past cols and scales past the last block do not count. */
+typedef struct gk_mxint8 {
+    void *codes;
+    size_t codes_len;
+    void *scales;
+    size_t scales_len;
+    size_t rows;
+    size_t cols;
+    size_t ld;
+    size_t lds;
+} gk_mxint8;
+
+/* Quantizes the matrix x into q (same rows and cols).  A block with largest
+ * magnitude m has e = max(floor(log2 m), -120), the scale byte e + 127, and as codes
+ * the whole numbers nearest x / 2^(e - 6), ties to even, at most 127 either way; a
+ * block with a NaN or an infinity the byte 255 and zero codes. */
+int gk_quantize_mxint8_f32(const gk_mat_ref *x, const gk_mxint8 *q);
+int gk_quantize_mxint8_bf16(const gk_mat_ref *x, const gk_mxint8 *q);
+/* c <- act(values of q), rounded once; without activation exact in f32 and bf16 for every
+ * q that quantization writes. */
+int gk_dequantize_mxint8_f32(const gk_mxint8 *q, int32_t act, float slope, const gk_mat_mut *c);
+int gk_dequantize_mxint8_bf16(const gk_mxint8 *q, int32_t act, float slope, const gk_mat_mut *c);
+
+/* The weight gradient from a checkpoint: C <- alpha * H^T * B + beta * C, H = act(values of
+ * a) rounded to bf16 (without activation exact), a rows x k, B rows x n, C k x n. */
+int gk_gemm_wgrad_mxint8_bf16(gk_workspace *ws, float alpha, const gk_mxint8 *a, int32_t act,
+                              float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                              gk_par par);
+int gk_gemm_wgrad_mxint8_f32(gk_workspace *ws, float alpha, const gk_mxint8 *a, int32_t act,
+                             float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c,
+                             gk_par par);
+
+/* Z = alpha*A*B + bias, C <- act(Z) + residual: A m x k, B k x n, C m x n.  bias: per
+ * column (GK_BIAS_PER_COL), bf16 or (bias_f32) f32, or NULL; residual: m x n of C's type, or
+ * NULL, and it may be C itself, element for element.  Z is kept in z (bf16) or zq
+ * (MXINT8), at most one of them; the activation takes it unrounded. */
+int gk_gemm_linear_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a, const gk_mat_ref *b,
+                        const gk_bias *bias, int32_t bias_f32, int32_t act, float slope,
+                        const gk_mat_ref *residual, const gk_mat_mut *z, const gk_mxint8 *zq,
+                        const gk_mat_mut *c, gk_par par);
+int gk_gemm_linear_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a, const gk_mat_ref *b,
+                          const gk_bias *bias, int32_t bias_f32, int32_t act, float slope,
+                          const gk_mat_ref *residual, const gk_mat_mut *z, const gk_mxint8 *zq,
+                          const gk_mat_mut *c, gk_par par);
+
+/* D <- (alpha*A*B) * act'(Z), elementwise: the gradient at the pre-activations Z (m x n, z or
+ * zq as gk_gemm_linear kept them; neither without activation) of the layer before.
+ * dbias (n floats, or NULL) <- the column sums of D before it is rounded. */
+int gk_gemm_linear_dgrad_bf16(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                              const gk_mat_ref *b, int32_t act, float slope, const gk_mat_ref *z,
+                              const gk_mxint8 *zq, float *dbias, size_t dbias_len,
+                              const gk_mat_mut *d, gk_par par);
+int gk_gemm_linear_dgrad_f32out(gk_workspace *ws, float alpha, const gk_mat_ref *a,
+                                const gk_mat_ref *b, int32_t act, float slope, const gk_mat_ref *z,
+                                const gk_mxint8 *zq, float *dbias, size_t dbias_len,
+                                const gk_mat_mut *d, gk_par par);
+
+/* D <- G * act'(Z) (bf16), dbias <- its column sums likewise, for a gradient G that is there
+ * already (bf16, which may be D itself, or f32); without activation D is G, rounded. */
+int gk_activation_grad_bf16(gk_workspace *ws, const gk_mat_ref *g, int32_t act, float slope,
+                            const gk_mat_ref *z, const gk_mxint8 *zq, float *dbias,
+                            size_t dbias_len, const gk_mat_mut *d);
+int gk_activation_grad_f32(gk_workspace *ws, const gk_mat_ref *g, int32_t act, float slope,
+                           const gk_mat_ref *z, const gk_mxint8 *zq, float *dbias,
+                           size_t dbias_len, const gk_mat_mut *d);
 
 #ifdef __cplusplus
 } /* extern "C" */
