@@ -216,6 +216,24 @@ __device__ __forceinline__ bool row_lines(const void *p, int64_t row_bytes) {
     return (((uint64_t)p | (uint64_t)row_bytes) & 127) == 0;
 }
 
+// Rows of a tile as a buffer: accesses past its rows or columns read zeros and write nothing.
+struct Rows {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t at, step;  // this lane's offset in the next pass, and from pass to pass
+    // base: the tile's first element; width: bytes of the tile's columns; in, col: the lane's
+    // column in bytes if it is one of them
+    __device__ __forceinline__ Rows(const void *base, int64_t ld, int rows, int width, int row,
+                                    int col, bool in, int rpp) {
+        const uint8_t *const b = uniform((const uint8_t *)base);
+        const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)ld);
+        r = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)b, (short)0, (int)__builtin_amdgcn_readfirstlane((rows - 1) * l + width),
+            kRsrcWord3);
+        at = in ? row * l + col : kOutOfRange;
+        step = rpp * l;
+    }
+};
+
 // Rows of a product for which sums holds one row: a tile's, or (256 x 256) half a tile's,
 // since the last round's tiles may go out as halves.
 constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }
@@ -271,55 +289,71 @@ struct LinearOut {
                 b[e] = p.bias_f32 ? ((const float *)p.bias)[col + e]
                                   : bf16_widen(((const uint16_t *)p.bias)[col + e]);
     }
-    // f: sums of products in, the output before rounding out.  Every lane of a row's block
-    // comes along.
+    // f: sums of products in; the gradient before rounding out.
+    __device__ __forceinline__ static void grad_map(const Params &p, float alpha, int kind,
+                                                    const In &in, float (&f)[CH]) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) f[e] *= alpha;
+        if (kind == 0) return;
+        float z[CH];
+        if (kind == 2) {
+            const float step = mxint8_step(in.byte);
+#pragma unroll
+            for (int e = 0; e < CH; e += 4) mxint8_values4(in.v[e / 4], step, z + e);
+        } else {
+            widen<false, CH>(in.v, z);
+        }
+        act_scale(f, z, p.act, p.slope);
+    }
+    // f: pre-activations in, the output before rounding out.
+    __device__ __forceinline__ static void act_map(const Params &p, bool res, const In &in,
+                                                   float (&f)[CH]) {
+        act_apply(f, p.act, p.slope);
+        if (res) {
+            float r[CH];
+            widen<F32, CH>(in.v, r);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) f[e] += r[e];
+        }
+    }
+    // The chunk's codes (in w) and its block's scale byte; every lane of the block comes along.
+    // cols: how many of the chunk's columns are in the matrix; the others become 0.
+    __device__ __forceinline__ static int quantize(float (&f)[CH], int cols, v2u &w) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+            if (e >= cols) f[e] = 0.0f;
+            top = max_bits(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+        }
+        const int byte = mxint8_byte(block_max<LB>(top));
+        w[0] = mxint8_codes4(f, byte);
+        w[1] = CH == 8 ? mxint8_codes4(f + CH - 4, byte) : 0;
+        return byte;
+    }
+    // The whole way of a chunk, whatever the views' strides and however few of its columns there
+    // are.
     __device__ __forceinline__ static void store(const Params &p, const Flags &fl, int row, int col,
                                                  int N, const float (&bias)[CH], const In &in,
                                                  float (&f)[CH]) {
         const int cols = N - col;  // (0 or less: outside the matrix)
         if constexpr (GRAD) {
-#pragma unroll
-            for (int e = 0; e < CH; ++e) f[e] *= p.alpha;
-            if (p.act != kActNone) {
-                float z[CH];
-                if (p.codes) {
-                    const float step = mxint8_step(in.byte);
-#pragma unroll
-                    for (int e = 0; e < CH; e += 4) mxint8_values4(in.v[e / 4], step, z + e);
-                } else {
-                    widen<false, CH>(in.v, z);
-                }
-                act_scale(f, z, p.act, p.slope);
-            }
+            grad_map(p, p.alpha, p.codes ? 2 : p.z ? 1 : 0, in, f);
         } else {
 #pragma unroll
             for (int e = 0; e < CH; ++e) f[e] = __builtin_fmaf(p.alpha, f[e], bias[e]);
             if (p.codes) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < CH; ++e) {
-                    if (e >= cols) f[e] = 0.0f;
-                    top = max_bits(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-                }
-                const int byte = mxint8_byte(block_max<LB>(top));
+                v2u w;
+                const int byte = quantize(f, cols, w);
                 if ((col >> 5) < (N + 31) >> 5) {
                     uint8_t *q = p.codes + row * p.ld + col;
-                    if constexpr (CH == 8)
-                        *(v2u *)q = v2u{mxint8_codes4(f, byte), mxint8_codes4(f + 4, byte)};
-                    else
-                        *(uint32_t *)q = mxint8_codes4(f, byte);
+                    if constexpr (CH == 8) *(v2u *)q = w;
+                    else *(uint32_t *)q = w[0];
                     if ((col & 31) == 0) p.scales[row * p.lds + (col >> 5)] = (uint8_t)byte;
                 }
             } else if (p.z && cols > 0) {
                 write_row<false, CH>(p.z, row * p.rsz + col * p.csz, p.csz, cols, fl.nt_z, f);
             }
-            act_apply(f, p.act, p.slope);
-            if (p.res) {
-                float r[CH];
-                widen<F32, CH>(in.v, r);
-#pragma unroll
-                for (int e = 0; e < CH; ++e) f[e] += r[e];
-            }
+            act_map(p, p.res != nullptr, in, f);
         }
         if (cols > 0) write_row<F32, CH>(p.c, row * p.rsc + col * p.csc, p.csc, cols, fl.nt_c, f);
     }
@@ -419,6 +453,11 @@ struct LinearOut {
                     *(v4f *)(sums + (wm * WTM + i * 16 + l16) * LD + wn * WTN + j * 16 + 4 * lq) =
                         acc[i][j];
             slabs<BM, BN, WM * WN * 64, 1>(p, t, N, sums);
+        } else if (p.chunks && (N - t.n0 >= BN || N % CH == 0)) {
+            if (GRAD && p.codes) chunked<BM, BN, WM, WN, SMEM, GRAD ? 2 : 0>(p, t, N, acc, smem, wave, lane);
+            else if (GRAD ? p.z != nullptr : p.res != nullptr)
+                chunked<BM, BN, WM, WN, SMEM, 1>(p, t, N, acc, smem, wave, lane);
+            else chunked<BM, BN, WM, WN, SMEM, 0>(p, t, N, acc, smem, wave, lane);
         } else {
             // Bands of 16 rows staged per wave, GB of them at a time, and read back as rows.
             // (The row loop stays rolled: its code, five activations long, would not fit the
@@ -471,27 +510,181 @@ struct LinearOut {
                 __builtin_amdgcn_s_waitcnt(0xC07F);
                 __builtin_amdgcn_wave_barrier();
             }
-            if (GRAD && p.sums) {
-                // Lanes of the same columns, then the waves above each other, in order.
+            if (GRAD && p.sums) tile_sums<BM, BN, WM, WN>(p, t, N, sum, smem, wave, lane);
+        }
+    }
+
+    // Column sums of a tile from its lanes': lanes of the same columns, then the waves above each
+    // other, in order.
+    template <int BM, int BN, int WM, int WN>
+    __device__ __forceinline__ static void tile_sums(const Params &p, const RaggedTile &t, int N,
+                                                     float (&sum)[CH], uint8_t *smem, int wave,
+                                                     int lane) {
+        constexpr int WTN = BN / WN, CPR = WTN / CH;
+        const int wm = wave / WN, wn = wave % WN;
 #pragma unroll
-                for (int d = CPR; d < 64; d <<= 1)
+        for (int d = CPR; d < 64; d <<= 1)
 #pragma unroll
-                    for (int e = 0; e < CH; ++e) sum[e] += __shfl_xor(sum[e], d);
-                __syncthreads();
-                float *const red = (float *)smem;
-                if (lane < CPR) {
+            for (int e = 0; e < CH; ++e) sum[e] += __shfl_xor(sum[e], d);
+        __syncthreads();
+        float *const red = (float *)smem;
+        if (lane < CPR) {
 #pragma unroll
-                    for (int e = 0; e < CH; ++e) red[wm * BN + wn * WTN + c + e] = sum[e];
+            for (int e = 0; e < CH; ++e) red[wm * BN + wn * WTN + lane * CH + e] = sum[e];
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < BN; j += WM * WN * 64) {
+            float s = red[j];
+#pragma unroll
+            for (int w = 1; w < WM; ++w) s += red[w * BN + j];
+            put_sum<BM>(p, t, N, j, s);
+        }
+    }
+
+    // tile() where every view has unit column stride and whole chunks, 4-byte aligned: no branch
+    // around any access, so that the wait for a band's inputs, which go out a band before it, is a
+    // wait for them alone.  (Loads and stores share one counter: behind branches the compiler
+    // waits for all of the stores too, every pass.)  One band is staged while the one before
+    // it is worked on; the code of a band is there once, with a branch for its registers.
+    // IN: the inputs, none, a matrix (the residual or bf16 pre-activations) or (2) a checkpoint.
+    template <int BM, int BN, int WM, int WN, int SMEM, int IN, int TM, int TN>
+    __device__ __forceinline__ static void chunked(const Params &p, const RaggedTile &t, int N,
+                                                   const v4f (&acc)[TM][TN], uint8_t *smem,
+                                                   int wave, int lane) {
+        constexpr int WTM = BM / WM, WTN = BN / WN, NW = WM * WN, LD = WTN + 4, ESZ = F32 ? 4 : 2;
+        constexpr int CPR = WTN / CH, RPP = 64 / CPR, P = 16 / RPP;
+        static_assert(NW * 2 * 16 * LD * 4 <= SMEM && WM * BN * 4 <= SMEM, "LDS");
+        const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, lq = lane >> 4;
+        const int r0 = lane / CPR, c = lane % CPR * CH, cw = wn * WTN + c, col = t.n0 + cw;
+        const int cols = N - t.n0 < BN ? N - t.n0 : BN, row = wm * WTM + r0;
+        const bool in_c = cw < cols, in_b = cw < ((cols + 31) & ~31);
+        const Flags fl(p);
+        const int64_t row0 = t.row0;
+        const int64_t ldc = (p.rsc > N ? p.rsc : N) * ESZ;  // (one row: any stride)
+        Rows rc((uint8_t *)p.c + row0 * ldc + t.n0 * ESZ, ldc, t.rows, cols * ESZ, row, cw * ESZ, in_c, RPP);
+        // inputs: the residual, or the pre-activations
+        constexpr int ISZ = GRAD ? 2 : ESZ;
+        const void *const ip = GRAD ? (const void *)p.z : p.res;
+        const int64_t ldi = (!GRAD ? p.rsr : p.rsz > N ? p.rsz : N) * ISZ;
+        Rows ri((const uint8_t *)ip + row0 * ldi + t.n0 * ISZ, ldi, t.rows, cols * ISZ, row, cw * ISZ, in_c, RPP);
+        const int64_t ldz = (p.rsz > N ? p.rsz : N) * 2;
+        Rows rz((uint8_t *)p.z + row0 * ldz + t.n0 * 2, ldz, t.rows, cols * 2, row, cw * 2, in_c, RPP);
+        Rows rq(p.codes + row0 * p.ld + t.n0, p.ld, t.rows, (cols + 31) & ~31, row, cw, in_b, RPP);
+        Rows rs(p.scales + row0 * p.lds + (t.n0 >> 5), p.lds, t.rows, (cols + 31) >> 5, row, cw >> 5,
+                in_b && (GRAD || (cw & 31) == 0), RPP);
+        float bias[CH], sum[CH] = {};
+        bias_of(p, col, N, bias);
+
+        auto load_in = [&](In &in) {
+            if constexpr (IN == 2) {
+                if constexpr (CH == 8) {
+                    const v2u w = __builtin_amdgcn_raw_buffer_load_b64(rq.r, rq.at, 0, 0);
+                    in.v[0] = w[0];
+                    in.v[1] = w[1];
+                } else {
+                    in.v[0] = __builtin_amdgcn_raw_buffer_load_b32(rq.r, rq.at, 0, 0);
                 }
-                __syncthreads();
-                for (int j = threadIdx.x; j < BN; j += NW * 64) {
-                    float s = red[j];
+                in.byte = (int)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs.r, rs.at, 0, 0);
+                rq.at += rq.step;
+                rs.at += rs.step;
+            } else if constexpr (IN == 1) {
+                if constexpr (CH * ISZ == 16) {
+                    in.v = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ri.r, ri.at, 0, 0));
+                } else {
+                    const v2u w = __builtin_amdgcn_raw_buffer_load_b64(ri.r, ri.at, 0, 0);
+                    in.v[0] = w[0];
+                    in.v[1] = w[1];
+                }
+                ri.at += ri.step;
+            }
+        };
+        float *const stg = (float *)smem + wave * 2 * 16 * LD;
+        auto stage = [&](int h) {  // band h of 1 .. TM - 1
+            float *const d = stg + (h & 1) * 16 * LD + l16 * LD + 4 * lq;
 #pragma unroll
-                    for (int w = 1; w < WM; ++w) s += red[w * BN + j];
-                    put_sum<BM>(p, t, N, j, s);
+            for (int i = 1; i < TM; ++i) {
+                // (opaque, so that the branches stay apart: merged they would index the
+                // accumulators through scratch memory)
+                int k = h;
+                asm volatile("" : "+s"(k));
+                if (k == i) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) *(v4f *)(d + j * 16) = acc[i][j];
                 }
             }
+        };
+        In next[P];
+#pragma unroll
+        for (int s = 0; s < P; ++s) load_in(next[s]);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * LD + 4 * lq + j * 16) = acc[0][j];
+        int at_row = row;
+#pragma unroll 1
+        for (int h = 0; h < TM; ++h) {
+            In in[P];
+#pragma unroll
+            for (int s = 0; s < P; ++s) in[s] = next[s];
+            // (past the wave's last band: rows of the next wave or none, not used)
+#pragma unroll
+            for (int s = 0; s < P; ++s) load_in(next[s]);
+            __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses take effect in order)
+            stage(h + 1);
+            const float *const src = stg + (h & 1) * 16 * LD + r0 * LD + c;
+#pragma unroll
+            for (int s = 0; s < P; ++s) {
+                float f[CH];
+#pragma unroll
+                for (int i = 0; i < CH; i += 4) {
+                    const v4f v = *(const v4f *)(src + s * RPP * LD + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[i + e] = v[e];
+                }
+                if constexpr (GRAD) {
+                    // (rows that are not there: 0 times anything, alpha too)
+                    grad_map(p, at_row < t.rows ? p.alpha : 0.0f, IN, in[s], f);
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) sum[e] += f[e];
+                    at_row += RPP;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) f[e] = __builtin_fmaf(p.alpha, f[e], bias[e]);
+                    if (p.codes) {
+                        v2u w;
+                        const int byte = quantize(f, N - col, w);
+                        if constexpr (CH == 8) __builtin_amdgcn_raw_buffer_store_b64(w, rq.r, rq.at, 0, 0);
+                        else __builtin_amdgcn_raw_buffer_store_b32(w[0], rq.r, rq.at, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs.r, rs.at, 0, 0);
+                        rq.at += rq.step;
+                        rs.at += rs.step;
+                    } else if (p.z) {
+                        put<false>(rz, fl.nt_z, f);
+                    }
+                    act_map(p, IN == 1, in[s], f);
+                }
+                put<F32>(rc, fl.nt_c, f);
+            }
         }
+        if (GRAD && p.sums) tile_sums<BM, BN, WM, WN>(p, t, N, sum, smem, wave, lane);
+    }
+
+    // A chunk, rounded once, to its place in the next pass.
+    template <bool W>
+    __device__ __forceinline__ static void put(Rows &r, bool nt, const float (&f)[CH]) {
+        v4u w = {};
+        if constexpr (W) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) w[e % 4] = __float_as_uint(f[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < CH / 2; ++e) w[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
+        }
+        if constexpr (W || CH == 8) {
+            if (nt) __builtin_amdgcn_raw_buffer_store_b128(w, r.r, r.at, 0, 2);
+            else __builtin_amdgcn_raw_buffer_store_b128(w, r.r, r.at, 0, 0);
+        } else {
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{w[0], w[1]}, r.r, r.at, 0, 0);
+        }
+        r.at += r.step;
     }
 };
 
@@ -507,10 +700,23 @@ static hipError_t linear_go(const RaggedArgs &g, const LinearParams &p, hipStrea
     return forward_tile<false, BT>(g, go);
 }
 
+// Whether a view's chunks are whole and in reach of a tile's 32-bit offsets (LinearOut::chunked).
+inline bool chunk_rows(const void *p, int64_t rs, int64_t cs, int64_t M, int64_t size) {
+    return cs == 1 && (uintptr_t)p % 4 == 0 &&
+           (M <= 1 || (rs * size % 4 == 0 && rs * size <= kMaxTileRowBytes));
+}
+
 template <bool GRAD>
-static hipError_t linear_launch(const RaggedArgs &g, RaggedB bl, EpiKind kind,
-                                const LinearParams &p, hipStream_t stream) {
+static hipError_t linear_launch(const RaggedArgs &g, RaggedB bl, EpiKind kind, LinearParams p,
+                                hipStream_t stream) {
     const bool cols = bl == RaggedB::Cols;
+    const int64_t size = kind == EpiKind::F32 ? 4 : 2;
+    p.chunks = chunk_rows(p.c, p.rsc, p.csc, g.M, size) &&
+               (!p.res || chunk_rows(p.res, p.rsr, p.csr, g.M, size)) &&
+               (!p.z || (chunk_rows(p.z, p.rsz, p.csz, g.M, 2) && (g.M <= 1 || p.rsz >= g.N))) &&
+               (!p.codes || (p.ld <= kMaxTileRowBytes && p.lds <= kMaxTileRowBytes)) &&
+               (int64_t)g.N * size <= kMaxTileRowBytes;
+    if (g.M == 1) p.rsc = p.rsr = p.rsz = 0;  // (never used)
     if (kind == EpiKind::BF16)
         return cols ? linear_go<true, EpiKind::BF16, GRAD>(g, p, stream)
                     : linear_go<false, EpiKind::BF16, GRAD>(g, p, stream);
