@@ -141,8 +141,9 @@ __device__ __forceinline__ uint32_t block_max(uint32_t top) {
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-// CH consecutive bf16 or f32 values of a row at p (element stride cs; cols of them exist), as
-// they lie in memory.
+// CH consecutive bf16 or f32 values of a row at p (element stride cs; cols of them, at least one,
+// exist), as they lie in memory.  (Alone they are loaded without branches, values past the last
+// one from there: behind branches each load would wait for the one before it.)
 template <bool F32, int CH>
 __device__ __forceinline__ v4u read_raw(const void *p, int64_t at, int64_t cs, int cols) {
     v4u w = {};
@@ -151,9 +152,11 @@ __device__ __forceinline__ v4u read_raw(const void *p, int64_t at, int64_t cs, i
         typedef v4u v4u_any4 __attribute__((aligned(4)));
         const uint32_t *q = (const uint32_t *)p + at;
         if (cs == 1 && cols >= CH) return *(const v4u_any4 *)q;
+        uint32_t v[CH];
 #pragma unroll
-        for (int e = 0; e < CH; ++e)
-            if (e < cols) w[e] = q[e * cs];
+        for (int e = 0; e < CH; ++e) v[e] = q[(e < cols ? e : cols - 1) * cs];
+#pragma unroll
+        for (int e = 0; e < CH; ++e) w[e] = e < cols ? v[e] : 0;
     } else {
         const uint16_t *q = (const uint16_t *)p + at;
         if (cs == 1 && cols >= CH) {
@@ -167,9 +170,11 @@ __device__ __forceinline__ v4u read_raw(const void *p, int64_t at, int64_t cs, i
                 return w;
             }
         }
+        uint16_t v[CH];
 #pragma unroll
-        for (int e = 0; e < CH; ++e)
-            if (e < cols) w[e / 2] |= (uint32_t)q[e * cs] << (16 * (e % 2));
+        for (int e = 0; e < CH; ++e) v[e] = q[(e < cols ? e : cols - 1) * cs];
+#pragma unroll
+        for (int e = 0; e < CH; ++e) w[e / 2] |= e < cols ? (uint32_t)v[e] << (16 * (e % 2)) : 0;
     }
     return w;
 }
@@ -232,7 +237,52 @@ struct Rows {
         at = in ? row * l + col : kOutOfRange;
         step = rpp * l;
     }
+    // A chunk of CH elements of SZ bytes, of which cols are in the matrix: one by one, zeros for
+    // the others.
+    template <int CH, int SZ>
+    __device__ __forceinline__ void load(uint32_t (&v)[CH], int cols) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+            const uint32_t o = e < cols ? at + e * SZ : kOutOfRange;
+            if constexpr (SZ == 4) v[e] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+            else v[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+        }
+        at += step;
+    }
+    // PART: some chunks of the wave are not whole.
+    template <int CH, int SZ, bool PART>
+    __device__ __forceinline__ void store(const v4u &w, int cols, bool nt) {
+        const uint32_t o = PART && cols < CH ? kOutOfRange : at;
+        if constexpr (CH * SZ == 16) {
+            if (nt) __builtin_amdgcn_raw_buffer_store_b128(w, r, o, 0, 2);
+            else __builtin_amdgcn_raw_buffer_store_b128(w, r, o, 0, 0);
+        } else {
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{w[0], w[1]}, r, o, 0, 0);
+        }
+        if constexpr (PART) {
+#pragma unroll
+            for (int e = 0; e < CH - 1; ++e) {
+                const uint32_t p = cols < CH && e < cols ? at + e * SZ : kOutOfRange;
+                if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(w[e % 4], r, p, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(w[e / 2] >> (16 * (e % 2))), r, p, 0, 0);
+            }
+        }
+        at += step;
+    }
 };
+
+// Elements loaded one by one, as they lie in memory.
+template <int CH, int SZ>
+__device__ __forceinline__ v4u packed(const uint32_t (&v)[CH]) {
+    v4u w = {};
+#pragma unroll
+    for (int e = 0; e < CH; ++e) {
+        if constexpr (SZ == 4) w[e % 4] = v[e];
+        else w[e / 2] |= v[e] << (16 * (e % 2));
+    }
+    return w;
+}
+
 
 // Rows of a product for which sums holds one row: a tile's, or (256 x 256) half a tile's,
 // since the last round's tiles may go out as halves.
@@ -369,24 +419,60 @@ struct LinearOut {
         if (UNIT < BM && t.rows > UNIT) q[N] = 0.0f;
     }
 
+    // What a tile reads beside its products, the chunks of each thread of a tile that goes out by
+    // slabs() and of each lane of one that goes out by bands, in registers before the
+    // products are done where they are few.
+    template <int BM, int BN, int THREADS>
+    struct EarlySlab {
+        static constexpr int CPR = BN / CH, CHUNKS = BM * CPR, U = (CHUNKS + THREADS - 1) / THREADS;
+        In in[U];
+        float bias[U][CH];
+        __device__ __forceinline__ void load(const Params &p, const RaggedTile &t, int N, int, int) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = threadIdx.x + u * THREADS, row = c / CPR, col = t.n0 + c % CPR * CH;
+                const bool live = c < CHUNKS && row < t.rows;
+                in[u] = LinearOut::load(p, t.row0 + row, col, N, live);
+                bias_of(p, live ? col : N, N, bias[u]);
+            }
+        }
+    };
+    template <int BM, int BN, int WM, int WN>
+    struct EarlyBands {
+        static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, CPR = WTN / CH;
+        static constexpr int RPP = 64 / CPR, P = 16 / RPP;
+        static constexpr bool ALL = TM * P <= 4;
+        In in[ALL ? TM * P : 1];
+        float bias[ALL ? CH : 1];
+        __device__ __forceinline__ void load(const Params &p, const RaggedTile &t, int N, int wave,
+                                             int lane) {
+            if constexpr (ALL) {
+                const int col = t.n0 + wave % WN * WTN + lane % CPR * CH;
+#pragma unroll
+                for (int i = 0; i < TM * P; ++i) {
+                    const int row = wave / WN * WTM + i * RPP + lane / CPR;
+                    in[i] = LinearOut::load(p, t.row0 + row, col, N, row < t.rows);
+                }
+                bias_of(p, col, N, bias);
+            }
+        }
+    };
+    template <int BM, int BN, int WM, int WN>
+    using EarlyTile = std::conditional_t<(BN / WN < 32), EarlySlab<BM, BN, WM * WN * 64>,
+                                         EarlyBands<BM, BN, WM, WN>>;
+    template <int BM, int BN, int KS>
+    using EarlyWaves = EarlySlab<BM, BN, KS * 64>;
+
     // Tiles that lie in LDS whole, SLABS partial sums of each element one after the other, of
     // which every thread takes chunks.
     template <int BM, int BN, int THREADS, int SLABS>
     __device__ __forceinline__ static void slabs(const Params &p, const RaggedTile &t, int N,
-                                                 float *sums) {
+                                                 float *sums,
+                                                 const EarlySlab<BM, BN, THREADS> &early) {
         constexpr int LD = BN + 4, CPR = BN / CH, CHUNKS = BM * CPR;
-        constexpr int U = (CHUNKS + THREADS - 1) / THREADS;
+        constexpr int U = EarlySlab<BM, BN, THREADS>::U;
         static_assert(CHUNKS % 64 == 0 && BN % 32 == 0, "whole waves, whole blocks");
         const Flags fl(p);
-        In in[U];
-        float bias[U][CH];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {  // (on their way while the sums meet)
-            const int c = threadIdx.x + u * THREADS, row = c / CPR, col = t.n0 + c % CPR * CH;
-            const bool live = c < CHUNKS && row < t.rows;
-            in[u] = load(p, t.row0 + row, col, N, live);
-            bias_of(p, live ? col : N, N, bias[u]);
-        }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -401,7 +487,7 @@ struct LinearOut {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[i + e] = v[e];
             }
-            store(p, fl, t.row0 + row, t.n0 + at, N, bias[u], in[u], f);
+            store(p, fl, t.row0 + row, t.n0 + at, N, early.bias[u], early.in[u], f);
             if (GRAD && p.sums) {
 #pragma unroll
                 for (int i = 0; i < CH; i += 4)
@@ -421,7 +507,7 @@ struct LinearOut {
     template <int BM, int BN, int KS, int SMEM, int TM, int TN>
     __device__ __forceinline__ static void waves(const Params &p, const RaggedTile &t, int N,
                                                  const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
-                                                 int lane) {
+                                                 int lane, const EarlyWaves<BM, BN, KS> &early) {
         constexpr int LD = BN + 4;
         static_assert(KS * BM * LD * 4 <= SMEM, "LDS");
         float *const sums = (float *)smem;
@@ -431,13 +517,13 @@ struct LinearOut {
             for (int j = 0; j < TN; ++j)
                 *(v4f *)(sums + (wave * BM + i * 16 + (lane & 15)) * LD + j * 16 + 4 * (lane >> 4)) =
                     acc[i][j];
-        slabs<BM, BN, KS * 64, KS>(p, t, N, sums);
+        slabs<BM, BN, KS * 64, KS>(p, t, N, sums, early);
     }
 
     template <int BM, int BN, int WM, int WN, int SMEM, int TM, int TN>
     __device__ __forceinline__ static void tile(const Params &p, const RaggedTile &t, int N,
                                                 const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
-                                                int lane) {
+                                                int lane, const EarlyTile<BM, BN, WM, WN> &early) {
         constexpr int WTM = BM / WM, WTN = BN / WN;
         const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, lq = lane >> 4;
         if constexpr (WTN < 32) {
@@ -452,12 +538,19 @@ struct LinearOut {
                 for (int j = 0; j < TN; ++j)
                     *(v4f *)(sums + (wm * WTM + i * 16 + l16) * LD + wn * WTN + j * 16 + 4 * lq) =
                         acc[i][j];
-            slabs<BM, BN, WM * WN * 64, 1>(p, t, N, sums);
-        } else if (p.chunks && (N - t.n0 >= BN || N % CH == 0)) {
-            if (GRAD && p.codes) chunked<BM, BN, WM, WN, SMEM, GRAD ? 2 : 0>(p, t, N, acc, smem, wave, lane);
-            else if (GRAD ? p.z != nullptr : p.res != nullptr)
-                chunked<BM, BN, WM, WN, SMEM, 1>(p, t, N, acc, smem, wave, lane);
-            else chunked<BM, BN, WM, WN, SMEM, 0>(p, t, N, acc, smem, wave, lane);
+            slabs<BM, BN, WM * WN * 64, 1>(p, t, N, sums, early);
+        } else if constexpr (EarlyBands<BM, BN, WM, WN>::ALL) {
+            bands<BM, BN, WM, WN, SMEM>(p, t, N, acc, smem, wave, lane, early);
+        } else if (p.chunks) {
+            const bool part = N - t.n0 < BN && N % CH != 0;
+            const auto go = [&](auto in) {
+                constexpr int IN = decltype(in)::value;
+                if (part) chunked<BM, BN, WM, WN, SMEM, IN, true>(p, t, N, acc, smem, wave, lane);
+                else chunked<BM, BN, WM, WN, SMEM, IN, false>(p, t, N, acc, smem, wave, lane);
+            };
+            if (GRAD && p.codes) go(std::integral_constant<int, GRAD ? 2 : 0>{});
+            else if (GRAD ? p.z != nullptr : p.res != nullptr) go(std::integral_constant<int, 1>{});
+            else go(std::integral_constant<int, 0>{});
         } else {
             // Bands of 16 rows staged per wave, GB of them at a time, and read back as rows.
             // (The row loop stays rolled: its code, five activations long, would not fit the
@@ -514,6 +607,51 @@ struct LinearOut {
         }
     }
 
+    // tile() of few passes, whose inputs are all there: bands of 16 rows staged per wave and read
+    // back as rows.
+    template <int BM, int BN, int WM, int WN, int SMEM, int TM, int TN>
+    __device__ __forceinline__ static void bands(const Params &p, const RaggedTile &t, int N,
+                                                 const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
+                                                 int lane, const EarlyBands<BM, BN, WM, WN> &early) {
+        using EB = EarlyBands<BM, BN, WM, WN>;
+        constexpr int WTN = EB::WTN, LD = WTN + 4, RPP = EB::RPP, P = EB::P;
+        constexpr int GB = WM * WN * TM * 16 * LD * 4 <= SMEM ? TM : TM / 2;  // bands staged at once
+        static_assert(WM * WN * GB * 16 * LD * 4 <= SMEM && WM * BN * 4 <= SMEM, "LDS");
+        const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, lq = lane >> 4;
+        const int r0 = lane / EB::CPR, c = lane % EB::CPR * CH, col = t.n0 + wn * WTN + c;
+        float *const stg = (float *)smem + wave * GB * 16 * LD;
+        const Flags fl(p);
+        float sum[CH] = {};
+#pragma unroll
+        for (int i = 0; i < TM * P; ++i) {
+            if (i % (GB * P) == 0) {
+                __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses take effect in order)
+#pragma unroll
+                for (int b = 0; b < GB; ++b)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        *(v4f *)(stg + (b * 16 + l16) * LD + j * 16 + 4 * lq) = acc[i / P + b][j];
+                __builtin_amdgcn_wave_barrier();
+            }
+            float f[CH];
+#pragma unroll
+            for (int k = 0; k < CH; k += 4) {
+                const v4f v = *(const v4f *)(stg + (i % (GB * P) * RPP + r0) * LD + c + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[k + e] = v[e];
+            }
+            const int row = wm * TM * 16 + i * RPP + r0;
+            if (row < t.rows) {
+                store(p, fl, t.row0 + row, col, N, early.bias, early.in[i], f);
+                if constexpr (GRAD) {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) sum[e] += f[e];
+                }
+            }
+        }
+        if (GRAD && p.sums) tile_sums<BM, BN, WM, WN>(p, t, N, sum, smem, wave, lane);
+    }
+
     // Column sums of a tile from its lanes': lanes of the same columns, then the waves above each
     // other, in order.
     template <int BM, int BN, int WM, int WN>
@@ -541,13 +679,14 @@ struct LinearOut {
         }
     }
 
-    // tile() where every view has unit column stride and whole chunks, 4-byte aligned: no branch
+    // tile() where every view has unit column stride, at any alignment: no branch
     // around any access, so that the wait for a band's inputs, which go out a band before it, is a
     // wait for them alone.  (Loads and stores share one counter: behind branches the compiler
     // waits for all of the stores too, every pass.)  One band is staged while the one before
     // it is worked on; the code of a band is there once, with a branch for its registers.
     // IN: the inputs, none, a matrix (the residual or bf16 pre-activations) or (2) a checkpoint.
-    template <int BM, int BN, int WM, int WN, int SMEM, int IN, int TM, int TN>
+    // PART: the matrix ends inside a chunk of this tile, whose elements go one by one.
+    template <int BM, int BN, int WM, int WN, int SMEM, int IN, bool PART, int TM, int TN>
     __device__ __forceinline__ static void chunked(const Params &p, const RaggedTile &t, int N,
                                                    const v4f (&acc)[TM][TN], uint8_t *smem,
                                                    int wave, int lane) {
@@ -575,7 +714,10 @@ struct LinearOut {
         float bias[CH], sum[CH] = {};
         bias_of(p, col, N, bias);
 
-        auto load_in = [&](In &in) {
+        struct Raw : In {
+            uint32_t raw[IN == 1 && PART ? CH : 1];
+        };
+        auto load_in = [&](Raw &in) {
             if constexpr (IN == 2) {
                 if constexpr (CH == 8) {
                     const v2u w = __builtin_amdgcn_raw_buffer_load_b64(rq.r, rq.at, 0, 0);
@@ -587,6 +729,8 @@ struct LinearOut {
                 in.byte = (int)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs.r, rs.at, 0, 0);
                 rq.at += rq.step;
                 rs.at += rs.step;
+            } else if constexpr (IN == 1 && PART) {
+                ri.template load<CH, ISZ>(in.raw, N - col);
             } else if constexpr (IN == 1) {
                 if constexpr (CH * ISZ == 16) {
                     in.v = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ri.r, ri.at, 0, 0));
@@ -613,7 +757,7 @@ struct LinearOut {
                 }
             }
         };
-        In next[P];
+        Raw next[P];
 #pragma unroll
         for (int s = 0; s < P; ++s) load_in(next[s]);
 #pragma unroll
@@ -621,7 +765,7 @@ struct LinearOut {
         int at_row = row;
 #pragma unroll 1
         for (int h = 0; h < TM; ++h) {
-            In in[P];
+            Raw in[P];
 #pragma unroll
             for (int s = 0; s < P; ++s) in[s] = next[s];
             // (past the wave's last band: rows of the next wave or none, not used)
@@ -639,6 +783,7 @@ struct LinearOut {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) f[i + e] = v[e];
                 }
+                if constexpr (IN == 1 && PART) in[s].v = packed<CH, ISZ>(in[s].raw);
                 if constexpr (GRAD) {
                     // (rows that are not there: 0 times anything, alpha too)
                     grad_map(p, at_row < t.rows ? p.alpha : 0.0f, IN, in[s], f);
@@ -657,19 +802,19 @@ struct LinearOut {
                         rq.at += rq.step;
                         rs.at += rs.step;
                     } else if (p.z) {
-                        put<false>(rz, fl.nt_z, f);
+                        put<false, PART>(rz, fl.nt_z, N - col, f);
                     }
                     act_map(p, IN == 1, in[s], f);
                 }
-                put<F32>(rc, fl.nt_c, f);
+                put<F32, PART>(rc, fl.nt_c, N - col, f);
             }
         }
         if (GRAD && p.sums) tile_sums<BM, BN, WM, WN>(p, t, N, sum, smem, wave, lane);
     }
 
     // A chunk, rounded once, to its place in the next pass.
-    template <bool W>
-    __device__ __forceinline__ static void put(Rows &r, bool nt, const float (&f)[CH]) {
+    template <bool W, bool PART>
+    __device__ __forceinline__ static void put(Rows &r, bool nt, int cols, const float (&f)[CH]) {
         v4u w = {};
         if constexpr (W) {
 #pragma unroll
@@ -678,32 +823,37 @@ struct LinearOut {
 #pragma unroll
             for (int e = 0; e < CH / 2; ++e) w[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
         }
-        if constexpr (W || CH == 8) {
-            if (nt) __builtin_amdgcn_raw_buffer_store_b128(w, r.r, r.at, 0, 2);
-            else __builtin_amdgcn_raw_buffer_store_b128(w, r.r, r.at, 0, 0);
-        } else {
-            __builtin_amdgcn_raw_buffer_store_b64(v2u{w[0], w[1]}, r.r, r.at, 0, 0);
-        }
-        r.at += r.step;
+        r.template store<CH, W ? 4 : 2, PART>(w, cols, nt);
     }
 };
 
 // ---------------------------------------------------------------- launch
 
-// The tiles of grouped.hip's rule.
+// f(the tile of a linear layer's product): that of forward_tile, but for products of which 16 x 32
+// pieces are more than a CU each and 32 x 32 pieces are not: those take 32 x 32, K split over four
+// waves.  Graph-timed with rotating weights, us against the other rule's: 64x14336x4096 38.5 / 56.0,
+// 64x4096x4096 12.6 / 18.0, 128x2048x2048 6.2 / 8.0, 100x1000x1504 4.7 / 6.0, 333x512x512 3.8 / 4.4
+// (n-contiguous weights 58.8 / 66.8, 19.1 / 21.4, 7.1 / 8.0, 5.1 / 6.0, 4.0 / 4.5).
+template <bool BT, typename F>
+static auto linear_tile(const RaggedArgs &g, F f) {
+    if (g.any_align) return any_align_tile(g, f);
+    const int64_t cols = ((int64_t)g.N + 31) / 32;
+    if (((int64_t)g.M + 15) / 16 * cols > g.cus && ((int64_t)g.M + 31) / 32 * cols <= g.cus &&
+        g.K >= 256)
+        return f(WaveTile<32, 32, 4, 3>{});
+    return forward_tile<false, BT>(g, f);
+}
+
 template <bool BT, EpiKind E, bool GRAD>
 static hipError_t linear_go(const RaggedArgs &g, const LinearParams &p, hipStream_t stream) {
-    const auto go = [&](auto t) {
+    return linear_tile<BT>(g, [&](auto t) {
         return ragged_go<false, false, BT, LinearOut<E, GRAD>, decltype(t)>(g, p, stream);
-    };
-    if (g.any_align) return any_align_tile(g, go);
-    return forward_tile<false, BT>(g, go);
+    });
 }
 
 // Whether a view's chunks are whole and in reach of a tile's 32-bit offsets (LinearOut::chunked).
-inline bool chunk_rows(const void *p, int64_t rs, int64_t cs, int64_t M, int64_t size) {
-    return cs == 1 && (uintptr_t)p % 4 == 0 &&
-           (M <= 1 || (rs * size % 4 == 0 && rs * size <= kMaxTileRowBytes));
+inline bool chunk_rows(int64_t rs, int64_t cs, int64_t M, int64_t size) {
+    return cs == 1 && (M <= 1 || rs * size <= kMaxTileRowBytes);
 }
 
 template <bool GRAD>
@@ -711,9 +861,9 @@ static hipError_t linear_launch(const RaggedArgs &g, RaggedB bl, EpiKind kind, L
                                 hipStream_t stream) {
     const bool cols = bl == RaggedB::Cols;
     const int64_t size = kind == EpiKind::F32 ? 4 : 2;
-    p.chunks = chunk_rows(p.c, p.rsc, p.csc, g.M, size) &&
-               (!p.res || chunk_rows(p.res, p.rsr, p.csr, g.M, size)) &&
-               (!p.z || (chunk_rows(p.z, p.rsz, p.csz, g.M, 2) && (g.M <= 1 || p.rsz >= g.N))) &&
+    p.chunks = chunk_rows(p.rsc, p.csc, g.M, size) &&
+               (!p.res || chunk_rows(p.rsr, p.csr, g.M, size)) &&
+               (!p.z || (chunk_rows(p.rsz, p.csz, g.M, 2) && (g.M <= 1 || p.rsz >= g.N))) &&
                (!p.codes || (p.ld <= kMaxTileRowBytes && p.lds <= kMaxTileRowBytes)) &&
                (int64_t)g.N * size <= kMaxTileRowBytes;
     if (g.M == 1) p.rsc = p.rsr = p.rsz = 0;  // (never used)

@@ -11,43 +11,51 @@ hipError_t launch_linear_grad(const RaggedArgs &g, RaggedB bl, EpiKind kind, con
     return linear_launch<true>(g, bl, kind, p, stream);
 }
 
-int linear_unit(const RaggedArgs &g, RaggedB bl) { return sum_unit(grouped_plan(g, bl).bm); }
+int linear_unit(const RaggedArgs &g, RaggedB bl) {
+    const auto unit = [](auto t) { return sum_unit(decltype(t)::BM); };
+    return bl == RaggedB::Cols ? linear_tile<true>(g, unit) : linear_tile<false>(g, unit);
+}
 
 // ---------------------------------------------------------------- activation gradient
 
-// C = A * act'(Z), a workgroup per 256 >> ty chunk columns of 8 and `unit` rows, 1 << ty rows
-// at a time; column sums of its rows before rounding to one row of p.sums.
+// C = A * act'(Z), a workgroup per strip of 1 << tx chunk columns of 8 and `unit` rows, as many rows at
+// a time as it has threads for; column sums of its rows before rounding to one row of p.sums.
+constexpr int kStripSums = 4 * 512;  // floats: four waves of 64 chunk columns
 
-// The workgroup's column sums from its threads': column j of the strip, its rows' sums in order.
-__device__ __forceinline__ void strip_sums(const LinearParams &p, int N, int tx, int ty, float *red,
-                                           const float (&sum)[8]) {
+// The workgroup's column sums from its threads': a wave's rows, then the waves, in order.
+__device__ __forceinline__ void strip_sums(const LinearParams &p, int N, int tx, float *red,
+                                           float (&sum)[8]) {
+    for (int d = 1 << tx; d < 64; d <<= 1)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = sum[e];
+        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], d);
+    const int width = 8 << tx, base = (int)blockIdx.x * width, lane = threadIdx.x & 63;
+    if (lane < 1 << tx) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) red[(threadIdx.x >> 6) * width + lane * 8 + e] = sum[e];
+    }
     __syncthreads();
-    const int width = 8 << tx, base = (int)blockIdx.x * width;
     for (int j = threadIdx.x; j < width; j += 256) {
-        float s = 0.0f;
-        for (int y = 0; y < 1 << ty; ++y) s += red[(y << tx) * 8 + j];
+        float s = red[j];
+        for (int w = 1; w < 4; ++w) s += red[w * width + j];
         if (base + j < N) p.sums[(int64_t)blockIdx.y * N + base + j] = s;
     }
 }
 
-// Every view of unit column stride and whole chunks (LinearOut::chunked): no branch around any
-// access, and the next U rows' inputs go out before this one's stores.
-// IN: pre-activations, none, bf16, or (2) a checkpoint.
-template <InType T, int IN>
-__global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p, int64_t M, int N,
-                                                            int unit, int ty) {
+// Views of unit column stride (LinearOut::chunked): no branch around any access, and the next U
+// rows' inputs go out before this one's stores.
+// IN: pre-activations, none, bf16, or (2) a checkpoint.  PART: the matrix ends inside a chunk.
+template <InType T, int IN, bool PART>
+__device__ __forceinline__ void act_grad_rows(const LinearParams &p, int64_t M, int N, int unit,
+                                              int tx, float *red) {
     constexpr bool F32 = T == InType::F32;
     constexpr int U = 2, SZ = F32 ? 4 : 2;
-    __shared__ float red[256 * 8];
-    const int tx = 8 - ty, cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx;
+    const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx;
     const int width = 8 << tx, n0 = (int)blockIdx.x * width, c = cx * 8;
     const int cols = N - n0 < width ? N - n0 : width;
     const int64_t row0 = (int64_t)blockIdx.y * unit;
     const int rows = M - row0 < unit ? (int)(M - row0) : unit;
     const bool in = c < cols, nt = row_lines(p.c, p.rsc * 2);
-    const int rpp = 1 << ty;
+    const int rpp = 256 >> tx;
     const int64_t ldc = (p.rsc > N ? p.rsc : N) * 2, ldz = (p.rsz > N ? p.rsz : N) * 2;
     const int64_t lda = (p.rsr > N ? p.rsr : N) * SZ;
     Rows rc((uint8_t *)p.c + row0 * ldc + n0 * 2, ldc, rows, cols * 2, ry, c * 2, in, rpp);
@@ -58,12 +66,24 @@ __global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p
     struct In {
         v4u a[F32 ? 2 : 1], z;
         int byte;
+        uint32_t ra[PART ? 8 : 1], rz[PART && IN == 1 ? 8 : 1];
     };
+    const int left = N - n0 - c;
     auto load = [&](In &i) {
-        i.a[0] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at, 0, 0));
-        if constexpr (F32)
-            i.a[1] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at + 16, 0, 0));
-        ra.at += ra.step;
+        if constexpr (PART) {
+            ra.template load<8, SZ>(i.ra, left);
+            if constexpr (IN == 1) rz.template load<8, 2>(i.rz, left);
+        }
+        if constexpr (!PART) {
+            i.a[0] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at, 0, 0));
+            if constexpr (F32)
+                i.a[1] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at + 16, 0, 0));
+            ra.at += ra.step;
+            if constexpr (IN == 1) {
+                i.z = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rz.r, rz.at, 0, 0));
+                rz.at += rz.step;
+            }
+        }
         if constexpr (IN == 2) {
             const v2u w = __builtin_amdgcn_raw_buffer_load_b64(rq.r, rq.at, 0, 0);
             i.z[0] = w[0];
@@ -71,9 +91,6 @@ __global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p
             i.byte = (int)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs.r, rs.at, 0, 0);
             rq.at += rq.step;
             rs.at += rs.step;
-        } else if constexpr (IN == 1) {
-            i.z = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rz.r, rz.at, 0, 0));
-            rz.at += rz.step;
         }
     };
     float sum[8] = {};
@@ -81,7 +98,7 @@ __global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p
 #pragma unroll
     for (int u = 0; u < U; ++u) load(next[u]);
 #pragma unroll 1
-    for (int r = 0; r < rows; r += U << ty) {
+    for (int r = 0; r < rows; r += U * rpp) {
         In i[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) i[u] = next[u];
@@ -90,7 +107,11 @@ __global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[8];
-            if constexpr (F32) {
+            if constexpr (PART) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(F32 ? i[u].ra[e] : i[u].ra[e] << 16);
+                if constexpr (IN == 1) i[u].z = packed<8, 2>(i[u].rz);
+            } else if constexpr (F32) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(i[u].a[F32 ? e / 4 : 0][e % 4]);
             } else {
@@ -110,42 +131,40 @@ __global__ __launch_bounds__(256) void act_grad_rows_kernel(const LinearParams p
             v4u w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = bf16x2_rne(f[2 * e], f[2 * e + 1]);
-            if (nt) __builtin_amdgcn_raw_buffer_store_b128(w, rc.r, rc.at, 0, 2);
-            else __builtin_amdgcn_raw_buffer_store_b128(w, rc.r, rc.at, 0, 0);
-            rc.at += rc.step;
+            rc.template store<8, 2, PART>(w, left, nt);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += f[e];
         }
     }
-    if (p.sums) strip_sums(p, N, tx, ty, red, sum);
+    if (p.sums) strip_sums(p, N, tx, red, sum);
 }
 
-// Views of any strides.
+// A strip of any strides and width.
 template <InType T>
-__global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int64_t M, int N,
-                                                       int unit, int ty) {
+__device__ __forceinline__ void act_grad_any(const LinearParams &p, int64_t M, int N, int unit, int tx,
+                                             float *red) {
     constexpr bool F32 = T == InType::F32;
-    constexpr int U = 4;  // rows whose loads are in flight together
-    __shared__ float red[256 * 8];
-    const int tx = 8 - ty, cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx;
+    constexpr int U = 2;  // rows whose loads are in flight together
+    const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx, rpp = 256 >> tx;
     const int col = ((int)blockIdx.x << tx | cx) * 8, cols = N - col;
     const int64_t first = (int64_t)blockIdx.y * unit;
     const int64_t end = first + unit < M ? first + unit : M;
     const bool nt = row_lines(p.c, p.rsc * 2);
     float sum[8] = {};
     if (cols > 0) {
-        for (int64_t r = first + ry; r < end; r += (int64_t)U << ty) {
+        for (int64_t r = first + ry; r < end; r += (int64_t)U * rpp) {
             v4u a[U][2], z[U];
             int byte[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t row = r + ((int64_t)u << ty);
+                const int64_t row = r + (int64_t)u * rpp;
                 a[u][0] = a[u][1] = z[u] = v4u{};
                 byte[u] = 0;
                 if (row >= end) continue;
                 if constexpr (F32) {
                     a[u][0] = read_raw<true, 4>(p.res, row * p.rsr + col * p.csr, p.csr, cols);
-                    a[u][1] = read_raw<true, 4>(p.res, row * p.rsr + (col + 4) * p.csr, p.csr, cols - 4);
+                    if (cols > 4)
+                        a[u][1] = read_raw<true, 4>(p.res, row * p.rsr + (col + 4) * p.csr, p.csr, cols - 4);
                 } else {
                     a[u][0] = read_raw<false, 8>(p.res, row * p.rsr + col * p.csr, p.csr, cols);
                 }
@@ -160,7 +179,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t row = r + ((int64_t)u << ty);
+                const int64_t row = r + (int64_t)u * rpp;
                 if (row >= end) break;
                 float f[8];
                 if constexpr (F32) {
@@ -192,85 +211,103 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int
             }
         }
     }
-    if (p.sums) strip_sums(p, N, tx, ty, red, sum);
+    if (p.sums) strip_sums(p, N, tx, red, sum);
 }
 
-// Rows that share a thread's columns: 64 chunk columns (a KiB of bf16 in a row) where the matrix
-// has them.
-static int act_grad_ty(int64_t n) {
+// IN 0..2: act_grad_rows; 3: views of any strides.
+template <InType T, int IN>
+__global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int64_t M, int N,
+                                                       int unit, int tx) {
+    __shared__ float red[kStripSums];
+    if constexpr (IN == 3) {
+        act_grad_any<T>(p, M, N, unit, tx, red);
+    } else {
+        const bool part = N % 8 != 0 && N - ((int)blockIdx.x << (3 + tx)) < 8 << tx;
+        if (part) act_grad_rows<T, IN, true>(p, M, N, unit, tx, red);
+        else act_grad_rows<T, IN, false>(p, M, N, unit, tx, red);
+    }
+}
+
+// A workgroup's part.  Strips of 64 chunk columns (a KiB of bf16 in a row) where the matrix has
+// them, rows for about eight workgroups per CU, at least two per thread.  Column sums of few rows:
+// strips of two chunk columns and all rows, which need no second launch (64 x 8192 5.8 us); such
+// strips read 32 bytes of a row at a time and are bound by their addresses, so that of more rows
+// two launches cost less (1003 x 777 12.7 us in one, 5.9 + 4.4 in two).
+struct ActGradShape {
+    int tx, unit;
+};
+static ActGradShape act_grad_shape(int64_t m, int64_t n, int cus, bool sums) {
     int tx = 6;
     while (tx > 0 && ((int64_t)8 << (tx - 1)) >= n) --tx;
-    return 8 - tx;
+    const int rpp = 256 >> tx;
+    const int64_t strips = (n + (8 << tx) - 1) / (8 << tx);
+    const int64_t parts = std::max<int64_t>(8 * (int64_t)cus / strips, 1), rows = (m + parts - 1) / parts;
+    int64_t unit = (rows + rpp - 1) / rpp * rpp;
+    unit = std::max<int64_t>(unit, 2 * rpp);
+    unit = std::max<int64_t>(unit, (m + 65534) / 65535);
+    if (sums && m > unit && m <= 512) return {1, (int)m};
+    return {tx, (int)unit};
 }
 
-int act_grad_unit(int64_t m, int64_t n, int cus) {
-    const int ty = act_grad_ty(n);
-    const int64_t strips = (n + (2048 >> ty) - 1) / (2048 >> ty);
-    // about eight workgroups per CU, of at least one row per thread
-    const int64_t parts = std::max<int64_t>(8 * (int64_t)cus / strips, 1), rows = (m + parts - 1) / parts;
-    int64_t unit = (rows + (1 << ty) - 1) >> ty << ty;
-    unit = std::max<int64_t>(unit, 1 << ty);
-    return (int)std::max<int64_t>(unit, (m + 65534) / 65535);
-}
+int act_grad_unit(int64_t m, int64_t n, int cus) { return act_grad_shape(m, n, cus, true).unit; }
 
 template <InType T>
-static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, int unit, int ty, dim3 grid,
+static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, const ActGradShape &shape,
                         hipStream_t stream) {
     // (32-bit offsets: the rows of a workgroup)
-    const int64_t most = (int64_t)kMaxRecords / (unit + (4 << ty));
-    const auto rows = [&](const void *q, int64_t rs, int64_t cs, int64_t size) {
-        return cs == 1 && (uintptr_t)q % 4 == 0 &&
-               (m <= 1 || (rs * size % 4 == 0 && rs >= n && rs * size <= most));
+    const int tx = shape.tx, unit = shape.unit;
+    const dim3 grid((uint32_t)((n + (8 << tx) - 1) / (8 << tx)), (uint32_t)((m + unit - 1) / unit));
+    const int64_t most = (int64_t)kMaxRecords / (unit + 4 * (256 >> tx));
+    const auto rows = [&](int64_t rs, int64_t cs, int64_t size) {
+        return cs == 1 && (m <= 1 || (rs >= n && rs * size <= most));
     };
-    const int64_t size = (int64_t)in_size(T);
-    const bool chunks = n % 8 == 0 && n * 4 <= most && rows(p.c, p.rsc, p.csc, 2) &&
-                        rows(p.res, p.rsr, p.csr, size) && (!p.z || rows(p.z, p.rsz, p.csz, 2)) &&
+    const bool chunks = n * 4 <= most && rows(p.rsc, p.csc, 2) &&
+                        rows(p.rsr, p.csr, (int64_t)in_size(T)) && (!p.z || rows(p.rsz, p.csz, 2)) &&
                         (!p.codes || (p.ld <= most && p.lds <= most));
     LinearParams q = p;
     if (m == 1) q.rsc = q.rsr = q.rsz = 0;  // (never used)
     if (!chunks)
-        hipLaunchKernelGGL((act_grad_kernel<T>), grid, dim3(256), 0, stream, q, m, (int)n, unit, ty);
+        hipLaunchKernelGGL((act_grad_kernel<T, 3>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
     else if (p.codes)
-        hipLaunchKernelGGL((act_grad_rows_kernel<T, 2>), grid, dim3(256), 0, stream, q, m, (int)n, unit, ty);
+        hipLaunchKernelGGL((act_grad_kernel<T, 2>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
     else if (p.z)
-        hipLaunchKernelGGL((act_grad_rows_kernel<T, 1>), grid, dim3(256), 0, stream, q, m, (int)n, unit, ty);
+        hipLaunchKernelGGL((act_grad_kernel<T, 1>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
     else
-        hipLaunchKernelGGL((act_grad_rows_kernel<T, 0>), grid, dim3(256), 0, stream, q, m, (int)n, unit, ty);
+        hipLaunchKernelGGL((act_grad_kernel<T, 0>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
 }
 
 hipError_t launch_act_grad(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,
                            hipStream_t stream) {
-    const int ty = act_grad_ty(n), unit = act_grad_unit(m, n, cus);
-    const dim3 grid((uint32_t)((n + (2048 >> ty) - 1) / (2048 >> ty)), (uint32_t)((m + unit - 1) / unit));
-    if (in == InType::BF16) act_grad_go<InType::BF16>(p, m, n, unit, ty, grid, stream);
-    else act_grad_go<InType::F32>(p, m, n, unit, ty, grid, stream);
+    const ActGradShape shape = act_grad_shape(m, n, cus, p.sums != nullptr);
+    if (in == InType::BF16) act_grad_go<InType::BF16>(p, m, n, shape, stream);
+    else act_grad_go<InType::F32>(p, m, n, shape, stream);
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- column sums
 
-// 32 columns a workgroup; eight lanes of rows each add every eighth row, then the eight.
+// 16 columns a workgroup; sixteen lanes of rows each add every sixteenth row, then the sixteen.
 __global__ __launch_bounds__(256) void col_sums_kernel(const float *part, int64_t rows, int64_t n,
                                                        float *out) {
     __shared__ float red[256];
-    const int c = threadIdx.x & 31, l = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c;
     float s = 0.0f;
     if (col < n) {
 #pragma unroll 8
-        for (int64_t r = l; r < rows; r += 8) s += part[r * n + col];
+        for (int64_t r = l; r < rows; r += 16) s += part[r * n + col];
     }
     red[threadIdx.x] = s;
     __syncthreads();
     if (l == 0 && col < n) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += red[i * 32 + c];
+        for (int i = 1; i < 16; ++i) s += red[i * 16 + c];
         out[col] = s;
     }
 }
 
 hipError_t launch_col_sums(const float *part, int64_t rows, int64_t n, float *out, hipStream_t stream) {
-    hipLaunchKernelGGL(col_sums_kernel, dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, stream, part,
+    hipLaunchKernelGGL(col_sums_kernel, dim3((uint32_t)((n + 15) / 16)), dim3(256), 0, stream, part,
                        rows, n, out);
     return hipGetLastError();
 }

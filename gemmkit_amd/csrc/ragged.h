@@ -620,14 +620,22 @@ __device__ __forceinline__ void wave_sums(const EpiParams &ep, const RaggedTile 
 
 // How a tile leaves the kernels: tile() of waves that each hold WTM x WTN of it, waves() of
 // waves that each hold sums of all of it, with SMEM bytes of LDS that nothing else uses any
-// more.  PlainOut: EpiParams' map.
+// more.  EarlyTile and EarlyWaves hold what these read from memory beside the products,
+// loaded behind the first stages' loads.  PlainOut: EpiParams' map.
 template <EpiKind E>
 struct PlainOut {
     using Params = EpiParams;
+    struct Nothing {
+        __device__ __forceinline__ void load(const Params &, const RaggedTile &, int, int, int) {}
+    };
+    template <int BM, int BN, int WM, int WN>
+    using EarlyTile = Nothing;
+    template <int BM, int BN, int KS>
+    using EarlyWaves = Nothing;
     template <int BM, int BN, int WM, int WN, int SMEM, int TM, int TN>
     __device__ __forceinline__ static void tile(const Params &ep, const RaggedTile &t, int N,
                                                 const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
-                                                int lane) {
+                                                int lane, const Nothing &) {
         constexpr int WTM = BM / WM, WTN = BN / WN;
         const int wm = wave / WN, wn = wave % WN;
         if (whole_lines<E>(ep)) ragged_store<E, true, WTM, WTN>(ep, t, N, acc, smem, wave, wm, wn, lane);
@@ -636,7 +644,7 @@ struct PlainOut {
     template <int BM, int BN, int KS, int SMEM, int TM, int TN>
     __device__ __forceinline__ static void waves(const Params &ep, const RaggedTile &t, int N,
                                                  const v4f (&acc)[TM][TN], uint8_t *smem, int wave,
-                                                 int lane) {
+                                                 int lane, const Nothing &) {
         if (whole_lines<E>(ep)) wave_sums<E, true, BM, BN, KS>(ep, t, N, acc, smem, wave, lane);
         else wave_sums<E, false, BM, BN, KS>(ep, t, N, acc, smem, wave, lane);
     }
@@ -756,6 +764,8 @@ void ragged_kernel(const RaggedArgs g, const typename O::Params ep) {
         }
         load_stage(smem + s * L::STAGE);
     }
+    typename O::template EarlyTile<BM, BN, WM, WN> early;
+    early.load(ep, t, g.N, wave, lane);
     int slot = 0;
     auto step = [&](int kt, auto par) {
         const int w = slot == 0 ? NS - 1 : slot - 1;
@@ -780,7 +790,7 @@ void ragged_kernel(const RaggedArgs g, const typename O::Params ep) {
         half(sa, sa + PA::BYTES, H1{});
         __syncthreads();
     }
-    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane, early);
 }
 
 // ---------------------------------------------------------------- 256 x 256 tile
@@ -896,6 +906,8 @@ void ragged_big_kernel(const RaggedArgs g, const typename O::Params ep) {
         for (int i = 0; i < LPB; ++i) B.load(b_slot(s), nullptr, i);
         B.next();
     }
+    typename O::template EarlyTile<BM, BN, WM, WN> early;
+    early.load(ep, t, g.N, wave, lane);
     wait_vmcnt<LPA + LPB>();
     stage_barrier();
     ops(a_slot(0), b_slot(0), I0{}, 0, FA{}, std::true_type{}, I0{}, [](int) {});
@@ -994,7 +1006,7 @@ void ragged_big_kernel(const RaggedArgs g, const typename O::Params ep) {
         }
         __syncthreads();
     }
-    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane, early);
 }
 
 // ---------------------------------------------------------------- few tiles
@@ -1105,6 +1117,8 @@ void ragged_wave_kernel(const RaggedArgs g, const typename O::Params ep) {
     };
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) load_stage(wave + i * KS, ring + i * L::STAGE);
+    typename O::template EarlyWaves<BM, BN, KS> early;
+    early.load(ep, t, g.N, wave, lane);
     int slot = 0, kt = wave;
     const int whole = MX && g.K % 32 ? t.KT - 1 : t.KT;  // stages without a cut block
     for (; kt < whole; kt += KS) {
@@ -1120,7 +1134,7 @@ void ragged_wave_kernel(const RaggedArgs g, const typename O::Params ep) {
         products(kt, ring + slot * L::STAGE);
     }
     __syncthreads();
-    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
+    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane, early);
 }
 
 // ---------------------------------------------------------------- operands of any alignment
@@ -1273,6 +1287,8 @@ void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
     };
     get(0);
     get(1);
+    typename O::template EarlyTile<BM, BN, WM, WN> early;
+    early.load(ep, t, g.N, wave, lane);
     put(0, smem);
     __builtin_amdgcn_s_waitcnt(0xC07F);
     stage_barrier();
@@ -1281,7 +1297,7 @@ void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
         if (kt + 1 < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
+    O::template tile<BM, BN, WM, WN, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane, early);
 }
 
 // The same with K split over the KS waves of a workgroup (see ragged_wave_kernel): a wave's
@@ -1346,12 +1362,14 @@ void ragged_reg_wave_kernel(const RaggedArgs g, const typename O::Params ep) {
     };
     get(0);
     get(1);
+    typename O::template EarlyWaves<BM, BN, KS> early;
+    early.load(ep, t, g.N, wave, lane);
     for (int kt = wave; kt < t.KT; kt += 2 * KS) {
         kstep(std::integral_constant<int, 0>{});
         if (kt + KS < t.KT) kstep(std::integral_constant<int, 1>{});
     }
     __syncthreads();
-    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane);
+    O::template waves<BM, BN, KS, sizeof(smem)>(ep, t, g.N, acc, smem, wave, lane, early);
 }
 
 // Workgroups go out in rows of at most 2^20 (a grid's x extent counts threads in 32 bits).
