@@ -288,6 +288,10 @@ __device__ __forceinline__ v4u packed(const uint32_t (&v)[CH]) {
 // since the last round's tiles may go out as halves.
 constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }
 
+// Bands whose inputs are in flight while one is worked on (LinearOut::chunked): 8192 x 4096 x 8192's
+// input gradient through a checkpoint 435 us with two, 445 with one; four spill.
+constexpr int kAhead = 2;
+
 template <EpiKind E, bool GRAD>
 struct LinearOut {
     using Params = LinearParams;
@@ -757,20 +761,26 @@ struct LinearOut {
                 }
             }
         };
-        Raw next[P];
+        constexpr int D = TM % kAhead == 0 ? kAhead : TM;
+        Raw next[D][P];
 #pragma unroll
-        for (int s = 0; s < P; ++s) load_in(next[s]);
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int s = 0; s < P; ++s) load_in(next[d][s]);
 #pragma unroll
         for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * LD + 4 * lq + j * 16) = acc[0][j];
         int at_row = row;
 #pragma unroll 1
-        for (int h = 0; h < TM; ++h) {
+        for (int h0 = 0; h0 < TM; h0 += D)
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int h = h0 + d;
             Raw in[P];
 #pragma unroll
-            for (int s = 0; s < P; ++s) in[s] = next[s];
+            for (int s = 0; s < P; ++s) in[s] = next[d][s];
             // (past the wave's last band: rows of the next wave or none, not used)
 #pragma unroll
-            for (int s = 0; s < P; ++s) load_in(next[s]);
+            for (int s = 0; s < P; ++s) load_in(next[d][s]);
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses take effect in order)
             stage(h + 1);
             const float *const src = stg + (h & 1) * 16 * LD + r0 * LD + c;
