@@ -936,6 +936,7 @@ void ragged_big_kernel(const RaggedArgs g, const typename O::Params ep) {
         mfma_rows(I1{}, 0);
 #pragma unroll
         for (int m = 0; m < NM; ++m) __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_barrier(0);  // (else these products move behind the barrier)
         wait_vmcnt<L0>();
         stage_barrier();
     };
