@@ -46,10 +46,7 @@ __global__ __launch_bounds__(256) void mxint8_quantize_kernel(const MxArgs g, ui
         const ChunkAt<CH> at(row0, c0, threadIdx.x + u * 256, cpr);
         float f[CH];
         widen<F32, CH>(raw[u], f);
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) top = max_bits(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-        const int byte = mxint8_byte(block_max<LB>(top));
+        const int byte = mxint8_byte(block_max<LB>(top_bits(f)));
         if (at.row >= g.rows) continue;
         uint8_t *q = g.codes + at.row * g.ld + at.col;
         if constexpr (CH == 8)

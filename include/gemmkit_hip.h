@@ -759,8 +759,8 @@ int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
  *   GK_ACT_GELU_TANH   z*s, s = sigmoid(2u)           s + z*s*(1-s)*2u',
  *                      u = sqrt(2/pi)*(z + 0.044715*z^3)
  *   GK_ACT_SILU        z*s, s = sigmoid(z)            s + z*s*(1-s)
- * with the normal distribution P and its density p.  The last three are off by at most
- * 2^-20 * max(|z|, 1) (derivatives: 2^-20 * max(|z|, 1) too), and NaN at -infinity.
+ * with the normal distribution P and its density p.  The last three and their derivatives
+ * are off by at most 2^-20 * max(|z|, 1); GELU_TANH and SILU are NaN at -infinity.
  */
 
 /* A rows x cols matrix in MXINT8: row r's elements as int8 codes at codes + r * ld,
