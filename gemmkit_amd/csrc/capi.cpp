@@ -2384,6 +2384,23 @@ int wgrad_run(gk_workspace *ws, EpiKind kind, float alpha, Opnd a, int64_t na, O
     g.N = (int32_t)N;
     g.K = (int32_t)K;
     g.splits = 1;
+    // A checkpoint of few rows is decoded on its way into the tiles: one launch, no workspace.
+    if (q) {
+        g.act = q->act;
+        g.slope = q->slope;
+    }
+    if (q && !swap && M > 0 && wgrad8_direct(g) && ragged_unit_rows(B, M, N) &&
+        (int64_t)std::max(q->args->ld, q->args->lds) * 64 <= (int64_t)kMaxTileRowBytes * 256) {
+        g.a = q->args->codes;
+        g.sa = q->args->scales;
+        g.lda = q->args->ld;
+        g.lsa = q->args->lds;
+        g.b = B.p;
+        g.ldb = ragged_ld(B, M, N);
+        const hipError_t e = launch_wgrad8(g, ep, tl_stream);
+        if (e != hipSuccess) return launch_failed(e, "weight gradient");
+        return finish("weight gradient");
+    }
     uint8_t *part = nullptr;
     if (M == 0) wgrad_plan(g, kind, false, 0);
     if (M > 0) {

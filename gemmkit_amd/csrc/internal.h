@@ -258,6 +258,9 @@ struct RaggedArgs {
     // bf16: the operands' rows are unit-stride, 16 bytes or more, at any alignment
     int32_t any_align;
     int32_t tile;              // what grouped_plan_any or wgrad_plan chose
+    // wgrad of an MXINT8 checkpoint: A's codes at a and scales at sa, through an activation
+    int32_t act;               // FusedAct
+    float slope;
 };
 // B_g of the forward product: N rows of K (k-contiguous), or K rows of N.
 enum class RaggedB : int { Rows = 0, Cols = 1 };
@@ -270,6 +273,11 @@ hipError_t launch_grouped_bf16(const RaggedArgs &g, RaggedB bl, const EpiParams 
 // gradient with `out` output, given the bytes that aligned copies of its operands take.
 void wgrad_plan(RaggedArgs &g, EpiKind out, bool can_any, int64_t copies);
 hipError_t launch_grouped_wgrad(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
+// The weight gradient of one group of rows whose left operand is an MXINT8 checkpoint, decoded on
+// its way into the tiles; B as for any_align.  wgrad8_direct: where that costs less than
+// decoding first.
+bool wgrad8_direct(const RaggedArgs &g);
+hipError_t launch_wgrad8(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream);
 // What such a launch runs: the kernel (ragged.h: 0 ring, 1 256 x 256, 2 K split over the waves,
 // 3 and 4 the same for rows of any alignment), its tile, how many waves K is split over, whether B is read nontemporally.
 struct RaggedPlan {

@@ -99,6 +99,105 @@ __global__ __launch_bounds__(256) void mxint8_dequantize_kernel(const MxArgs g, 
     }
 }
 
+// ---------------------------------------------------------------- weight gradient
+
+// A's stages of a weight gradient whose left operand is a checkpoint: loaded as codes, and put in
+// the stage as act(values), rounded to bf16.  (RegPanel's transposed stage; each thread decodes
+// LP chunks of eight values a stage, once for every tile of its columns.)
+template <int W, int NW>
+struct CodePanel {
+    static constexpr int BYTES = W * 128, NI = BYTES / 1024, LP = NI / NW;
+    static_assert(NI % NW == 0, "every wave has chunks");
+    static constexpr int kNone = INT32_MAX;
+    static constexpr bool CODES = true;
+    using Reg = v4i;  // eight codes, their scale byte
+    const uint8_t *codes, *scales;  // of the next stage
+    int ld, lds, left, act;
+    float slope;
+    uint32_t vc[LP], vs[LP];  // this lane's offsets from them
+    int pos[LP];              // its rows, kNone: outside the tile
+    int wave, lane;
+
+    __device__ __forceinline__ void init(const RaggedArgs &g, const RaggedTile &t, int wave_, int lane_) {
+        codes = uniform((const uint8_t *)g.a + t.row0);
+        scales = uniform(g.sa + (t.row0 >> 5));
+        ld = (int)g.lda;
+        lds = (int)g.lsa;
+        left = t.k;
+        act = g.act;
+        slope = g.slope;
+        wave = wave_;
+        lane = lane_;
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const int at = (wave * LP + i) * 64 + lane, row = at / (W / 8), slot = at % (W / 8);
+            const int c = ((((slot >> 1) ^ tr_unit<W>(row)) << 1) | (slot & 1)) * 8;  // column
+            vc[i] = (uint32_t)(row * ld + c);
+            vs[i] = (uint32_t)(row * lds + (c >> 5));
+            pos[i] = c < t.rows ? row : kNone;
+        }
+    }
+    __device__ __forceinline__ void load(Reg (&r)[LP]) const {
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            v4i v = {};
+            if (pos[i] < left) {
+                const v2i w = *(const v2i *)(codes + vc[i]);
+                v = v4i{w[0], w[1], scales[vs[i]], 0};
+            }
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void skip(int stages) {
+        codes += (int64_t)stages * 64 * ld;
+        scales += (int64_t)stages * 64 * lds;
+        left -= stages * 64;
+    }
+    __device__ __forceinline__ void store(const Reg (&r)[LP], uint8_t *dst) const {
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const float step = mxint8_step(r[i][2]);
+            float f[8];
+            mxint8_values4((uint32_t)r[i][0], step, f);
+            mxint8_values4((uint32_t)r[i][1], step, f + 4);
+            act_apply(f, act, slope);
+            const v4i v = {(int)bf16x2_rne(f[0], f[1]), (int)bf16x2_rne(f[2], f[3]),
+                           (int)bf16x2_rne(f[4], f[5]), (int)bf16x2_rne(f[6], f[7])};
+            *(v4i *)(dst + (wave * LP + i) * 1024 + lane * 16) = v;
+        }
+    }
+};
+
+template <EpiKind E>
+static hipError_t wgrad8_go(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+    constexpr int BM = 64, BN = 64;
+    const int64_t per = (int64_t)((g.K + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    // (32-bit offsets inside a stage of 64 rows)
+    if (per > INT32_MAX / 16 || 64 * std::max(std::max(g.lda, g.lsa), g.ldb) > (int64_t)kMaxRecords)
+        return hipErrorInvalidValue;
+    hipLaunchKernelGGL((ragged_reg_kernel<true, true, PlainOut<E>, BM, BN, 2, 2, CodePanel<BM, 4>>),
+                       ragged_grid((int64_t)wgrad_share((int)per) * 8), dim3(256), 0, stream, g, ep);
+    return hipGetLastError();
+}
+
+// Few rows and tiles.  Traced kernels / calls one after the other, us, decoded in the tiles against
+// decoded first (two launches and a workspace): 64x1024x704 5.3 / 8.4 against 6.5 / 14.5, 256x1024x704
+// 7.4 / 8.6 against 7.1 / 14.4, 512x1024x704 10.2 / 9.4 against 8.1 / 14.4; through GELU 64 rows 6.6 / 8.5
+// against 6.7 / 14.2, 256 rows 10.4 / 9.6 against 7.4 / 14.1 (each tile of a column computes it again).
+bool wgrad8_direct(const RaggedArgs &g) {
+    const int64_t tiles = (int64_t)((g.K + 63) / 64) * ((g.N + 63) / 64);
+    const bool smooth = g.act != kActNone && g.act != kActRelu && g.act != kActLeakyRelu;
+    return g.M <= (smooth ? 128 : 256) && tiles <= 2 * (int64_t)g.cus;
+}
+
+hipError_t launch_wgrad8(const RaggedArgs &g, const EpiParams &ep, hipStream_t stream) {
+    if (ep.kind == EpiKind::BF16) return wgrad8_go<EpiKind::BF16>(g, ep, stream);
+    if (ep.kind == EpiKind::F32) return wgrad8_go<EpiKind::F32>(g, ep, stream);
+    return hipErrorInvalidValue;
+}
+
+// ---------------------------------------------------------------- launch
+
 // Small matrices: a chunk a thread, so that they reach more CUs.
 template <InType T, typename F>
 static hipError_t mxint8_grid(const MxArgs &g, F f) {

@@ -1149,6 +1149,8 @@ template <bool TR, int W, int NW>
 struct RegPanel {
     static constexpr int BYTES = W * 128, NI = BYTES / 1024, LP = (NI + NW - 1) / NW;
     static constexpr int kNone = INT32_MAX;
+    static constexpr bool CODES = false;
+    using Reg = v4i;
     // 16 bytes before the next stage (a chunk across the end of a row is read back from that
     // end, which may lie before the stage's first byte).
     const uint8_t *base;
@@ -1221,12 +1223,14 @@ struct RegPanel {
     }
 };
 
-template <bool AT, bool BT, typename O, int BM, int BN, int WM, int WN>
+// LEFT: A's panel, with RegPanel's members.
+template <bool AT, bool BT, typename O, int BM, int BN, int WM, int WN,
+          typename LEFT = RegPanel<AT, BM, WM * WN>>
 __global__ __launch_bounds__(WM * WN * 64)
 void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
     constexpr int NW = WM * WN;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
-    using PA = RegPanel<AT, BM, NW>;
+    using PA = LEFT;
     using PB = RegPanel<BT, BN, NW>;
     constexpr int STAGE = PA::BYTES + PB::BYTES, SUMS = NW * 16 * (WTN + 4) * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE > SUMS ? 2 * STAGE : SUMS];
@@ -1240,7 +1244,8 @@ void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
     const int kb = AT ? t.k : g.K * 2;
     PA A;
     PB B;
-    A.init(t.a, g.lda, kb, AT ? t.rows * 2 : t.rows, wave, lane);
+    if constexpr (PA::CODES) A.init(g, t, wave, lane);
+    else A.init(t.a, g.lda, kb, AT ? t.rows * 2 : t.rows, wave, lane);
     B.init(t.b, g.ldb, BT && !AT ? g.K : kb, BT ? t.cols * 2 : t.cols, wave, lane);
 
     Frag<AT, BM> fa;
@@ -1253,21 +1258,22 @@ void ragged_reg_kernel(const RaggedArgs g, const typename O::Params ep) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v4f{};
 
-    v4i ra[2][PA::LP], rb[2][PB::LP];
-    auto get = [&](int set) {
+    typename PA::Reg ra[2][PA::LP];
+    v4i rb[2][PB::LP];
+    auto get = [&](int set) __attribute__((always_inline)) {
         A.load(ra[set]);
         B.load(rb[set]);
         A.skip(1);
         B.skip(1);
     };
-    auto put = [&](int set, uint8_t *d) {
+    auto put = [&](int set, uint8_t *d) __attribute__((always_inline)) {
         A.store(ra[set], d);
         B.store(rb[set], d + PA::BYTES);
         get(set);
     };
     // Stage kt from slot PAR; stage kt+1, in registers, goes to the other one, and the loads
     // of stage kt+3 take its registers.
-    auto kstep = [&](auto par) {
+    auto kstep = [&](auto par) __attribute__((always_inline)) {
         constexpr int PAR = decltype(par)::value;
         const uint8_t *const sa = smem + PAR * STAGE, *const sb = sa + PA::BYTES;
         put(1 - PAR, smem + (1 - PAR) * STAGE);
