@@ -303,7 +303,6 @@ __device__ __forceinline__ v4u packed(const uint32_t (&v)[CH]) {
     return w;
 }
 
-
 // Rows of a product for which sums holds one row: a tile's, or (256 x 256) half a tile's,
 // since the last round's tiles may go out as halves.
 constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }
@@ -785,52 +784,53 @@ struct LinearOut {
         for (int j = 0; j < TN; ++j) *(v4f *)(stg + l16 * LD + 4 * lq + j * 16) = acc[0][j];
         int at_row = row;
 #pragma unroll 1
-        for (int h0 = 0; h0 < TM; h0 += D)
+        for (int h0 = 0; h0 < TM; h0 += D) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int h = h0 + d;
-            Raw in[P];
+            for (int d = 0; d < D; ++d) {
+                const int h = h0 + d;
+                Raw in[P];
 #pragma unroll
-            for (int s = 0; s < P; ++s) in[s] = next[d][s];
-            // (past the wave's last band: rows of the next wave or none, not used)
+                for (int s = 0; s < P; ++s) in[s] = next[d][s];
+                // (past the wave's last band: rows of the next wave or none, not used)
 #pragma unroll
-            for (int s = 0; s < P; ++s) load_in(next[d][s]);
-            __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses take effect in order)
-            stage(h + 1);
-            const float *const src = stg + (h & 1) * 16 * LD + r0 * LD + c;
+                for (int s = 0; s < P; ++s) load_in(next[d][s]);
+                __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses take effect in order)
+                stage(h + 1);
+                const float *const src = stg + (h & 1) * 16 * LD + r0 * LD + c;
 #pragma unroll
-            for (int s = 0; s < P; ++s) {
-                float f[CH];
+                for (int s = 0; s < P; ++s) {
+                    float f[CH];
 #pragma unroll
-                for (int i = 0; i < CH; i += 4) {
-                    const v4f v = *(const v4f *)(src + s * RPP * LD + i);
+                    for (int i = 0; i < CH; i += 4) {
+                        const v4f v = *(const v4f *)(src + s * RPP * LD + i);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[i + e] = v[e];
-                }
-                if constexpr (IN == 1 && PART) in[s].v = packed<CH, ISZ>(in[s].raw);
-                if constexpr (GRAD) {
-                    // (rows that are not there: 0 times anything, alpha too)
-                    grad_map(p, at_row < t.rows ? p.alpha : 0.0f, IN, in[s], f);
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) sum[e] += f[e];
-                    at_row += RPP;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) f[e] = __builtin_fmaf(p.alpha, f[e], bias[e]);
-                    if (p.codes) {
-                        v2u w;
-                        const int byte = quantize(f, w);
-                        if constexpr (CH == 8) __builtin_amdgcn_raw_buffer_store_b64(w, rq.r, rq.at, 0, 0);
-                        else __builtin_amdgcn_raw_buffer_store_b32(w[0], rq.r, rq.at, 0, 0);
-                        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs.r, rs.at, 0, 0);
-                        rq.at += rq.step;
-                        rs.at += rs.step;
-                    } else if (p.z) {
-                        put<false, PART>(rz, fl.nt_z, N - col, f);
+                        for (int e = 0; e < 4; ++e) f[i + e] = v[e];
                     }
-                    act_map(p, IN == 1, in[s], f);
+                    if constexpr (IN == 1 && PART) in[s].v = packed<CH, ISZ>(in[s].raw);
+                    if constexpr (GRAD) {
+                        grad_map(p, p.alpha, IN, in[s], f);
+                        // (rows that are not there: no zeros where a column of B is infinite)
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) sum[e] += at_row < t.rows ? f[e] : 0.0f;
+                        at_row += RPP;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e) f[e] = __builtin_fmaf(p.alpha, f[e], bias[e]);
+                        if (p.codes) {
+                            v2u w;
+                            const int byte = quantize(f, w);
+                            if constexpr (CH == 8) __builtin_amdgcn_raw_buffer_store_b64(w, rq.r, rq.at, 0, 0);
+                            else __builtin_amdgcn_raw_buffer_store_b32(w[0], rq.r, rq.at, 0, 0);
+                            __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rs.r, rs.at, 0, 0);
+                            rq.at += rq.step;
+                            rs.at += rs.step;
+                        } else if (p.z) {
+                            put<false, PART>(rz, fl.nt_z, N - col, f);
+                        }
+                        act_map(p, IN == 1, in[s], f);
+                    }
+                    put<F32, PART>(rc, fl.nt_c, N - col, f);
                 }
-                put<F32, PART>(rc, fl.nt_c, N - col, f);
             }
         }
         if (GRAD && p.sums) tile_sums<BM, BN, WM, WN>(p, t, N, sum, smem, wave, lane);

@@ -518,6 +518,26 @@ def test_dgrad_of_nothing_is_zero(dev, alpha, k):
         run_grad(dev, m, k, n, "gelu", BF16, z="mx", alpha=alpha)
 
 
+@pytest.mark.parametrize("m,k,n", [(9, 64, 72), (130, 264, 520), (300, 1024, 1024), (2500, 256, 3000)])
+@pytest.mark.parametrize("z", [None, "row", "mx"])
+def test_dgrad_sums_of_infinite_columns(dev, m, k, n, z):
+    """A column of B with an infinity: its sum is infinite, whatever the rows past the last one
+    hold.  (Exact: every finite product is 2^-10, so that the sums are below 2^24 of them.)"""
+    a = torch.ones((m, k), dtype=BF16)
+    w = torch.full((k, n), 2.0 ** -10, dtype=BF16)
+    w[k - 1, n - 1] = w[0, 5] = float("inf")
+    zs = torch.ones((m, n), dtype=BF16)
+    zv = None if z is None else mx_of(zs, dev) if z == "mx" else ref(zs, "row", dev)
+    sums = torch.full((n,), float("nan"), device=dev)
+    d = Out(m, n, BF16, "row", dev)
+    gk.gemm_linear_dgrad(1.0, ref(a, "row", dev), ref(w, "row", dev), d.view,
+                         act=ACTS["none" if z is None else "relu"], z=zv, dbias=sums)
+    got = sums.cpu()
+    want = torch.full((n,), m * k * 2.0 ** -10)
+    want[n - 1] = want[5] = float("inf")
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("m,n", [(1, 1), (1, 700), (3, 8), (700, 1), (333, 777), (1003, 520), (64, 5000),
                                  (5000, 40), (2048, 2048)])
 @pytest.mark.parametrize("act", ["none", "gelu", "leaky"])
@@ -585,6 +605,38 @@ def test_wgrad(dev, rows, k, n, out, act):
         tol = (rows + 2) * E23 * (s + (abs(beta) * c0.double().abs() if beta else 0))
         tol = tol + 1.25 * (dh.t() @ b.double().abs()) * (1 + rows * E23)
         close(c.get(), want, tol + HALF[out] * (want.abs() + tol), f"{rows}x{k}x{n} {act} {how_c}")
+
+
+@pytest.mark.parametrize("rows", [1, 63, 64, 127, 128, 129, 256, 257])
+@pytest.mark.parametrize("k,n", [(1, 8), (40, 72), (1025, 711), (2047, 1100), (64, 2048)])
+@pytest.mark.parametrize("act", ["none", "leaky", "silu"])
+def test_wgrad_of_few_rows(dev, rows, k, n, act):
+    """Rows and tiles on both sides of where a checkpoint is decoded in the tiles; a block
+    of NaN stays in its columns; what lies past the matrices' rows and columns is
+    not read into them."""
+    x = rnd((rows, k), F32, 5, 2.0)
+    q = mx_of(x, dev, 16)
+    if k % 32:
+        torch.as_strided(q.codes, (rows, -(-k // 32) * 32), (q.ld, 1))[:, k:] = 55
+    b = rnd((rows, n), BF16, 6)
+    h = act64(values8(q)[0], act)
+    dh = E20 * values8(q)[0].abs().clamp(min=1) if act in SMOOTH else torch.zeros_like(h)
+    if act != "none":
+        dh = dh + HALF[BF16] * (h.abs() + dh)
+    p, s = product(h.t(), b)
+    tol = (rows + 2) * E23 * s + (dh.t() @ b.double().abs()) * (1 + rows * E23)
+    for how_b in ("row", "mis"):
+        c = Out(k, n, F32, "row", dev)
+        gk.gemm_wgrad_mxint8(1.0, q, ref(b, how_b, dev), 0.0, c.view, act=ACTS[act])
+        close(c.get(), p, tol + HALF[F32] * (p.abs() + tol), f"{rows}x{k}x{n} {act} {how_b}")
+    q.scales[(rows - 1) * q.lds] = 255
+    c = Out(k, n, F32, "row", dev)
+    gk.gemm_wgrad_mxint8(1.0, q, ref(b, "row", dev), 0.0, c.view, act=ACTS[act])
+    got = c.get()
+    bad = slice(0, min(k, 32))
+    if act == "silu" or act == "none":
+        assert torch.isnan(got[bad]).all()
+    assert torch.isfinite(got[32:]).all()
 
 
 def test_wgrad_of_no_rows_scales_c(dev):
