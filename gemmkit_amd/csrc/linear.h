@@ -303,6 +303,10 @@ __device__ __forceinline__ v4u packed(const uint32_t (&v)[CH]) {
     return w;
 }
 
+// Matrices read once from this size on, a quarter of the Infinity Cache, are read nontemporally by the
+// kernels that do nothing else; smaller ones may lie in the caches, and lose.
+constexpr int64_t kOnceBytes = (int64_t)64 << 20;
+
 // Rows of a product for which sums holds one row: a tile's, or (256 x 256) half a tile's,
 // since the last round's tiles may go out as halves.
 constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }

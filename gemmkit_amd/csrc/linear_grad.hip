@@ -44,11 +44,12 @@ __device__ __forceinline__ void strip_sums(const LinearParams &p, int N, int tx,
 // Views of unit column stride (LinearOut::chunked): no branch around any access, and the next U
 // rows' inputs go out before this one's stores.
 // IN: pre-activations, none, bf16, or (2) a checkpoint.  PART: the matrix ends inside a chunk.
-template <InType T, int IN, bool PART>
+// ONCE: G nontemporally.
+template <InType T, int IN, bool PART, bool ONCE>
 __device__ __forceinline__ void act_grad_rows(const LinearParams &p, int64_t M, int N, int unit,
                                               int tx, float *red) {
     constexpr bool F32 = T == InType::F32;
-    constexpr int U = 2, SZ = F32 ? 4 : 2;
+    constexpr int U = 2, SZ = F32 ? 4 : 2, AUX = ONCE ? 2 : 0;
     const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx;
     const int width = 8 << tx, n0 = (int)blockIdx.x * width, c = cx * 8;
     const int cols = N - n0 < width ? N - n0 : width;
@@ -75,9 +76,9 @@ __device__ __forceinline__ void act_grad_rows(const LinearParams &p, int64_t M, 
             if constexpr (IN == 1) rz.template load<8, 2>(i.rz, left);
         }
         if constexpr (!PART) {
-            i.a[0] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at, 0, 0));
+            i.a[0] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at, 0, AUX));
             if constexpr (F32)
-                i.a[1] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at + 16, 0, 0));
+                i.a[1] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(ra.r, ra.at + 16, 0, AUX));
             ra.at += ra.step;
             if constexpr (IN == 1) {
                 i.z = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rz.r, rz.at, 0, 0));
@@ -215,7 +216,7 @@ __device__ __forceinline__ void act_grad_any(const LinearParams &p, int64_t M, i
 }
 
 // IN 0..2: act_grad_rows; 3: views of any strides.
-template <InType T, int IN>
+template <InType T, int IN, bool ONCE>
 __global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int64_t M, int N,
                                                        int unit, int tx) {
     __shared__ float red[kStripSums];
@@ -223,8 +224,8 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int
         act_grad_any<T>(p, M, N, unit, tx, red);
     } else {
         const bool part = N % 8 != 0 && N - ((int)blockIdx.x << (3 + tx)) < 8 << tx;
-        if (part) act_grad_rows<T, IN, true>(p, M, N, unit, tx, red);
-        else act_grad_rows<T, IN, false>(p, M, N, unit, tx, red);
+        if (part) act_grad_rows<T, IN, true, ONCE>(p, M, N, unit, tx, red);
+        else act_grad_rows<T, IN, false, ONCE>(p, M, N, unit, tx, red);
     }
 }
 
@@ -266,14 +267,22 @@ static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, const ActGr
                         (!p.codes || (p.ld <= most && p.lds <= most));
     LinearParams q = p;
     if (m == 1) q.rsc = q.rsr = q.rsz = 0;  // (never used)
-    if (!chunks)
-        hipLaunchKernelGGL((act_grad_kernel<T, 3>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
-    else if (p.codes)
-        hipLaunchKernelGGL((act_grad_kernel<T, 2>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
-    else if (p.z)
-        hipLaunchKernelGGL((act_grad_kernel<T, 1>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
-    else
-        hipLaunchKernelGGL((act_grad_kernel<T, 0>), grid, dim3(256), 0, stream, q, m, (int)n, unit, tx);
+    const auto go = [&](auto in, auto once) {
+        hipLaunchKernelGGL((act_grad_kernel<T, decltype(in)::value, decltype(once)::value>), grid,
+                           dim3(256), 0, stream, q, m, (int)n, unit, tx);
+    };
+    // (kernels, us, plain loads of G / nontemporal ones: bf16 8192 x 8192 70.4 / 65.1, 4096 x 8192
+    // 37.6 / 36.9, 1024 x 8192 12.0 / 12.6; f32 4096 x 8192 54.4 / 49.3, 1024 x 8192 13.8 / 15.2; the
+    // pre-activations nontemporally too 69.2 for the first)
+    const bool once = m * n * (int64_t)in_size(T) >= kOnceBytes;
+    const auto either = [&](auto in) {
+        if (once) go(in, std::true_type{});
+        else go(in, std::false_type{});
+    };
+    if (!chunks) go(std::integral_constant<int, 3>{}, std::false_type{});
+    else if (p.codes) either(std::integral_constant<int, 2>{});
+    else if (p.z) either(std::integral_constant<int, 1>{});
+    else either(std::integral_constant<int, 0>{});
 }
 
 hipError_t launch_act_grad(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,

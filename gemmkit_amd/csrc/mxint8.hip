@@ -26,7 +26,10 @@ struct ChunkAt {
     }
 };
 
-template <InType T, int U>
+// ONCE: x of whole chunks, nontemporally and without a branch around a load (kernels, us, plain loads
+// / so: bf16 16384 x 4096 51 / 40.4 (5.1 TB/s), 8192 x 4096 28.7 / 19.6, f32 16384 x 4000 91.7 / 64.6;
+// nontemporally 4096 x 4096 loses, 10.8 / 11.9).
+template <InType T, int U, bool ONCE>
 __global__ __launch_bounds__(256) void mxint8_quantize_kernel(const MxArgs g, uint32_t cpr) {
     constexpr bool F32 = T == InType::F32;
     constexpr int CH = F32 ? 4 : 8, LB = 32 / CH;
@@ -37,9 +40,16 @@ __global__ __launch_bounds__(256) void mxint8_quantize_kernel(const MxArgs g, ui
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const ChunkAt<CH> at(row0, c0, threadIdx.x + u * 256, cpr);
+        const bool in = at.row < g.rows && at.col < g.K;
         raw[u] = v4u{};
-        if (at.row < g.rows && at.col < g.K)
+        if constexpr (ONCE) {
+            typedef v4u v4u_any2 __attribute__((aligned(2)));
+            const uint8_t *x = (const uint8_t *)g.x + (in ? at.row * g.rs + at.col : 0) * (F32 ? 4 : 2);
+            const v4u v = __builtin_nontemporal_load((const v4u_any2 *)x);
+            raw[u] = in ? v : v4u{};
+        } else if (in) {
             raw[u] = read_raw<F32, CH>(g.x, at.row * g.rs + at.col * g.cs, g.cs, (int)g.K - at.col);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -224,11 +234,15 @@ static hipError_t mxint8_grid(const MxArgs &g, F f) {
 
 template <InType T>
 static hipError_t quantize_go(const MxArgs &g, hipStream_t stream) {
+    const bool once = g.rows * g.K * (int64_t)in_size(T) >= kOnceBytes && g.cs == 1 &&
+                      g.K % (T == InType::F32 ? 4 : 8) == 0;
     return mxint8_grid<T>(g, [&](const MxArgs &p, dim3 grid, uint32_t cpr, bool wide) {
-        if (wide)
-            hipLaunchKernelGGL((mxint8_quantize_kernel<T, 4>), grid, dim3(256), 0, stream, p, cpr);
+        if (wide && once)
+            hipLaunchKernelGGL((mxint8_quantize_kernel<T, 4, true>), grid, dim3(256), 0, stream, p, cpr);
+        else if (wide)
+            hipLaunchKernelGGL((mxint8_quantize_kernel<T, 4, false>), grid, dim3(256), 0, stream, p, cpr);
         else
-            hipLaunchKernelGGL((mxint8_quantize_kernel<T, 1>), grid, dim3(256), 0, stream, p, cpr);
+            hipLaunchKernelGGL((mxint8_quantize_kernel<T, 1, false>), grid, dim3(256), 0, stream, p, cpr);
     });
 }
 

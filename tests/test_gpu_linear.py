@@ -199,6 +199,37 @@ def test_quantize_and_back(dev, dt, rows, k, how):
         assert torch.equal(c.get().double(), want)
 
 
+@pytest.mark.parametrize("dt,rows", [(BF16, 4100), (F32, 2050)])
+def test_large_matrices_as_their_halves(dev, dt, rows):
+    """Matrices from 64 MiB on are read another way: the same bits as half of the rows at a time,
+    with a last block that is not whole."""
+    k = 8200
+    x = torch.randn(rows, k, device=dev, generator=torch.Generator(dev).manual_seed(9)).to(dt)
+    z = torch.randn(rows, k, device=dev, generator=torch.Generator(dev).manual_seed(10)).to(BF16)
+    assert x.numel() * x.element_size() >= 64 << 20
+    cuts = [(0, rows), (0, rows // 2), (rows // 2, rows)]
+    codes, grads, sums = [], [], []
+    for lo, hi in cuts:
+        n = hi - lo
+        xv = gk.MatRef(x[lo:hi], n, k, k, 1)
+        q = mx_empty(n, k, dev)
+        gk.quantize_mxint8(xv, q)
+        codes.append((torch.as_strided(q.codes, (n, -(-k // 32) * 32), (q.ld, 1)),
+                      torch.as_strided(q.scales, (n, -(-k // 32)), (q.lds, 1))))
+        for act, zv in (("none", None), ("gelu", gk.MatRef(z[lo:hi], n, k, k, 1)), ("silu", q)):
+            d, s = torch.empty(n, k, dtype=BF16, device=dev), torch.empty(k, device=dev)
+            gk.activation_grad(xv, gk.MatMut(d, n, k, k, 1), act=ACTS[act], z=zv, dbias=s)
+            grads.append(d)
+            sums.append(s)
+    for i in range(2):
+        assert torch.equal(codes[0][i], torch.cat([codes[1][i], codes[2][i]]))
+    for i in range(3):
+        assert torch.equal(grads[i], torch.cat([grads[3 + i], grads[6 + i]]))
+        # (two orders of one sum of `rows` terms, each off by rows half steps of the magnitudes' sum)
+        bound = 2 * rows * E23 * (grads[i].double().abs().sum(0) * (1 + 2.0 ** -8) + 1e-30)
+        assert ((sums[i].double() - sums[3 + i].double() - sums[6 + i].double()).abs() <= bound).all()
+
+
 def test_quantize_extremes(dev):
     big, tiny, sub = 3.3895313892515355e38, 2.0 ** -126, 2.0 ** -133
     for dt in (BF16, F32):
