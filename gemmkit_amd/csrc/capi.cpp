@@ -2981,7 +2981,7 @@ int act_grad_checked(gk_workspace *ws, InType in, const LinearSpec &s, const gk_
         return (r = add_col_sums(nullptr, 0, s)) ? r : finish("activation gradient");
     }
     LinearParams p = linear_params(s, 1.0f, c);
-    const int64_t unit = act_grad_unit(M, N, g_num_cus), parts = s.dbias ? (M + unit - 1) / unit : 0;
+    const int64_t unit = act_grad_unit(in, M, N, g_num_cus, p), parts = s.dbias ? (M + unit - 1) / unit : 0;
     void *part = nullptr;
     if (parts > 1 && (r = ws_reserve(resolve_ws(ws), (size_t)parts * N * 4, &part))) return r;
     p.sums = parts > 1 ? (float *)part : s.dbias;

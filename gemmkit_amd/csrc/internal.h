@@ -340,7 +340,7 @@ hipError_t launch_linear_grad(const RaggedArgs &g, RaggedB bl, EpiKind kind, con
 int linear_unit(const RaggedArgs &g, RaggedB bl);
 // C = A * act'(Z), elementwise over M x N (A of either type at p.res, C bf16), with column
 // sums per act_grad_unit() rows.
-int act_grad_unit(int64_t m, int64_t n, int cus);
+int act_grad_unit(InType in, int64_t m, int64_t n, int cus, const LinearParams &p);
 hipError_t launch_act_grad(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,
                            hipStream_t stream);
 // out[j] = the sum over i < rows of part[i*n + j], in a fixed order.

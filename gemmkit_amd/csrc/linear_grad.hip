@@ -20,23 +20,25 @@ int linear_unit(const RaggedArgs &g, RaggedB bl) {
 
 // C = A * act'(Z), a workgroup per strip of 1 << tx chunk columns of 8 and `unit` rows, as many rows at
 // a time as it has threads for; column sums of its rows before rounding to one row of p.sums.
-constexpr int kStripSums = 4 * 512;  // floats: four waves of 64 chunk columns
+constexpr int kStripSums = 4 * 512;  // floats: four waves of 64 chunk columns, or 16 of four
+constexpr int kStripTx = 2;  // narrow strips of aligned rows
 
 // The workgroup's column sums from its threads': a wave's rows, then the waves, in order.
-__device__ __forceinline__ void strip_sums(const LinearParams &p, int N, int tx, float *red,
+template <int THREADS>
+__device__ __forceinline__ void strip_sums(const LinearParams &p, int strip, int N, int tx, float *red,
                                            float (&sum)[8]) {
     for (int d = 1 << tx; d < 64; d <<= 1)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], d);
-    const int width = 8 << tx, base = (int)blockIdx.x * width, lane = threadIdx.x & 63;
+    const int width = 8 << tx, base = strip * width, lane = threadIdx.x & 63;
     if (lane < 1 << tx) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) red[(threadIdx.x >> 6) * width + lane * 8 + e] = sum[e];
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < width; j += 256) {
+    for (int j = threadIdx.x; j < width; j += THREADS) {
         float s = red[j];
-        for (int w = 1; w < 4; ++w) s += red[w * width + j];
+        for (int w = 1; w < THREADS / 64; ++w) s += red[w * width + j];
         if (base + j < N) p.sums[(int64_t)blockIdx.y * N + base + j] = s;
     }
 }
@@ -45,18 +47,18 @@ __device__ __forceinline__ void strip_sums(const LinearParams &p, int N, int tx,
 // rows' inputs go out before this one's stores.
 // IN: pre-activations, none, bf16, or (2) a checkpoint.  PART: the matrix ends inside a chunk.
 // ONCE: G nontemporally.
-template <InType T, int IN, bool PART, bool ONCE>
-__device__ __forceinline__ void act_grad_rows(const LinearParams &p, int64_t M, int N, int unit,
-                                              int tx, float *red) {
+template <InType T, int IN, bool PART, bool ONCE, int THREADS>
+__device__ __forceinline__ void act_grad_rows(const LinearParams &p, int strip, int64_t M, int N,
+                                              int unit, int tx, float *red) {
     constexpr bool F32 = T == InType::F32;
     constexpr int U = 2, SZ = F32 ? 4 : 2, AUX = ONCE ? 2 : 0;
     const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx;
-    const int width = 8 << tx, n0 = (int)blockIdx.x * width, c = cx * 8;
+    const int width = 8 << tx, n0 = strip * width, c = cx * 8;
     const int cols = N - n0 < width ? N - n0 : width;
     const int64_t row0 = (int64_t)blockIdx.y * unit;
     const int rows = M - row0 < unit ? (int)(M - row0) : unit;
     const bool in = c < cols, nt = row_lines(p.c, p.rsc * 2);
-    const int rpp = 256 >> tx;
+    const int rpp = THREADS >> tx;
     const int64_t ldc = (p.rsc > N ? p.rsc : N) * 2, ldz = (p.rsz > N ? p.rsz : N) * 2;
     const int64_t lda = (p.rsr > N ? p.rsr : N) * SZ;
     Rows rc((uint8_t *)p.c + row0 * ldc + n0 * 2, ldc, rows, cols * 2, ry, c * 2, in, rpp);
@@ -137,17 +139,17 @@ __device__ __forceinline__ void act_grad_rows(const LinearParams &p, int64_t M, 
             for (int e = 0; e < 8; ++e) sum[e] += f[e];
         }
     }
-    if (p.sums) strip_sums(p, N, tx, red, sum);
+    if (p.sums) strip_sums<THREADS>(p, strip, N, tx, red, sum);
 }
 
 // A strip of any strides and width.
-template <InType T>
-__device__ __forceinline__ void act_grad_any(const LinearParams &p, int64_t M, int N, int unit, int tx,
-                                             float *red) {
+template <InType T, int THREADS>
+__device__ __forceinline__ void act_grad_any(const LinearParams &p, int strip, int64_t M, int N,
+                                             int unit, int tx, float *red) {
     constexpr bool F32 = T == InType::F32;
     constexpr int U = 2;  // rows whose loads are in flight together
-    const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx, rpp = 256 >> tx;
-    const int col = ((int)blockIdx.x << tx | cx) * 8, cols = N - col;
+    const int cx = threadIdx.x & ((1 << tx) - 1), ry = threadIdx.x >> tx, rpp = THREADS >> tx;
+    const int col = (strip << tx | cx) * 8, cols = N - col;
     const int64_t first = (int64_t)blockIdx.y * unit;
     const int64_t end = first + unit < M ? first + unit : M;
     const bool nt = row_lines(p.c, p.rsc * 2);
@@ -212,32 +214,49 @@ __device__ __forceinline__ void act_grad_any(const LinearParams &p, int64_t M, i
             }
         }
     }
-    if (p.sums) strip_sums(p, N, tx, red, sum);
+    if (p.sums) strip_sums<THREADS>(p, strip, N, tx, red, sum);
 }
 
 // IN 0..2: act_grad_rows; 3: views of any strides.
-template <InType T, int IN, bool ONCE>
-__global__ __launch_bounds__(256) void act_grad_kernel(const LinearParams p, int64_t M, int N,
-                                                       int unit, int tx) {
+template <InType T, int IN, bool ONCE, int THREADS>
+__global__ __launch_bounds__(THREADS) void act_grad_kernel(const LinearParams p, int64_t M, int N,
+                                                           int unit, int tx) {
     __shared__ float red[kStripSums];
-    if constexpr (IN == 3) {
-        act_grad_any<T>(p, M, N, unit, tx, red);
-    } else {
-        const bool part = N % 8 != 0 && N - ((int)blockIdx.x << (3 + tx)) < 8 << tx;
-        if (part) act_grad_rows<T, IN, true, ONCE>(p, M, N, unit, tx, red);
-        else act_grad_rows<T, IN, false, ONCE>(p, M, N, unit, tx, red);
+    int strip = (int)blockIdx.x;
+    if (tx == kStripTx && gridDim.y == 1) {  // neighbours, which share lines, on one XCD
+        const int x = strip % 8, per = (int)gridDim.x / 8, more = (int)gridDim.x % 8;
+        strip = x * per + (x < more ? x : more) + strip / 8;
     }
+    if constexpr (IN == 3) {
+        act_grad_any<T, THREADS>(p, strip, M, N, unit, tx, red);
+    } else {
+        const bool part = N % 8 != 0 && N - (strip << (3 + tx)) < 8 << tx;
+        if (part) act_grad_rows<T, IN, true, ONCE, THREADS>(p, strip, M, N, unit, tx, red);
+        else act_grad_rows<T, IN, false, ONCE, THREADS>(p, strip, M, N, unit, tx, red);
+    }
+}
+
+// Whether every row of the views starts at 16 bytes.
+static bool act_grad_aligned(InType in, int64_t m, const LinearParams &p) {
+    const auto rows = [&](const void *q, int64_t rs, int64_t cs, int64_t size) {
+        return cs == 1 && (((uint64_t)q | (m > 1 ? (uint64_t)(rs * size) : 0)) & 15) == 0;
+    };
+    return rows(p.c, p.rsc, p.csc, 2) && rows(p.res, p.rsr, p.csr, (int64_t)in_size(in)) &&
+           (!p.z || rows(p.z, p.rsz, p.csz, 2));
 }
 
 // A workgroup's part.  Strips of 64 chunk columns (a KiB of bf16 in a row) where the matrix has
 // them, rows for about eight workgroups per CU, at least two per thread.  Column sums of few rows:
-// strips of two chunk columns and all rows, which need no second launch (64 x 8192 5.8 us); such
-// strips read 32 bytes of a row at a time and are bound by their addresses, so that of more rows
-// two launches cost less (1003 x 777 12.7 us in one, 5.9 + 4.4 in two).
+// narrow strips of all rows, which need no second launch.  Aligned rows up to 1024, four chunk
+// columns (calls, us, against two launches: bf16 512 x 8192 9.4 / 12.0, 1024 x 1024 9.6 / 14.3, 1024 x 8192
+// 10.9 / 14.9; 2048 x 4096 14.3 / 14.6, 2048 x 8192 18.8 / 19.2).  Others are bound by their addresses on
+// the few CUs of narrow strips: up to 512 rows, two chunk columns (333 x 1501 9.0 / 13.5; f32
+// 1003 x 777 14.6 / 13.5).
 struct ActGradShape {
-    int tx, unit;
+    int tx, unit, threads;
 };
-static ActGradShape act_grad_shape(int64_t m, int64_t n, int cus, bool sums) {
+static ActGradShape act_grad_shape(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,
+                                   bool sums) {
     int tx = 6;
     while (tx > 0 && ((int64_t)8 << (tx - 1)) >= n) --tx;
     const int rpp = 256 >> tx;
@@ -246,19 +265,25 @@ static ActGradShape act_grad_shape(int64_t m, int64_t n, int cus, bool sums) {
     int64_t unit = (rows + rpp - 1) / rpp * rpp;
     unit = std::max<int64_t>(unit, 2 * rpp);
     unit = std::max<int64_t>(unit, (m + 65534) / 65535);
-    if (sums && m > unit && m <= 512) return {1, (int)m};
-    return {tx, (int)unit};
+    if (sums && m > unit) {
+        if (m <= 1024 && m * n * (int64_t)in_size(in) < kOnceBytes && act_grad_aligned(in, m, p))
+            return {kStripTx, (int)m, m <= 256 ? 256 : 1024};
+        if (m <= 512) return {1, (int)m, 256};
+    }
+    return {tx, (int)unit, 256};
 }
 
-int act_grad_unit(int64_t m, int64_t n, int cus) { return act_grad_shape(m, n, cus, true).unit; }
+int act_grad_unit(InType in, int64_t m, int64_t n, int cus, const LinearParams &p) {
+    return act_grad_shape(in, m, n, cus, p, true).unit;
+}
 
 template <InType T>
 static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, const ActGradShape &shape,
                         hipStream_t stream) {
     // (32-bit offsets: the rows of a workgroup)
-    const int tx = shape.tx, unit = shape.unit;
+    const int tx = shape.tx, unit = shape.unit, threads = shape.threads;
     const dim3 grid((uint32_t)((n + (8 << tx) - 1) / (8 << tx)), (uint32_t)((m + unit - 1) / unit));
-    const int64_t most = (int64_t)kMaxRecords / (unit + 4 * (256 >> tx));
+    const int64_t most = (int64_t)kMaxRecords / (unit + 4 * (threads >> tx));
     const auto rows = [&](int64_t rs, int64_t cs, int64_t size) {
         return cs == 1 && (m <= 1 || (rs >= n && rs * size <= most));
     };
@@ -268,8 +293,14 @@ static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, const ActGr
     LinearParams q = p;
     if (m == 1) q.rsc = q.rsr = q.rsz = 0;  // (never used)
     const auto go = [&](auto in, auto once) {
-        hipLaunchKernelGGL((act_grad_kernel<T, decltype(in)::value, decltype(once)::value>), grid,
-                           dim3(256), 0, stream, q, m, (int)n, unit, tx);
+        constexpr int IN = decltype(in)::value;
+        constexpr bool ONCE = decltype(once)::value;
+        if (threads == 1024)
+            hipLaunchKernelGGL((act_grad_kernel<T, IN, false, 1024>), grid, dim3(1024), 0, stream, q, m,
+                               (int)n, unit, tx);
+        else
+            hipLaunchKernelGGL((act_grad_kernel<T, IN, ONCE, 256>), grid, dim3(256), 0, stream, q, m,
+                               (int)n, unit, tx);
     };
     // (kernels, us, plain loads of G / nontemporal ones: bf16 8192 x 8192 70.4 / 65.1, 4096 x 8192
     // 37.6 / 36.9, 1024 x 8192 12.0 / 12.6; f32 4096 x 8192 54.4 / 49.3, 1024 x 8192 13.8 / 15.2; the
@@ -287,7 +318,7 @@ static void act_grad_go(const LinearParams &p, int64_t m, int64_t n, const ActGr
 
 hipError_t launch_act_grad(InType in, int64_t m, int64_t n, int cus, const LinearParams &p,
                            hipStream_t stream) {
-    const ActGradShape shape = act_grad_shape(m, n, cus, p.sums != nullptr);
+    const ActGradShape shape = act_grad_shape(in, m, n, cus, p, p.sums != nullptr);
     if (in == InType::BF16) act_grad_go<InType::BF16>(p, m, n, shape, stream);
     else act_grad_go<InType::F32>(p, m, n, shape, stream);
     return hipGetLastError();

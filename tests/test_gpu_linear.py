@@ -585,6 +585,14 @@ def test_activation_grad_strides(dev, act, how):
     run_grad(dev, 130, 0, 141, act, z="mx", product_first=False, hows=(how, how, how), in_place=True)
 
 
+@pytest.mark.parametrize("m", [64, 256, 257, 512, 513, 1023, 1024, 1025, 2048])
+@pytest.mark.parametrize("n", [8, 72, 1000, 1001, 2080])
+@pytest.mark.parametrize("z", ["row", "mx", "odd"])
+def test_activation_grad_column_sums(dev, m, n, z):
+    """Rows, widths and alignments on both sides of where the sums need no second launch."""
+    run_grad(dev, m, 0, n, act="silu", z=z, product_first=False, gt=BF16 if m % 2 else F32)
+
+
 def test_gradients_against_differences(dev):
     """d/dx and d/db of sum(G * act(X W + b)) against central differences in 64 bits."""
     m, k, n = 6, 40, 33
