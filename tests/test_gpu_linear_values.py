@@ -1,0 +1,98 @@
+"""Values of the linear layers' activations and derivatives where they are small, infinite or
+NaN.  An activation's argument reaches it exactly as an f32 bias of a product without alpha, a
+derivative's as a bfloat16 pre-activation under a gradient of 1."""
+import pytest
+import torch
+
+import gemmkit_amd as gk
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+E20, E23 = 2.0 ** -20, 2.0 ** -23
+
+
+def row(t):
+    return gk.MatRef.from_row_major(t, *t.shape)
+
+
+def out(t):
+    return gk.MatMut.from_row_major(t, *t.shape)
+
+
+def ones(dev, *shape, dt=BF16):
+    return torch.ones(*shape, dtype=dt, device=dev)
+
+
+def activated(z, act, dev):
+    """act(z) of f32 values, in f32."""
+    n = z.numel()
+    c = torch.empty(1, n, device=dev)
+    gk.gemm_linear(0.0, row(ones(dev, 1, 1)), row(ones(dev, 1, n)), out(c),
+                   bias=gk.Bias.PerCol(z.to(dev)), act=act)
+    return c.cpu().flatten()
+
+
+def derivative(z, act, dev):
+    """act'(z) of bfloat16 values, in f32."""
+    n = z.numel()
+    d = torch.empty(1, n, device=dev)
+    gk.gemm_linear_dgrad(1.0, row(ones(dev, 1, 1)), row(ones(dev, 1, n)), out(d), act=act,
+                         z=row(z.to(dev).view(1, n)))
+    return d.cpu().flatten()
+
+
+def bf16_between(lo, hi):
+    """Every bfloat16 value of [lo, hi]."""
+    v = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(BF16)
+    return v[(v >= lo) & (v <= hi)]
+
+
+def tail(z):
+    """(P(-|z|), |z| p(z), how far either may be off, relative to itself) in 64 bits.
+
+    An exponent of z^2 log2(e) / 2 that is rounded three times, by 2^-24 each, moves the exponential by
+    z^2 / 2 * 3 * 2^-24, less than z^2 2^-23 of itself; the exponential, a reciprocal and the nine
+    steps of a polynomial with positive sum, whose error the fit adds to by 2^-22, stay
+    within 2^-20.  (P by erfc: as 1 + erf it would end at 2^-53.)"""
+    a = z.double().abs()
+    return torch.special.erfc(a * 0.5 ** 0.5) / 2, a * torch.exp(-a * a / 2) * 0.3989422804014327, E20 + a * a * E23
+
+
+def test_gelu_keeps_the_tail(dev):
+    """GELU of negative z is z P(z) to its own last bits, not only to those of 1: its sign is
+    z's as far as f32 reaches."""
+    g = torch.Generator().manual_seed(1)
+    z = torch.cat([bf16_between(-13, 13).float(), torch.rand(20001, generator=g) * 26 - 13])
+    got = activated(z, gk.Activation.Gelu, dev).double()
+    p, _, rel = tail(z)
+    z64 = z.double()
+    want = torch.where(z64 < 0, z64 * p, z64 * (1 - p))
+    tol = z64.abs() * p * rel + torch.where(z64 < 0, 0.0, E23 * z64) + 2.0 ** -126
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+    assert (got[(z < -0.01) & (z > -12.5)] < 0).all()
+
+
+def test_gelu_derivative_keeps_the_tail(dev):
+    z = bf16_between(-13, 13)
+    got = derivative(z, gk.Activation.Gelu, dev).double()
+    p, zp, rel = tail(z)
+    want = torch.where(z < 0, p - zp, 1 - p + zp)
+    tol = (p + zp) * rel + torch.where(z < 0, 0.0, 2 * E23) + 2.0 ** -126
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+def test_gelu_of_a_checkpoint_keeps_the_tail(dev):
+    """The same through dequantization, in f32 and rounded once to bfloat16."""
+    z = -torch.arange(32, 128).float().div(8).view(3, 32)  # -4 .. -15.9: codes of one scale each
+    q = gk.quantize_mxint8(row(z.to(dev)))
+    kept = torch.empty(3, 32, device=dev)
+    gk.dequantize_mxint8(q, out(kept))
+    assert torch.equal(kept.cpu(), z)
+    p, _, rel = tail(z)
+    want = z.double() * p
+    for dt, half in ((F32, 0.0), (BF16, 2.0 ** -8)):
+        c = torch.empty(3, 32, dtype=dt, device=dev)
+        gk.dequantize_mxint8(q, out(c), act=gk.Activation.Gelu)
+        tol = want.abs() * (rel + half * (1 + rel)) + 2.0 ** -126
+        assert ((c.cpu().double() - want).abs() <= tol).all()
