@@ -100,8 +100,9 @@ __device__ __forceinline__ void act_scale(float (&f)[N], const float (&z)[N], in
     } else if (act == kActSilu) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float s = sigmoid(z[e]);
-            f[e] *= s * __builtin_fmaf(z[e], 1.0f - s, 1.0f);
+            // (beyond 128 s is 1 or 0: an infinity would make NaN of the limits)
+            const float s = sigmoid(z[e]), b = __builtin_amdgcn_fmed3f(z[e], -128.0f, 128.0f);
+            f[e] *= s * __builtin_fmaf(b, 1.0f - s, 1.0f);
         }
     } else if (act != kActNone) {
         const float s = act == kActRelu ? 0.0f : slope;

@@ -762,7 +762,8 @@ int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
  * with the normal distribution P and its density p.  The last three and their derivatives
  * are off by at most 2^-20 * max(|z|, 1); left of 0 GELU is off by at most 2^-20 + z^2 2^-23 of
  * itself and its derivative by as much of P(z) + |z| p(z), but for what f32 cannot hold.
- * GELU_TANH and SILU are NaN at -infinity.
+ * At infinities these three and their derivatives have their limits, but GELU_TANH and SILU
+ * themselves are NaN at -infinity.
  */
 
 /* A rows x cols matrix in MXINT8: row r's elements as int8 codes at codes + r * ld,

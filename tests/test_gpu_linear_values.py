@@ -96,3 +96,36 @@ def test_gelu_of_a_checkpoint_keeps_the_tail(dev):
         gk.dequantize_mxint8(q, out(c), act=gk.Activation.Gelu)
         tol = want.abs() * (rel + half * (1 + rel)) + 2.0 ** -126
         assert ((c.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("act", ["Relu", "LeakyRelu", "Gelu", "GeluTanh", "Silu"])
+def test_derivatives_at_infinity(dev, act):
+    """Their limits: a pre-activation past bfloat16's range is kept as an infinity, and its column
+    sum stays finite."""
+    a = gk.Activation.LeakyRelu(-0.5) if act == "LeakyRelu" else getattr(gk.Activation, act)
+    inf = float("inf")
+    z = torch.tensor([inf, -inf, 1.0, inf, -inf], dtype=BF16)
+    low = -0.5 if act == "LeakyRelu" else 0.0
+    limits = torch.tensor([1.0, low])
+    assert torch.equal(derivative(z, a, dev)[[0, 1]], limits)
+    for rows in (1, 40, 700):
+        zm = z.to(dev).repeat(rows, 1)
+        d, sums = torch.empty(rows, 5, dtype=BF16, device=dev), torch.empty(5, device=dev)
+        gk.activation_grad(row(ones(dev, rows, 5)), out(d), act=a, z=row(zm), dbias=sums)
+        assert torch.equal(d.float().cpu()[:, [0, 1, 3, 4]], limits.repeat(rows, 2))
+        assert torch.equal(sums.cpu()[[0, 1, 3, 4]], limits.repeat(2) * rows)
+    big = torch.tensor([3.4e38], device=dev)  # rounds to an infinity in bfloat16
+    zk, c = torch.empty(1, 1, dtype=BF16, device=dev), torch.empty(1, 1, device=dev)
+    gk.gemm_linear(0.0, row(ones(dev, 1, 1)), row(ones(dev, 1, 1)), out(c), bias=gk.Bias.PerCol(big),
+                   act=a, z=out(zk))
+    assert torch.isinf(zk).all() and torch.isfinite(c).all()
+
+
+def test_activations_at_infinity(dev):
+    z = torch.tensor([float("inf"), -float("inf")])
+    for act, low in ((gk.Activation.Relu, 0.0), (gk.Activation.LeakyRelu(0.25), -float("inf")),
+                     (gk.Activation.Gelu, 0.0), (gk.Activation.GeluTanh, None),
+                     (gk.Activation.Silu, None)):
+        got = activated(z, act, dev)
+        assert got[0] == float("inf")
+        assert torch.isnan(got[1]) if low is None else got[1] == low
