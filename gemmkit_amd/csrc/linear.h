@@ -52,7 +52,8 @@ __device__ __forceinline__ float gelu_inner(float z) {
     return z * __builtin_fmaf(kGeluC2 * kGeluCubic, z * z, kGeluC2);
 }
 
-// f = act(f).  (ReLU and LeakyReLU as fused_apply's: NaN and -0 give 0.)
+// f = act(f).  NaN stays NaN, through ReLU and LeakyReLU too (unlike fused_apply's): a checkpoint's
+// mark of an overflow is to be seen behind them.  Their -0 gives 0.
 template <int N>
 __device__ __forceinline__ void act_apply(float (&f)[N], int act, float slope) {
     if (act == kActGelu) {
@@ -71,13 +72,13 @@ __device__ __forceinline__ void act_apply(float (&f)[N], int act, float slope) {
         const float s = act == kActRelu ? 0.0f : slope;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float hi = f[e] > 0.0f ? f[e] : 0.0f, lo = f[e] < 0.0f ? f[e] : 0.0f;
+            const float hi = f[e] <= 0.0f ? 0.0f : f[e], lo = f[e] < 0.0f ? f[e] : 0.0f;
             f[e] = act == kActRelu ? hi : __builtin_fmaf(s, lo, hi);
         }
     }
 }
 
-// f *= act'(z); at 0 ReLU's derivative is 0 and LeakyReLU's the slope.
+// f *= act'(z); at 0 ReLU's derivative is 0 and LeakyReLU's the slope, at a NaN every one is NaN.
 template <int N>
 __device__ __forceinline__ void act_scale(float (&f)[N], const float (&z)[N], int act, float slope) {
     if (act == kActGelu) {
@@ -107,7 +108,7 @@ __device__ __forceinline__ void act_scale(float (&f)[N], const float (&z)[N], in
     } else if (act != kActNone) {
         const float s = act == kActRelu ? 0.0f : slope;
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] *= z[e] > 0.0f ? 1.0f : s;
+        for (int e = 0; e < N; ++e) f[e] *= z[e] > 0.0f ? 1.0f : z[e] <= 0.0f ? s : z[e];
     }
 }
 

@@ -764,6 +764,8 @@ int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
  * itself and its derivative by as much of P(z) + |z| p(z), but for what f32 cannot hold.
  * At infinities these three and their derivatives have their limits, but GELU_TANH and SILU
  * themselves are NaN at -infinity.
+ * A NaN gives NaN, in the value and in the derivative of every activation (through the fused
+ * entries' ReLU and LeakyReLU it gives 0), so a checkpoint's block of NaN is not lost behind one.
  */
 
 /* A rows x cols matrix in MXINT8: row r's elements as int8 codes at codes + r * ld,

@@ -129,3 +129,44 @@ def test_activations_at_infinity(dev):
         got = activated(z, act, dev)
         assert got[0] == float("inf")
         assert torch.isnan(got[1]) if low is None else got[1] == low
+
+
+NAN_ACTS = [gk.Activation.Relu, gk.Activation.LeakyRelu(-0.3), gk.Activation.LeakyRelu(0.0),
+            gk.Activation.Gelu, gk.Activation.GeluTanh, gk.Activation.Silu]
+
+
+@pytest.mark.parametrize("act", NAN_ACTS)
+def test_nan_stays_nan(dev, act):
+    """Through every activation and derivative, from a value and from a checkpoint's block."""
+    nan = float("nan")
+    got = activated(torch.tensor([1.0, nan, -1.0, nan]), act, dev)
+    assert torch.equal(torch.isnan(got), torch.tensor([False, True, False, True]))
+    got = derivative(torch.tensor([1.0, nan, -1.0, nan], dtype=BF16), act, dev)
+    assert torch.equal(torch.isnan(got), torch.tensor([False, True, False, True]))
+    for rows in (70, 600):
+        x = torch.randn(rows, 100, generator=torch.Generator().manual_seed(2))
+        x[rows - 3, 40] = float("inf")
+        q = gk.quantize_mxint8(row(x.to(dev)))
+        bad = torch.zeros(rows, 100, dtype=torch.bool)
+        bad[rows - 3, 32:64] = True
+        c = torch.empty(rows, 100, device=dev)
+        gk.dequantize_mxint8(q, out(c), act=act)
+        assert torch.equal(torch.isnan(c.cpu()), bad)
+        b = torch.randn(rows, 24, generator=torch.Generator().manual_seed(3)).to(BF16).to(dev)
+        w = torch.empty(100, 24, device=dev)
+        gk.gemm_wgrad_mxint8(1.0, q, row(b), 0.0, out(w), act=act)
+        assert torch.equal(torch.isnan(w.cpu()), bad.any(0).unsqueeze(1).expand(100, 24))
+        g = ones(dev, rows, 100)
+        d, sums = torch.empty(rows, 100, dtype=BF16, device=dev), torch.empty(100, device=dev)
+        gk.activation_grad(row(g), out(d), act=act, z=q, dbias=sums)
+        assert torch.equal(torch.isnan(d.cpu()), bad) and torch.equal(torch.isnan(sums.cpu()), bad.any(0))
+        a, k = ones(dev, rows, 8), ones(dev, 8, 100)
+        gk.gemm_linear_dgrad(1.0, row(a), row(k), out(d), act=act, z=q, dbias=sums)
+        assert torch.equal(torch.isnan(d.cpu()), bad) and torch.equal(torch.isnan(sums.cpu()), bad.any(0))
+
+
+@pytest.mark.parametrize("act", [gk.Activation.Relu, gk.Activation.LeakyRelu(-0.3)])
+def test_zeros_of_either_sign(dev, act):
+    z = torch.tensor([0.0, -0.0])
+    assert torch.equal(activated(z, act, dev), torch.zeros(2))
+    assert torch.equal(derivative(z.to(BF16), act, dev), torch.full((2,), act.slope))
