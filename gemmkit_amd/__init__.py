@@ -1304,12 +1304,14 @@ def _kept(z, *tensors):
     return MatRef._c(z, torch.bfloat16, "Z"), None
 
 
-def _dbias(dbias: Optional[torch.Tensor]):
+def _dbias(dbias: Optional[torch.Tensor], cols: int):
     if dbias is None:
         return None, 0
     d = _slice(dbias, "dbias")
     if d.dtype != torch.float32:
         raise TypeError(f"gemmkit_amd: dbias must be float32, got {d.dtype}")
+    if d.numel() != cols:  # (here, since an empty tensor's pointer is null: no dbias)
+        raise GemmkitError(-1, f"gemmkit_amd: dbias length ({d.numel()}) != the output's columns ({cols})")
     return d.data_ptr(), d.numel()
 
 
@@ -1361,7 +1363,7 @@ def gemm_linear_dgrad(alpha: float, a: MatRef, b: MatRef, d: MatMut,
     is rounded, the gradient of that layer's bias."""
     fn, dt = _out_entry(d, "gk_gemm_linear_dgrad_bf16", "gk_gemm_linear_dgrad_f32out",
                         "gemm_linear_dgrad")
-    sums = _dbias(dbias)
+    sums = _dbias(dbias, d.cols)
     zc, zq = _kept(z, a.data, b.data, d.data, *(() if dbias is None else (dbias,)))
     _check(getattr(_lib.lib(), fn)(_ws(ws), float(alpha), MatRef._c(a, torch.bfloat16, "A"),
                                    MatRef._c(b, torch.bfloat16, "B"), *_act_args(act), zc, zq,
@@ -1378,7 +1380,7 @@ def activation_grad(g: MatRef, d: MatMut, act: Optional[Activation] = None,
     if dt not in (torch.float32, torch.bfloat16):
         raise TypeError(f"gemmkit_amd: activation_grad supports float32 and bfloat16, got {dt}")
     fn = "gk_activation_grad_f32" if dt == torch.float32 else "gk_activation_grad_bf16"
-    sums = _dbias(dbias)
+    sums = _dbias(dbias, d.cols)
     zc, zq = _kept(z, g.data, d.data, *(() if dbias is None else (dbias,)))
     _check(getattr(_lib.lib(), fn)(_ws(ws), MatRef._c(g, dt, "G"), *_act_args(act), zc, zq, *sums,
                                    d._c(torch.bfloat16, "D")))

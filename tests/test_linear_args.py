@@ -234,3 +234,17 @@ def test_python_types():
                  lambda: gk.dequantize_mxint8(None, m)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("n", [0, 5, 7])
+def test_python_dbias_length(n):
+    """A dbias of any wrong length, one of no elements (whose pointer is null) among them."""
+    t = torch.zeros(60, dtype=torch.bfloat16)
+    d = gk.MatMut(t, 10, 6, 6, 1)
+    dbias = torch.empty(n)
+    for call in (lambda: gk.gemm_linear_dgrad(1.0, gk.MatRef(t, 10, 6, 6, 1), gk.MatRef(t, 6, 6, 6, 1), d,
+                                              dbias=dbias),
+                 lambda: gk.activation_grad(gk.MatRef(t, 10, 6, 6, 1), d, dbias=dbias)):
+        with pytest.raises(gk.GemmkitError, match=rf"dbias length \({n}\) != the output's columns \(6\)") as e:
+            call()
+        assert e.value.code == -1
