@@ -1307,11 +1307,13 @@ def _kept(z, *tensors):
 def _dbias(dbias: Optional[torch.Tensor], cols: int):
     if dbias is None:
         return None, 0
+    # (here, since an empty tensor's pointer is null, which stands for no dbias)
+    if isinstance(dbias, torch.Tensor) and dbias.numel() != cols:
+        raise GemmkitError(-1, f"gemmkit_amd: dbias length ({dbias.numel()}) != the output's columns "
+                               f"({cols})")
     d = _slice(dbias, "dbias")
     if d.dtype != torch.float32:
         raise TypeError(f"gemmkit_amd: dbias must be float32, got {d.dtype}")
-    if d.numel() != cols:  # (here, since an empty tensor's pointer is null: no dbias)
-        raise GemmkitError(-1, f"gemmkit_amd: dbias length ({d.numel()}) != the output's columns ({cols})")
     return d.data_ptr(), d.numel()
 
 
