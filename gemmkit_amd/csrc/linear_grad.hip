@@ -331,7 +331,7 @@ __global__ __launch_bounds__(256) void col_sums_kernel(const float *part, int64_
                                                        float *out) {
     __shared__ float red[256];
     const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
-    const int64_t col = (int64_t)blockIdx.x * 16 + c;
+    const int64_t col = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + c;
     float s = 0.0f;
     if (col < n) {
 #pragma unroll 8
@@ -347,8 +347,9 @@ __global__ __launch_bounds__(256) void col_sums_kernel(const float *part, int64_
 }
 
 hipError_t launch_col_sums(const float *part, int64_t rows, int64_t n, float *out, hipStream_t stream) {
-    hipLaunchKernelGGL(col_sums_kernel, dim3((uint32_t)((n + 15) / 16)), dim3(256), 0, stream, part,
-                       rows, n, out);
+    // (from 2^28 columns on one row of workgroups would have more threads than 32 bits count)
+    hipLaunchKernelGGL(col_sums_kernel, ragged_grid((n + 15) / 16), dim3(256), 0, stream, part, rows, n,
+                       out);
     return hipGetLastError();
 }
 

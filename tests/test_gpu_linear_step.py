@@ -374,3 +374,21 @@ def test_offsets_past_32_bits(dev):
     want = (codes * torch.pow(2.0, scales - 133)).t() @ b.double()
     mags = (codes * torch.pow(2.0, scales - 133)).t().abs() @ b.double().abs()
     near(g[cols], want, (m + 2) * E23 * mags, "g")
+
+
+def test_column_sums_of_more_than_2_28_columns(dev):
+    """Their launch has more threads than 32 bits count: of no rows, and of two tiles' partial sums
+    (whole numbers, exact)."""
+    n, m, k = 2 ** 28 + 40, 129, 8
+    db = torch.full((n,), float("nan"), device=dev)
+    none = torch.empty(0, dtype=BF16, device=dev)
+    gk.gemm_linear_dgrad(1.0, gk.MatRef(none, 0, 0, 0, 1), gk.MatRef(none, 0, n, n, 1),
+                         gk.MatMut(none, 0, n, n, 1), dbias=db)
+    assert not db.any()  # (a NaN counts as true)
+    w = torch.randint(-8, 9, (n, k), dtype=torch.int8, device=dev).to(BF16)
+    d = torch.empty(m, n, dtype=BF16, device=dev)
+    gk.gemm_linear_dgrad(1.0, row(torch.ones(m, k, dtype=BF16, device=dev)), transposed(w), out(d), dbias=db)
+    want = w.sum(1, dtype=F32)
+    assert torch.equal(db, want * m)
+    for r in (0, 64, 128):
+        assert torch.equal(d[r], want.to(BF16))
