@@ -22,6 +22,7 @@ int linear_unit(const RaggedArgs &g, RaggedB bl) {
 // a time as it has threads for; column sums of its rows before rounding to one row of p.sums.
 constexpr int kStripSums = 4 * 512;  // floats: four waves of 64 chunk columns, or 16 of four
 constexpr int kStripTx = 2;  // narrow strips of aligned rows
+constexpr int64_t kStripElems = (int64_t)3 << 20;  // ... of others, at most
 
 // The workgroup's column sums from its threads': a wave's rows, then the waves, in order.
 template <int THREADS>
@@ -250,8 +251,10 @@ static bool act_grad_aligned(InType in, int64_t m, const LinearParams &p) {
 // narrow strips of all rows, which need no second launch.  Aligned rows up to 1024, four chunk
 // columns (calls, us, against two launches: bf16 512 x 8192 9.4 / 12.0, 1024 x 1024 9.6 / 14.3, 1024 x 8192
 // 10.9 / 14.9; 2048 x 4096 14.3 / 14.6, 2048 x 8192 18.8 / 19.2).  Others are bound by their addresses on
-// the few CUs of narrow strips: up to 512 rows, two chunk columns (333 x 1501 9.0 / 13.5; f32
-// 1003 x 777 14.6 / 13.5).
+// the few CUs of narrow strips, and from about 3 Mi elements on by the cache lines that strips of two
+// chunk columns share: up to 512 rows (calls: 333 x 1501 9.0 / 13.5, 256 x 8001 10.3 / 14.5, 512 x 4001
+// 10.4 / 14.3; 256 x 16001 18.8 / 14.4, 512 x 8001 17.5 / 15.6, f32 18.8 / 17.7, 512 x 65536 167 / 39;
+// more rows: f32 1003 x 777 14.6 / 13.5).
 struct ActGradShape {
     int tx, unit, threads;
 };
@@ -268,7 +271,7 @@ static ActGradShape act_grad_shape(InType in, int64_t m, int64_t n, int cus, con
     if (sums && m > unit) {
         if (m <= 1024 && m * n * (int64_t)in_size(in) < kOnceBytes && act_grad_aligned(in, m, p))
             return {kStripTx, (int)m, m <= 256 ? 256 : 1024};
-        if (m <= 512) return {1, (int)m, 256};
+        if (m <= 512 && m * n <= kStripElems) return {1, (int)m, 256};
     }
     return {tx, (int)unit, 256};
 }

@@ -697,3 +697,10 @@ def test_wgrad_of_nan_blocks(dev):
     gk.gemm_wgrad_mxint8(1.0, q, ref(rnd((100, 50), BF16, 2), "row", dev), 0.0, c.view)
     got = c.get()
     assert torch.isnan(got[32:64]).all() and torch.isfinite(got[:32]).all() and torch.isfinite(got[64:]).all()
+
+
+@pytest.mark.parametrize("m,n", [(512, 6143), (512, 6145), (96, 32767), (96, 32769), (512, 8192)])
+@pytest.mark.parametrize("z", ["row", "mx"])
+def test_activation_grad_column_sums_of_wide_rows(dev, m, n, z):
+    """On both sides of 3 Mi elements, up to which rows without alignment are summed in one launch."""
+    run_grad(dev, m, 0, n, act="silu", z=z, product_first=False)
