@@ -330,7 +330,9 @@ struct LinearParams {
     uint8_t *codes, *scales;   // row i at codes + i*ld, scales + i*lds
     int64_t ld, lds;
     float *sums;               // row of N column sums for each linear_unit() rows of the product
-    int32_t chunks;            // (set by the launch: every view has whole chunks of 16 bytes)
+    // (set by the launch: every view has unit column stride, at any alignment, and rows within a
+    // tile's 32-bit offsets; chunks that the matrix cuts go element by element)
+    int32_t chunks;
 };
 // A product without offsets (one group).  kind: C's type.
 hipError_t launch_linear(const RaggedArgs &g, RaggedB bl, EpiKind kind, const LinearParams &p,

@@ -317,7 +317,7 @@ constexpr int64_t kOnceBytes = (int64_t)64 << 20;
 constexpr int sum_unit(int bm) { return bm == 256 ? 128 : bm; }
 
 // Bands whose inputs are in flight while one is worked on (LinearOut::chunked): 8192 x 4096 x 8192's
-// input gradient through a checkpoint 435 us with two, 445 with one; four spill.
+// input gradient through a checkpoint 440 us with two, 444 with one; four spill.
 constexpr int kAhead = 2;
 
 template <EpiKind E, bool GRAD>
@@ -884,7 +884,8 @@ static hipError_t linear_go(const RaggedArgs &g, const LinearParams &p, hipStrea
     });
 }
 
-// Whether a view's chunks are whole and in reach of a tile's 32-bit offsets (LinearOut::chunked).
+// Whether a view has unit column stride, at any alignment, and rows in reach of a tile's 32-bit
+// offsets (LinearOut::chunked, whose PART takes chunks that the matrix cuts).
 inline bool chunk_rows(int64_t rs, int64_t cs, int64_t M, int64_t size) {
     return cs == 1 && (M <= 1 || rs * size <= kMaxTileRowBytes);
 }

@@ -254,7 +254,7 @@ static bool act_grad_aligned(InType in, int64_t m, const LinearParams &p) {
 // the few CUs of narrow strips, and from about 3 Mi elements on by the cache lines that strips of two
 // chunk columns share: up to 512 rows (calls: 333 x 1501 9.0 / 13.5, 256 x 8001 10.3 / 14.5, 512 x 4001
 // 10.4 / 14.3; 256 x 16001 18.8 / 14.4, 512 x 8001 17.5 / 15.6, f32 18.8 / 17.7, 512 x 65536 167 / 39;
-// more rows: f32 1003 x 777 14.6 / 13.5).
+// more rows: f32 1003 x 777 12.8 / 12.1 to 16, its kernels 12.8 / 10.1).
 struct ActGradShape {
     int tx, unit, threads;
 };

@@ -112,8 +112,11 @@ __global__ __launch_bounds__(256) void mxint8_dequantize_kernel(const MxArgs g, 
 // ---------------------------------------------------------------- weight gradient
 
 // A's stages of a weight gradient whose left operand is a checkpoint: loaded as codes, and put in
-// the stage as act(values), rounded to bf16.  (RegPanel's transposed stage; each thread decodes
-// LP chunks of eight values a stage, once for every tile of its columns.)
+// the stage as act(values), rounded to bf16: what the bf16 instructions take.  Their rounding, half of 2^-7 of a value's power of two, is
+// at most the checkpoint's own, half of 2^-6 of its block's largest: 1003x1024x704 through GELU is
+// off by 0.0019 of its norm where f32 activations would leave 0.0017 (bf16 output).  (RegPanel's
+// transposed stage; each thread decodes LP chunks of eight values a stage, once for every tile of its
+// columns.)
 template <int W, int NW>
 struct CodePanel {
     static constexpr int BYTES = W * 128, NI = BYTES / 1024, LP = NI / NW;
@@ -191,9 +194,11 @@ static hipError_t wgrad8_go(const RaggedArgs &g, const EpiParams &ep, hipStream_
 }
 
 // Few rows and tiles.  Traced kernels / calls one after the other, us, decoded in the tiles against
-// decoded first (two launches and a workspace): 64x1024x704 5.3 / 8.4 against 6.5 / 14.5, 256x1024x704
-// 7.4 / 8.6 against 7.1 / 14.4, 512x1024x704 10.2 / 9.4 against 8.1 / 14.4; through GELU 64 rows 6.6 / 8.5
-// against 6.7 / 14.2, 256 rows 10.4 / 9.6 against 7.4 / 14.1 (each tile of a column computes it again).
+// decoded first (two launches and a workspace): 64x1024x704 5.3 / 8.8 against 6.5 / 14.8, 256x1024x704
+// 7.3 / 8.7 against 7.2 / 14.8, 512x1024x704 10.2 / 9.4 against 8.3 / 14.8; through GELU 64 rows 6.6 / 8.8
+// against 6.8 / 14.8, 128 rows 8.0 / 8.8 against 6.9 / 14.8, 256 rows 10.7 / 9.8 against 7.5 / 14.9 (each
+// tile of a column computes it again).  The bounds lie where a device that other work keeps busy, to
+// which the kernels' times count, loses no more than 1 us; one that waits for the host gains 6.
 bool wgrad8_direct(const RaggedArgs &g) {
     const int64_t tiles = (int64_t)((g.K + 63) / 64) * ((g.N + 63) / 64);
     const bool smooth = g.act != kActNone && g.act != kActRelu && g.act != kActLeakyRelu;

@@ -803,8 +803,8 @@ void ragged_kernel(const RaggedArgs g, const typename O::Params ep) {
 //   phase 3  half 1, block rows 4-7   reads half 0 of stage kt+1; loads the rest of kt+2
 // bf16: three A slots and two B slots, all of the LDS; MXFP4: two of each and the scales.
 // A full round's stage, 2048 cycles of matrix instructions on each SIMD, takes 1.39 us (bf16) or
-// 1.76 us (MXFP4, four times the k): 8192 x 4096 x 8192 367 and 130 us (1.50 and 4.2 PFLOP/s);
-// prologue, epilogue and launch take 7 to 9 us.  bf16 is bound by the matrix cores, 0.8 of them
+// 1.76 us (MXFP4, four times the k): m x n x k 8192 x 4096 x 8192 367 and 130 us (1.50 and 4.2
+// PFLOP/s); prologue, epilogue and launch take 7 to 9 us.  bf16 is bound by the matrix cores, 0.8 of them
 // at the 1.8 GHz that the power limit leaves.  MXFP4 is not: at 2.08 GHz a stage is 3660 cycles,
 // of which the scales' LDS reads, waits and lane swaps at its end, and eight loads and twelve
 // fragment reads in one phase, take their part.

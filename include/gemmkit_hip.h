@@ -772,7 +772,8 @@ int gk_gemm_grouped_mxfp4_f32(gk_workspace *ws, float alpha, const gk_mxfp4 *a,
  * whole blocks of 32; one e8m0 scale per block at scales + r * lds.  A code stands for
  * code * 2^(byte - 133), 255 for NaN.  Strides are bytes, multiples of 16, and both
  * arrays 16-byte aligned; a row's scales are padded to a multiple of 16 bytes.  Codes
- * past cols and scales past the last block do not count. */
+ * past cols and scales past the last block do not count: both ways of writing put zero codes
+ * there, quantization zero scales too, and gk_gemm_linear leaves those scales as they were. */
 typedef struct gk_mxint8 {
     void *codes;
     size_t codes_len;
@@ -796,7 +797,8 @@ int gk_dequantize_mxint8_f32(const gk_mxint8 *q, int32_t act, float slope, const
 int gk_dequantize_mxint8_bf16(const gk_mxint8 *q, int32_t act, float slope, const gk_mat_mut *c);
 
 /* The weight gradient from a checkpoint: C <- alpha * H^T * B + beta * C, H = act(values of
- * a) rounded to bf16 (without activation exact), a rows x k, B rows x n, C k x n. */
+ * a) rounded to bf16 whatever C's type (without activation exact), a rows x k, B rows x n,
+ * C k x n. */
 int gk_gemm_wgrad_mxint8_bf16(gk_workspace *ws, float alpha, const gk_mxint8 *a, int32_t act,
                               float slope, const gk_mat_ref *b, float beta, const gk_mat_mut *c,
                               gk_par par);
