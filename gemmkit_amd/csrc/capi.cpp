@@ -1495,15 +1495,19 @@ bool dims_fit(size_t m, size_t k, size_t n, size_t batch) {
 }
 
 // Calls fn(z0, nb, i0, mm, j0, nn) over blocks of a (batch x) m x n user-frame
-// C of at most kMaxGridZ elements, kMaxSide rows and kMaxSide columns (the
-// element-wise fill kernels index one block per launch).
+// C of at most kMaxGridZ elements, kMaxSide rows and kMaxSide columns, and
+// 2 * kMaxSide elements of each batch element (the element-wise fill kernels
+// index one block per launch, a thread each, whose count has 32 bits: beyond
+// them a launch covers the remainder only and reports nothing).
 template <typename F>
 hipError_t for_c_blocks(int64_t m, int64_t n, int64_t batch, F fn) {
+    const int64_t cols = std::min(kMaxSide, std::max<int64_t>(n, 1));
+    const int64_t rows = std::min(kMaxSide, 2 * kMaxSide / cols);
     for (int64_t z0 = 0; z0 < batch; z0 += kMaxGridZ)
-        for (int64_t i0 = 0; i0 < m; i0 += kMaxSide)
-            for (int64_t j0 = 0; j0 < n; j0 += kMaxSide) {
+        for (int64_t i0 = 0; i0 < m; i0 += rows)
+            for (int64_t j0 = 0; j0 < n; j0 += cols) {
                 hipError_t e = fn(z0, std::min(kMaxGridZ, batch - z0), i0,
-                                  std::min(kMaxSide, m - i0), j0, std::min(kMaxSide, n - j0));
+                                  std::min(rows, m - i0), j0, std::min(cols, n - j0));
                 if (e != hipSuccess) return e;
             }
     return hipSuccess;

@@ -290,3 +290,31 @@ def test_capture_needs_a_sized_workspace(dev):
             assert np.array_equal(c.cpu().numpy(), want)
     finally:
         gk.set_synchronous(True)
+
+
+def test_empty_contraction_of_more_than_2_32_outputs(dev):
+    """k = 0: beta * C, the fused map of it and the requantized zero, element by element, more of them
+    than a launch's 32-bit thread count."""
+    m, n = 65600, 65600
+    rows = [0, 1, 128, 65472, m - 1]
+
+    def same(c, want):  # (compared in bands of rows: no matrix of flags)
+        return all(bool((c[r:r + 4096] == want).all()) for r in range(0, m, 4096)) and \
+            all(torch.equal(c[r], want.expand(n).to(c.dtype)) for r in rows)
+
+    none = torch.empty(0, dtype=torch.bfloat16, device=dev)
+    a, b = gk.MatRef(none, m, 0, 0, 1), gk.MatRef(none, 0, n, n, 1)
+    c = torch.full((m, n), 3.0, dtype=torch.bfloat16, device=dev)
+    view = gk.MatMut.from_row_major(c, m, n)
+    gk.gemm(1.0, a, b, 0.5, view)
+    assert same(c, torch.full((n,), 1.5, dtype=torch.bfloat16, device=dev))
+    bias = (torch.arange(n, device=dev) % 251).to(torch.bfloat16)
+    gk.gemm_fused(1.0, a, b, 0.0, view, bias=gk.Bias.PerCol(bias))
+    assert same(c, bias)
+    del c, view
+    none = torch.empty(0, dtype=torch.int8, device=dev)
+    q = torch.full((m, n), 3, dtype=torch.int8, device=dev)
+    gk.gemm_i8_requant(gk.MatRef(none, m, 0, 0, 1), gk.MatRef(none, 0, n, n, 1),
+                       gk.Requantize(gk.RequantScale.PerTensor(1.0), zero_point=7),
+                       gk.MatMut.from_row_major(q, m, n))
+    assert same(q, torch.full((n,), 7, dtype=torch.int8, device=dev))
